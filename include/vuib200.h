@@ -502,6 +502,83 @@ int32_t vuib_codec_enc_check_flag(VuibCodecEnc* c, void* stream);
 int32_t vuib_codec_enc_read_latent(VuibCodecEnc* c, float* out_host, int32_t n, void* stream);
 int64_t vuib_codec_enc_launch_count(VuibCodecEnc* c);
 
+/* ---------------------------------------------------------------------------
+ * Paged KV cache in 4 bits: for servers whose conversations outgrow the (slots, max_seq) bf16 cache above.  No
+ * counterpart in the reference.  Positions live in blocks of block_size that any sequence may own; the GPU itself
+ * extends the sequences' block tables (vuib_kv4_plan), so a captured step needs no host when a sequence crosses into
+ * a new block.  A vector (position, kv head) is stored in groups of 32 elements as 4-bit codes with an f16 scale and
+ * zero: 80 bytes a position and kv head at head_dim 64 (keys and values), where bf16 takes 256.
+ *   zero = f16(min x), scale = f16((max x - zero) / 15), code = nearest of 0..15; it stands for f16(scale*code + zero).
+ * Sequences are slots 0 .. max_seqs-1; their lengths are the device's.  A step is
+ *   vuib_kv4_plan once, then for every layer vuib_kv4_append and vuib_kv4_attention with that plan.
+ * All calls are asynchronous on `stream`, can be captured, allocate nothing and launch on the current device, which is
+ * the one that was current at vuib_kv4_bind.  Calls that read or write one cache, and calls that share a plan, are
+ * ordered by the caller; attention calls of one plan may overlap if their workspaces and outputs differ.
+ * Out-of-range slots, lengths and values are left out or clamped and recorded in the flag (vuib_kv4_check_flag).
+ * ------------------------------------------------------------------------- */
+typedef struct VuibKv4Config {
+    int32_t n_layers;
+    int32_t n_heads, n_kv_heads;   /* up to 16 query heads per kv head */
+    int32_t head_dim;              /* 64, 96 or 128 */
+    int32_t n_blocks, block_size;  /* block_size: 16, 32, 64, 128 or 256 positions */
+    int32_t max_seqs, max_blocks;  /* sequences (up to 4096) and blocks of one sequence */
+} VuibKv4Config;
+
+/* One step's rows: n_seqs entries (a sequence and the rows it brings) and at most n_rows rows in all, max_new of one
+ * entry.  The arrays are the caller's, written by vuib_kv4_plan and read by the calls that take the plan. */
+typedef struct VuibKv4Plan {
+    int32_t n_seqs, n_rows, max_new;
+    int32_t* entries;    /* (n_seqs, 4), 16-byte aligned: slot (-1: takes no part), first position, rows, first row */
+    int32_t* cu_rows;    /* (n_seqs + 1): first row of every entry, and the number of rows */
+    int32_t* cu_units;   /* (n_seqs + 1): first unit of attention work of every entry */
+    int32_t* row_slot;   /* (n_rows): a row's sequence, -1 behind the last row */
+    int32_t* row_pos;    /* (n_rows): its position, -1 behind the last row */
+    int64_t* slot_map;   /* (n_rows): block * block_size + position in the block, -1 behind the last row */
+} VuibKv4Plan;
+
+typedef struct VuibKv4 VuibKv4;
+
+int32_t vuib_kv4_create(const VuibKv4Config* cfg, VuibKv4** out);
+int32_t vuib_kv4_destroy(VuibKv4* c);
+int32_t vuib_kv4_last_error(VuibKv4* c, char* buf, size_t n);
+/* Bytes of the pool, all layers.  The caller allocates it (128-byte aligned), ZEROES it once and binds it with
+ * seq_lens int32[max_seqs], block_table int32[max_seqs][max_blocks] (-1: no block), free_blocks int32[n_blocks] (a
+ * stack, n_free int32[1] blocks deep) and flag int32[1]; vuib_kv4_reset gives these their first contents. */
+int32_t vuib_kv4_pool_bytes(VuibKv4* c, size_t* bytes);
+int32_t vuib_kv4_bind(VuibKv4* c, void* pool_dev, size_t bytes, int32_t* seq_lens_dev, int32_t* block_table_dev,
+                      int32_t* free_blocks_dev, int32_t* n_free_dev, int32_t* flag_dev);
+/* Every sequence empty, every block free, the flag cleared. */
+int32_t vuib_kv4_reset(VuibKv4* c, void* stream);
+
+/* Extends sequences and lays out the rows of a step.  Entry i: slots[i] (distinct; -1 takes no part) is cut back to
+ * at[i] positions (at = NULL: its length; never lengthened by it) and gets new[i] (NULL: 1 each) more.  Blocks it no
+ * longer needs go back on the stack, the first entry's first block on top; those it lacks come off the top in entry
+ * order.  Rows get the entries' new positions in entry order.
+ * An entry is left as it is, brings no rows and is recorded in the flag if its slot is out of range or named before,
+ * its lengths are out of range or above max_new, the rows up to and including it are more than n_rows, or it asks for
+ * blocks and those asked for up to and including it are more than there are.  at = 0 and new = 0 release a sequence. */
+int32_t vuib_kv4_plan(VuibKv4* c, const VuibKv4Plan* plan, const int32_t* slots_dev, const int32_t* new_dev,
+                      const int32_t* at_dev, void* stream);
+
+/* Stores the plan's rows: k, v bf16 (n_rows, n_kv_heads * head_dim), rows k_stride / v_stride elements apart (multiples
+ * of 8, 16-byte aligned).  NaN is stored as 0, magnitudes beyond 60000 as 60000 (recorded in the flag). */
+int32_t vuib_kv4_append(VuibKv4* c, int32_t layer, const VuibKv4Plan* plan, const void* k_dev, int64_t k_stride,
+                        const void* v_dev, int64_t v_stride, void* stream);
+/* What is stored for rows (row_slot, row_pos), as bf16 (n_rows, n_kv_heads * head_dim); slot -1 gives zeros. */
+int32_t vuib_kv4_read(VuibKv4* c, int32_t layer, int32_t n_rows, const int32_t* row_slot_dev, const int32_t* row_pos_dev,
+                      void* k_out_dev, int64_t k_stride, void* v_out_dev, int64_t v_stride, void* stream);
+
+/* Causal attention of the plan's rows over their sequences: row r of a sequence attends positions [0, its own], its own
+ * row included (store it first).  q, out: bf16 (n_rows, n_heads * head_dim), strides as in vuib_kv4_append; query head j
+ * reads kv head j / (n_heads / n_kv_heads).  scale 0: 1/sqrt(head_dim).  Rows behind the plan's last row are not
+ * written.  The workspace (256-byte aligned, contents of no account) holds the parts of long sequences. */
+int32_t vuib_kv4_attention_workspace(VuibKv4* c, const VuibKv4Plan* plan, size_t* bytes);
+int32_t vuib_kv4_attention(VuibKv4* c, int32_t layer, const VuibKv4Plan* plan, const void* q_dev, int64_t q_stride,
+                           void* out_dev, int64_t out_stride, float scale, void* ws_dev, size_t ws_bytes, void* stream);
+/* Reads and clears the flag.  Synchronises `stream`. */
+int32_t vuib_kv4_check_flag(VuibKv4* c, void* stream);
+int64_t vuib_kv4_launch_count(VuibKv4* c);
+
 #ifdef __cplusplus
 }
 #endif

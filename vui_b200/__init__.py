@@ -4,7 +4,8 @@ reference's Engine / Row / GenConfig API."""
 from .codec import CodecCtx, QwenCodecDecoder
 from .codec_encoder import QwenCodecEncoder, StreamingCodecEncoder
 from .engine import Engine, GenConfig, RenderRequest, Row, Segment
+from .kv4 import Kv4Cache, Kv4Plan
 from .model import VuiB200, VuiShape
 
-__all__ = ["CodecCtx", "Engine", "GenConfig", "QwenCodecDecoder", "QwenCodecEncoder", "RenderRequest", "Row", "Segment",
+__all__ = ["CodecCtx", "Engine", "GenConfig", "Kv4Cache", "Kv4Plan", "QwenCodecDecoder", "QwenCodecEncoder", "RenderRequest", "Row", "Segment",
            "StreamingCodecEncoder", "VuiB200", "VuiShape"]

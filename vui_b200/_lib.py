@@ -22,6 +22,7 @@ UNITS = {
     "vuib200.cu": ["decode_kernels.cuh", "tc_gemm.cuh", "fused_blocks.cuh", "fused_rows.cuh", "depth_tc.cuh", "prefill_attn.cuh"],
     "codec.cu": ["codec_kernels.cuh", "codec_batch.cuh", "split_ops.cuh", "split_gemm.cuh"],
     "codec_enc.cu": ["codec_enc_kernels.cuh", "split_ops.cuh", "split_gemm.cuh"],
+    "kv4.cu": ["kv4_kernels.cuh", "kv4_attn.cuh"],
 }
 SOURCES = [os.path.join(_CSRC, u) for u in UNITS]
 HEADERS = sorted({os.path.join(_CSRC, h) for hs in UNITS.values() for h in hs}) + [_API_H]
@@ -139,6 +140,17 @@ class VuibCodecEncWeights(C.Structure):
     ]
 
 
+class VuibKv4Config(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n_layers", "n_heads", "n_kv_heads", "head_dim", "n_blocks", "block_size", "max_seqs",
+                                         "max_blocks")]
+
+
+class VuibKv4Plan(C.Structure):
+    _fields_ = [("n_seqs", C.c_int32), ("n_rows", C.c_int32), ("max_new", C.c_int32),
+                ("entries", C.c_void_p), ("cu_rows", C.c_void_p), ("cu_units", C.c_void_p),
+                ("row_slot", C.c_void_p), ("row_pos", C.c_void_p), ("slot_map", C.c_void_p)]
+
+
 # name -> (restype, argtypes); every symbol include/vuib200.h declares
 _P = C.c_void_p
 SYMBOLS = {
@@ -203,6 +215,20 @@ SYMBOLS = {
     "vuib_codec_enc_check_flag": (C.c_int32, [_P, _P]),
     "vuib_codec_enc_read_latent": (C.c_int32, [_P, C.POINTER(C.c_float), C.c_int32, _P]),
     "vuib_codec_enc_launch_count": (C.c_int64, [_P]),
+    "vuib_kv4_create": (C.c_int32, [C.POINTER(VuibKv4Config), C.POINTER(_P)]),
+    "vuib_kv4_destroy": (C.c_int32, [_P]),
+    "vuib_kv4_last_error": (C.c_int32, [_P, C.c_char_p, C.c_size_t]),
+    "vuib_kv4_pool_bytes": (C.c_int32, [_P, C.POINTER(C.c_size_t)]),
+    "vuib_kv4_bind": (C.c_int32, [_P, _P, C.c_size_t, _P, _P, _P, _P, _P]),
+    "vuib_kv4_reset": (C.c_int32, [_P, _P]),
+    "vuib_kv4_plan": (C.c_int32, [_P, C.POINTER(VuibKv4Plan), _P, _P, _P, _P]),
+    "vuib_kv4_append": (C.c_int32, [_P, C.c_int32, C.POINTER(VuibKv4Plan), _P, C.c_int64, _P, C.c_int64, _P]),
+    "vuib_kv4_read": (C.c_int32, [_P, C.c_int32, C.c_int32, _P, _P, _P, C.c_int64, _P, C.c_int64, _P]),
+    "vuib_kv4_attention_workspace": (C.c_int32, [_P, C.POINTER(VuibKv4Plan), C.POINTER(C.c_size_t)]),
+    "vuib_kv4_attention": (C.c_int32, [_P, C.c_int32, C.POINTER(VuibKv4Plan), _P, C.c_int64, _P, C.c_int64, C.c_float, _P,
+                                       C.c_size_t, _P]),
+    "vuib_kv4_check_flag": (C.c_int32, [_P, _P]),
+    "vuib_kv4_launch_count": (C.c_int64, [_P]),
 }
 
 

@@ -1,0 +1,331 @@
+// Host side of the paged 4-bit KV cache: checks, sizes and launches (kernels: kv4_kernels.cuh, kv4_attn.cuh).  Entry points:
+// include/vuib200.h, section "Paged KV cache in 4 bits".
+#include <cuda_runtime.h>
+#include <stdarg.h>
+#include <stdio.h>
+#include <string.h>
+
+#include <new>
+
+#include "../../include/vuib200.h"
+#include "kv4_attn.cuh"
+#include "kv4_kernels.cuh"
+
+using namespace vuik;
+
+struct VuibKv4 {
+    VuibKv4Config cfg;
+    Kv4Cache cache;           // pool: of layer 0
+    size_t layer_bytes;
+    bool bound;
+    int block_shift, ng, sms, device;
+    int64_t launches;
+    char err[256];
+};
+
+namespace {
+
+int32_t fail(VuibKv4* c, int32_t code, const char* fmt, ...) {
+    if (c) {
+        va_list ap;
+        va_start(ap, fmt);
+        vsnprintf(c->err, sizeof(c->err), fmt, ap);
+        va_end(ap);
+    }
+    return code;
+}
+
+#define CK(call)                                                                              \
+    do {                                                                                      \
+        cudaError_t _err = (call);                                                            \
+        if (_err != cudaSuccess)                                                              \
+            return fail(c, VUIB_ERR_CUDA, "%s failed: %s", #call, cudaGetErrorString(_err));  \
+    } while (0)
+
+template <class... KArgs, class... Args>
+cudaError_t launch(VuibKv4* c, void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, int cluster, void* stream, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    c->launches++;
+    return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+}
+
+long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+
+// What a plan's shape decides for attention: columns of a tile (rows x query heads of a kv head) and positions of a split.
+// Single tokens: splits of 256 positions, four warps at 64 each, whatever the batch, so that a row's bits depend on its own keys alone.
+struct Shape { int nt, cols, split; };
+Shape shape_of(const VuibKv4* c, const VuibKv4Plan* p) {
+    Shape s;
+    const int group = c->cfg.n_heads / c->cfg.n_kv_heads;
+    const long long most = (long long)p->max_new * group;       // columns of one sequence
+    s.nt = most <= 8 ? 1 : most <= 16 || c->ng > 2 ? 2 : 4;
+    s.cols = 8 * s.nt;
+    s.split = 256;
+    if (most > 16) {
+        const long long tiles = ceil_div((long long)p->n_rows * group, s.cols) + p->n_seqs;
+        const long long len = (long long)c->cfg.max_blocks << c->block_shift;
+        s.split = 512;
+        while ((long long)s.split * 32 < len) s.split *= 2;
+        if (tiles * c->cfg.n_kv_heads >= 2 * c->sms) s.split = 1 << 30;
+    }
+    return s;
+}
+
+// Most units (of one kv head) that a plan of this shape can have.  Sequences share no blocks, so their lengths sum up to the pool's.
+long long most_units(const VuibKv4* c, const VuibKv4Plan* p, const Shape& s) {
+    const long long len = (long long)c->cfg.max_blocks << c->block_shift, pool = (long long)c->cfg.n_blocks << c->block_shift;
+    const int group = c->cfg.n_heads / c->cfg.n_kv_heads;
+    const long long a_seq = ceil_div((long long)p->max_new * group, s.cols);
+    const long long tiles = min((long long)p->n_seqs * a_seq, ceil_div((long long)p->n_rows * group, s.cols) + p->n_seqs);
+    return min(tiles * ceil_div(len, s.split), a_seq * (p->n_seqs + pool / s.split));
+}
+
+size_t acc_bytes(const VuibKv4* c, long long items, int cols) { return ((size_t)items * cols * c->cfg.head_dim * 4 + 255) & ~size_t(255); }
+
+int32_t check_plan(VuibKv4* c, const VuibKv4Plan* p) {
+    if (!p || !p->entries || !p->cu_rows || !p->cu_units) return fail(c, VUIB_ERR_NULL, "a plan needs its arrays");
+    if (p->n_rows > 0 && (!p->row_slot || !p->row_pos || !p->slot_map)) return fail(c, VUIB_ERR_NULL, "a plan of rows needs its row arrays");
+    if (p->n_seqs < 1 || p->n_seqs > KV4_MAX_SEQS) return fail(c, VUIB_ERR_RANGE, "n_seqs %d not in 1..%d", p->n_seqs, KV4_MAX_SEQS);
+    if (p->n_rows < 0 || p->n_rows > 1 << 24) return fail(c, VUIB_ERR_RANGE, "n_rows %d not in 0..%d", p->n_rows, 1 << 24);
+    if (p->max_new < 0 || p->max_new > p->n_rows) return fail(c, VUIB_ERR_RANGE, "max_new %d not in 0..n_rows", p->max_new);
+    if (reinterpret_cast<uintptr_t>(p->entries) & 15) return fail(c, VUIB_ERR_WORKSPACE, "entries must be 16-byte aligned");
+    if (!c->bound) return fail(c, VUIB_ERR_UNBOUND, "vuib_kv4_bind has not been called");
+    return VUIB_OK;
+}
+
+// A matrix of rows: 16-byte aligned, rows at a multiple of 8 elements and not overlapping.
+int32_t check_rows(VuibKv4* c, const char* name, const void* p, int64_t stride, int64_t width) {
+    if (!p) return fail(c, VUIB_ERR_NULL, "%s is NULL", name);
+    if (reinterpret_cast<uintptr_t>(p) & 15 || stride % 8 || stride < width)
+        return fail(c, VUIB_ERR_SHAPE, "%s: rows must be 16-byte aligned, a multiple of 8 elements and at least %lld apart (stride %lld)", name,
+                    (long long)width, (long long)stride);
+    return VUIB_OK;
+}
+
+template <int NG, int NT>
+cudaError_t launch_attn(VuibKv4* c, const Kv4AttnArgs& a, long long items, bool merge, void* stream) {
+    // as many CTAs as can be resident: their number is asked for once a kernel
+    static int resident = 0;
+    cudaError_t e = cudaSuccess;
+    if (!resident) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, k_kv4_attn<NG, NT>, KA_THREADS, 0);
+    if (e != cudaSuccess) return e;
+    const long long grid = min(items, (long long)c->sms * (resident > 0 ? resident : 1));
+    e = launch(c, k_kv4_attn<NG, NT>, dim3((unsigned)grid), KA_THREADS, 0, 1, stream, a);
+    if (e != cudaSuccess || !merge) return e;
+    return launch(c, k_kv4_merge<NG>, dim3((unsigned)ceil_div((long long)a.n_rows * c->cfg.n_heads, 8)), 256, 0, 1, stream, a, NT * 8);
+}
+
+}  // namespace
+
+extern "C" int32_t vuib_kv4_create(const VuibKv4Config* cfg, VuibKv4** out) {
+    if (!cfg || !out) return VUIB_ERR_NULL;
+    *out = nullptr;
+    const VuibKv4Config& g = *cfg;
+    if (g.head_dim != 64 && g.head_dim != 96 && g.head_dim != 128) return VUIB_ERR_SHAPE;
+    if (g.n_kv_heads < 1 || g.n_heads < g.n_kv_heads || g.n_heads % g.n_kv_heads || g.n_heads / g.n_kv_heads > 16 || g.n_heads > 1024)
+        return VUIB_ERR_SHAPE;
+    int shift = 4;
+    while (shift < 8 && 1 << shift < g.block_size) ++shift;
+    if (1 << shift != g.block_size) return VUIB_ERR_SHAPE;
+    if (g.n_layers < 1 || g.n_layers > 1024 || g.n_blocks < 1 || g.n_blocks > 1 << 24 || g.max_seqs < 1 || g.max_seqs > KV4_MAX_SEQS ||
+        g.max_blocks < 1 || (long long)g.max_blocks << shift > 1 << 24)
+        return VUIB_ERR_RANGE;
+    VuibKv4* c = new (std::nothrow) VuibKv4();
+    if (!c) return VUIB_ERR_NULL;
+    memset(c, 0, sizeof(*c));
+    c->cfg = g;
+    c->block_shift = shift;
+    c->ng = g.head_dim / KV4_GROUP;
+    c->layer_bytes = (size_t)g.n_blocks * g.n_kv_heads * (g.block_size / KV4_TILE) * c->ng * KV4_GT;
+    *out = c;
+    return VUIB_OK;
+}
+
+extern "C" int32_t vuib_kv4_destroy(VuibKv4* c) {
+    delete c;
+    return VUIB_OK;
+}
+
+extern "C" int32_t vuib_kv4_last_error(VuibKv4* c, char* buf, size_t n) {
+    if (!c || !buf || !n) return VUIB_ERR_NULL;
+    snprintf(buf, n, "%s", c->err);
+    return VUIB_OK;
+}
+
+extern "C" int32_t vuib_kv4_pool_bytes(VuibKv4* c, size_t* bytes) {
+    if (!c || !bytes) return VUIB_ERR_NULL;
+    *bytes = c->layer_bytes * c->cfg.n_layers;
+    return VUIB_OK;
+}
+
+extern "C" int32_t vuib_kv4_bind(VuibKv4* c, void* pool, size_t bytes, int32_t* seq_lens, int32_t* block_table, int32_t* free_blocks,
+                                 int32_t* n_free, int32_t* flag) {
+    if (!c) return VUIB_ERR_NULL;
+    c->bound = false;
+    if (!pool || !seq_lens || !block_table || !free_blocks || !n_free || !flag) return fail(c, VUIB_ERR_NULL, "a pointer is NULL");
+    if (reinterpret_cast<uintptr_t>(pool) & 127) return fail(c, VUIB_ERR_WORKSPACE, "the pool must be 128-byte aligned");
+    if (bytes < c->layer_bytes * c->cfg.n_layers)
+        return fail(c, VUIB_ERR_WORKSPACE, "pool of %zu bytes, %zu needed", bytes, c->layer_bytes * c->cfg.n_layers);
+    CK(cudaGetDevice(&c->device));
+    CK(cudaDeviceGetAttribute(&c->sms, cudaDevAttrMultiProcessorCount, c->device));
+    c->cache = {static_cast<unsigned char*>(pool), block_table, seq_lens, free_blocks, n_free, flag, c->cfg.n_kv_heads, c->block_shift,
+                c->cfg.n_blocks, c->cfg.max_seqs, c->cfg.max_blocks};
+    c->bound = true;
+    return VUIB_OK;
+}
+
+extern "C" int32_t vuib_kv4_reset(VuibKv4* c, void* stream) {
+    if (!c) return VUIB_ERR_NULL;
+    if (!c->bound) return fail(c, VUIB_ERR_UNBOUND, "vuib_kv4_bind has not been called");
+    const long long n = (long long)c->cfg.max_seqs * c->cfg.max_blocks;
+    CK(launch(c, k_kv4_reset, dim3((unsigned)min(ceil_div(max(n, (long long)c->cfg.n_blocks), 256), 1024ll)), 256, 0, 1, stream, c->cache));
+    return VUIB_OK;
+}
+
+extern "C" int32_t vuib_kv4_plan(VuibKv4* c, const VuibKv4Plan* p, const int32_t* slots_dev, const int32_t* new_dev, const int32_t* at_dev,
+                                 void* stream) {
+    if (!c) return VUIB_ERR_NULL;
+    if (int32_t rc = check_plan(c, p)) return rc;
+    if (!slots_dev) return fail(c, VUIB_ERR_NULL, "slots is NULL");
+    if (!new_dev && p->max_new < 1) return fail(c, VUIB_ERR_RANGE, "one new row each, but max_new is %d", p->max_new);
+    const Shape s = shape_of(c, p);
+    if (most_units(c, p, s) > 0x7fffffffll / 2) return fail(c, VUIB_ERR_RANGE, "too many units of work for one plan");
+    Kv4PlanArgs a = {};
+    a.c = c->cache;
+    a.slots = slots_dev; a.new_lens = new_dev; a.at = at_dev;
+    a.n = p->n_seqs; a.n_rows = p->n_rows; a.max_new = p->max_new;
+    a.group = c->cfg.n_heads / c->cfg.n_kv_heads; a.cols = s.cols; a.split = s.split;
+    a.entries = reinterpret_cast<int4*>(p->entries); a.cu_rows = p->cu_rows; a.cu_units = p->cu_units;
+    a.row_slot = p->row_slot; a.row_pos = p->row_pos; a.slot_map = reinterpret_cast<long long*>(p->slot_map);
+    const size_t smem = (8 * (size_t)p->n_seqs + 3 + c->cfg.max_seqs) * 4;
+    if (smem > 48 * 1024) CK(cudaFuncSetAttribute(k_kv4_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    const int cluster = p->n_rows > 4096 ? 8 : 1;
+    CK(launch(c, k_kv4_plan, dim3(cluster), 1024, smem, cluster, stream, a));
+    return VUIB_OK;
+}
+
+extern "C" int32_t vuib_kv4_append(VuibKv4* c, int32_t layer, const VuibKv4Plan* p, const void* k_dev, int64_t k_stride, const void* v_dev,
+                                   int64_t v_stride, void* stream) {
+    if (!c) return VUIB_ERR_NULL;
+    if (int32_t rc = check_plan(c, p)) return rc;
+    if (layer < 0 || layer >= c->cfg.n_layers) return fail(c, VUIB_ERR_RANGE, "layer %d not in 0..%d", layer, c->cfg.n_layers - 1);
+    if (!p->n_rows) return VUIB_OK;
+    const int64_t width = (int64_t)c->cfg.n_kv_heads * c->cfg.head_dim;
+    if (int32_t rc = check_rows(c, "k", k_dev, k_stride, width)) return rc;
+    if (int32_t rc = check_rows(c, "v", v_dev, v_stride, width)) return rc;
+    Kv4RowsArgs a = {};
+    a.c = c->cache;
+    a.c.pool += c->layer_bytes * layer;
+    a.k = static_cast<const __nv_bfloat16*>(k_dev); a.k_stride = k_stride;
+    a.v = static_cast<const __nv_bfloat16*>(v_dev); a.v_stride = v_stride;
+    a.slot_map = reinterpret_cast<const long long*>(p->slot_map);
+    a.n_rows = p->n_rows;
+    const dim3 grid((unsigned)ceil_div((long long)p->n_rows * width / 8, 256), 2);
+    CK(c->ng == 2 ? launch(c, k_kv4_append<2>, grid, 256, 0, 1, stream, a)
+                  : c->ng == 3 ? launch(c, k_kv4_append<3>, grid, 256, 0, 1, stream, a) : launch(c, k_kv4_append<4>, grid, 256, 0, 1, stream, a));
+    return VUIB_OK;
+}
+
+extern "C" int32_t vuib_kv4_read(VuibKv4* c, int32_t layer, int32_t n_rows, const int32_t* row_slot_dev, const int32_t* row_pos_dev,
+                                 void* k_out_dev, int64_t k_stride, void* v_out_dev, int64_t v_stride, void* stream) {
+    if (!c) return VUIB_ERR_NULL;
+    if (!c->bound) return fail(c, VUIB_ERR_UNBOUND, "vuib_kv4_bind has not been called");
+    if (layer < 0 || layer >= c->cfg.n_layers) return fail(c, VUIB_ERR_RANGE, "layer %d not in 0..%d", layer, c->cfg.n_layers - 1);
+    if (n_rows < 0 || n_rows > 1 << 24) return fail(c, VUIB_ERR_RANGE, "n_rows %d not in 0..%d", n_rows, 1 << 24);
+    if (!n_rows) return VUIB_OK;
+    if (!row_slot_dev || !row_pos_dev) return fail(c, VUIB_ERR_NULL, "row_slot or row_pos is NULL");
+    const int64_t width = (int64_t)c->cfg.n_kv_heads * c->cfg.head_dim;
+    if (int32_t rc = check_rows(c, "k_out", k_out_dev, k_stride, width)) return rc;
+    if (int32_t rc = check_rows(c, "v_out", v_out_dev, v_stride, width)) return rc;
+    Kv4RowsArgs a = {};
+    a.c = c->cache;
+    a.c.pool += c->layer_bytes * layer;
+    a.k_out = static_cast<__nv_bfloat16*>(k_out_dev); a.k_stride = k_stride;
+    a.v_out = static_cast<__nv_bfloat16*>(v_out_dev); a.v_stride = v_stride;
+    a.row_slot = row_slot_dev; a.row_pos = row_pos_dev;
+    a.n_rows = n_rows;
+    const dim3 grid((unsigned)ceil_div((long long)n_rows * width / 8, 256), 2);
+    CK(c->ng == 2 ? launch(c, k_kv4_read<2>, grid, 256, 0, 1, stream, a)
+                  : c->ng == 3 ? launch(c, k_kv4_read<3>, grid, 256, 0, 1, stream, a) : launch(c, k_kv4_read<4>, grid, 256, 0, 1, stream, a));
+    return VUIB_OK;
+}
+
+extern "C" int32_t vuib_kv4_attention_workspace(VuibKv4* c, const VuibKv4Plan* p, size_t* bytes) {
+    if (!c || !bytes) return VUIB_ERR_NULL;
+    if (int32_t rc = check_plan(c, p)) return rc;
+    *bytes = 0;
+    if (!p->n_rows || !p->max_new) return VUIB_OK;
+    const Shape s = shape_of(c, p);
+    if (((long long)c->cfg.max_blocks << c->block_shift) <= s.split) return VUIB_OK;
+    const long long items = most_units(c, p, s) * c->cfg.n_kv_heads;
+    *bytes = acc_bytes(c, items, s.cols) + (size_t)items * s.cols * 8;
+    return VUIB_OK;
+}
+
+extern "C" int32_t vuib_kv4_attention(VuibKv4* c, int32_t layer, const VuibKv4Plan* p, const void* q_dev, int64_t q_stride, void* out_dev,
+                                      int64_t out_stride, float scale, void* ws_dev, size_t ws_bytes, void* stream) {
+    if (!c) return VUIB_ERR_NULL;
+    if (int32_t rc = check_plan(c, p)) return rc;
+    if (layer < 0 || layer >= c->cfg.n_layers) return fail(c, VUIB_ERR_RANGE, "layer %d not in 0..%d", layer, c->cfg.n_layers - 1);
+    if (!(scale >= 0.f) || scale > 1e30f) return fail(c, VUIB_ERR_RANGE, "scale must be positive, or 0 for 1/sqrt(head_dim)");
+    if (!p->n_rows || !p->max_new) return VUIB_OK;
+    const int64_t width = (int64_t)c->cfg.n_heads * c->cfg.head_dim;
+    if (int32_t rc = check_rows(c, "q", q_dev, q_stride, width)) return rc;
+    if (int32_t rc = check_rows(c, "out", out_dev, out_stride, width)) return rc;
+    size_t need = 0;
+    if (int32_t rc = vuib_kv4_attention_workspace(c, p, &need)) return rc;
+    if (need && (!ws_dev || ws_bytes < need || reinterpret_cast<uintptr_t>(ws_dev) & 255))
+        return fail(c, VUIB_ERR_WORKSPACE, "workspace of %zu bytes, 256-byte aligned, needed", need);
+    const Shape s = shape_of(c, p);
+    const long long items = most_units(c, p, s) * c->cfg.n_kv_heads;
+    Kv4AttnArgs a = {};
+    a.c = c->cache;
+    a.c.pool += c->layer_bytes * layer;
+    a.entries = reinterpret_cast<const int4*>(p->entries); a.cu_rows = p->cu_rows; a.cu_units = p->cu_units;
+    a.n = p->n_seqs; a.n_rows = p->n_rows; a.group = c->cfg.n_heads / c->cfg.n_kv_heads; a.split = s.split;
+    a.q = static_cast<const __nv_bfloat16*>(q_dev); a.q_stride = q_stride;
+    a.out = static_cast<__nv_bfloat16*>(out_dev); a.out_stride = out_stride;
+    a.scale_log2 = (scale > 0.f ? scale : 1.f / sqrtf((float)c->cfg.head_dim)) * 1.4426950408889634f;
+    a.acc = static_cast<float*>(ws_dev);
+    a.ml = reinterpret_cast<float2*>(static_cast<char*>(ws_dev) + acc_bytes(c, items, s.cols));
+    const bool merge = need != 0;
+    switch (c->ng * 8 + s.nt) {
+        case 17: CK((launch_attn<2, 1>(c, a, items, merge, stream))); break;
+        case 18: CK((launch_attn<2, 2>(c, a, items, merge, stream))); break;
+        case 20: CK((launch_attn<2, 4>(c, a, items, merge, stream))); break;
+        case 25: CK((launch_attn<3, 1>(c, a, items, merge, stream))); break;
+        case 26: CK((launch_attn<3, 2>(c, a, items, merge, stream))); break;
+        case 33: CK((launch_attn<4, 1>(c, a, items, merge, stream))); break;
+        default: CK((launch_attn<4, 2>(c, a, items, merge, stream))); break;
+    }
+    return VUIB_OK;
+}
+
+extern "C" int32_t vuib_kv4_check_flag(VuibKv4* c, void* stream) {
+    if (!c) return VUIB_ERR_NULL;
+    if (!c->bound) return fail(c, VUIB_ERR_UNBOUND, "vuib_kv4_bind has not been called");
+    int32_t v = 0;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    CK(cudaMemcpyAsync(&v, c->cache.flag, 4, cudaMemcpyDeviceToHost, s));
+    CK(cudaStreamSynchronize(s));
+    if (!v) return VUIB_OK;
+    CK(cudaMemsetAsync(c->cache.flag, 0, 4, s));
+    return fail(c, VUIB_ERR_DEVICE_FLAG, "device flag %d:%s%s%s%s%s%s", v, v & KV4_BAD_SLOT ? " slot or position out of range or named twice;" : "",
+                v & KV4_BAD_LEN ? " length out of range;" : "", v & KV4_NO_ROWS ? " more rows than the plan holds;" : "",
+                v & KV4_NO_BLOCKS ? " out of blocks;" : "", v & KV4_BAD_VALUE ? " NaN or a value beyond 60000 stored;" : "",
+                v & KV4_BAD_BLOCK ? " no block for a position;" : "");
+}
+
+extern "C" int64_t vuib_kv4_launch_count(VuibKv4* c) { return c ? c->launches : 0; }

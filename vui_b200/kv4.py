@@ -1,0 +1,213 @@
+"""A paged KV cache held in 4 bits, with the attention that reads it (``vuib_kv4_*`` of libvuib200).
+
+Next to the engine's bf16 cache of ``max_seq`` positions a slot (48 KB a position for Vui Nano), for servers that keep
+many or long conversations: positions live in blocks that any sequence may own, and keys and values take 5 bits an
+element with their scales (3.2 times less memory, and 3.2 times fewer bytes for a decode step to read).  The block
+tables are built and extended on the GPU, so that a captured step needs no host when a sequence crosses into a new
+block.  The reference has no counterpart.
+
+A step::
+
+    plan = cache.plan(slots)                       # one new row for every sequence: tables, positions, slot map
+    for layer in range(n_layers):
+        cache.append(layer, k, v, plan)            # (rows, n_kv_heads, head_dim) bf16, keys with RoPE applied
+        out = cache.attention(layer, q, plan)      # (rows, n_heads, head_dim) bf16
+
+A prompt is the same with ``cache.plan(slots, lengths)``; its rows are the sequences' new positions behind one another.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+from torch import Tensor
+
+from . import _lib
+
+
+class Kv4Plan:
+    """The rows of one step, all on the device: ``row_slot`` and ``row_pos`` (int32) say which position of which sequence
+    a row is, ``slot_map`` (int64) where it lies (block * block_size + offset), ``cu_rows`` (int32, one more than
+    sequences) where each sequence's rows begin.  Rows behind the last are -1."""
+
+    def __init__(self, device, n_seqs: int, n_rows: int, max_new: int):
+        self.n_seqs, self.n_rows, self.max_new = n_seqs, n_rows, max_new
+        self._ints = torch.empty(6 * n_seqs + 4 + 2 * n_rows, dtype=torch.int32, device=device)
+        self._entries, self.cu_rows, self._cu_units, self.row_slot, self.row_pos = self._ints.split(
+            [4 * n_seqs, n_seqs + 1, n_seqs + 3, n_rows, n_rows])
+        self.slot_map = torch.empty(n_rows, dtype=torch.int64, device=device)
+        P = lambda t: t.data_ptr()  # noqa: E731
+        self._c = _lib.VuibKv4Plan(n_seqs, n_rows, max_new, P(self._entries), P(self.cu_rows), P(self._cu_units),
+                                   P(self.row_slot) if n_rows else None, P(self.row_pos) if n_rows else None,
+                                   P(self.slot_map) if n_rows else None)
+
+
+class Kv4Cache:
+    """``n_blocks`` blocks of ``block_size`` positions (16, 32, 64, 128 or 256) for ``max_seqs`` sequences of at most
+    ``max_blocks`` blocks each; ``head_dim`` 64, 96 or 128, up to 16 query heads per kv head.  ``seq_lens``,
+    ``block_table`` and ``n_free`` are the device's own state, to be read but not written by the caller."""
+
+    def __init__(self, *, n_layers: int, n_heads: int, n_kv_heads: int, head_dim: int, n_blocks: int, block_size: int = 64,
+                 max_seqs: int, max_blocks: int | None = None, device="cuda"):
+        self._h = C.c_void_p()
+        max_blocks = n_blocks if max_blocks is None else max_blocks
+        cfg = _lib.VuibKv4Config(n_layers, n_heads, n_kv_heads, head_dim, n_blocks, block_size, max_seqs, max_blocks)
+        self._lib = _lib.load()
+        rc = self._lib.vuib_kv4_create(C.byref(cfg), C.byref(self._h))
+        if rc:
+            raise ValueError(f"unsupported 4-bit cache (status {rc}): {n_layers} layers, {n_heads}/{n_kv_heads} heads of {head_dim}, "
+                             f"{n_blocks} blocks of {block_size}, {max_seqs} sequences of up to {max_blocks} blocks")
+        if not torch.cuda.is_available():
+            raise RuntimeError("vui_b200.Kv4Cache needs a CUDA device (sm_100a); there is no CPU path")
+        dev = torch.device(device)
+        self.device = dev if dev.index is not None else torch.device("cuda", torch.cuda.current_device())
+        self.n_layers, self.n_heads, self.n_kv_heads, self.head_dim = n_layers, n_heads, n_kv_heads, head_dim
+        self.n_blocks, self.block_size, self.max_seqs, self.max_blocks = n_blocks, block_size, max_seqs, max_blocks
+        n = C.c_size_t()
+        self._ck(self._lib.vuib_kv4_pool_bytes(self._h, C.byref(n)))
+        self.pool_bytes = n.value
+        i32 = lambda *shape: torch.zeros(*shape, dtype=torch.int32, device=self.device)  # noqa: E731
+        with torch.cuda.device(self.device):
+            self._pool = torch.zeros(n.value, dtype=torch.uint8, device=self.device)
+            self.seq_lens, self.block_table = i32(max_seqs), i32(max_seqs, max_blocks)
+            self._free, self.n_free, self._flag = i32(n_blocks), i32(1), i32(1)
+            P = lambda t: t.data_ptr()  # noqa: E731
+            self._ck(self._lib.vuib_kv4_bind(self._h, P(self._pool), n.value, P(self.seq_lens), P(self.block_table), P(self._free),
+                                             P(self.n_free), P(self._flag)))
+            self._ck(self._lib.vuib_kv4_reset(self._h, self._stream))
+
+    def __del__(self):
+        try:
+            if self._h:
+                self._lib.vuib_kv4_destroy(self._h)
+                self._h = C.c_void_p()
+        except Exception:
+            pass
+
+    def _ck(self, rc: int) -> None:
+        if rc:
+            buf = C.create_string_buffer(256)
+            self._lib.vuib_kv4_last_error(self._h, buf, 256)
+            raise _lib.VuibError(rc, buf.value.decode(errors="replace") or "(no message)")
+
+    @property
+    def _stream(self):
+        return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+
+    def _ints(self, v, name: str, n: int | None = None) -> Tensor:
+        t = v if torch.is_tensor(v) else torch.as_tensor(v, dtype=torch.int64 if len(v) == 0 else None)
+        if t.dim() != 1 or t.is_floating_point() or t.is_complex() or (n is not None and t.numel() != n):
+            raise ValueError(f"{name}: a one-dimensional list of {'whole numbers' if n is None else f'{n} whole numbers'} is wanted, "
+                             f"got {t.dtype} {tuple(t.shape)}")
+        return t.to(self.device, torch.int32).contiguous()
+
+    # ------------------------------------------------------------------ tables
+    def reset(self) -> None:
+        """Empties every sequence."""
+        with torch.cuda.device(self.device):
+            self._ck(self._lib.vuib_kv4_reset(self._h, self._stream))
+
+    def plan(self, slots, new_lens=None, at=None, *, n_rows: int | None = None, max_new: int | None = None) -> Kv4Plan:
+        """Lengthens sequence ``slots[i]`` by ``new_lens[i]`` positions (None: one each), after cutting it back to ``at[i]``
+        where ``at`` is given, and lays out the new rows.  Lists or tensors; with lengths that are on the device, ``n_rows``
+        (rows that the plan has room for) and ``max_new`` (most rows of one sequence) have to be given, so that nothing waits
+        for them.  Slot -1 takes no part.  A sequence for which rows or blocks run out, or whose numbers are out of range,
+        stays as it is, brings no rows and is recorded (``check_device``)."""
+        if new_lens is not None and not (torch.is_tensor(new_lens) and new_lens.is_cuda):
+            host = [int(x) for x in new_lens]
+            n_rows = sum(max(x, 0) for x in host) if n_rows is None else n_rows
+            max_new = min(n_rows, max(host, default=0)) if max_new is None else max_new
+        slots = self._ints(slots, "slots")
+        n = slots.numel()
+        if n == 0:
+            raise ValueError("slots is empty")
+        if new_lens is None:
+            n_rows, max_new = n if n_rows is None else n_rows, 1 if max_new is None else max_new
+        if n_rows is None or max_new is None:
+            raise ValueError("new_lens on the device need n_rows and max_new")
+        with torch.cuda.device(self.device):
+            new = None if new_lens is None else self._ints(new_lens, "new_lens", n)
+            at = None if at is None else self._ints(at, "at", n)
+            if n_rows < 0 or max_new < 0:
+                raise ValueError("n_rows and max_new must not be negative")
+            plan = Kv4Plan(self.device, n, int(n_rows), min(int(max_new), int(n_rows)))
+            self._ck(self._lib.vuib_kv4_plan(self._h, C.byref(plan._c), slots.data_ptr(), None if new is None else new.data_ptr(),
+                                             None if at is None else at.data_ptr(), self._stream))
+        return plan
+
+    def release(self, slots) -> None:
+        """Empties these sequences and gives their blocks back."""
+        slots = self._ints(slots, "slots")
+        none = torch.zeros_like(slots)
+        self.plan(slots, none, at=none, n_rows=0, max_new=0)
+
+    # -------------------------------------------------------------------- rows
+    def _rows(self, t: Tensor, name: str, n: int, heads: int, *, out: bool = False) -> Tensor:
+        """(n, heads, head_dim) or (n, heads * head_dim) as the library takes it: bf16 on this device, heads behind one
+        another, rows a multiple of 16 bytes apart.  An input that lies otherwise is copied, an output refused."""
+        if not torch.is_tensor(t) or tuple(t.shape) not in ((n, heads, self.head_dim), (n, heads * self.head_dim)):
+            raise ValueError(f"{name}: ({n}, {heads}, {self.head_dim}) is wanted, got {tuple(t.shape) if torch.is_tensor(t) else type(t)}")
+        good = t.device == self.device and t.dtype == torch.bfloat16
+        if not out:
+            t = t.to(self.device, torch.bfloat16)
+        flat = t.stride(-1) == 1 and (t.dim() == 2 or heads == 1 or t.stride(1) == self.head_dim)
+        step = t.stride(0) if n > 1 else heads * self.head_dim
+        if flat and step % 8 == 0 and step >= heads * self.head_dim and t.data_ptr() % 16 == 0 and (good or not out):
+            return t
+        if out:
+            raise ValueError(f"{name}: bf16 on {self.device} with heads behind one another and rows a multiple of 16 bytes apart is wanted")
+        t = t.contiguous()
+        return t if t.data_ptr() % 16 == 0 else t.clone()
+
+    def _step(self, t: Tensor, heads: int) -> int:
+        return t.stride(0) if t.shape[0] > 1 else heads * self.head_dim
+
+    def append(self, layer: int, k: Tensor, v: Tensor, plan: Kv4Plan) -> None:
+        """Stores the plan's rows: k, v (n_rows, n_kv_heads, head_dim), keys with RoPE applied.  NaN is stored as 0 and
+        magnitudes beyond 60000 as 60000, which ``check_device`` reports."""
+        with torch.cuda.device(self.device):
+            k, v = (self._rows(t, name, plan.n_rows, self.n_kv_heads) for t, name in ((k, "k"), (v, "v")))
+            self._ck(self._lib.vuib_kv4_append(self._h, layer, C.byref(plan._c), k.data_ptr(), self._step(k, self.n_kv_heads),
+                                               v.data_ptr(), self._step(v, self.n_kv_heads), self._stream))
+
+    def read(self, layer: int, row_slot, row_pos, *, k_out: Tensor | None = None, v_out: Tensor | None = None) -> tuple[Tensor, Tensor]:
+        """The keys and values stored for position ``row_pos[i]`` of sequence ``row_slot[i]``: (n, n_kv_heads, head_dim) bf16,
+        new tensors or ``k_out`` and ``v_out`` (a stretch of an engine's bf16 cache, say).  Slot -1 gives zeros."""
+        with torch.cuda.device(self.device):
+            row_slot = self._ints(row_slot, "row_slot")
+            n = row_slot.numel()
+            row_pos = self._ints(row_pos, "row_pos", n)
+            new = lambda: torch.empty(n, self.n_kv_heads, self.head_dim, dtype=torch.bfloat16, device=self.device)  # noqa: E731
+            k = new() if k_out is None else self._rows(k_out, "k_out", n, self.n_kv_heads, out=True)
+            v = new() if v_out is None else self._rows(v_out, "v_out", n, self.n_kv_heads, out=True)
+            if n:
+                self._ck(self._lib.vuib_kv4_read(self._h, layer, n, row_slot.data_ptr(), row_pos.data_ptr(), k.data_ptr(),
+                                                 self._step(k, self.n_kv_heads), v.data_ptr(), self._step(v, self.n_kv_heads), self._stream))
+        return k, v
+
+    def attention(self, layer: int, q: Tensor, plan: Kv4Plan, *, scale: float | None = None, out: Tensor | None = None) -> Tensor:
+        """Causal attention of the plan's rows, each over its sequence up to and with its own position (append first):
+        q (n_rows, n_heads, head_dim) with RoPE applied -> the same shape, bf16.  ``scale`` defaults to 1 / sqrt(head_dim).
+        Rows behind the plan's last are not written."""
+        if scale is not None and not 0 < scale <= 1e30:
+            raise ValueError("scale must be positive")
+        with torch.cuda.device(self.device):
+            q = self._rows(q, "q", plan.n_rows, self.n_heads)
+            out = torch.empty(q.shape, dtype=torch.bfloat16, device=self.device) if out is None else self._rows(out, "out", plan.n_rows, self.n_heads, out=True)
+            n = C.c_size_t()
+            self._ck(self._lib.vuib_kv4_attention_workspace(self._h, C.byref(plan._c), C.byref(n)))
+            ws = torch.empty(n.value, dtype=torch.uint8, device=self.device) if n.value else None
+            self._ck(self._lib.vuib_kv4_attention(self._h, layer, C.byref(plan._c), q.data_ptr(), self._step(q, self.n_heads), out.data_ptr(),
+                                                  self._step(out, self.n_heads), float(scale or 0.0), None if ws is None else ws.data_ptr(), n.value,
+                                                  self._stream))
+        return out
+
+    # ------------------------------------------------------------- diagnostics
+    def check_device(self) -> None:
+        """Raises if a call since the last check met a slot, length or value out of range, or ran out of rows or blocks."""
+        with torch.cuda.device(self.device):
+            self._ck(self._lib.vuib_kv4_check_flag(self._h, self._stream))
+
+    def launch_count(self) -> int:
+        return int(self._lib.vuib_kv4_launch_count(self._h))
