@@ -119,10 +119,12 @@ cudaError_t launch_attn(VuibKv4* c, const Kv4AttnArgs& a, long long items, bool 
     // as many CTAs as can be resident: their number is asked for once a kernel
     static int resident = 0;
     cudaError_t e = cudaSuccess;
-    if (!resident) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, k_kv4_attn<NG, NT>, KA_THREADS, 0);
+    constexpr int smem = KaShared<NG, NT>::TOTAL;
+    e = cudaFuncSetAttribute(k_kv4_attn<NG, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess && !resident) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, k_kv4_attn<NG, NT>, KA_THREADS + 32, smem);
     if (e != cudaSuccess) return e;
     const long long grid = min(items, (long long)c->sms * (resident > 0 ? resident : 1));
-    e = launch(c, k_kv4_attn<NG, NT>, dim3((unsigned)grid), KA_THREADS, 0, 1, stream, a);
+    e = launch(c, k_kv4_attn<NG, NT>, dim3((unsigned)grid), KA_THREADS + 32, smem, 1, stream, a);
     if (e != cudaSuccess || !merge) return e;
     return launch(c, k_kv4_merge<NG>, dim3((unsigned)ceil_div((long long)a.n_rows * c->cfg.n_heads, 8)), 256, 0, 1, stream, a, NT * 8);
 }
@@ -322,10 +324,10 @@ extern "C" int32_t vuib_kv4_check_flag(VuibKv4* c, void* stream) {
     CK(cudaStreamSynchronize(s));
     if (!v) return VUIB_OK;
     CK(cudaMemsetAsync(c->cache.flag, 0, 4, s));
-    return fail(c, VUIB_ERR_DEVICE_FLAG, "device flag %d:%s%s%s%s%s%s", v, v & KV4_BAD_SLOT ? " slot or position out of range or named twice;" : "",
+    return fail(c, VUIB_ERR_DEVICE_FLAG, "device flag %d:%s%s%s%s%s%s%s", v, v & KV4_BAD_SLOT ? " slot or position out of range or named twice;" : "",
                 v & KV4_BAD_LEN ? " length out of range;" : "", v & KV4_NO_ROWS ? " more rows than the plan holds;" : "",
                 v & KV4_NO_BLOCKS ? " out of blocks;" : "", v & KV4_BAD_VALUE ? " NaN or a value beyond 60000 stored;" : "",
-                v & KV4_BAD_BLOCK ? " no block for a position;" : "");
+                v & KV4_BAD_BLOCK ? " no block for a position;" : "", v & KV4_TIMEOUT ? " a wait inside a kernel ran out;" : "");
 }
 
 extern "C" int64_t vuib_kv4_launch_count(VuibKv4* c) { return c ? c->launches : 0; }

@@ -29,7 +29,8 @@ constexpr float KV4_LIMIT = 60000.f;      // larger magnitudes are stored as thi
 constexpr int KV4_MAX_SEQS = 4096;
 
 // bits of the device flag
-constexpr int KV4_BAD_SLOT = 1, KV4_BAD_LEN = 2, KV4_NO_ROWS = 4, KV4_NO_BLOCKS = 8, KV4_BAD_VALUE = 16, KV4_BAD_BLOCK = 32;
+constexpr int KV4_BAD_SLOT = 1, KV4_BAD_LEN = 2, KV4_NO_ROWS = 4, KV4_NO_BLOCKS = 8, KV4_BAD_VALUE = 16, KV4_BAD_BLOCK = 32, KV4_TIMEOUT = 64;
+constexpr unsigned KV4_POLLS = 1u << 22;  // bound of every wait
 
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
