@@ -272,26 +272,43 @@ class Filled:
         return plan
 
     def want(self, q, new, scale=None):
-        """Softmax attention in 64 bits, and the same of the values' magnitudes."""
-        outs, mags, a = [], [], 0
+        """Softmax attention in 64 bits, the same of the values' magnitudes, and what fixed-point queries and weights may add to an error.
+
+        Queries enter as whole numbers of 2^-13 of the power of two below their largest element: exact (8 digits) but for elements below
+        2^-6 of it, each half a unit off at most.  Weights times value scales enter in units of 2^-16 of the largest scale R, half a unit off at
+        most, against codes up to 15.  Both kinds of errors are independent of one another: six standard deviations (a unit's over the
+        square root of 12)."""
+        outs, mags, more, a = [], [], [], 0
+        scale = self.dim ** -0.5 if scale is None else scale
         for i, m in enumerate(new):
             n = self.k[i].shape[0]
             k, v = (x[i].repeat_interleave(self.heads // self.kv, 1) for x in (self.k, self.v))
-            s = torch.einsum("rhd,nhd->hrn", q[a:a + m].double(), k) * (self.dim ** -0.5 if scale is None else scale)
+            x = q[a:a + m].double()
+            s = torch.einsum("rhd,nhd->hrn", x, k) * scale
             late = torch.arange(n, device="cuda")[None, :] > torch.arange(n - m, n, device="cuda")[:, None]
             p = s.masked_fill(late, float("-inf")).softmax(-1)
             outs.append(torch.einsum("hrn,nhd->rhd", p, v))
             mags.append(torch.einsum("hrn,nhd->rhd", p, v.abs()))
+            if m and n:
+                unit = torch.exp2(x.abs().amax(-1).clamp(min=1e-300).log2().floor())                # (rows, heads)
+                small = (x.abs() < unit[..., None] / 64).double()
+                score = torch.einsum("rhd,nhd->rhn", small, k * k).amax(-1).sqrt() * unit * scale * 2.0 ** -13 / 12 ** 0.5 * 6
+                span = (v.unflatten(-1, (-1, 32)).amax(-1) - v.unflatten(-1, (-1, 32)).amin(-1)).amax() / 15 * 1.001
+                sums = n ** 0.5 * span * 15 * 2.0 ** -16 / 12 ** 0.5 * 6 * p.amax(-1).T               # the largest weight is 1 of the sum
+                more.append(2 * score[..., None] * mags[-1] + sums[..., None])
+            else:
+                more.append(torch.zeros_like(mags[-1]))
             a += m
-        return torch.cat(outs), torch.cat(mags)
+        return torch.cat(outs), torch.cat(mags), torch.cat(more)
 
 
 def close(out, want):
-    # one rounding to bf16 (2^-8 of the value); the weights' rounding to f16 (2^-11 each) and what fp32 scores below 64 in magnitude are off
-    # (128 products and sums of 2^-24 each: 2^-24 * 128 * 64 = 2^-11 in the exponent), both of the magnitudes that are added up
-    ref, mag = want
+    # one rounding to bf16 (2^-8 of the value); the weights' rounding to f16, where they are (2^-11 each), and what fp32 scores below 64 in
+    # magnitude are off (128 products and sums of 2^-24 each: 2^-24 * 128 * 64 = 2^-11 in the exponent), both of the magnitudes that are added
+    # up; what fixed-point operands add
+    ref, mag, more = want
     err = (out.double() - ref).abs()
-    assert (err <= 2.0 ** -8 * ref.abs() + 2.0 ** -10 * mag + 1e-30).all(), (err / mag).max()
+    assert (err <= 2.0 ** -8 * ref.abs() + 2.0 ** -10 * mag + more + 1e-30).all(), (err / mag).max()
 
 
 EDGES = [1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 127, 129, 192, 255, 256, 257, 320, 511, 512, 513, 777, 1024]
@@ -361,8 +378,8 @@ def test_peaked_scores():
     f = Filled([500, 40, 1500], 16, 8, 64, 64, key_scale=30.0)
     plan = f.add([1, 1, 1])
     q = torch.randn(3, 16, 64, device="cuda", generator=f.g).bfloat16()
-    ref, mag = f.want(q, [1, 1, 1])
-    close(f.cache.attention(0, q, plan), (ref, 2 * mag))
+    ref, mag, more = f.want(q, [1, 1, 1])
+    close(f.cache.attention(0, q, plan), (ref, 2 * mag, more))
 
 
 def test_a_row_of_nan_stays_its_own():

@@ -19,7 +19,7 @@ def _handle(**kw):
 
 
 def _plan(**kw):
-    base = dict(n_seqs=2, n_rows=3, max_new=2, entries=4096, cu_rows=4096, cu_units=4096, row_slot=4096, row_pos=4096, slot_map=4096)
+    base = dict(n_seqs=2, n_rows=3, max_new=2, work=4096, cu_rows=4096, row_slot=4096, row_pos=4096, slot_map=4096)
     base.update(kw)
     return C.byref(_lib.VuibKv4Plan(**base))
 
@@ -63,8 +63,8 @@ def test_null_and_unbound():
     assert lib.vuib_kv4_bind(h, p, 100, p, p, p, p, p) == -6
     buf = C.create_string_buffer(256)
     assert lib.vuib_kv4_last_error(h, buf, 256) == 0 and b"needed" in buf.value
-    for bad, status in ((dict(entries=None), -1), (dict(slot_map=None), -1), (dict(n_seqs=0), -3), (dict(n_seqs=5000), -3),
-                        (dict(n_rows=-1), -3), (dict(max_new=4), -3), (dict(max_new=-1), -3), (dict(entries=4100), -6)):
+    for bad, status in ((dict(work=None), -1), (dict(slot_map=None), -1), (dict(n_seqs=0), -3), (dict(n_seqs=5000), -3),
+                        (dict(n_rows=-1), -3), (dict(max_new=4), -3), (dict(max_new=-1), -3), (dict(work=4100), -6)):
         assert lib.vuib_kv4_plan(h, _plan(**bad), p, p, None, None) == status
     assert lib.vuib_kv4_plan(h, None, p, p, None, None) == -1
     assert lib.vuib_kv4_launch_count(h) == 0

@@ -147,7 +147,7 @@ class VuibKv4Config(C.Structure):
 
 class VuibKv4Plan(C.Structure):
     _fields_ = [("n_seqs", C.c_int32), ("n_rows", C.c_int32), ("max_new", C.c_int32),
-                ("entries", C.c_void_p), ("cu_rows", C.c_void_p), ("cu_units", C.c_void_p),
+                ("work", C.c_void_p), ("cu_rows", C.c_void_p),
                 ("row_slot", C.c_void_p), ("row_pos", C.c_void_p), ("slot_map", C.c_void_p)]
 
 

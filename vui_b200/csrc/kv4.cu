@@ -19,6 +19,7 @@ struct VuibKv4 {
     size_t layer_bytes;
     bool bound;
     int block_shift, ng, sms, device;
+    int resident[5];          // CTAs of each attention form that fit an SM of the device, 0: not asked for yet
     int64_t launches;
     char err[256];
 };
@@ -42,6 +43,7 @@ int32_t fail(VuibKv4* c, int32_t code, const char* fmt, ...) {
             return fail(c, VUIB_ERR_CUDA, "%s failed: %s", #call, cudaGetErrorString(_err));  \
     } while (0)
 
+// cluster 0: without an early launch
 template <class... KArgs, class... Args>
 cudaError_t launch(VuibKv4* c, void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, int cluster, void* stream, Args... args) {
     cudaLaunchConfig_t cfg = {};
@@ -56,7 +58,7 @@ cudaError_t launch(VuibKv4* c, void (*kern)(KArgs...), dim3 grid, dim3 block, si
     attr[1].val.clusterDim.x = cluster;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    cfg.numAttrs = cluster > 1 ? 2 : cluster;
     c->launches++;
     return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
 }
@@ -65,15 +67,17 @@ long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
 // What a plan's shape decides for attention: columns of a tile (rows x query heads of a kv head) and positions of a split.
 // Single tokens: splits of 256 positions, four warps at 64 each, whatever the batch, so that a row's bits depend on its own keys alone.
-struct Shape { int nt, cols, split; };
+// Up to 16 columns the form for a few (4, 8 or 16 columns a tile), else the one for many.
+struct Shape { bool few; int nt, cols, split; };
 Shape shape_of(const VuibKv4* c, const VuibKv4Plan* p) {
     Shape s;
     const int group = c->cfg.n_heads / c->cfg.n_kv_heads;
     const long long most = (long long)p->max_new * group;       // columns of one sequence
-    s.nt = most <= 8 ? 1 : most <= 16 || c->ng > 2 ? 2 : 4;
-    s.cols = 8 * s.nt;
+    s.few = most <= 16;
+    s.nt = s.few ? (most <= 4 ? 1 : most <= 8 ? 2 : 4) : c->ng > 2 ? 2 : 4;
+    s.cols = (s.few ? 4 : 8) * s.nt;
     s.split = 256;
-    if (most > 16) {
+    if (!s.few) {
         const long long tiles = ceil_div((long long)p->n_rows * group, s.cols) + p->n_seqs;
         const long long len = (long long)c->cfg.max_blocks << c->block_shift;
         s.split = 512;
@@ -94,13 +98,19 @@ long long most_units(const VuibKv4* c, const VuibKv4Plan* p, const Shape& s) {
 
 size_t acc_bytes(const VuibKv4* c, long long items, int cols) { return ((size_t)items * cols * c->cfg.head_dim * 4 + 255) & ~size_t(255); }
 
+// The parts of a plan's work array.
+int4* plan_entries(const VuibKv4Plan* p) { return reinterpret_cast<int4*>(p->work); }
+int32_t* plan_units(const VuibKv4Plan* p) { return p->work + 4 * (size_t)p->n_seqs; }
+int32_t* plan_tiles(const VuibKv4Plan* p) { return p->work + 5 * (size_t)p->n_seqs + 1; }
+int32_t* plan_row_entry(const VuibKv4Plan* p) { return p->work + 6 * (size_t)p->n_seqs + 2; }
+
 int32_t check_plan(VuibKv4* c, const VuibKv4Plan* p) {
-    if (!p || !p->entries || !p->cu_rows || !p->cu_units) return fail(c, VUIB_ERR_NULL, "a plan needs its arrays");
+    if (!p || !p->work || !p->cu_rows) return fail(c, VUIB_ERR_NULL, "a plan needs its arrays");
     if (p->n_rows > 0 && (!p->row_slot || !p->row_pos || !p->slot_map)) return fail(c, VUIB_ERR_NULL, "a plan of rows needs its row arrays");
     if (p->n_seqs < 1 || p->n_seqs > KV4_MAX_SEQS) return fail(c, VUIB_ERR_RANGE, "n_seqs %d not in 1..%d", p->n_seqs, KV4_MAX_SEQS);
     if (p->n_rows < 0 || p->n_rows > 1 << 24) return fail(c, VUIB_ERR_RANGE, "n_rows %d not in 0..%d", p->n_rows, 1 << 24);
     if (p->max_new < 0 || p->max_new > p->n_rows) return fail(c, VUIB_ERR_RANGE, "max_new %d not in 0..n_rows", p->max_new);
-    if (reinterpret_cast<uintptr_t>(p->entries) & 15) return fail(c, VUIB_ERR_WORKSPACE, "entries must be 16-byte aligned");
+    if (reinterpret_cast<uintptr_t>(p->work) & 15) return fail(c, VUIB_ERR_WORKSPACE, "work must be 16-byte aligned");
     if (!c->bound) return fail(c, VUIB_ERR_UNBOUND, "vuib_kv4_bind has not been called");
     return VUIB_OK;
 }
@@ -114,19 +124,35 @@ int32_t check_rows(VuibKv4* c, const char* name, const void* p, int64_t stride, 
     return VUIB_OK;
 }
 
-template <int NG, int NT>
-cudaError_t launch_attn(VuibKv4* c, const Kv4AttnArgs& a, long long items, bool merge, void* stream) {
-    // as many CTAs as can be resident: their number is asked for once a kernel
-    static int resident = 0;
+template <int NG, int COLS>
+cudaError_t launch_attn(VuibKv4* c, void (*kern)(Kv4AttnArgs), int& resident, const Kv4AttnArgs& a, long long items, bool merge, void* stream) {
+    constexpr int smem = KaShared<NG, COLS>::TOTAL;
     cudaError_t e = cudaSuccess;
-    constexpr int smem = KaShared<NG, NT>::TOTAL;
-    e = cudaFuncSetAttribute(k_kv4_attn<NG, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess && !resident) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, k_kv4_attn<NG, NT>, KA_THREADS + 32, smem);
-    if (e != cudaSuccess) return e;
-    const long long grid = min(items, (long long)c->sms * (resident > 0 ? resident : 1));
-    e = launch(c, k_kv4_attn<NG, NT>, dim3((unsigned)grid), KA_THREADS + 32, smem, 1, stream, a);
+    if (!resident) {     // as many CTAs as fit the SMs: asked for, and attributes set, once a handle and form
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+        if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kern, KA_THREADS + 32, smem);
+        if (e != cudaSuccess) return e;
+        if (resident < 1) resident = 1;
+    }
+    e = launch(c, kern, dim3((unsigned)min(items, (long long)c->sms * resident)), KA_THREADS + 32, smem, 1, stream, a);
     if (e != cudaSuccess || !merge) return e;
-    return launch(c, k_kv4_merge<NG>, dim3((unsigned)ceil_div((long long)a.n_rows * c->cfg.n_heads, 8)), 256, 0, 1, stream, a, NT * 8);
+    const long long rows = (long long)a.n_rows * c->cfg.n_heads;
+    if (((long long)c->cfg.max_blocks << c->block_shift) <= 32ll * a.split)
+        return launch(c, k_kv4_merge<NG, 1>, dim3((unsigned)ceil_div(rows, 4)), 128, 0, 1, stream, a, COLS);
+    return launch(c, k_kv4_merge<NG, 8>, dim3((unsigned)rows), 256, 0, 1, stream, a, COLS);
+}
+
+template <int NG>
+cudaError_t launch_form(VuibKv4* c, const Shape& s, const Kv4AttnArgs& a, long long items, bool merge, void* stream) {
+    int* resident = c->resident;
+    if (s.few) {
+        if (s.nt == 1) return launch_attn<NG, 4>(c, k_kv4_attn_few<NG, 1>, resident[0], a, items, merge, stream);
+        if (s.nt == 2) return launch_attn<NG, 8>(c, k_kv4_attn_few<NG, 2>, resident[1], a, items, merge, stream);
+        return launch_attn<NG, 16>(c, k_kv4_attn_few<NG, 4>, resident[2], a, items, merge, stream);
+    }
+    if constexpr (NG == 2) return launch_attn<NG, 32>(c, k_kv4_attn<NG, 4>, resident[3], a, items, merge, stream);
+    else return launch_attn<NG, 16>(c, k_kv4_attn<NG, 2>, resident[4], a, items, merge, stream);
 }
 
 }  // namespace
@@ -180,6 +206,7 @@ extern "C" int32_t vuib_kv4_bind(VuibKv4* c, void* pool, size_t bytes, int32_t* 
     if (reinterpret_cast<uintptr_t>(pool) & 127) return fail(c, VUIB_ERR_WORKSPACE, "the pool must be 128-byte aligned");
     if (bytes < c->layer_bytes * c->cfg.n_layers)
         return fail(c, VUIB_ERR_WORKSPACE, "pool of %zu bytes, %zu needed", bytes, c->layer_bytes * c->cfg.n_layers);
+    memset(c->resident, 0, sizeof(c->resident));
     CK(cudaGetDevice(&c->device));
     CK(cudaDeviceGetAttribute(&c->sms, cudaDevAttrMultiProcessorCount, c->device));
     c->cache = {static_cast<unsigned char*>(pool), block_table, seq_lens, free_blocks, n_free, flag, c->cfg.n_kv_heads, c->block_shift,
@@ -209,12 +236,14 @@ extern "C" int32_t vuib_kv4_plan(VuibKv4* c, const VuibKv4Plan* p, const int32_t
     a.slots = slots_dev; a.new_lens = new_dev; a.at = at_dev;
     a.n = p->n_seqs; a.n_rows = p->n_rows; a.max_new = p->max_new;
     a.group = c->cfg.n_heads / c->cfg.n_kv_heads; a.cols = s.cols; a.split = s.split;
-    a.entries = reinterpret_cast<int4*>(p->entries); a.cu_rows = p->cu_rows; a.cu_units = p->cu_units;
+    a.entries = plan_entries(p); a.cu_units = plan_units(p); a.cu_tiles = plan_tiles(p); a.row_entry = plan_row_entry(p);
+    a.cu_rows = p->cu_rows;
     a.row_slot = p->row_slot; a.row_pos = p->row_pos; a.slot_map = reinterpret_cast<long long*>(p->slot_map);
     const size_t smem = (8 * (size_t)p->n_seqs + 3 + c->cfg.max_seqs) * 4;
     if (smem > 48 * 1024) CK(cudaFuncSetAttribute(k_kv4_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     const int cluster = p->n_rows > 4096 ? 8 : 1;
-    CK(launch(c, k_kv4_plan, dim3(cluster), 1024, smem, cluster, stream, a));
+    const int threads = p->n_seqs <= 256 && p->n_rows <= 1024 ? 256 : 1024;
+    CK(launch(c, k_kv4_plan, dim3(cluster), threads, smem, cluster, stream, a));
     return VUIB_OK;
 }
 
@@ -232,11 +261,13 @@ extern "C" int32_t vuib_kv4_append(VuibKv4* c, int32_t layer, const VuibKv4Plan*
     a.c.pool += c->layer_bytes * layer;
     a.k = static_cast<const __nv_bfloat16*>(k_dev); a.k_stride = k_stride;
     a.v = static_cast<const __nv_bfloat16*>(v_dev); a.v_stride = v_stride;
-    a.slot_map = reinterpret_cast<const long long*>(p->slot_map);
+    a.entries = plan_entries(p); a.cu_tiles = plan_tiles(p); a.n = p->n_seqs;
     a.n_rows = p->n_rows;
-    const dim3 grid((unsigned)ceil_div((long long)p->n_rows * width / 8, 256), 2);
-    CK(c->ng == 2 ? launch(c, k_kv4_append<2>, grid, 256, 0, 1, stream, a)
-                  : c->ng == 3 ? launch(c, k_kv4_append<3>, grid, 256, 0, 1, stream, a) : launch(c, k_kv4_append<4>, grid, 256, 0, 1, stream, a));
+    // a sequence's m rows touch (m + 30) / 16 tiles at most, and no more than m
+    const long long tiles = min((long long)p->n_rows, p->n_rows / 16 + 2ll * p->n_seqs);
+    const dim3 grid((unsigned)ceil_div(tiles * c->cfg.n_kv_heads, 4));
+    CK(c->ng == 2 ? launch(c, k_kv4_append<2>, grid, 128, 0, 1, stream, a)
+                  : c->ng == 3 ? launch(c, k_kv4_append<3>, grid, 128, 0, 1, stream, a) : launch(c, k_kv4_append<4>, grid, 128, 0, 1, stream, a));
     return VUIB_OK;
 }
 
@@ -258,9 +289,9 @@ extern "C" int32_t vuib_kv4_read(VuibKv4* c, int32_t layer, int32_t n_rows, cons
     a.v_out = static_cast<__nv_bfloat16*>(v_out_dev); a.v_stride = v_stride;
     a.row_slot = row_slot_dev; a.row_pos = row_pos_dev;
     a.n_rows = n_rows;
-    const dim3 grid((unsigned)ceil_div((long long)n_rows * width / 8, 256), 2);
-    CK(c->ng == 2 ? launch(c, k_kv4_read<2>, grid, 256, 0, 1, stream, a)
-                  : c->ng == 3 ? launch(c, k_kv4_read<3>, grid, 256, 0, 1, stream, a) : launch(c, k_kv4_read<4>, grid, 256, 0, 1, stream, a));
+    const dim3 grid((unsigned)ceil_div(n_rows, 256 / (c->ng * 4)), c->cfg.n_kv_heads, 2);
+    CK(c->ng == 2 ? launch(c, k_kv4_read<2>, grid, 256, 0, 0, stream, a)
+                  : c->ng == 3 ? launch(c, k_kv4_read<3>, grid, 256, 0, 0, stream, a) : launch(c, k_kv4_read<4>, grid, 256, 0, 0, stream, a));
     return VUIB_OK;
 }
 
@@ -295,7 +326,7 @@ extern "C" int32_t vuib_kv4_attention(VuibKv4* c, int32_t layer, const VuibKv4Pl
     Kv4AttnArgs a = {};
     a.c = c->cache;
     a.c.pool += c->layer_bytes * layer;
-    a.entries = reinterpret_cast<const int4*>(p->entries); a.cu_rows = p->cu_rows; a.cu_units = p->cu_units;
+    a.entries = plan_entries(p); a.cu_units = plan_units(p); a.row_entry = plan_row_entry(p);
     a.n = p->n_seqs; a.n_rows = p->n_rows; a.group = c->cfg.n_heads / c->cfg.n_kv_heads; a.split = s.split;
     a.q = static_cast<const __nv_bfloat16*>(q_dev); a.q_stride = q_stride;
     a.out = static_cast<__nv_bfloat16*>(out_dev); a.out_stride = out_stride;
@@ -303,15 +334,8 @@ extern "C" int32_t vuib_kv4_attention(VuibKv4* c, int32_t layer, const VuibKv4Pl
     a.acc = static_cast<float*>(ws_dev);
     a.ml = reinterpret_cast<float2*>(static_cast<char*>(ws_dev) + acc_bytes(c, items, s.cols));
     const bool merge = need != 0;
-    switch (c->ng * 8 + s.nt) {
-        case 17: CK((launch_attn<2, 1>(c, a, items, merge, stream))); break;
-        case 18: CK((launch_attn<2, 2>(c, a, items, merge, stream))); break;
-        case 20: CK((launch_attn<2, 4>(c, a, items, merge, stream))); break;
-        case 25: CK((launch_attn<3, 1>(c, a, items, merge, stream))); break;
-        case 26: CK((launch_attn<3, 2>(c, a, items, merge, stream))); break;
-        case 33: CK((launch_attn<4, 1>(c, a, items, merge, stream))); break;
-        default: CK((launch_attn<4, 2>(c, a, items, merge, stream))); break;
-    }
+    CK(c->ng == 2 ? launch_form<2>(c, s, a, items, merge, stream)
+                  : c->ng == 3 ? launch_form<3>(c, s, a, items, merge, stream) : launch_form<4>(c, s, a, items, merge, stream));
     return VUIB_OK;
 }
 

@@ -9,7 +9,7 @@ constexpr int KA_THREADS = 128, KA_WARPS = 4;
 
 struct Kv4AttnArgs {
     Kv4Cache c;
-    const int4* entries; const int32_t* cu_rows; const int32_t* cu_units;
+    const int4* entries; const int32_t* cu_units; const int32_t* row_entry;
     int n, n_rows, group, split;
     const __nv_bfloat16* q; long long q_stride;
     __nv_bfloat16* out; long long out_stride;
@@ -44,21 +44,22 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
 
 // The eight codes of a word as four pairs of the values that they stand for.  A nibble under the exponent of 1024 is 1024 + c, one
 // that sits four bits higher 1024 + 16 c: both are exact in f16, and so is what is left when 1024 is taken off again.
-__device__ __forceinline__ void kv4_values(uint32_t w, uint32_t s, uint32_t z, uint32_t (&r)[4]) {
+__device__ __forceinline__ __half2 as_h2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
+// s0, z0: scale and zero of the first two pairs, s1, z1 of the others.
+__device__ __forceinline__ void kv4_values(uint32_t w, __half2 s0, __half2 z0, __half2 s1, __half2 z1, uint32_t (&r)[4]) {
     const uint32_t v = w >> 8;
     uint32_t x[4];
     asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(x[0]) : "r"(w));
     asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(x[1]) : "r"(w));
     asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(x[2]) : "r"(v));
     asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(x[3]) : "r"(v));
-    const __half2 hs = *reinterpret_cast<const __half2*>(&s), hz = *reinterpret_cast<const __half2*>(&z);
     const __half2 low = __half2half2(__ushort_as_half(0xE400)), sixteenth = __half2half2(__ushort_as_half(0x2C00)),
                   less = __half2half2(__ushort_as_half(0xD400));   // -1024, 1 / 16, -64
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const __half2 h = *reinterpret_cast<const __half2*>(&x[j]);
         const __half2 code = j & 1 ? __hfma2(h, sixteenth, less) : __hadd2(h, low);
-        const __half2 value = __hfma2(hs, code, hz);
+        const __half2 value = j < 2 ? __hfma2(s0, code, z0) : __hfma2(s1, code, z1);
         r[j] = *reinterpret_cast<const uint32_t*>(&value);
     }
 }
@@ -166,115 +167,170 @@ __device__ __noinline__ void give_up(int32_t* flag) {
     for (int i = 0; i < 100; ++i) __nanosleep(100000);
 }
 
-// Shared memory of the mma.sync form, in bytes.
-template <int NG, int NT>
+#ifndef KV4_STAGES
+#define KV4_STAGES 2
+#endif
+// Shared memory of the mma.sync forms, in bytes.
+template <int NG, int COLS>
 struct KaShared {
     static constexpr int KT = NG == 2 ? 4 : 2;                                  // tiles of 16 positions a warp takes at once
     static constexpr int KEYS = KA_WARPS * KT * KV4_TILE;                         // positions of a stage
     static constexpr int TILE = NG * KV4_GT, QCOL = NG * KV4_GROUP * 2;
-    static constexpr int KV = KA_WARPS * KT * TILE, Q = NT * 8 * QCOL;
+    static constexpr int KV = KA_WARPS * KT * TILE, Q = COLS * QCOL;
     static constexpr int STAGE = KV + Q + (int)sizeof(Kv4Item);
-    static constexpr int STAGES = 3;
-    static constexpr int ACC = KA_WARPS * NT * 8 * (NG * KV4_GROUP + 4) * 4, ML = KA_WARPS * NT * 8 * 8;
+    static constexpr int STAGES = KV4_STAGES;
+    static constexpr int ACC = KA_WARPS * COLS * (NG * KV4_GROUP + 4) * 4, ML = KA_WARPS * COLS * 8;
     static constexpr int TOTAL = STAGES * STAGE + ACC + ML + 8 * (2 * STAGES + 2);
 };
 
-// mma.sync form: a producer warp walks the CTA's units and brings keys, values and queries into a ring of stages (bulk copies), four
-// consumer warps take KT tiles of 16 positions each.  Keys are the A operand, queries the B operand (8 columns), so that one or a few
-// query heads waste nothing but columns; the scores' transpose for the second product is one movmatrix a fragment.  Softmax statistics
-// and sums are fp32; the weights enter the second product as f16 (2^-11 of each, where bf16's 2^-8 would be as much as the output's own
-// rounding).
+// A CTA's shared memory and barriers: full and empty of every stage, and of the place where the consumer warps' states meet.
+template <int NG, int COLS>
+struct KaRing {
+    using S = KaShared<NG, COLS>;
+    unsigned char* smem;
+    float* acc;          // [warp][column][HD + 4]
+    float2* ml;          // [warp][column]
+    uint32_t bars;
+    __device__ __forceinline__ explicit KaRing(unsigned char* p)
+        : smem(p), acc(reinterpret_cast<float*>(p + S::STAGES * S::STAGE)), ml(reinterpret_cast<float2*>(p + S::STAGES * S::STAGE + S::ACC)),
+          bars(smem_addr(p + S::STAGES * S::STAGE + S::ACC + S::ML)) {}
+    __device__ __forceinline__ uint32_t full(int s) const { return bars + 8 * s; }
+    __device__ __forceinline__ uint32_t empty(int s) const { return bars + 8 * (S::STAGES + s); }
+    __device__ __forceinline__ uint32_t acc_full() const { return bars + 16 * S::STAGES; }
+    __device__ __forceinline__ uint32_t acc_empty() const { return bars + 16 * S::STAGES + 8; }
+    __device__ __forceinline__ void init() const {
+        if (threadIdx.x == 0) {
+            for (int s = 0; s < S::STAGES; ++s) { bar_init(full(s), 1); bar_init(empty(s), KA_WARPS); }
+            bar_init(acc_full(), KA_WARPS);
+            bar_init(acc_empty(), KA_WARPS);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        __syncthreads();
+    }
+};
+
+// The producer warp: walks the CTA's units and brings keys, values and queries into the ring (bulk copies), a stage at a time.
+template <int NG, int COLS>
+__device__ __forceinline__ void ka_produce(const Kv4AttnArgs& a, const KaRing<NG, COLS>& ring, int lane) {
+    using S = KaShared<NG, COLS>;
+    constexpr int HD = NG * KV4_GROUP, KT = S::KT, D = S::STAGES;
+    const int tiles = 1 << (a.c.block_shift - 4);     // of a block
+    const long long total = (long long)__ldcg(a.cu_units + a.n) * a.c.n_kv;
+    long long w = total * blockIdx.x / gridDim.x;
+    const long long last = total * (blockIdx.x + 1) / gridDim.x;
+    Kv4Walk u = {};
+    int id = 0;     // the lane's tile's block
+    auto block_of = [&]() {
+        const int pos = u.base + lane * KV4_TILE;
+        return lane < KA_WARPS * KT && pos < u.hi ? __ldcg(a.c.table + (size_t)u.e.x * a.c.max_blocks + (pos >> a.c.block_shift)) : 0;
+    };
+    bool queries = true, begins = true;
+    if (w < last) {
+        u = walk_at<COLS>(a, w, lane);
+        id = block_of();
+    }
+    const int run = min(tiles, KA_WARPS * KT);    // tiles that lie behind one another
+    for (unsigned k = 0;; ++k) {
+        const int s = k % D;
+        if (k >= D && !bar_wait(ring.empty(s), (k / D - 1) & 1)) { give_up(a.c.flag); return; }
+        unsigned char* const stage = ring.smem + s * S::STAGE;
+        Kv4Item* const item = reinterpret_cast<Kv4Item*>(stage + S::KV + S::Q);
+        if (w >= last) {
+            if (lane == 0) {
+                item->flags = KI_END;
+                bar_arrive(ring.full(s));
+            }
+            return;
+        }
+        if ((unsigned)id >= (unsigned)a.c.n_blocks) {
+            atomicOr(a.c.flag, KV4_BAD_BLOCK);
+            id = 0;
+        }
+        const bool ends = u.base + S::KEYS >= u.hi;
+        const int valid = max(min((u.hi - u.base + KV4_TILE - 1) / KV4_TILE, KA_WARPS * KT), 0);   // none: a tile that does not see this split
+        const int cols = min(u.e.z * a.group - u.ctile * COLS, COLS);
+        if (lane == 0) {
+            Kv4Item d;
+            d.flags = (begins ? KI_FIRST : 0) | (ends ? KI_LAST : 0) | (queries ? KI_QUERIES : 0);
+            d.start = u.e.y; d.rows = u.e.z; d.row0 = u.e.w;
+            d.ctile = u.ctile; d.head = u.head; d.splits = u.splits; d.base = u.base;
+            d.hi = u.hi; d.pad = 0; d.w = w;
+            *item = d;
+            bar_expect(ring.full(s), valid * S::TILE + (queries ? cols * S::QCOL : 0));
+        }
+        __syncwarp();
+        const int pos = u.base + lane * KV4_TILE;
+        if (lane < valid && lane % run == 0) {
+            const unsigned char* src = a.c.pool + ((size_t)((long long)id * a.c.n_kv + u.head) * tiles + ((pos & ((1 << a.c.block_shift) - 1)) >> 4)) * S::TILE;
+            bulk_copy(smem_addr(stage + lane * S::TILE), src, min(run, valid - lane) * S::TILE, ring.full(s));
+        }
+        if (queries && lane < cols) {     // the heads of a row lie behind one another
+            const int c = u.ctile * COLS + lane, row = c / a.group, in = c % a.group;
+            if (lane == 0 || in == 0)
+                bulk_copy(smem_addr(stage + S::KV + lane * S::QCOL), a.q + (long long)(u.e.w + row) * a.q_stride + (u.head * a.group + in) * HD,
+                          min(a.group - in, cols - lane) * S::QCOL, ring.full(s));
+        }
+        queries = false;
+        begins = ends;
+        u.base += S::KEYS;
+        if (ends) {
+            if (++w < last) {
+                walk_next<COLS>(a, u);
+                queries = u.split == 0;
+            }
+        }
+        if (w < last) id = block_of();
+    }
+}
+
+// The end of a unit: the four consumer warps' states, which lie in the ring's place for them, added in the order of the warps; written out,
+// or kept as the split's part.
+template <int NG, int COLS>
+__device__ __forceinline__ void ka_finish(const Kv4AttnArgs& a, const KaRing<NG, COLS>& ring, const Kv4Item& d, int cols) {
+    constexpr int HD = NG * KV4_GROUP;
+    for (int i = threadIdx.x; i < min(cols, COLS) * (HD / 4); i += KA_THREADS) {
+        const int col = i / (HD / 4), dim = i % (HD / 4) * 4;
+        float best = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int k2 = 0; k2 < KA_WARPS; ++k2) best = fmaxf(best, ring.ml[k2 * COLS + col].x);
+        const float now = best == -INFINITY ? 0.f : best;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k2 = 0; k2 < KA_WARPS; ++k2) {
+            const float2 part = ring.ml[k2 * COLS + col];
+            const float f = ex2(part.x - now);
+            const float4 v = *reinterpret_cast<const float4*>(ring.acc + (k2 * COLS + col) * (HD + 4) + dim);
+            sum += f * part.y;
+            o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
+        }
+        if (d.splits == 1) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            const int c = d.ctile * COLS + col;
+            __nv_bfloat162 lo2 = __floats2bfloat162_rn(o.x * inv, o.y * inv), hi2 = __floats2bfloat162_rn(o.z * inv, o.w * inv);
+            uint2 v = make_uint2(*reinterpret_cast<uint32_t*>(&lo2), *reinterpret_cast<uint32_t*>(&hi2));
+            *reinterpret_cast<uint2*>(a.out + (long long)(d.row0 + c / a.group) * a.out_stride + (d.head * a.group + c % a.group) * HD + dim) = v;
+        } else {
+            *reinterpret_cast<float4*>(a.acc + (size_t)(d.w * COLS + col) * HD + dim) = o;
+            if (dim == 0) a.ml[d.w * COLS + col] = make_float2(best, sum);
+        }
+    }
+}
+
+// Form for tiles of more columns than a few: keys as the A operand, queries as the B operand (8 columns), values as f16; the scores'
+// transpose for the second product is one movmatrix a fragment.  Softmax statistics and sums are fp32; the weights enter the second
+// product as f16 (2^-11 of each, where bf16's 2^-8 would be as much as the output's own rounding).
 template <int NG, int NT>
 __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn(const Kv4AttnArgs a) {
-    using S = KaShared<NG, NT>;
-    constexpr int HD = NG * KV4_GROUP, COLS = NT * 8, KT = S::KT, D = S::STAGES;
+    constexpr int HD = NG * KV4_GROUP, COLS = NT * 8;
+    using S = KaShared<NG, COLS>;
+    constexpr int KT = S::KT, D = S::STAGES;
     extern __shared__ __align__(128) unsigned char smem[];
-    float* const sm_acc = reinterpret_cast<float*>(smem + D * S::STAGE);                 // [warp][column][HD + 4]
-    float2* const sm_ml = reinterpret_cast<float2*>(smem + D * S::STAGE + S::ACC);       // [warp][column]
-    const uint32_t bars = smem_addr(smem + D * S::STAGE + S::ACC + S::ML);
-    auto full = [&](int s) { return bars + 8 * s; };
-    auto empty = [&](int s) { return bars + 8 * (D + s); };
-    const uint32_t acc_full = bars + 16 * D, acc_empty = acc_full + 8;
+    const KaRing<NG, COLS> ring(smem);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < D; ++s) { bar_init(full(s), 1); bar_init(empty(s), KA_WARPS); }
-        bar_init(acc_full, KA_WARPS);
-        bar_init(acc_empty, KA_WARPS);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    __syncthreads();
-    const int tiles = 1 << (a.c.block_shift - 4);     // of a block
+    ring.init();
     pdl_wait();
     pdl_launch();
-
-    if (warp == KA_WARPS) {
-        const long long total = (long long)__ldcg(a.cu_units + a.n) * a.c.n_kv;
-        long long w = total * blockIdx.x / gridDim.x;
-        const long long last = total * (blockIdx.x + 1) / gridDim.x;
-        Kv4Walk u = {};
-        int id = 0;     // the lane's tile's block
-        auto block_of = [&]() {
-            const int pos = u.base + lane * KV4_TILE;
-            return lane < KA_WARPS * KT && pos < u.hi ? __ldcg(a.c.table + (size_t)u.e.x * a.c.max_blocks + (pos >> a.c.block_shift)) : 0;
-        };
-        bool queries = true, begins = true;
-        if (w < last) {
-            u = walk_at<COLS>(a, w, lane);
-            id = block_of();
-        }
-        const int run = min(tiles, KA_WARPS * KT);    // tiles that lie behind one another
-        for (unsigned k = 0;; ++k) {
-            const int s = k % D;
-            if (k >= D && !bar_wait(empty(s), (k / D - 1) & 1)) { give_up(a.c.flag); return; }
-            unsigned char* const stage = smem + s * S::STAGE;
-            Kv4Item* const item = reinterpret_cast<Kv4Item*>(stage + S::KV + S::Q);
-            if (w >= last) {
-                if (lane == 0) {
-                    item->flags = KI_END;
-                    bar_arrive(full(s));
-                }
-                return;
-            }
-            if ((unsigned)id >= (unsigned)a.c.n_blocks) {
-                atomicOr(a.c.flag, KV4_BAD_BLOCK);
-                id = 0;
-            }
-            const bool ends = u.base + S::KEYS >= u.hi;
-            const int valid = max(min((u.hi - u.base + KV4_TILE - 1) / KV4_TILE, KA_WARPS * KT), 0);   // none: a tile that does not see this split
-            const int cols = min(u.e.z * a.group - u.ctile * COLS, COLS);
-            if (lane == 0) {
-                Kv4Item d;
-                d.flags = (begins ? KI_FIRST : 0) | (ends ? KI_LAST : 0) | (queries ? KI_QUERIES : 0);
-                d.start = u.e.y; d.rows = u.e.z; d.row0 = u.e.w;
-                d.ctile = u.ctile; d.head = u.head; d.splits = u.splits; d.base = u.base;
-                d.hi = u.hi; d.pad = 0; d.w = w;
-                *item = d;
-                bar_expect(full(s), valid * S::TILE + (queries ? cols * S::QCOL : 0));
-            }
-            __syncwarp();
-            const int pos = u.base + lane * KV4_TILE;
-            if (lane < valid && lane % run == 0) {
-                const unsigned char* src = a.c.pool + ((size_t)((long long)id * a.c.n_kv + u.head) * tiles + ((pos & ((1 << a.c.block_shift) - 1)) >> 4)) * S::TILE;
-                bulk_copy(smem_addr(stage + lane * S::TILE), src, min(run, valid - lane) * S::TILE, full(s));
-            }
-            if (queries && lane < cols) {     // the heads of a row lie behind one another
-                const int c = u.ctile * COLS + lane, row = c / a.group, in = c % a.group;
-                if (lane == 0 || in == 0)
-                    bulk_copy(smem_addr(stage + S::KV + lane * S::QCOL), a.q + (long long)(u.e.w + row) * a.q_stride + (u.head * a.group + in) * HD,
-                              min(a.group - in, cols - lane) * S::QCOL, full(s));
-            }
-            queries = false;
-            begins = ends;
-            u.base += S::KEYS;
-            if (ends) {
-                if (++w < last) {
-                    walk_next<COLS>(a, u);
-                    queries = u.split == 0;
-                }
-            }
-            if (w < last) id = block_of();
-        }
-    }
+    if (warp == KA_WARPS) return ka_produce<NG, COLS>(a, ring, lane);
 
     uint32_t qf[NT][NG][4];
     float factor[NT][2];
@@ -283,8 +339,8 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn(const Kv4AttnArgs 
     unsigned merged = 0;
     for (unsigned k = 0;; ++k) {
         const int s = k % D;
-        if (!bar_wait(full(s), (k / D) & 1)) { give_up(a.c.flag); return; }
-        const unsigned char* const stage = smem + s * S::STAGE;
+        if (!bar_wait(ring.full(s), (k / D) & 1)) { give_up(a.c.flag); return; }
+        const unsigned char* const stage = ring.smem + s * S::STAGE;
         const Kv4Item d = *reinterpret_cast<const Kv4Item*>(stage + S::KV + S::Q);
         if (d.flags & KI_END) return;
         const int cols = d.rows * a.group - d.ctile * COLS;                 // valid ones of this tile, if fewer than COLS
@@ -314,7 +370,7 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn(const Kv4AttnArgs 
                     for (int j = 0; j < 4; ++j)
                         qf[nt][i][j] = pack_h2(__uint_as_float(x[j] << 16) * down, __uint_as_float(x[j] & 0xffff0000u) * down);
                 }
-                const float f = a.scale_log2 * up;
+                const float f = fmaxf(a.scale_log2 * up, 1e-37f);      // not 0, which would make NaN of masked scores
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const int c2 = nt * 8 + 2 * t + j;
@@ -349,8 +405,8 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn(const Kv4AttnArgs 
                         const uint2 code = *reinterpret_cast<const uint2*>(p + lane * 8);
                         const uint2 par = *reinterpret_cast<const uint2*>(p + KV4_KPAR + g * 8);
                         uint32_t x[4], y[4];
-                        kv4_values(code.x, __byte_perm(par.x, 0, 0x1010), __byte_perm(par.x, 0, 0x3232), x);
-                        kv4_values(code.y, __byte_perm(par.y, 0, 0x1010), __byte_perm(par.y, 0, 0x3232), y);
+                        kv4_values(code.x, __low2half2(as_h2(par.x)), __high2half2(as_h2(par.x)), __low2half2(as_h2(par.x)), __high2half2(as_h2(par.x)), x);
+                        kv4_values(code.y, __low2half2(as_h2(par.y)), __high2half2(as_h2(par.y)), __low2half2(as_h2(par.y)), __high2half2(as_h2(par.y)), y);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
                             mma16816(sc[k2][nt], x[0], y[0], x[1], y[1], qf[nt][i][0], qf[nt][i][1]);
@@ -359,26 +415,37 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn(const Kv4AttnArgs 
                     }
                 }
             }
-            uint32_t p[KT][NT][2];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                float top[2] = {-INFINITY, -INFINITY};
+            if (!whole) {
 #pragma unroll
                 for (int k2 = 0; k2 < KT; ++k2) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        sc[k2][nt][j] *= factor[nt][j & 1];
-                        if (!whole && base + k2 * 16 + g + (j >> 1) * 8 > limit[nt][j & 1]) sc[k2][nt][j] = -INFINITY;
-                        top[j & 1] = fmaxf(top[j & 1], sc[k2][nt][j]);
+                    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (base + k2 * 16 + g + (j >> 1) * 8 > limit[nt][j & 1]) sc[k2][nt][j] = -INFINITY;
                     }
+                }
+            }
+            uint32_t p[KT][NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float top[2] = {sc[0][nt][0], sc[0][nt][1]};
+#pragma unroll
+                for (int k2 = 0; k2 < KT; ++k2) {
+                    top[0] = fmaxf(fmaxf(top[0], sc[k2][nt][0]), sc[k2][nt][2]);
+                    top[1] = fmaxf(fmaxf(top[1], sc[k2][nt][1]), sc[k2][nt][3]);
                 }
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) {
                     top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], o));
                     top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], o));
                 }
-                float now[2];
-                if (__any_sync(0xffffffffu, top[0] > m[nt][0] || top[1] > m[nt][1])) {
+                top[0] *= factor[nt][0];
+                top[1] *= factor[nt][1];
+                if (d.flags & KI_FIRST) {
+                    m[nt][0] = top[0];
+                    m[nt][1] = top[1];
+                } else if (__any_sync(0xffffffffu, top[0] > m[nt][0] || top[1] > m[nt][1])) {
                     float old[2];
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
@@ -393,14 +460,14 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn(const Kv4AttnArgs 
                         acc[nt][i][2] *= old[0]; acc[nt][i][3] *= old[1];
                     }
                 }
-#pragma unroll
-                for (int j = 0; j < 2; ++j) now[j] = m[nt][j] == -INFINITY ? 0.f : m[nt][j];    // nothing seen yet: weights of exp(-inf) = 0
+                // minus the maximum, as the addend of a fused multiply; nothing seen yet: weights of exp(-inf) = 0
+                const float less[2] = {m[nt][0] == -INFINITY ? 0.f : -m[nt][0], m[nt][1] == -INFINITY ? 0.f : -m[nt][1]};
 #pragma unroll
                 for (int k2 = 0; k2 < KT; ++k2) {
                     float e[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        e[j] = ex2(sc[k2][nt][j] - now[j & 1]);
+                        e[j] = ex2(fmaf(sc[k2][nt][j], factor[nt][j & 1], less[j & 1]));
                         l[nt][j & 1] += e[j];
                     }
                     p[k2][nt][0] = movmatrix(pack_h2(e[0], e[1]));
@@ -414,24 +481,26 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn(const Kv4AttnArgs 
                     for (int i = 0; i < NG; ++i) {
                         const unsigned char* q = mine + k2 * S::TILE + i * KV4_GT;
                         const uint2 code = *reinterpret_cast<const uint2*>(q + KV4_VCODE + lane * 8);
-                        const uint4 par = *reinterpret_cast<const uint4*>(q + KV4_VPAR + t * 16);
+                        const uint4 par = *reinterpret_cast<const uint4*>(q + KV4_VPAR + t * 16);   // of keys 2t, 2t+8, 2t+1, 2t+9
+                        const __half2 s0 = as_h2(__byte_perm(par.x, par.z, 0x5410)), z0 = as_h2(__byte_perm(par.x, par.z, 0x7632));
+                        const __half2 s8 = as_h2(__byte_perm(par.y, par.w, 0x5410)), z8 = as_h2(__byte_perm(par.y, par.w, 0x7632));
                         uint32_t x[4], y[4];
-                        kv4_values(code.x, par.x, par.y, x);
-                        kv4_values(code.y, par.z, par.w, y);
+                        kv4_values(code.x, s0, z0, s8, z8, x);
+                        kv4_values(code.y, s0, z0, s8, z8, y);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            mma16816(acc[nt][2 * i], x[0], x[1], y[0], y[1], p[k2][nt][0], p[k2][nt][1]);
-                            mma16816(acc[nt][2 * i + 1], x[2], x[3], y[2], y[3], p[k2][nt][0], p[k2][nt][1]);
+                            mma16816(acc[nt][2 * i], x[0], x[1], x[2], x[3], p[k2][nt][0], p[k2][nt][1]);
+                            mma16816(acc[nt][2 * i + 1], y[0], y[1], y[2], y[3], p[k2][nt][0], p[k2][nt][1]);
                         }
                     }
                 }
             }
         }
         __syncwarp();
-        if (lane == 0) bar_arrive(empty(s));
+        if (lane == 0) bar_arrive(ring.empty(s));
         if (!(d.flags & KI_LAST)) continue;
         // the warps' states, added in the order of the warps
-        if (merged && !bar_wait(acc_empty, (merged - 1) & 1)) { give_up(a.c.flag); return; }
+        if (merged && !bar_wait(ring.acc_empty(), (merged - 1) & 1)) { give_up(a.c.flag); return; }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -443,91 +512,396 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn(const Kv4AttnArgs 
             for (int j = 0; j < 2; ++j) {
                 const int col = nt * 8 + 2 * t + j;
                 if (col < cols) {
-                    if (g == 0) sm_ml[warp * COLS + col] = make_float2(m[nt][j], l[nt][j]);
+                    if (g == 0) ring.ml[warp * COLS + col] = make_float2(m[nt][j], l[nt][j]);
 #pragma unroll
                     for (int i = 0; i < NG; ++i)
-                        *reinterpret_cast<float4*>(sm_acc + (warp * COLS + col) * (HD + 4) + i * KV4_GROUP + 4 * g) =
+                        *reinterpret_cast<float4*>(ring.acc + (warp * COLS + col) * (HD + 4) + i * KV4_GROUP + 4 * g) =
                             make_float4(acc[nt][2 * i][j], acc[nt][2 * i][2 + j], acc[nt][2 * i + 1][j], acc[nt][2 * i + 1][2 + j]);
                 }
             }
         }
         __syncwarp();
-        if (lane == 0) bar_arrive(acc_full);
-        if (!bar_wait(acc_full, merged & 1)) { give_up(a.c.flag); return; }
-        for (int i = threadIdx.x; i < min(cols, COLS) * (HD / 4); i += KA_THREADS) {
-            const int col = i / (HD / 4), dim = i % (HD / 4) * 4;
-            float best = -INFINITY, sum = 0.f;
-#pragma unroll
-            for (int k2 = 0; k2 < KA_WARPS; ++k2) best = fmaxf(best, sm_ml[k2 * COLS + col].x);
-            const float now = best == -INFINITY ? 0.f : best;
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int k2 = 0; k2 < KA_WARPS; ++k2) {
-                const float2 part = sm_ml[k2 * COLS + col];
-                const float f = ex2(part.x - now);
-                const float4 v = *reinterpret_cast<const float4*>(sm_acc + (k2 * COLS + col) * (HD + 4) + dim);
-                sum += f * part.y;
-                o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
-            }
-            if (d.splits == 1) {
-                const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                const int c = d.ctile * COLS + col;
-                __nv_bfloat162 lo2 = __floats2bfloat162_rn(o.x * inv, o.y * inv), hi2 = __floats2bfloat162_rn(o.z * inv, o.w * inv);
-                uint2 v = make_uint2(*reinterpret_cast<uint32_t*>(&lo2), *reinterpret_cast<uint32_t*>(&hi2));
-                *reinterpret_cast<uint2*>(a.out + (long long)(d.row0 + c / a.group) * a.out_stride + (d.head * a.group + c % a.group) * HD + dim) = v;
-            } else {
-                *reinterpret_cast<float4*>(a.acc + (size_t)(d.w * COLS + col) * HD + dim) = o;
-                if (dim == 0) a.ml[d.w * COLS + col] = make_float2(best, sum);
-            }
-        }
+        if (lane == 0) bar_arrive(ring.acc_full());
+        if (!bar_wait(ring.acc_full(), merged & 1)) { give_up(a.c.flag); return; }
+        ka_finish<NG, COLS>(a, ring, d, cols);
         __syncwarp();
-        if (lane == 0) bar_arrive(acc_empty);
+        if (lane == 0) bar_arrive(ring.acc_empty());
         ++merged;
     }
 }
 
-// Adds up the splits of every row that has more than one, in the order of the positions: a warp a (row, query head).
-template <int NG>
-__global__ void __launch_bounds__(256) k_kv4_merge(const Kv4AttnArgs a, const int cols) {
-    constexpr int HD = NG * KV4_GROUP;
-    const int lane = threadIdx.x & 31, heads = a.c.n_kv * a.group;
-    const long long id = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+// m16n8k32, bytes in, 32-bit sums out: D += A B, the codes A always unsigned.
+template <bool SIGNED>
+__device__ __forceinline__ void mma16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (SIGNED)
+        asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Sums that start as the bits of 1.5 * 2^23 are that float plus the sum (below 2^22 in magnitude), bit for bit.
+constexpr int KA_ORIGIN = 0x4B400000;
+__device__ __forceinline__ float from_origin(int x) { return __int_as_float(x) - 12582912.f; }
+
+// Form for a few columns (single tokens): what bounds it is the arithmetic a stored byte costs, not the tensor cores, so the codes enter
+// the products as they are, as bytes: three logic operations for eight codes, where their f16 values take thirteen instructions, half of
+// them at half rate.
+//   scores:  q . K = sum over groups of scale * (q . code) + zero * (sum of the group's q)
+//   outputs: sum_i w_i V_i = sum_i (w_i scale_i) code_i + sum_i w_i zero_i
+// A query column, times a power of two, is a 15-bit whole number: exact for elements down to 2^-6 of the largest, the others to 2^-14 of
+// it.  The weights times the value scales are 16-bit whole numbers in units of 2^-16 of the largest value scale among the warp's positions
+// (half a unit off, each on its own, a quarter of what bf16 weights would be off at one position and less the more there are).  Both are
+// cut into two bytes that take two of the 8 columns of a product, so a product holds four queries.  The tensor cores' sums are exact;
+// what is added to them, statistics and outputs, is fp32.
+// Measured (B200, 256 sequences of 512 to 2048 positions, 16 query and 8 key heads of 64): see the table of forms in kv4.cu.
+template <int NG, int NT>
+__global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn_few(const Kv4AttnArgs a) {
+    constexpr int HD = NG * KV4_GROUP, COLS = NT * 4;
+    using S = KaShared<NG, COLS>;
+    constexpr int KT = S::KT, D = S::STAGES;
+    extern __shared__ __align__(128) unsigned char smem[];
+    const KaRing<NG, COLS> ring(smem);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    ring.init();
+    pdl_wait();
+    pdl_launch();
+    if (warp == KA_WARPS) return ka_produce<NG, COLS>(a, ring, lane);
+
+    const uint32_t pick = g & 1 ? 0x6240 : 0x7351;      // low or high bytes of four 16-bit weights, in the order of a word's keys
+    uint32_t qf[NT][NG][2];         // bytes of column g: query g / 2, high byte (even g) or low byte
+    float qsum[NT][NG], factor[NT]; // of query t, as all below
+    int limit[NT];                  // last position that it sees
+    float acc[NT][2 * NG][2], zsum[NT][NG], m[NT], l[NT];
+    unsigned merged = 0;
+    for (unsigned k = 0;; ++k) {
+        const int s = k % D;
+        if (!bar_wait(ring.full(s), (k / D) & 1)) { give_up(a.c.flag); return; }
+        const unsigned char* const stage = ring.smem + s * S::STAGE;
+        const Kv4Item d = *reinterpret_cast<const Kv4Item*>(stage + S::KV + S::Q);
+        if (d.flags & KI_END) return;
+        const int cols = d.rows * a.group - d.ctile * COLS;                 // valid ones of this tile, if fewer than COLS
+        if (d.flags & KI_QUERIES) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const int col = nt * 4 + (g >> 1);
+                uint4 raw[NG];
+                uint32_t big = 0;
+#pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    raw[i] = make_uint4(0, 0, 0, 0);
+                    if (col < cols) raw[i] = *reinterpret_cast<const uint4*>(stage + S::KV + col * S::QCOL + i * 64 + t * 16);
+                    big = max(big, most_bits(raw[i]));
+                }
+                big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+                big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+                // times a power of two, so that the largest element lies in [2^13, 2^14)
+                const int e = min(max((int)(big >> 7), 1), 253);
+                const float down = __int_as_float((254 - e) << 23), up = __int_as_float(e << 23);
+                float total[NG];
+#pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    const uint32_t x[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                    int v[8], part = 0;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        v[j] = __float2int_rn(__uint_as_float(j & 1 ? x[j >> 1] & 0xffff0000u : x[j >> 1] << 16) * down * 8192.f);
+                        part += v[j];
+                        const int low = (int)(signed char)(v[j] & 255);
+                        v[j] = g & 1 ? low & 255 : (v[j] - low) >> 8 & 255;
+                    }
+                    qf[nt][i][0] = v[0] | v[4] << 8 | v[1] << 16 | v[5] << 24;      // the order of a key word's low nibbles
+                    qf[nt][i][1] = v[2] | v[6] << 8 | v[3] << 16 | v[7] << 24;      // and of its high ones
+                    part += __shfl_xor_sync(0xffffffffu, part, 1);
+                    part += __shfl_xor_sync(0xffffffffu, part, 2);
+                    total[i] = (float)part;
+                }
+                // a masked score times the factor has to stay -inf, and a query that is not finite makes all its weights NaN
+                const float f = big >= 0x7f80u ? __int_as_float(0x7fffffff) : fmaxf(a.scale_log2 * up * (1.f / 8192.f), 1e-37f);
+                factor[nt] = __shfl_sync(0xffffffffu, f, t * 8);
+#pragma unroll
+                for (int i = 0; i < NG; ++i) qsum[nt][i] = __shfl_sync(0xffffffffu, total[i], t * 8);
+                const int mine = nt * 4 + t;
+                limit[nt] = mine < cols ? d.start + (d.ctile * COLS + mine) / a.group : -1;
+            }
+        }
+        if (d.flags & KI_FIRST) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                m[nt] = -INFINITY;
+                l[nt] = factor[nt] * 0.f;
+#pragma unroll
+                for (int i = 0; i < NG; ++i) zsum[nt][i] = 0.f;
+#pragma unroll
+                for (int i = 0; i < 2 * NG; ++i) acc[nt][i][0] = acc[nt][i][1] = 0.f;
+            }
+        }
+        const int base = d.base + warp * (KT * KV4_TILE);
+        const int nk = min(KT, (d.hi - base + KV4_TILE - 1) / KV4_TILE);    // tiles that are there
+        if (nk > 0) {
+            const unsigned char* const mine = stage + warp * (KT * S::TILE);
+            const bool whole = base + KT * KV4_TILE - 1 <= d.start + d.ctile * COLS / a.group;   // every column sees all of them
+            float sc[KT][NT][2];      // scores of keys g and g + 8 of every tile, then weights
+#pragma unroll
+            for (int k2 = 0; k2 < KT; ++k2) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) sc[k2][nt][0] = sc[k2][nt][1] = 0.f;
+                if (k2 < nk) {
+#pragma unroll
+                    for (int i = 0; i < NG; ++i) {
+                        const unsigned char* p = mine + k2 * S::TILE + i * KV4_GT;
+                        const uint2 code = *reinterpret_cast<const uint2*>(p + lane * 8);
+                        const uint2 par = *reinterpret_cast<const uint2*>(p + KV4_KPAR + g * 8);
+                        const float2 p0 = __half22float2(as_h2(par.x)), p1 = __half22float2(as_h2(par.y));     // scale, zero
+                        const uint32_t a0 = code.x & 0x0f0f0f0fu, a1 = code.y & 0x0f0f0f0fu;
+                        const uint32_t a2 = code.x >> 4 & 0x0f0f0f0fu, a3 = code.y >> 4 & 0x0f0f0f0fu;
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            int x[4] = {KA_ORIGIN, KA_ORIGIN, KA_ORIGIN, KA_ORIGIN};
+                            mma16832<true>(x, a0, a1, a2, a3, qf[nt][i][0], qf[nt][i][1]);
+                            sc[k2][nt][0] = fmaf(p0.x, fmaf(from_origin(x[0]), 256.f, from_origin(x[1])), fmaf(p0.y, qsum[nt][i], sc[k2][nt][0]));
+                            sc[k2][nt][1] = fmaf(p1.x, fmaf(from_origin(x[2]), 256.f, from_origin(x[3])), fmaf(p1.y, qsum[nt][i], sc[k2][nt][1]));
+                        }
+                    }
+                }
+            }
+            if (!whole) {
+#pragma unroll
+                for (int k2 = 0; k2 < KT; ++k2) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        if (base + k2 * 16 + g > limit[nt]) sc[k2][nt][0] = -INFINITY;
+                        if (base + k2 * 16 + g + 8 > limit[nt]) sc[k2][nt][1] = -INFINITY;
+                    }
+                }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float top = sc[0][nt][0];
+#pragma unroll
+                for (int k2 = 0; k2 < KT; ++k2) top = fmaxf(fmaxf(top, sc[k2][nt][0]), sc[k2][nt][1]);
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                top *= factor[nt];
+                if (d.flags & KI_FIRST) {
+                    m[nt] = top;
+                } else if (__any_sync(0xffffffffu, top > m[nt])) {
+                    const float best = fmaxf(m[nt], top), old = best == -INFINITY ? 1.f : ex2(m[nt] - best);
+                    m[nt] = best;
+                    l[nt] *= old;
+#pragma unroll
+                    for (int i = 0; i < NG; ++i) zsum[nt][i] *= old;
+#pragma unroll
+                    for (int i = 0; i < 2 * NG; ++i) { acc[nt][i][0] *= old; acc[nt][i][1] *= old; }
+                }
+                const float less = m[nt] == -INFINITY ? 0.f : -m[nt];       // nothing seen yet: weights of exp(-inf) = 0
+#pragma unroll
+                for (int k2 = 0; k2 < KT; ++k2) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        sc[k2][nt][j] = ex2(fminf(fmaf(sc[k2][nt][j], factor[nt], less), 0.f));
+                        l[nt] += sc[k2][nt][j];
+                    }
+                }
+            }
+            // value scales, and the largest of each group
+            float vs[KT][NG][2], unit[NG];
+#pragma unroll
+            for (int i = 0; i < NG; ++i) unit[i] = 0.f;
+#pragma unroll
+            for (int k2 = 0; k2 < KT; ++k2) {
+#pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    vs[k2][i][0] = vs[k2][i][1] = 0.f;
+                    if (k2 < nk) {
+                        const uint2 par = *reinterpret_cast<const uint2*>(mine + k2 * S::TILE + i * KV4_GT + KV4_VPAR + g * 8);
+                        const float2 p0 = __half22float2(as_h2(par.x)), p1 = __half22float2(as_h2(par.y));
+                        vs[k2][i][0] = p0.x;
+                        vs[k2][i][1] = p1.x;
+                        unit[i] = fmaxf(fmaxf(unit[i], p0.x), p1.x);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) zsum[nt][i] = fmaf(sc[k2][nt][0], p0.y, fmaf(sc[k2][nt][1], p1.y, zsum[nt][i]));
+                    }
+                }
+            }
+            float units[NG];
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                unit[i] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(unit[i])));
+                units[i] = unit[i] > 0.f ? __fdividef(65280.f, unit[i]) : 0.f;
+                unit[i] *= 1.f / 65280.f;
+            }
+#pragma unroll
+            for (int k2 = 0; k2 < KT; ++k2) {
+#pragma unroll
+                for (int i = 0; i < NG; ++i) { vs[k2][i][0] *= units[i]; vs[k2][i][1] *= units[i]; }
+            }
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                int x[NT][2][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[nt][0][j] = x[nt][1][j] = KA_ORIGIN;
+                }
+#pragma unroll
+                for (int k2 = 0; k2 < KT; k2 += 2) {
+                    if (k2 < nk) {       // of a second tile that is not there the weights are 0
+                        const uint2 first = *reinterpret_cast<const uint2*>(mine + k2 * S::TILE + i * KV4_GT + KV4_VCODE + lane * 8);
+                        const uint2 second = *reinterpret_cast<const uint2*>(mine + (k2 + 1) * S::TILE + i * KV4_GT + KV4_VCODE + lane * 8);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            uint32_t b[2];
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                // the nearest whole number in the low 16 bits, twice over, for the columns of both bytes
+                                const uint32_t w0 = __float_as_uint(fmaf(sc[k2 + j][nt][0], vs[k2 + j][i][0], 8388608.f));
+                                const uint32_t w8 = __float_as_uint(fmaf(sc[k2 + j][nt][1], vs[k2 + j][i][1], 8388608.f));
+                                b[j] = __byte_perm(movmatrix(__byte_perm(w0, 0, 0x1010)), movmatrix(__byte_perm(w8, 0, 0x1010)), pick);
+                            }
+                            mma16832<false>(x[nt][0], first.x & 0x0f0f0f0fu, first.x >> 4 & 0x0f0f0f0fu, second.x & 0x0f0f0f0fu, second.x >> 4 & 0x0f0f0f0fu, b[0], b[1]);
+                            mma16832<false>(x[nt][1], first.y & 0x0f0f0f0fu, first.y >> 4 & 0x0f0f0f0fu, second.y & 0x0f0f0f0fu, second.y >> 4 & 0x0f0f0f0fu, b[0], b[1]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        acc[nt][2 * i + j][0] = fmaf(unit[i], fmaf(from_origin(x[nt][j][0]), 256.f, from_origin(x[nt][j][1])), acc[nt][2 * i + j][0]);
+                        acc[nt][2 * i + j][1] = fmaf(unit[i], fmaf(from_origin(x[nt][j][2]), 256.f, from_origin(x[nt][j][3])), acc[nt][2 * i + j][1]);
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        if (lane == 0) bar_arrive(ring.empty(s));
+        if (!(d.flags & KI_LAST)) continue;
+        if (merged && !bar_wait(ring.acc_empty(), (merged - 1) & 1)) { give_up(a.c.flag); return; }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int col = nt * 4 + t;
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+                l[nt] += __shfl_xor_sync(0xffffffffu, l[nt], o);
+#pragma unroll
+                for (int i = 0; i < NG; ++i) zsum[nt][i] += __shfl_xor_sync(0xffffffffu, zsum[nt][i], o);
+            }
+            if (col < cols) {
+                if (g == 0) ring.ml[warp * COLS + col] = make_float2(m[nt], l[nt]);
+#pragma unroll
+                for (int i = 0; i < NG; ++i)
+                    *reinterpret_cast<float4*>(ring.acc + (warp * COLS + col) * (HD + 4) + i * KV4_GROUP + 4 * g) =
+                        make_float4(acc[nt][2 * i][0] + zsum[nt][i], acc[nt][2 * i][1] + zsum[nt][i], acc[nt][2 * i + 1][0] + zsum[nt][i], acc[nt][2 * i + 1][1] + zsum[nt][i]);
+            }
+        }
+        __syncwarp();
+        if (lane == 0) bar_arrive(ring.acc_full());
+        if (!bar_wait(ring.acc_full(), merged & 1)) { give_up(a.c.flag); return; }
+        ka_finish<NG, COLS>(a, ring, d, cols);
+        __syncwarp();
+        if (lane == 0) bar_arrive(ring.acc_empty());
+        ++merged;
+    }
+}
+
+// Adds up the splits of every row that has more than one: a CTA a (row, query head), WARPS warps.  Split i belongs to class i % 32; a class
+// adds its splits in order, and the classes are added in order, so that a row's bits do not depend on WARPS, which goes by the
+// cache's size: with up to 32 splits one warp, as each class then has one member at most.
+template <int NG, int WARPS>
+__global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) k_kv4_merge(const Kv4AttnArgs a, const int cols) {
+    constexpr int HD = NG * KV4_GROUP, CLASSES = 32 / WARPS;
+    __shared__ float part_acc[WARPS == 1 ? 1 : 32][HD];
+    __shared__ float part_sum[WARPS == 1 ? 1 : 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, heads = a.c.n_kv * a.group;
+    const long long id = WARPS == 1 ? (long long)blockIdx.x * 4 + warp : blockIdx.x;
     pdl_wait();
     pdl_launch();
     const int row = (int)(id / heads), head = (int)(id % heads), kv = head / a.group;
-    if (row >= a.n_rows || row >= __ldcg(a.cu_rows + a.n)) return;
-    int lo = 0, hi = a.n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (__ldcg(a.cu_rows + mid) <= row) lo = mid; else hi = mid;
-    }
-    const int4 e = __ldcg(a.entries + lo);
+    if (row >= a.n_rows) return;
+    const int entry = __ldcg(a.row_entry + row);
+    if (entry < 0) return;
+    const int4 e = __ldcg(a.entries + entry);
+    const long long unit = __ldcg(a.cu_units + entry);
     const int all = (e.y + e.z + a.split - 1) / a.split;
     if (all == 1) return;
     const int own = (e.y + row - e.w) / a.split + 1;        // splits that the row sees
     const int c = (row - e.w) * a.group + head % a.group;
-    const long long w = (long long)__ldcg(a.cu_units + lo) * a.c.n_kv + ((long long)(c / cols) * a.c.n_kv + kv) * all;
+    const long long w = unit * a.c.n_kv + ((long long)(c / cols) * a.c.n_kv + kv) * all;
     const float2* ml = a.ml + w * cols + c % cols;
     const float* acc = a.acc + (size_t)(w * cols + c % cols) * HD + lane * NG;
-    float best = -INFINITY;
-    for (int i = lane; i < own; i += 32) best = fmaxf(best, __ldcg(&ml[(size_t)i * cols].x));
-#pragma unroll
-    for (int o = 16; o; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
-    const float now = best == -INFINITY ? 0.f : best;
-    float sum = 0.f, out[NG];
+    const size_t step = (size_t)cols * HD;
+    __nv_bfloat16* dst = a.out + (long long)row * a.out_stride + head * HD;
+    float best = -INFINITY, sum = 0.f, out[NG];
 #pragma unroll
     for (int j = 0; j < NG; ++j) out[j] = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < own; ++i) {
-        const float2 part = __ldcg(ml + (size_t)i * cols);
-        const float f = ex2(part.x - now);
-        sum += f * part.y;
+    if constexpr (WARPS == 1) {
+        const float2 mine = lane < own ? __ldcg(ml + (size_t)lane * cols) : make_float2(-INFINITY, 0.f);
+        best = mine.x;
 #pragma unroll
-        for (int j = 0; j < NG; ++j) out[j] += f * __ldcg(acc + (size_t)i * cols * HD + j);
+        for (int o = 16; o; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+        const float f = ex2(mine.x - (best == -INFINITY ? 0.f : best)), l = f * mine.y;
+        for (int i = 0; i < own; i += 8) {
+            float v[8][NG];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+#pragma unroll
+                for (int j = 0; j < NG; ++j) v[k][j] = i + k < own ? __ldcg(acc + (i + k) * step + j) : 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float fk = __shfl_sync(0xffffffffu, f, i + k);
+                sum = __fadd_rn(sum, __shfl_sync(0xffffffffu, l, i + k));
+#pragma unroll
+                for (int j = 0; j < NG; ++j) out[j] = __fadd_rn(out[j], __fmul_rn(fk, v[k][j]));
+            }
+        }
+    } else {
+        for (int i = lane; i < own; i += 32) best = fmaxf(best, __ldcg(&ml[(size_t)i * cols].x));
+#pragma unroll
+        for (int o = 16; o; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+        const float now = best == -INFINITY ? 0.f : best;
+        float s[CLASSES], o[CLASSES][NG];
+#pragma unroll
+        for (int k = 0; k < CLASSES; ++k) {
+            s[k] = 0.f;
+#pragma unroll
+            for (int j = 0; j < NG; ++j) o[k][j] = 0.f;
+        }
+        for (int i = warp * CLASSES; i < own; i += 32) {
+            float2 p[CLASSES];
+            float v[CLASSES][NG];
+#pragma unroll
+            for (int k = 0; k < CLASSES; ++k) {
+                p[k] = i + k < own ? __ldcg(ml + (size_t)(i + k) * cols) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+                for (int j = 0; j < NG; ++j) v[k][j] = i + k < own ? __ldcg(acc + (i + k) * step + j) : 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < CLASSES; ++k) {
+                const float f = ex2(p[k].x - now);
+                s[k] = __fadd_rn(s[k], f * p[k].y);
+#pragma unroll
+                for (int j = 0; j < NG; ++j) o[k][j] = __fadd_rn(o[k][j], __fmul_rn(f, v[k][j]));
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < CLASSES; ++k) {
+            if (lane == 0) part_sum[warp * CLASSES + k] = s[k];
+#pragma unroll
+            for (int j = 0; j < NG; ++j) part_acc[warp * CLASSES + k][lane * NG + j] = o[k][j];
+        }
+        __syncthreads();
+        if (warp) return;
+        for (int k = 0; k < 32; ++k) {
+            sum = __fadd_rn(sum, part_sum[k]);
+#pragma unroll
+            for (int j = 0; j < NG; ++j) out[j] = __fadd_rn(out[j], part_acc[k][lane * NG + j]);
+        }
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-    for (int j = 0; j < NG; ++j) a.out[(long long)row * a.out_stride + head * HD + lane * NG + j] = __float2bfloat16_rn(out[j] * inv);
+    for (int j = 0; j < NG; ++j) dst[lane * NG + j] = __float2bfloat16_rn(out[j] * inv);
 }
 
 }  // namespace vuik

@@ -4,15 +4,16 @@
 //   zero = f16(min x), scale = f16((max x - zero) * fl(1/15)), code = rint((x - zero) / scale) in 0 .. 15,
 // and a code stands for f16(scale * code + zero).
 //
-// Layout of a layer's pool: [block][kv head][16 positions][32 elements] -> 640 bytes, laid out as the m16n8k16 fragments that the
-// attention feeds to the tensor cores (lane = 4 g + t):
+// Layout of a layer's pool: [block][kv head][16 positions][32 elements] -> 640 bytes, laid out as the fragments that the attention
+// feeds to the tensor cores (lane = 4 g + t of a warp; keys 0 .. 15 are the positions of a tile):
 //   [  0, 256)  key codes: lane's 8 bytes = word of key g, word of key g + 8; nibble j of a word's low half is element 8 t + 2 j,
 //               of its high half element 8 t + 2 j + 1
 //   [256, 320)  key scale and zero: (scale, zero) of key g, of key g + 8, g = 0 .. 7
-//   [320, 576)  value codes: lane's 8 bytes = keys 2t, 2t+1, 2t+8, 2t+9, 16 bits each; nibble j of a key's half is element 4 g + j
-//   [576, 640)  value scales and zeros of those keys, for t = 0 .. 3: s(2t) s(2t+1) z(2t) z(2t+1) s(2t+8) s(2t+9) z(2t+8) z(2t+9)
-// So a tile is read with one 8-byte load a lane and operand, without a shuffle, and a position owns whole 32-bit (keys) and 16-bit
-// (values) pieces: storing one position never reads or rewrites another's.
+//   [320, 576)  value codes: lane's 8 bytes = two words, each a byte of the keys 2t, 2t+8, 2t+1, 2t+9; a byte of the first word holds
+//               elements 4 g (low nibble) and 4 g + 1, of the second 4 g + 2 and 4 g + 3
+//   [576, 640)  value scale and zero, as the keys'
+// So a tile is read with one 8-byte load a lane and operand, without a shuffle, and a position owns whole words (keys) and bytes
+// (values): storing one position never reads or rewrites another's.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -35,7 +36,7 @@ constexpr unsigned KV4_POLLS = 1u << 22;  // bound of every wait
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-struct Kv4Entry { int32_t slot, start, rows, row0; };   // as int4 in memory
+// A plan's entry, as int4: slot (-1: takes no part), first new position, rows, first row.
 
 struct Kv4Cache {
     unsigned char* pool;        // of the layer
@@ -53,7 +54,8 @@ struct Kv4PlanArgs {
     const int32_t* slots; const int32_t* new_lens; const int32_t* at;
     int n, n_rows, max_new;
     int group, cols, split;     // query heads a kv head, columns of a tile, positions of a split: attention's units are counted here
-    int4* entries; int32_t* cu_rows; int32_t* cu_units; int32_t* row_slot; int32_t* row_pos; long long* slot_map;
+    int4* entries; int32_t* cu_units; int32_t* cu_tiles; int32_t* row_entry;    // the plan's work array
+    int32_t* cu_rows; int32_t* row_slot; int32_t* row_pos; long long* slot_map;
 };
 
 __device__ __forceinline__ unsigned cluster_rank() { unsigned r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
@@ -65,27 +67,43 @@ __device__ __forceinline__ void plan_sync(unsigned size) {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// Exclusive prefix sum over the block of one number a thread; the total comes back too.
-__device__ __forceinline__ long long block_scan(long long v, long long* warp_sums, long long& total) {
+// Exclusive prefix sums over the block of N non-negative numbers a thread, side by side; v becomes the sum before the thread, total the
+// whole.  Sums stop at KV4_MANY, which no size that can be served reaches.
+constexpr int KV4_MANY = 1 << 30;
+template <int N>
+__device__ __forceinline__ void block_scan(int (&v)[N], int (*warp_sums)[32], int (&total)[N]) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-    long long x = v;
+    int x[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = v[j];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-    }
-    __syncthreads();
-    if (lane == 31) warp_sums[warp] = x;
-    __syncthreads();
-    long long s = lane < nw ? warp_sums[lane] : 0, p = s;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, p, o);
-        if (lane >= o) p += y;
+        for (int j = 0; j < N; ++j) {
+            const int y = __shfl_up_sync(0xffffffffu, x[j], o);
+            if (lane >= o) x[j] = min(x[j] + y, KV4_MANY);
+        }
     }
-    total = __shfl_sync(0xffffffffu, p, 31);
-    const long long before = __shfl_sync(0xffffffffu, p - s, warp);
-    return before + x - v;
+    if (lane == 31) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) warp_sums[j][warp] = x[j];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const int s = lane < nw ? warp_sums[j][lane] : 0;
+        int p = s;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, p, o);
+            if (lane >= o) p = min(p + y, KV4_MANY);
+        }
+        total[j] = __shfl_sync(0xffffffffu, p, 31);
+        const int excl = __shfl_up_sync(0xffffffffu, p, 1);
+        const int before = __shfl_sync(0xffffffffu, lane ? excl : 0, warp);
+        const int in = __shfl_up_sync(0xffffffffu, x[j], 1);
+        v[j] = min(before + (lane ? in : 0), KV4_MANY);
+    }
 }
 
 // The last i with first[i] <= x, for a non-decreasing first[0 .. n] with first[0] = 0 and x < first[n].
@@ -102,7 +120,7 @@ __device__ __forceinline__ int find_in(const int* first, int n, int x) {
 // rows and blocks many.  Latency bound: three dependent reads (entry, length, table) and five barriers.
 __global__ void __launch_bounds__(1024) k_kv4_plan(const Kv4PlanArgs a) {
     extern __shared__ int sm[];
-    __shared__ long long warp_sums[32];
+    __shared__ int scan_a[1][32], scan_b[2][32], scan_c[4][32];
     const int n = a.n, per = (n + blockDim.x - 1) / blockDim.x;
     int* s_slot = sm;               // n each; slot -1: takes no part
     int* s_start = s_slot + n;
@@ -155,80 +173,72 @@ __global__ void __launch_bounds__(1024) k_kv4_plan(const Kv4PlanArgs a) {
     __syncthreads();
     // Who is served: the rows of the entries so far have to fit, and so have the blocks that they ask for (an entry that asks for none
     // is served all the same).
-    long long total, sum = 0;
-    for (int i = first; i < last; ++i) sum += s_new[i];
-    long long run = block_scan(sum, warp_sums, total);
-    long long grow = 0, drop = 0;
+    auto leave_out = [&](int i) { s_slot[i] = -1; s_new[i] = 0; s_need[i] = s_have[i]; };
+    int rows_to[1] = {0}, all[1];
+    for (int i = first; i < last; ++i) rows_to[0] = min(rows_to[0] + s_new[i], KV4_MANY);
+    block_scan<1>(rows_to, scan_a, all);
+    int blocks[2] = {0, 0}, sum[2];     // given back, asked for
     for (int i = first; i < last; ++i) {
-        run += s_new[i];
-        if (run > a.n_rows) {
+        rows_to[0] = min(rows_to[0] + s_new[i], KV4_MANY);
+        if (rows_to[0] > a.n_rows) {
             if (s_slot[i] >= 0) bad |= KV4_NO_ROWS;
-            s_slot[i] = -1;
-            s_new[i] = 0;
-            s_need[i] = s_have[i];
+            leave_out(i);
         }
-        grow += max(s_need[i] - s_have[i], 0);
-        drop += max(s_have[i] - s_need[i], 0);
+        blocks[0] += max(s_have[i] - s_need[i], 0);
+        blocks[1] = min(blocks[1] + max(s_need[i] - s_have[i], 0), KV4_MANY);
     }
-    long long dropped;
-    run = block_scan(drop, warp_sums, dropped);
+    block_scan<2>(blocks, scan_b, sum);
+    const int dropped = sum[0], top = n_free + dropped;
+    int part[4] = {0, 0, 0, 0}, whole[4];   // blocks got, rows, units of attention (of a kv head), tiles of 16 positions written
+    auto units_of = [&](int i) { return s_new[i] ? (int)min(((long long)s_new[i] * a.group + a.cols - 1) / a.cols * ((s_start[i] + (long long)s_new[i] + a.split - 1) / a.split), (long long)KV4_MANY) : 0; };
+    auto tiles_of = [&](int i) { return s_new[i] ? ((s_start[i] + s_new[i] - 1) >> 4) - (s_start[i] >> 4) + 1 : 0; };
     for (int i = first; i < last; ++i) {
-        s_drop[i] = (int)run;
-        run += max(s_have[i] - s_need[i], 0);
-    }
-    run = block_scan(grow, warp_sums, total);
-    grow = 0;
-    sum = 0;
-    for (int i = first; i < last; ++i) {
+        s_drop[i] = blocks[0];
+        blocks[0] += max(s_have[i] - s_need[i], 0);
         const int g = max(s_need[i] - s_have[i], 0);
-        run += g;
-        if (g > 0 && run > n_free + dropped) {
+        blocks[1] = min(blocks[1] + g, KV4_MANY);
+        if (g > 0 && blocks[1] > top) {
             bad |= KV4_NO_BLOCKS;
-            s_slot[i] = -1;
-            s_new[i] = 0;
-            s_need[i] = s_have[i];
+            leave_out(i);
         } else {
-            grow += g;
+            part[0] += g;
         }
-        sum += s_new[i];
+        part[1] += s_new[i];
+        part[2] = min(part[2] + units_of(i), KV4_MANY);
+        part[3] += tiles_of(i);
     }
-    long long grown, rows, units;
-    run = block_scan(grow, warp_sums, grown);
+    block_scan<4>(part, scan_c, whole);
+    const int grown = whole[0], rows = whole[1];
+    int units = part[2], tiles = part[3];
     for (int i = first; i < last; ++i) {
-        s_grow[i] = (int)run;
-        run += max(s_need[i] - s_have[i], 0);
+        s_grow[i] = part[0];
+        s_cu[i] = part[1];
+        part[0] += max(s_need[i] - s_have[i], 0);
+        part[1] += s_new[i];
     }
-    run = block_scan(sum, warp_sums, rows);
-    sum = 0;
-    for (int i = first; i < last; ++i) {
-        s_cu[i] = (int)run;
-        run += s_new[i];
-        const int end = s_start[i] + s_new[i];
-        if (s_new[i]) sum += (long long)((s_new[i] * (long long)a.group + a.cols - 1) / a.cols) * ((end + a.split - 1) / a.split);
-    }
-    run = block_scan(sum, warp_sums, units);
-    if (tid == 0) { s_cu[n] = (int)rows; s_grow[n] = (int)grown; s_drop[n] = (int)dropped; }
+    if (tid == 0) { s_cu[n] = rows; s_grow[n] = grown; s_drop[n] = dropped; }
     if (bad && rank == 0) atomicOr(a.c.flag, bad);
     plan_sync(size);                   // every CTA has read the lengths and the number of free blocks
     const int step = blockDim.x * size, me = rank * blockDim.x + tid;
     if (rank == 0) {
         if (tid == 0) {
-            *a.c.n_free = n_free + (int)(dropped - grown);
-            a.cu_rows[n] = (int)rows;
-            a.cu_units[n] = (int)units;
+            *a.c.n_free = top - grown;
+            a.cu_rows[n] = rows;
+            a.cu_units[n] = whole[2];
+            a.cu_tiles[n] = whole[3];
         }
         for (int i = first; i < last; ++i) {
-            a.cu_units[i] = (int)run;
-            const int end = s_start[i] + s_new[i];
-            if (s_new[i]) run += (long long)((s_new[i] * (long long)a.group + a.cols - 1) / a.cols) * ((end + a.split - 1) / a.split);
+            a.cu_units[i] = units;
+            a.cu_tiles[i] = tiles;
+            units = min(units + units_of(i), KV4_MANY);
+            tiles += tiles_of(i);
             a.cu_rows[i] = s_cu[i];
             a.entries[i] = make_int4(s_slot[i], s_start[i], s_new[i], s_cu[i]);
-            if (s_slot[i] >= 0) a.c.lens[s_slot[i]] = end;
+            if (s_slot[i] >= 0) a.c.lens[s_slot[i]] = s_start[i] + s_new[i];
         }
     }
     // Blocks given back go on the stack so that the first entry's first one is on top; those taken come off the top in entry order:
     // what was given back and is taken again in the same order gets its places again.
-    const int top = n_free + (int)dropped;
     for (int r = me; r < dropped; r += step) {
         const int i = find_in(s_drop, n, r);
         int32_t* at = a.c.table + (size_t)s_slot[i] * a.c.max_blocks + s_need[i] + (r - s_drop[i]);
@@ -242,16 +252,17 @@ __global__ void __launch_bounds__(1024) k_kv4_plan(const Kv4PlanArgs a) {
     }
     if (grown || dropped) plan_sync(size);
     for (int r = me; r < a.n_rows; r += step) {
-        int slot = -1, pos = -1;
+        int slot = -1, pos = -1, i = -1;
         long long where = -1;
         if (r < rows) {
-            const int i = find_in(s_cu, n, r);
+            i = find_in(s_cu, n, r);
             slot = s_slot[i];
             pos = s_start[i] + (r - s_cu[i]);
             const int b = __ldcg(a.c.table + (size_t)slot * a.c.max_blocks + (pos >> a.c.block_shift));
             if (b >= 0 && b < a.c.n_blocks) where = ((long long)b << a.c.block_shift) + (pos & (bs - 1));
             else atomicOr(a.c.flag, KV4_BAD_BLOCK);
         }
+        a.row_entry[r] = i;
         a.row_slot[r] = slot;
         a.row_pos[r] = pos;
         a.slot_map[r] = where;
@@ -283,97 +294,162 @@ struct Kv4RowsArgs {
     const __nv_bfloat16* k; const __nv_bfloat16* v;      // append: rows in
     __nv_bfloat16* k_out; __nv_bfloat16* v_out;          // read: rows out
     long long k_stride, v_stride;                        // elements between rows
-    const long long* slot_map;                           // append
+    const int4* entries; const int32_t* cu_tiles; int n; // append: the plan's entries, their first tiles
     const int32_t* row_slot; const int32_t* row_pos;     // read
     int n_rows;
 };
 
-// A thread quantises 8 elements of a row; the four threads of a group share its extremes.  blockIdx.y: keys or values.
+// The largest magnitude of 8 bf16 as bits (infinity and NaN are larger than any number).
+__device__ __forceinline__ uint32_t most_bits(const uint4& r) {
+    const uint32_t m = __vmaxu2(__vmaxu2(r.x & 0x7fff7fffu, r.y & 0x7fff7fffu), __vmaxu2(r.z & 0x7fff7fffu, r.w & 0x7fff7fffu));
+    return max(m & 0xffffu, m >> 16);
+}
+constexpr uint32_t KV4_LIMIT_BITS = 0x476a;   // 59904, the largest bf16 below KV4_LIMIT
+
+__device__ __noinline__ float tame(float x) { return x == x ? fminf(fmaxf(x, -KV4_LIMIT), KV4_LIMIT) : 0.f; }
+__device__ __noinline__ void codes_by_division(const float (&x)[8], float z, float s, uint32_t (&code)[8]) {
+    for (int j = 0; j < 8; ++j) code[j] = (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[j], z), s)), 0.f), 15.f);
+}
+
+// A warp stores one tile of 16 positions of one kv head, or those of its positions that are new: NG * 4 lanes a row, 8 elements a lane,
+// the four lanes of a group share its extremes; the codes are gathered in shared memory as they lie in the pool and leave it 16 bytes a
+// lane where the whole tile is new, else in the words and bytes of the new positions.
+// The nearest code: (x - zero) times the reciprocal of the scale is 2^-19 off at most (three roundings of a quotient below 16), so unless
+// that lies within 2^-17 of the middle between two codes it rounds as the quotient does; the few that do are divided.
 template <int NG>
-__global__ void __launch_bounds__(256) k_kv4_append(const Kv4RowsArgs a) {
-    constexpr int CH = NG * 4;   // threads of a vector
-    const bool value = blockIdx.y != 0;
-    const long long id = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    const int ch = (int)(id % CH);
-    const long long rest = id / CH;
-    const int h = (int)(rest % a.c.n_kv);
-    const long long row = rest / a.c.n_kv;
+__global__ void __launch_bounds__(128) k_kv4_append(const Kv4RowsArgs a) {
+    constexpr int LANES = NG * 4, ROWS = 32 / LANES;     // lanes of a row, rows side by side: 4, 2 (8 lanes idle), 2
+    constexpr int IMG = NG * KV4_GT;
+    __shared__ __align__(16) unsigned char image[4][IMG];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    unsigned char* const img = image[warp];
+    const long long id = (long long)blockIdx.x * 4 + warp;
+    const int h = (int)(id % a.c.n_kv), want = (int)(id / a.c.n_kv);
     pdl_wait();
     pdl_launch();
-    long long where = -1;
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (row < a.n_rows) {
-        where = __ldcg(a.slot_map + row);
-        const __nv_bfloat16* src = (value ? a.v + row * a.v_stride : a.k + row * a.k_stride) + (size_t)h * (NG * KV4_GROUP) + ch * 8;
-        raw = __ldcg(reinterpret_cast<const uint4*>(src));
+    int lo = 0, hi = a.n;      // the entry that tile number `want` belongs to
+    if (want >= __ldcg(a.cu_tiles + a.n)) return;
+    int before = 0;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+        const int f = at < hi ? __ldcg(a.cu_tiles + at) : 0x7fffffff;
+        const int k = 31 - __clz(__ballot_sync(0xffffffffu, f <= want));
+        before = __shfl_sync(0xffffffffu, f, k);
+        lo += k * step;
+        hi = min(hi, lo + step);
     }
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-    float x[8];
-    bool odd = false;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        x[j] = __uint_as_float(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16);
-        odd |= !(fabsf(x[j]) <= KV4_LIMIT);
-        x[j] = x[j] == x[j] ? fminf(fmaxf(x[j], -KV4_LIMIT), KV4_LIMIT) : 0.f;   // so that what is stored is finite
+    const int4 e = __ldcg(a.entries + lo);
+    const int pos0 = ((e.y >> 4) + want - before) << 4;                       // the tile's first position
+    const int from = max(e.y, pos0) - pos0, to = min(e.y + e.z, pos0 + 16) - pos0;
+    int b = __ldcg(a.c.table + (size_t)e.x * a.c.max_blocks + (pos0 >> a.c.block_shift));
+    if ((unsigned)b >= (unsigned)a.c.n_blocks) {
+        if (lane == 0) atomicOr(a.c.flag, KV4_BAD_BLOCK);
+        return;
     }
-    float lo = x[0], hi = x[0];
+    unsigned char* const tile = a.c.pool + tile_at<NG>(a.c, ((long long)b << a.c.block_shift) + (pos0 & ((1 << a.c.block_shift) - 1)), h);
+    const int sub = lane / LANES, ch = lane % LANES, grp = ch >> 2, t = ch & 3;
+    unsigned char* const gimg = img + grp * KV4_GT;
 #pragma unroll
-    for (int j = 1; j < 8; ++j) { lo = fminf(lo, x[j]); hi = fmaxf(hi, x[j]); }
+    for (int half = 0; half < 2; ++half) {       // keys, values
+        const __nv_bfloat16* src = (half ? a.v : a.k) + (long long)(e.w + pos0 - e.y) * (half ? a.v_stride : a.k_stride) + h * (NG * KV4_GROUP) + ch * 8;
+        const long long stride = half ? a.v_stride : a.k_stride;
 #pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
-    if (where < 0) return;
-    if (odd) atomicOr(a.c.flag, KV4_BAD_VALUE);
-    const __half zero = __float2half_rn(lo);
-    const float z = __half2float(zero);
-    const __half scale = __float2half_rn(__fmul_rn(__fsub_rn(hi, z), 1.f / 15.f));
-    const float s = __half2float(scale);
-    uint32_t code[8];
+        for (int part = 0; part < 16 / ROWS; part += 4) {       // four rows a lane in flight
+            uint4 raw[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-        code[j] = s > 0.f ? (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[j], z), s)), 0.f), 15.f) : 0u;
-    const int key = (int)(where & 15), key8 = key & 7, upper = key >> 3, grp = ch >> 2, t = ch & 3;
-    unsigned char* tile = a.c.pool + tile_at<NG>(a.c, where, h) + grp * KV4_GT;
-    if (!value) {
-        uint32_t word = 0;
+            for (int j = 0; j < 4; ++j) {
+                const int key = (part + j) * ROWS + sub;
+                raw[j] = make_uint4(0, 0, 0, 0);
+                if (sub < ROWS && key >= from && key < to) raw[j] = __ldcg(reinterpret_cast<const uint4*>(src + key * stride));
+            }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) word |= code[j] << (4 * (j >> 1) + 16 * (j & 1));
-        *reinterpret_cast<uint32_t*>(tile + (key8 * 4 + t) * 8 + upper * 4) = word;
-        if (t == 0)
-            *reinterpret_cast<__half2*>(tile + KV4_KPAR + key8 * 8 + upper * 4) = __halves2half2(scale, zero);
-    } else {
+            for (int r = 0; r < 4; ++r) {
+                const int key = (part + r) * ROWS + sub;
+                if ((part + r) * ROWS >= to) break;              // the whole warp
+                if ((part + r + 1) * ROWS <= from) continue;
+                const uint32_t w[4] = {raw[r].x, raw[r].y, raw[r].z, raw[r].w};
+                float x[8];
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            const uint32_t half = code[4 * q] | code[4 * q + 1] << 4 | code[4 * q + 2] << 8 | code[4 * q + 3] << 12;
-            *reinterpret_cast<uint16_t*>(tile + KV4_VCODE + ((2 * t + q) * 4 + (key8 >> 1)) * 8 + upper * 4 + (key8 & 1) * 2) = (uint16_t)half;
+                for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16);
+                if (most_bits(raw[r]) > KV4_LIMIT_BITS) {      // so that what is stored is finite
+                    atomicOr(a.c.flag, KV4_BAD_VALUE);
+                    for (int j = 0; j < 8; ++j) x[j] = tame(x[j]);
+                }
+                float low = x[0], high = x[0];
+#pragma unroll
+                for (int j = 1; j < 8; ++j) { low = fminf(low, x[j]); high = fmaxf(high, x[j]); }
+#pragma unroll
+                for (int o = 1; o < 4; o <<= 1) {
+                    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+                    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+                }
+                const __half zero = __float2half_rn(low);
+                const float z = __half2float(zero);
+                const __half scale = __float2half_rn(__fmul_rn(__fsub_rn(high, z), 1.f / 15.f));
+                const float s = __half2float(scale), inv = s > 0.f ? __frcp_rn(s) : 0.f;
+                uint32_t code[8];
+                float near = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float q = fminf(fmaxf(__fsub_rn(x[j], z), 0.f) * inv, 15.f);
+                    const float c = q + 8388608.f;             // 2^23: the nearest whole number is in the low bits
+                    near = fmaxf(near, fabsf(q - (c - 8388608.f)));
+                    code[j] = __float_as_uint(c) & 15u;
+                }
+                if (near > 0.5f - 7.62939453125e-6f && s > 0.f) codes_by_division(x, z, s, code);
+                if (sub >= ROWS || key < from || key >= to) continue;
+                const int key8 = key & 7, upper = key >> 3;
+                if (!half) {
+                    uint32_t word = 0;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) word |= code[j] << (4 * (j >> 1) + 16 * (j & 1));
+                    *reinterpret_cast<uint32_t*>(gimg + (key8 * 4 + t) * 8 + upper * 4) = word;
+                    if (t == 0) *reinterpret_cast<__half2*>(gimg + KV4_KPAR + key8 * 8 + upper * 4) = __halves2half2(scale, zero);
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        gimg[KV4_VCODE + ((2 * t + (q >> 1)) * 4 + (key8 >> 1)) * 8 + (q & 1) * 4 + (key8 & 1) * 2 + upper] =
+                            (unsigned char)(code[2 * q] | code[2 * q + 1] << 4);
+                    if (t == 0) *reinterpret_cast<__half2*>(gimg + KV4_VPAR + key8 * 8 + upper * 4) = __halves2half2(scale, zero);
+                }
+            }
         }
-        if (t == 0) {
-            __half* par = reinterpret_cast<__half*>(tile + KV4_VPAR + (key8 >> 1) * 16 + upper * 8) + (key8 & 1);
-            par[0] = scale;
-            par[2] = zero;
+    }
+    __syncwarp();
+    if (to - from == 16) {
+        for (int i = lane; i < IMG / 16; i += 32) reinterpret_cast<uint4*>(tile)[i] = reinterpret_cast<const uint4*>(img)[i];
+        return;
+    }
+    for (int i = lane; i < IMG / 4; i += 32) {      // word i of the image: whose is it?
+        const int in = i * 4 % KV4_GT;
+        if (in < KV4_VCODE || in >= KV4_VPAR) {     // one key's
+            const int key = (in < KV4_KPAR ? in >> 5 : in < KV4_VCODE ? (in - KV4_KPAR) >> 3 : (in - KV4_VPAR) >> 3) + (in >> 2 & 1) * 8;
+            if (key >= from && key < to) reinterpret_cast<uint32_t*>(tile)[i] = reinterpret_cast<const uint32_t*>(img)[i];
+        } else {                                    // four keys', a byte each
+            const int key = (in >> 3 & 3) * 2;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int k = key + (q >> 1) + (q & 1) * 8;
+                if (k >= from && k < to) tile[4 * i + q] = img[4 * i + q];
+            }
         }
     }
 }
 
-// The reverse: 8 elements a thread, bf16 out.  Rows whose slot or position is out of range, or whose block the table lacks, come out as zeros.
+// The reverse: 8 elements a thread, bf16 out.  Rows whose slot or position is out of range, or whose block the table lacks, come out as
+// zeros.  A CTA takes the rows next to one another of one kv head, keys or values (blockIdx.z), because those of a tile share its lines in
+// the L1; that is why this kernel starts only when the kernel before it has ended (no early launch: an SM's L1 could hold older lines).
 template <int NG>
 __global__ void __launch_bounds__(256) k_kv4_read(const Kv4RowsArgs a) {
-    constexpr int CH = NG * 4;
-    const bool value = blockIdx.y != 0;
-    const long long id = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    const int ch = (int)(id % CH);
-    const long long rest = id / CH;
-    const int h = (int)(rest % a.c.n_kv);
-    const long long row = rest / a.c.n_kv;
-    pdl_wait();
-    pdl_launch();
-    if (row >= a.n_rows) return;
-    const int slot = __ldcg(a.row_slot + row), pos = __ldcg(a.row_pos + row);
+    constexpr int CH = NG * 4, ROWS = 256 / CH;
+    const bool value = blockIdx.z != 0;
+    const int ch = threadIdx.x % CH, h = blockIdx.y;
+    const long long row = (long long)blockIdx.x * ROWS + threadIdx.x / CH;
+    if (threadIdx.x >= ROWS * CH || row >= a.n_rows) return;
+    const int slot = __ldg(a.row_slot + row), pos = __ldg(a.row_pos + row);
     long long where = -1;
     if (slot >= 0 && slot < a.c.max_seqs && pos >= 0 && (pos >> a.c.block_shift) < a.c.max_blocks) {
-        const int b = __ldcg(a.c.table + (size_t)slot * a.c.max_blocks + (pos >> a.c.block_shift));
+        const int b = __ldg(a.c.table + (size_t)slot * a.c.max_blocks + (pos >> a.c.block_shift));
         if (b >= 0 && b < a.c.n_blocks) where = ((long long)b << a.c.block_shift) + (pos & ((1 << a.c.block_shift) - 1));
     }
     if (where < 0 && slot != -1) atomicOr(a.c.flag, KV4_BAD_SLOT);
@@ -383,23 +459,20 @@ __global__ void __launch_bounds__(256) k_kv4_read(const Kv4RowsArgs a) {
         const unsigned char* tile = a.c.pool + tile_at<NG>(a.c, where, h) + grp * KV4_GT;
         float s, z;
         uint32_t code[8];
+        const uint32_t par = __ldg(reinterpret_cast<const uint32_t*>(tile + (value ? KV4_VPAR : KV4_KPAR) + key8 * 8 + upper * 4));
+        s = __half2float(__ushort_as_half((unsigned short)(par & 0xffff)));
+        z = __half2float(__ushort_as_half((unsigned short)(par >> 16)));
         if (!value) {
-            const uint32_t word = __ldcg(reinterpret_cast<const uint32_t*>(tile + (key8 * 4 + t) * 8 + upper * 4));
-            const uint32_t par = __ldcg(reinterpret_cast<const uint32_t*>(tile + KV4_KPAR + key8 * 8 + upper * 4));
-            s = __half2float(__ushort_as_half((unsigned short)(par & 0xffff)));
-            z = __half2float(__ushort_as_half((unsigned short)(par >> 16)));
+            const uint32_t word = __ldg(reinterpret_cast<const uint32_t*>(tile + (key8 * 4 + t) * 8 + upper * 4));
 #pragma unroll
             for (int j = 0; j < 8; ++j) code[j] = word >> (4 * (j >> 1) + 16 * (j & 1)) & 15;
         } else {
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const uint32_t half = __ldcg(reinterpret_cast<const unsigned short*>(tile + KV4_VCODE + ((2 * t + q) * 4 + (key8 >> 1)) * 8 + upper * 4 + (key8 & 1) * 2));
-#pragma unroll
-                for (int j = 0; j < 4; ++j) code[4 * q + j] = half >> (4 * j) & 15;
+            for (int q = 0; q < 4; ++q) {
+                const uint32_t two = __ldg(tile + KV4_VCODE + ((2 * t + (q >> 1)) * 4 + (key8 >> 1)) * 8 + (q & 1) * 4 + (key8 & 1) * 2 + upper);
+                code[2 * q] = two & 15;
+                code[2 * q + 1] = two >> 4;
             }
-            const unsigned short* par = reinterpret_cast<const unsigned short*>(tile + KV4_VPAR + (key8 >> 1) * 16 + upper * 8) + (key8 & 1);
-            s = __half2float(__ushort_as_half(__ldcg(par)));
-            z = __half2float(__ushort_as_half(__ldcg(par + 2)));
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = __half2float(__float2half_rn(__fmaf_rn(s, (float)code[j], z)));   // the product is exact

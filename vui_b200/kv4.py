@@ -18,12 +18,15 @@ A prompt is the same with ``cache.plan(slots, lengths)``; its rows are the seque
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 import torch
 from torch import Tensor
 
 from . import _lib
+
+_NOTHING = contextlib.nullcontext()
 
 
 class Kv4Plan:
@@ -33,14 +36,19 @@ class Kv4Plan:
 
     def __init__(self, device, n_seqs: int, n_rows: int, max_new: int):
         self.n_seqs, self.n_rows, self.max_new = n_seqs, n_rows, max_new
-        self._ints = torch.empty(6 * n_seqs + 4 + 2 * n_rows, dtype=torch.int32, device=device)
-        self._entries, self.cu_rows, self._cu_units, self.row_slot, self.row_pos = self._ints.split(
-            [4 * n_seqs, n_seqs + 1, n_seqs + 3, n_rows, n_rows])
-        self.slot_map = torch.empty(n_rows, dtype=torch.int64, device=device)
-        P = lambda t: t.data_ptr()  # noqa: E731
-        self._c = _lib.VuibKv4Plan(n_seqs, n_rows, max_new, P(self._entries), P(self.cu_rows), P(self._cu_units),
-                                   P(self.row_slot) if n_rows else None, P(self.row_pos) if n_rows else None,
-                                   P(self.slot_map) if n_rows else None)
+        work = (6 * n_seqs + 2 + n_rows + 3) & ~3          # the parts behind it: 16-byte aligned
+        row = (n_rows + 3) & ~3
+        # one allocation: work, slot_map (int64), row_slot, row_pos, cu_rows
+        self._ints = ints = torch.empty(work + 4 * row + n_seqs + 1, dtype=torch.int32, device=device)
+        self.slot_map = ints[work:work + 2 * n_rows].view(torch.int64)
+        self.row_slot = ints[work + 2 * row:work + 2 * row + n_rows]
+        self.row_pos = ints[work + 3 * row:work + 3 * row + n_rows]
+        self.cu_rows = ints[work + 4 * row:]
+        at = ints.data_ptr()
+        self._c = _lib.VuibKv4Plan(n_seqs, n_rows, max_new, at, at + 4 * (work + 4 * row), at + 4 * (work + 2 * row), at + 4 * (work + 3 * row),
+                                   at + 4 * work)
+        self._ref = C.byref(self._c)
+        self._ws_bytes = -1        # of its attention calls, asked for once
 
 
 class Kv4Cache:
@@ -62,13 +70,14 @@ class Kv4Cache:
             raise RuntimeError("vui_b200.Kv4Cache needs a CUDA device (sm_100a); there is no CPU path")
         dev = torch.device(device)
         self.device = dev if dev.index is not None else torch.device("cuda", torch.cuda.current_device())
+        self._index = self.device.index
         self.n_layers, self.n_heads, self.n_kv_heads, self.head_dim = n_layers, n_heads, n_kv_heads, head_dim
         self.n_blocks, self.block_size, self.max_seqs, self.max_blocks = n_blocks, block_size, max_seqs, max_blocks
         n = C.c_size_t()
         self._ck(self._lib.vuib_kv4_pool_bytes(self._h, C.byref(n)))
         self.pool_bytes = n.value
         i32 = lambda *shape: torch.zeros(*shape, dtype=torch.int32, device=self.device)  # noqa: E731
-        with torch.cuda.device(self.device):
+        with self._here():
             self._pool = torch.zeros(n.value, dtype=torch.uint8, device=self.device)
             self.seq_lens, self.block_table = i32(max_seqs), i32(max_seqs, max_blocks)
             self._free, self.n_free, self._flag = i32(n_blocks), i32(1), i32(1)
@@ -93,10 +102,16 @@ class Kv4Cache:
 
     @property
     def _stream(self):
-        return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def _here(self):
+        """Makes the cache's device the current one, where it is not."""
+        return _NOTHING if torch.cuda.current_device() == self._index else torch.cuda.device(self._index)
 
     def _ints(self, v, name: str, n: int | None = None) -> Tensor:
         t = v if torch.is_tensor(v) else torch.as_tensor(v, dtype=torch.int64 if len(v) == 0 else None)
+        if t.dtype is torch.int32 and t.device == self.device and t.dim() == 1 and t.is_contiguous() and (n is None or t.numel() == n):
+            return t
         if t.dim() != 1 or t.is_floating_point() or t.is_complex() or (n is not None and t.numel() != n):
             raise ValueError(f"{name}: a one-dimensional list of {'whole numbers' if n is None else f'{n} whole numbers'} is wanted, "
                              f"got {t.dtype} {tuple(t.shape)}")
@@ -105,7 +120,7 @@ class Kv4Cache:
     # ------------------------------------------------------------------ tables
     def reset(self) -> None:
         """Empties every sequence."""
-        with torch.cuda.device(self.device):
+        with self._here():
             self._ck(self._lib.vuib_kv4_reset(self._h, self._stream))
 
     def plan(self, slots, new_lens=None, at=None, *, n_rows: int | None = None, max_new: int | None = None) -> Kv4Plan:
@@ -126,13 +141,13 @@ class Kv4Cache:
             n_rows, max_new = n if n_rows is None else n_rows, 1 if max_new is None else max_new
         if n_rows is None or max_new is None:
             raise ValueError("new_lens on the device need n_rows and max_new")
-        with torch.cuda.device(self.device):
+        with self._here():
             new = None if new_lens is None else self._ints(new_lens, "new_lens", n)
             at = None if at is None else self._ints(at, "at", n)
             if n_rows < 0 or max_new < 0:
                 raise ValueError("n_rows and max_new must not be negative")
             plan = Kv4Plan(self.device, n, int(n_rows), min(int(max_new), int(n_rows)))
-            self._ck(self._lib.vuib_kv4_plan(self._h, C.byref(plan._c), slots.data_ptr(), None if new is None else new.data_ptr(),
+            self._ck(self._lib.vuib_kv4_plan(self._h, plan._ref, slots.data_ptr(), None if new is None else new.data_ptr(),
                                              None if at is None else at.data_ptr(), self._stream))
         return plan
 
@@ -146,6 +161,9 @@ class Kv4Cache:
     def _rows(self, t: Tensor, name: str, n: int, heads: int, *, out: bool = False) -> Tensor:
         """(n, heads, head_dim) or (n, heads * head_dim) as the library takes it: bf16 on this device, heads behind one
         another, rows a multiple of 16 bytes apart.  An input that lies otherwise is copied, an output refused."""
+        if torch.is_tensor(t) and t.dtype is torch.bfloat16 and t.device == self.device and t.shape == (n, heads, self.head_dim) and \
+                t.is_contiguous() and t.data_ptr() % 16 == 0:
+            return t
         if not torch.is_tensor(t) or tuple(t.shape) not in ((n, heads, self.head_dim), (n, heads * self.head_dim)):
             raise ValueError(f"{name}: ({n}, {heads}, {self.head_dim}) is wanted, got {tuple(t.shape) if torch.is_tensor(t) else type(t)}")
         good = t.device == self.device and t.dtype == torch.bfloat16
@@ -166,15 +184,15 @@ class Kv4Cache:
     def append(self, layer: int, k: Tensor, v: Tensor, plan: Kv4Plan) -> None:
         """Stores the plan's rows: k, v (n_rows, n_kv_heads, head_dim), keys with RoPE applied.  NaN is stored as 0 and
         magnitudes beyond 60000 as 60000, which ``check_device`` reports."""
-        with torch.cuda.device(self.device):
+        with self._here():
             k, v = (self._rows(t, name, plan.n_rows, self.n_kv_heads) for t, name in ((k, "k"), (v, "v")))
-            self._ck(self._lib.vuib_kv4_append(self._h, layer, C.byref(plan._c), k.data_ptr(), self._step(k, self.n_kv_heads),
+            self._ck(self._lib.vuib_kv4_append(self._h, layer, plan._ref, k.data_ptr(), self._step(k, self.n_kv_heads),
                                                v.data_ptr(), self._step(v, self.n_kv_heads), self._stream))
 
     def read(self, layer: int, row_slot, row_pos, *, k_out: Tensor | None = None, v_out: Tensor | None = None) -> tuple[Tensor, Tensor]:
         """The keys and values stored for position ``row_pos[i]`` of sequence ``row_slot[i]``: (n, n_kv_heads, head_dim) bf16,
         new tensors or ``k_out`` and ``v_out`` (a stretch of an engine's bf16 cache, say).  Slot -1 gives zeros."""
-        with torch.cuda.device(self.device):
+        with self._here():
             row_slot = self._ints(row_slot, "row_slot")
             n = row_slot.numel()
             row_pos = self._ints(row_pos, "row_pos", n)
@@ -192,21 +210,24 @@ class Kv4Cache:
         Rows behind the plan's last are not written."""
         if scale is not None and not 0 < scale <= 1e30:
             raise ValueError("scale must be positive")
-        with torch.cuda.device(self.device):
+        with self._here():
             q = self._rows(q, "q", plan.n_rows, self.n_heads)
             out = torch.empty(q.shape, dtype=torch.bfloat16, device=self.device) if out is None else self._rows(out, "out", plan.n_rows, self.n_heads, out=True)
-            n = C.c_size_t()
-            self._ck(self._lib.vuib_kv4_attention_workspace(self._h, C.byref(plan._c), C.byref(n)))
-            ws = torch.empty(n.value, dtype=torch.uint8, device=self.device) if n.value else None
-            self._ck(self._lib.vuib_kv4_attention(self._h, layer, C.byref(plan._c), q.data_ptr(), self._step(q, self.n_heads), out.data_ptr(),
-                                                  self._step(out, self.n_heads), float(scale or 0.0), None if ws is None else ws.data_ptr(), n.value,
+            if plan._ws_bytes < 0:
+                n = C.c_size_t()
+                self._ck(self._lib.vuib_kv4_attention_workspace(self._h, plan._ref, C.byref(n)))
+                plan._ws_bytes = n.value
+            n = plan._ws_bytes
+            ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None     # the call's own: calls may overlap
+            self._ck(self._lib.vuib_kv4_attention(self._h, layer, plan._ref, q.data_ptr(), self._step(q, self.n_heads), out.data_ptr(),
+                                                  self._step(out, self.n_heads), float(scale or 0.0), None if ws is None else ws.data_ptr(), n,
                                                   self._stream))
         return out
 
     # ------------------------------------------------------------- diagnostics
     def check_device(self) -> None:
         """Raises if a call since the last check met a slot, length or value out of range, or ran out of rows or blocks."""
-        with torch.cuda.device(self.device):
+        with self._here():
             self._ck(self._lib.vuib_kv4_check_flag(self._h, self._stream))
 
     def launch_count(self) -> int:
