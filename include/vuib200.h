@@ -528,7 +528,7 @@ typedef struct VuibKv4Config {
  * entry.  The arrays are the caller's, written by vuib_kv4_plan and read by the calls that take the plan. */
 typedef struct VuibKv4Plan {
     int32_t n_seqs, n_rows, max_new;
-    int32_t* work;       /* (6 * n_seqs + 2 + n_rows), 16-byte aligned: how the calls share out the rows */
+    int32_t* work;       /* (7 * n_seqs + 3 + n_rows), 16-byte aligned: how the calls share out the rows */
     int32_t* cu_rows;    /* (n_seqs + 1): first row of every entry, and the number of rows */
     int32_t* row_slot;   /* (n_rows): a row's sequence, -1 behind the last row */
     int32_t* row_pos;    /* (n_rows): its position, -1 behind the last row */

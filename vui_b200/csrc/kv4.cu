@@ -19,7 +19,7 @@ struct VuibKv4 {
     size_t layer_bytes;
     bool bound;
     int block_shift, ng, sms, device;
-    int resident[5];          // CTAs of each attention form that fit an SM of the device, 0: not asked for yet
+    int resident[6];          // CTAs of each attention form that fit an SM of the device, 0: not asked for yet
     int64_t launches;
     char err[256];
 };
@@ -66,34 +66,45 @@ cudaError_t launch(VuibKv4* c, void (*kern)(KArgs...), dim3 grid, dim3 block, si
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
 // What a plan's shape decides for attention: columns of a tile (rows x query heads of a kv head) and positions of a split.
-// Single tokens: splits of 256 positions, four warps at 64 each, whatever the batch, so that a row's bits depend on its own keys alone.
-// Up to 16 columns the form for a few (4, 8 or 16 columns a tile), else the one for many.
-struct Shape { bool few; int nt, cols, split; };
+// A few columns: splits of 256 positions in sequences of up to 1024, 512 beyond, whatever the batch.
+// Up to 16 columns the form for a few (2, 4, 8 or 16 columns a tile), else the one for many.
+struct Shape { bool few, halves; int nt, cols; Kv4Split split; };
 Shape shape_of(const VuibKv4* c, const VuibKv4Plan* p) {
     Shape s;
     const int group = c->cfg.n_heads / c->cfg.n_kv_heads;
     const long long most = (long long)p->max_new * group;       // columns of one sequence
     s.few = most <= 16;
     s.nt = s.few ? (most <= 4 ? 1 : most <= 8 ? 2 : 4) : c->ng > 2 ? 2 : 4;
-    s.cols = (s.few ? 4 : 8) * s.nt;
-    s.split = 256;
+    s.halves = most <= 2 && c->ng != 3;
+    s.cols = s.halves ? 2 : (s.few ? 4 : 8) * s.nt;
+#ifndef KV4_LONG
+#define KV4_LONG 512
+#endif
+    s.split = {256, KV4_LONG, true};
     if (!s.few) {
         const long long tiles = ceil_div((long long)p->n_rows * group, s.cols) + p->n_seqs;
         const long long len = (long long)c->cfg.max_blocks << c->block_shift;
-        s.split = 512;
-        while ((long long)s.split * 32 < len) s.split *= 2;
-        if (tiles * c->cfg.n_kv_heads >= 2 * c->sms) s.split = 1 << 30;
+        int split = 512;
+        while ((long long)split * 32 < len) split *= 2;
+        if (tiles * c->cfg.n_kv_heads >= 2 * c->sms) split = 1 << 30;
+        s.split = {split, split, false};
     }
     return s;
 }
 
+// Most splits of one sequence.
+long long most_parts(const VuibKv4* c, const Shape& s) {
+    const long long len = (long long)c->cfg.max_blocks << c->block_shift;
+    return max(s.split.parts(min(len, 1024ll)), s.split.parts(len));
+}
+
 // Most units (of one kv head) that a plan of this shape can have.  Sequences share no blocks, so their lengths sum up to the pool's.
 long long most_units(const VuibKv4* c, const VuibKv4Plan* p, const Shape& s) {
-    const long long len = (long long)c->cfg.max_blocks << c->block_shift, pool = (long long)c->cfg.n_blocks << c->block_shift;
+    const long long pool = (long long)c->cfg.n_blocks << c->block_shift;
     const int group = c->cfg.n_heads / c->cfg.n_kv_heads;
     const long long a_seq = ceil_div((long long)p->max_new * group, s.cols);
     const long long tiles = min((long long)p->n_seqs * a_seq, ceil_div((long long)p->n_rows * group, s.cols) + p->n_seqs);
-    return min(tiles * ceil_div(len, s.split), a_seq * (p->n_seqs + pool / s.split));
+    return min(tiles * most_parts(c, s), a_seq * (p->n_seqs + pool / s.split.up_to_1024));
 }
 
 size_t acc_bytes(const VuibKv4* c, long long items, int cols) { return ((size_t)items * cols * c->cfg.head_dim * 4 + 255) & ~size_t(255); }
@@ -101,8 +112,9 @@ size_t acc_bytes(const VuibKv4* c, long long items, int cols) { return ((size_t)
 // The parts of a plan's work array.
 int4* plan_entries(const VuibKv4Plan* p) { return reinterpret_cast<int4*>(p->work); }
 int32_t* plan_units(const VuibKv4Plan* p) { return p->work + 4 * (size_t)p->n_seqs; }
-int32_t* plan_tiles(const VuibKv4Plan* p) { return p->work + 5 * (size_t)p->n_seqs + 1; }
-int32_t* plan_row_entry(const VuibKv4Plan* p) { return p->work + 6 * (size_t)p->n_seqs + 2; }
+int32_t* plan_work(const VuibKv4Plan* p) { return p->work + 5 * (size_t)p->n_seqs + 1; }
+int32_t* plan_tiles(const VuibKv4Plan* p) { return p->work + 6 * (size_t)p->n_seqs + 2; }
+int32_t* plan_row_entry(const VuibKv4Plan* p) { return p->work + 7 * (size_t)p->n_seqs + 3; }
 
 int32_t check_plan(VuibKv4* c, const VuibKv4Plan* p) {
     if (!p || !p->work || !p->cu_rows) return fail(c, VUIB_ERR_NULL, "a plan needs its arrays");
@@ -125,7 +137,7 @@ int32_t check_rows(VuibKv4* c, const char* name, const void* p, int64_t stride, 
 }
 
 template <int NG, int COLS>
-cudaError_t launch_attn(VuibKv4* c, void (*kern)(Kv4AttnArgs), int& resident, const Kv4AttnArgs& a, long long items, bool merge, void* stream) {
+cudaError_t launch_attn(VuibKv4* c, const Shape& s, void (*kern)(Kv4AttnArgs), int& resident, const Kv4AttnArgs& a, long long items, bool merge, void* stream) {
     constexpr int smem = KaShared<NG, COLS>::TOTAL;
     cudaError_t e = cudaSuccess;
     if (!resident) {     // as many CTAs as fit the SMs: asked for, and attributes set, once a handle and form
@@ -138,7 +150,7 @@ cudaError_t launch_attn(VuibKv4* c, void (*kern)(Kv4AttnArgs), int& resident, co
     e = launch(c, kern, dim3((unsigned)min(items, (long long)c->sms * resident)), KA_THREADS + 32, smem, 1, stream, a);
     if (e != cudaSuccess || !merge) return e;
     const long long rows = (long long)a.n_rows * c->cfg.n_heads;
-    if (((long long)c->cfg.max_blocks << c->block_shift) <= 32ll * a.split)
+    if (most_parts(c, s) <= 32)
         return launch(c, k_kv4_merge<NG, 1>, dim3((unsigned)ceil_div(rows, 4)), 128, 0, 1, stream, a, COLS);
     return launch(c, k_kv4_merge<NG, 8>, dim3((unsigned)rows), 256, 0, 1, stream, a, COLS);
 }
@@ -147,12 +159,14 @@ template <int NG>
 cudaError_t launch_form(VuibKv4* c, const Shape& s, const Kv4AttnArgs& a, long long items, bool merge, void* stream) {
     int* resident = c->resident;
     if (s.few) {
-        if (s.nt == 1) return launch_attn<NG, 4>(c, k_kv4_attn_few<NG, 1>, resident[0], a, items, merge, stream);
-        if (s.nt == 2) return launch_attn<NG, 8>(c, k_kv4_attn_few<NG, 2>, resident[1], a, items, merge, stream);
-        return launch_attn<NG, 16>(c, k_kv4_attn_few<NG, 4>, resident[2], a, items, merge, stream);
+        if constexpr (NG != 3)
+            if (s.halves) return launch_attn<NG, 2>(c, s, k_kv4_attn_few<NG, 1, true>, resident[5], a, items, merge, stream);
+        if (s.nt == 1) return launch_attn<NG, 4>(c, s, k_kv4_attn_few<NG, 1, false>, resident[0], a, items, merge, stream);
+        if (s.nt == 2) return launch_attn<NG, 8>(c, s, k_kv4_attn_few<NG, 2, false>, resident[1], a, items, merge, stream);
+        return launch_attn<NG, 16>(c, s, k_kv4_attn_few<NG, 4, false>, resident[2], a, items, merge, stream);
     }
-    if constexpr (NG == 2) return launch_attn<NG, 32>(c, k_kv4_attn<NG, 4>, resident[3], a, items, merge, stream);
-    else return launch_attn<NG, 16>(c, k_kv4_attn<NG, 2>, resident[4], a, items, merge, stream);
+    if constexpr (NG == 2) return launch_attn<NG, 32>(c, s, k_kv4_attn<NG, 4>, resident[3], a, items, merge, stream);
+    else return launch_attn<NG, 16>(c, s, k_kv4_attn<NG, 2>, resident[4], a, items, merge, stream);
 }
 
 }  // namespace
@@ -236,7 +250,7 @@ extern "C" int32_t vuib_kv4_plan(VuibKv4* c, const VuibKv4Plan* p, const int32_t
     a.slots = slots_dev; a.new_lens = new_dev; a.at = at_dev;
     a.n = p->n_seqs; a.n_rows = p->n_rows; a.max_new = p->max_new;
     a.group = c->cfg.n_heads / c->cfg.n_kv_heads; a.cols = s.cols; a.split = s.split;
-    a.entries = plan_entries(p); a.cu_units = plan_units(p); a.cu_tiles = plan_tiles(p); a.row_entry = plan_row_entry(p);
+    a.entries = plan_entries(p); a.cu_units = plan_units(p); a.cu_work = plan_work(p); a.cu_tiles = plan_tiles(p); a.row_entry = plan_row_entry(p);
     a.cu_rows = p->cu_rows;
     a.row_slot = p->row_slot; a.row_pos = p->row_pos; a.slot_map = reinterpret_cast<long long*>(p->slot_map);
     const size_t smem = (8 * (size_t)p->n_seqs + 3 + c->cfg.max_seqs) * 4;
@@ -301,7 +315,7 @@ extern "C" int32_t vuib_kv4_attention_workspace(VuibKv4* c, const VuibKv4Plan* p
     *bytes = 0;
     if (!p->n_rows || !p->max_new) return VUIB_OK;
     const Shape s = shape_of(c, p);
-    if (((long long)c->cfg.max_blocks << c->block_shift) <= s.split) return VUIB_OK;
+    if (most_parts(c, s) <= 1) return VUIB_OK;
     const long long items = most_units(c, p, s) * c->cfg.n_kv_heads;
     *bytes = acc_bytes(c, items, s.cols) + (size_t)items * s.cols * 8;
     return VUIB_OK;
@@ -326,8 +340,9 @@ extern "C" int32_t vuib_kv4_attention(VuibKv4* c, int32_t layer, const VuibKv4Pl
     Kv4AttnArgs a = {};
     a.c = c->cache;
     a.c.pool += c->layer_bytes * layer;
-    a.entries = plan_entries(p); a.cu_units = plan_units(p); a.row_entry = plan_row_entry(p);
+    a.entries = plan_entries(p); a.cu_units = plan_units(p); a.cu_work = plan_work(p); a.row_entry = plan_row_entry(p);
     a.n = p->n_seqs; a.n_rows = p->n_rows; a.group = c->cfg.n_heads / c->cfg.n_kv_heads; a.split = s.split;
+    a.group_inv = a.group > 1 ? (uint32_t)(((1ull << 32) + a.group - 1) / a.group) : 0;
     a.q = static_cast<const __nv_bfloat16*>(q_dev); a.q_stride = q_stride;
     a.out = static_cast<__nv_bfloat16*>(out_dev); a.out_stride = out_stride;
     a.scale_log2 = (scale > 0.f ? scale : 1.f / sqrtf((float)c->cfg.head_dim)) * 1.4426950408889634f;

@@ -9,8 +9,10 @@ constexpr int KA_THREADS = 128, KA_WARPS = 4;
 
 struct Kv4AttnArgs {
     Kv4Cache c;
-    const int4* entries; const int32_t* cu_units; const int32_t* row_entry;
-    int n, n_rows, group, split;
+    const int4* entries; const int32_t* cu_units; const int32_t* cu_work; const int32_t* row_entry;
+    int n, n_rows, group;
+    uint32_t group_inv;                         // 2^32 / group, rounded up (group > 1)
+    Kv4Split split;
     const __nv_bfloat16* q; long long q_stride;
     __nv_bfloat16* out; long long out_stride;
     float scale_log2;                          // scale * log2(e)
@@ -64,63 +66,48 @@ __device__ __forceinline__ void kv4_values(uint32_t w, __half2 s0, __half2 z0, _
     }
 }
 
+// x / group for x below 2^28 (what is left over, x times less than 16, stays below 2^32).
+__device__ __forceinline__ int by_group(const Kv4AttnArgs& a, int x) { return a.group == 1 ? x : (int)__umulhi((unsigned)x, a.group_inv); }
+
 // A unit: a tile of columns of one sequence (its rows times the query heads of a kv head, COLS at a time), a kv head, a split of the
 // positions.  Units lie in the order sequence, column tile, kv head, split.  What the consumers are told of one, a stage at a time:
 struct __align__(16) Kv4Item {
     int flags;                                  // KI_*
     int start, rows, row0;                      // the sequence's first new position, its rows, the first of them
     int ctile, head, splits, base;              // base: position of the stage's first key
-    int hi, pad;                                // one past the last position of the stage that any column of the tile sees
+    int hi, all;                                // one past the last position that any column of the tile sees, the last that all see
     long long w;                                // number of the unit times kv heads: where its partial sums go
 };
 constexpr int KI_FIRST = 1, KI_LAST = 2, KI_QUERIES = 4, KI_END = 8;
 
 struct Kv4Walk {       // the producer's place
-    int entry, ctile, head, split, splits, base, hi;
+    int entry, ctile, head, split, splits, size, base, hi;     // size: positions of a split
     int4 e, next;      // this entry and, read ahead, the one behind it
+    int units, next_units;    // and their first units
+    long long w, at;   // number of the unit; work of all units before it
 };
 
 template <int COLS>
 __device__ __forceinline__ void walk_range(const Kv4AttnArgs& a, Kv4Walk& u) {
-    u.base = u.split * a.split;
-    const int end_row = (min((u.ctile + 1) * COLS, u.e.z * a.group) - 1) / a.group;
-    u.hi = (int)min((long long)u.base + a.split, (long long)u.e.y + end_row + 1);
+    u.base = u.split * u.size;
+    const int end_row = by_group(a, min((u.ctile + 1) * COLS, u.e.z * a.group) - 1);
+    u.hi = (int)min((long long)u.base + u.size, (long long)u.e.y + end_row + 1);
 }
 
-__device__ __forceinline__ void walk_enter(const Kv4AttnArgs& a, Kv4Walk& u, int4 e) {
+__device__ __forceinline__ void walk_enter(const Kv4AttnArgs& a, Kv4Walk& u, int4 e, int units) {
     u.e = e;
-    u.splits = (e.y + e.z + a.split - 1) / a.split;
+    u.size = a.split.of((long long)e.y + e.z);
+    u.splits = a.split.parts((long long)e.y + e.z);
+    u.w = (long long)units * a.c.n_kv;
     u.next = __ldcg(a.entries + min(u.entry + 1, a.n - 1));
-}
-
-// The place of work item w (< cu_units[n] * n_kv), found by the whole warp, 32 sequences' first units at a time.
-template <int COLS>
-__device__ __forceinline__ Kv4Walk walk_at(const Kv4AttnArgs& a, long long w, int lane) {
-    Kv4Walk u;
-    int lo = 0, hi = a.n;      // first unit of lo <= w < first unit of hi
-    long long before = 0;
-    while (hi - lo > 1) {
-        const int step = (hi - lo + 31) / 32, at = lo + lane * step;
-        const long long first = at < hi ? (long long)__ldcg(a.cu_units + at) * a.c.n_kv : 0x7fffffffffffffffll;
-        const int k = 31 - __clz(__ballot_sync(0xffffffffu, first <= w));
-        before = __shfl_sync(0xffffffffu, first, k);
-        lo += k * step;
-        hi = min(hi, lo + step);
-    }
-    u.entry = lo;
-    walk_enter(a, u, __ldcg(a.entries + lo));
-    const long long off = w - before;
-    u.split = (int)(off % u.splits);
-    const long long rest = off / u.splits;
-    u.head = (int)(rest % a.c.n_kv);
-    u.ctile = (int)(rest / a.c.n_kv);
-    walk_range<COLS>(a, u);
-    return u;
+    u.next_units = __ldcg(a.cu_units + min(u.entry + 1, a.n - 1));
 }
 
 // To the next unit.
 template <int COLS>
 __device__ __forceinline__ void walk_next(const Kv4AttnArgs& a, Kv4Walk& u) {
+    u.at += a.split.work_of(min(u.size, u.e.y + u.e.z - u.split * u.size));
+    ++u.w;
     if (++u.split == u.splits) {
         u.split = 0;
         if (++u.head == a.c.n_kv) {
@@ -128,13 +115,43 @@ __device__ __forceinline__ void walk_next(const Kv4AttnArgs& a, Kv4Walk& u) {
             if (++u.ctile * COLS >= u.e.z * a.group) {
                 u.ctile = 0;
                 while (++u.entry < a.n) {
-                    walk_enter(a, u, u.next);
+                    walk_enter(a, u, u.next, u.next_units);
                     if (u.e.z) break;
                 }
             }
         }
     }
     walk_range<COLS>(a, u);
+}
+
+// The first unit that has at least `at` work before it (at < the work of all), found by the whole warp, 32 sequences at a time.
+template <int COLS>
+__device__ __forceinline__ Kv4Walk walk_at(const Kv4AttnArgs& a, long long at, int lane) {
+    Kv4Walk u;
+    int lo = 0, hi = a.n;      // work before lo <= at < work before hi
+    long long before = 0;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, i = lo + lane * step;
+        const long long first = i < hi ? (long long)__ldcg(a.cu_work + i) * a.c.n_kv : 0x7fffffffffffffffll;
+        const int k = 31 - __clz(__ballot_sync(0xffffffffu, first <= at));
+        before = __shfl_sync(0xffffffffu, first, k);
+        lo += k * step;
+        hi = min(hi, lo + step);
+    }
+    u.entry = lo;
+    const int4 e = __ldcg(a.entries + lo);
+    walk_enter(a, u, e, __ldcg(a.cu_units + lo));
+    const int one = a.split.work((long long)e.y + e.z), full = a.split.work_of(u.size);     // of a (column tile, head), of a split
+    const long long turn = (at - before) / one;
+    const int into = (int)((at - before) % one);
+    u.split = min((into + full - 1) / full, u.splits - 1);
+    u.head = (int)(turn % a.c.n_kv);
+    u.ctile = (int)(turn / a.c.n_kv);
+    u.w += turn * u.splits + u.split;
+    u.at = before + turn * one + u.split * full;
+    walk_range<COLS>(a, u);
+    if (u.at < at) walk_next<COLS>(a, u);
+    return u;
 }
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -215,19 +232,19 @@ __device__ __forceinline__ void ka_produce(const Kv4AttnArgs& a, const KaRing<NG
     using S = KaShared<NG, COLS>;
     constexpr int HD = NG * KV4_GROUP, KT = S::KT, D = S::STAGES;
     const int tiles = 1 << (a.c.block_shift - 4);     // of a block
-    const long long total = (long long)__ldcg(a.cu_units + a.n) * a.c.n_kv;
-    long long w = total * blockIdx.x / gridDim.x;
-    const long long last = total * (blockIdx.x + 1) / gridDim.x;
+    const long long total = (long long)__ldcg(a.cu_work + a.n) * a.c.n_kv;
+    const long long from = total * blockIdx.x / gridDim.x, last = total * (blockIdx.x + 1) / gridDim.x;
     Kv4Walk u = {};
     int id = 0;     // the lane's tile's block
     auto block_of = [&]() {
         const int pos = u.base + lane * KV4_TILE;
         return lane < KA_WARPS * KT && pos < u.hi ? __ldcg(a.c.table + (size_t)u.e.x * a.c.max_blocks + (pos >> a.c.block_shift)) : 0;
     };
-    bool queries = true, begins = true;
-    if (w < last) {
-        u = walk_at<COLS>(a, w, lane);
-        id = block_of();
+    bool queries = true, begins = true, more = from < last;
+    if (more) {
+        u = walk_at<COLS>(a, from, lane);
+        more = u.at < last && u.entry < a.n;
+        if (more) id = block_of();
     }
     const int run = min(tiles, KA_WARPS * KT);    // tiles that lie behind one another
     for (unsigned k = 0;; ++k) {
@@ -235,7 +252,7 @@ __device__ __forceinline__ void ka_produce(const Kv4AttnArgs& a, const KaRing<NG
         if (k >= D && !bar_wait(ring.empty(s), (k / D - 1) & 1)) { give_up(a.c.flag); return; }
         unsigned char* const stage = ring.smem + s * S::STAGE;
         Kv4Item* const item = reinterpret_cast<Kv4Item*>(stage + S::KV + S::Q);
-        if (w >= last) {
+        if (!more) {
             if (lane == 0) {
                 item->flags = KI_END;
                 bar_arrive(ring.full(s));
@@ -254,7 +271,7 @@ __device__ __forceinline__ void ka_produce(const Kv4AttnArgs& a, const KaRing<NG
             d.flags = (begins ? KI_FIRST : 0) | (ends ? KI_LAST : 0) | (queries ? KI_QUERIES : 0);
             d.start = u.e.y; d.rows = u.e.z; d.row0 = u.e.w;
             d.ctile = u.ctile; d.head = u.head; d.splits = u.splits; d.base = u.base;
-            d.hi = u.hi; d.pad = 0; d.w = w;
+            d.hi = u.hi; d.all = u.e.y + by_group(a, u.ctile * COLS); d.w = u.w;
             *item = d;
             bar_expect(ring.full(s), valid * S::TILE + (queries ? cols * S::QCOL : 0));
         }
@@ -265,7 +282,7 @@ __device__ __forceinline__ void ka_produce(const Kv4AttnArgs& a, const KaRing<NG
             bulk_copy(smem_addr(stage + lane * S::TILE), src, min(run, valid - lane) * S::TILE, ring.full(s));
         }
         if (queries && lane < cols) {     // the heads of a row lie behind one another
-            const int c = u.ctile * COLS + lane, row = c / a.group, in = c % a.group;
+            const int c = u.ctile * COLS + lane, row = by_group(a, c), in = c - row * a.group;
             if (lane == 0 || in == 0)
                 bulk_copy(smem_addr(stage + S::KV + lane * S::QCOL), a.q + (long long)(u.e.w + row) * a.q_stride + (u.head * a.group + in) * HD,
                           min(a.group - in, cols - lane) * S::QCOL, ring.full(s));
@@ -274,12 +291,11 @@ __device__ __forceinline__ void ka_produce(const Kv4AttnArgs& a, const KaRing<NG
         begins = ends;
         u.base += S::KEYS;
         if (ends) {
-            if (++w < last) {
-                walk_next<COLS>(a, u);
-                queries = u.split == 0;
-            }
+            walk_next<COLS>(a, u);
+            more = u.at < last && u.entry < a.n;
+            queries = u.split == 0;
         }
-        if (w < last) id = block_of();
+        if (more) id = block_of();
     }
 }
 
@@ -305,10 +321,10 @@ __device__ __forceinline__ void ka_finish(const Kv4AttnArgs& a, const KaRing<NG,
         }
         if (d.splits == 1) {
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            const int c = d.ctile * COLS + col;
+            const int c = d.ctile * COLS + col, row = by_group(a, c);
             __nv_bfloat162 lo2 = __floats2bfloat162_rn(o.x * inv, o.y * inv), hi2 = __floats2bfloat162_rn(o.z * inv, o.w * inv);
             uint2 v = make_uint2(*reinterpret_cast<uint32_t*>(&lo2), *reinterpret_cast<uint32_t*>(&hi2));
-            *reinterpret_cast<uint2*>(a.out + (long long)(d.row0 + c / a.group) * a.out_stride + (d.head * a.group + c % a.group) * HD + dim) = v;
+            *reinterpret_cast<uint2*>(a.out + (long long)(d.row0 + row) * a.out_stride + (d.head * a.group + c - row * a.group) * HD + dim) = v;
         } else {
             *reinterpret_cast<float4*>(a.acc + (size_t)(d.w * COLS + col) * HD + dim) = o;
             if (dim == 0) a.ml[d.w * COLS + col] = make_float2(best, sum);
@@ -375,7 +391,7 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn(const Kv4AttnArgs 
                 for (int j = 0; j < 2; ++j) {
                     const int c2 = nt * 8 + 2 * t + j;
                     factor[nt][j] = __shfl_sync(0xffffffffu, f, (2 * t + j) * 4);
-                    limit[nt][j] = c2 < cols ? d.start + (d.ctile * COLS + c2) / a.group : -1;
+                    limit[nt][j] = c2 < cols ? d.start + by_group(a, d.ctile * COLS + c2) : -1;
                 }
             }
         }
@@ -388,11 +404,12 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn(const Kv4AttnArgs 
                 for (int i = 0; i < 2 * NG; ++i) acc[nt][i][0] = acc[nt][i][1] = acc[nt][i][2] = acc[nt][i][3] = 0.f;
             }
         }
-        const int base = d.base + warp * (KT * KV4_TILE);
-        const int nk = min(KT, (d.hi - base + KV4_TILE - 1) / KV4_TILE);    // tiles that are there
+        const int base = d.base + warp * KV4_TILE;                          // a warp takes every fourth tile
+        const int nk = min(KT, ((d.hi - base + KV4_TILE - 1) / KV4_TILE + KA_WARPS - 1) / KA_WARPS);    // tiles that are there
         if (nk > 0) {
-            const unsigned char* const mine = stage + warp * (KT * S::TILE);
-            const bool whole = base + KT * KV4_TILE - 1 <= d.start + d.ctile * COLS / a.group;   // every column sees all of them
+            constexpr int NEXT = KA_WARPS * S::TILE;
+            const unsigned char* const mine = stage + warp * S::TILE;
+            const bool whole = d.base + S::KEYS - 1 <= d.all;   // every column sees all of them
             float sc[KT][NT][4];
 #pragma unroll
             for (int k2 = 0; k2 < KT; ++k2) {
@@ -401,7 +418,7 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn(const Kv4AttnArgs 
                 if (k2 < nk) {
 #pragma unroll
                     for (int i = 0; i < NG; ++i) {
-                        const unsigned char* p = mine + k2 * S::TILE + i * KV4_GT;
+                        const unsigned char* p = mine + k2 * NEXT + i * KV4_GT;
                         const uint2 code = *reinterpret_cast<const uint2*>(p + lane * 8);
                         const uint2 par = *reinterpret_cast<const uint2*>(p + KV4_KPAR + g * 8);
                         uint32_t x[4], y[4];
@@ -422,7 +439,7 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn(const Kv4AttnArgs 
                     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            if (base + k2 * 16 + g + (j >> 1) * 8 > limit[nt][j & 1]) sc[k2][nt][j] = -INFINITY;
+                            if (base + k2 * (KA_WARPS * 16) + g + (j >> 1) * 8 > limit[nt][j & 1]) sc[k2][nt][j] = -INFINITY;
                     }
                 }
             }
@@ -479,7 +496,7 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn(const Kv4AttnArgs 
                 if (k2 < nk) {
 #pragma unroll
                     for (int i = 0; i < NG; ++i) {
-                        const unsigned char* q = mine + k2 * S::TILE + i * KV4_GT;
+                        const unsigned char* q = mine + k2 * NEXT + i * KV4_GT;
                         const uint2 code = *reinterpret_cast<const uint2*>(q + KV4_VCODE + lane * 8);
                         const uint4 par = *reinterpret_cast<const uint4*>(q + KV4_VPAR + t * 16);   // of keys 2t, 2t+8, 2t+1, 2t+9
                         const __half2 s0 = as_h2(__byte_perm(par.x, par.z, 0x5410)), z0 = as_h2(__byte_perm(par.x, par.z, 0x7632));
@@ -530,19 +547,17 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn(const Kv4AttnArgs 
     }
 }
 
-// m16n8k32, bytes in, 32-bit sums out: D += A B, the codes A always unsigned.
+// m16n8k32, bytes in, 32-bit sums out: D = A B + C, the codes A always unsigned.
+#define KA_MMA8(types)                                                                                                              \
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32." types ".s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"    \
+                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])                                                                     \
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c0), "r"(c1), "r"(c2), "r"(c3))
 template <bool SIGNED>
-__device__ __forceinline__ void mma16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    if constexpr (SIGNED)
-        asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    else
-        asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, int c0, int c1, int c2, int c3) {
+    if constexpr (SIGNED) KA_MMA8("u8.s8");
+    else KA_MMA8("u8.u8");
 }
-// Sums that start as the bits of 1.5 * 2^23 are that float plus the sum (below 2^22 in magnitude), bit for bit.
-constexpr int KA_ORIGIN = 0x4B400000;
-__device__ __forceinline__ float from_origin(int x) { return __int_as_float(x) - 12582912.f; }
+#undef KA_MMA8
 
 // Form for a few columns (single tokens): what bounds it is the arithmetic a stored byte costs, not the tensor cores, so the codes enter
 // the products as they are, as bytes: three logic operations for eight codes, where their f16 values take thirteen instructions, half of
@@ -552,14 +567,22 @@ __device__ __forceinline__ float from_origin(int x) { return __int_as_float(x) -
 // A query column, times a power of two, is a 15-bit whole number: exact for elements down to 2^-6 of the largest, the others to 2^-14 of
 // it.  The weights times the value scales are 16-bit whole numbers in units of 2^-16 of the largest value scale among the warp's positions
 // (half a unit off, each on its own, a quarter of what bf16 weights would be off at one position and less the more there are).  Both are
-// cut into two bytes that take two of the 8 columns of a product, so a product holds four queries.  The tensor cores' sums are exact;
-// what is added to them, statistics and outputs, is fp32.
-// Measured (B200, 256 sequences of 512 to 2048 positions, 16 query and 8 key heads of 64): see the table of forms in kv4.cu.
-template <int NG, int NT>
+// cut into two bytes that take two of the 8 columns of a product.  The tensor cores' sums are exact; what is added to them, statistics and
+// outputs, is fp32.
+// A product's columns hold four queries; or (HALVES, for up to two queries a tile, heads of 64 and 128) two queries twice, once for the
+// even groups of 32 elements and once for the odd ones, zeros elsewhere: a lane then has one group of two to scale and to weigh.
+constexpr int KA_ORIGIN = 0x4B400000;   // sums that start as the bits of 1.5 * 2^23 are that float plus the sum (below 2^22 in magnitude)
+__device__ __forceinline__ float two_bytes(int high, int low) {
+    return fmaf(__int_as_float(high) - 12582912.f, 256.f, __int_as_float(low) - 12582912.f);
+}
+
+template <int NG, int NT, bool HALVES>
 __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn_few(const Kv4AttnArgs a) {
-    constexpr int HD = NG * KV4_GROUP, COLS = NT * 4;
+    static_assert(!HALVES || (NT == 1 && NG % 2 == 0), "two halves of an even number of groups");
+    constexpr int HD = NG * KV4_GROUP, COLS = HALVES ? 2 : NT * 4;
+    constexpr int OWN = HALVES ? NG / 2 : NG, SIDES = HALVES ? 2 : 1;      // groups that a lane scales; group i * SIDES + side
     using S = KaShared<NG, COLS>;
-    constexpr int KT = S::KT, D = S::STAGES;
+    constexpr int KT = S::KT, D = S::STAGES, NEXT = KA_WARPS * S::TILE;
     extern __shared__ __align__(128) unsigned char smem[];
     const KaRing<NG, COLS> ring(smem);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -568,23 +591,27 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn_few(const Kv4AttnA
     pdl_launch();
     if (warp == KA_WARPS) return ka_produce<NG, COLS>(a, ring, lane);
 
+    const int side = HALVES ? t & 1 : 0, query = HALVES ? t >> 1 : t;
     const uint32_t pick = g & 1 ? 0x6240 : 0x7351;      // low or high bytes of four 16-bit weights, in the order of a word's keys
-    uint32_t qf[NT][NG][2];         // bytes of column g: query g / 2, high byte (even g) or low byte
-    float qsum[NT][NG], factor[NT]; // of query t, as all below
+    uint32_t qf[NT][NG][2];         // bytes of column g: high byte (even g) or low byte of its query
+    float qsum[NT][OWN], factor[NT];  // of the lane's query, as all below
     int limit[NT];                  // last position that it sees
-    float acc[NT][2 * NG][2], zsum[NT][NG], m[NT], l[NT];
+    float acc[NT][2 * OWN][2], zsum[NT][OWN], m[NT], l[NT];
     unsigned merged = 0;
     for (unsigned k = 0;; ++k) {
         const int s = k % D;
         if (!bar_wait(ring.full(s), (k / D) & 1)) { give_up(a.c.flag); return; }
         const unsigned char* const stage = ring.smem + s * S::STAGE;
-        const Kv4Item d = *reinterpret_cast<const Kv4Item*>(stage + S::KV + S::Q);
-        if (d.flags & KI_END) return;
-        const int cols = d.rows * a.group - d.ctile * COLS;                 // valid ones of this tile, if fewer than COLS
-        if (d.flags & KI_QUERIES) {
+        const Kv4Item& d = *reinterpret_cast<const Kv4Item*>(stage + S::KV + S::Q);
+        const int flags = d.flags, base = d.base + warp * KV4_TILE;         // a warp takes every fourth tile
+        if (flags & KI_END) return;
+        const int left = d.hi - base;
+        const bool whole = d.base + S::KEYS - 1 <= d.all;                   // every column sees all of the stage
+        if (flags & KI_QUERIES) {
+            const int cols = d.rows * a.group - d.ctile * COLS;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                const int col = nt * 4 + (g >> 1);
+                const int col = HALVES ? g >> 2 : nt * 4 + (g >> 1);
                 uint4 raw[NG];
                 uint32_t big = 0;
 #pragma unroll
@@ -612,56 +639,74 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn_few(const Kv4AttnA
                     }
                     qf[nt][i][0] = v[0] | v[4] << 8 | v[1] << 16 | v[5] << 24;      // the order of a key word's low nibbles
                     qf[nt][i][1] = v[2] | v[6] << 8 | v[3] << 16 | v[7] << 24;      // and of its high ones
+                    if (HALVES && (g >> 1 & 1) != (i & 1)) qf[nt][i][0] = qf[nt][i][1] = 0;
                     part += __shfl_xor_sync(0xffffffffu, part, 1);
                     part += __shfl_xor_sync(0xffffffffu, part, 2);
                     total[i] = (float)part;
                 }
                 // a masked score times the factor has to stay -inf, and a query that is not finite makes all its weights NaN
                 const float f = big >= 0x7f80u ? __int_as_float(0x7fffffff) : fmaxf(a.scale_log2 * up * (1.f / 8192.f), 1e-37f);
-                factor[nt] = __shfl_sync(0xffffffffu, f, t * 8);
+                const int from = HALVES ? query * 16 : t * 8;        // a lane of the query's columns
+                factor[nt] = __shfl_sync(0xffffffffu, f, from);
 #pragma unroll
-                for (int i = 0; i < NG; ++i) qsum[nt][i] = __shfl_sync(0xffffffffu, total[i], t * 8);
-                const int mine = nt * 4 + t;
-                limit[nt] = mine < cols ? d.start + (d.ctile * COLS + mine) / a.group : -1;
+                for (int i = 0; i < OWN; ++i) {
+                    qsum[nt][i] = __shfl_sync(0xffffffffu, total[i * SIDES], from);
+                    if constexpr (HALVES) {
+                        const float other = __shfl_sync(0xffffffffu, total[i * SIDES + 1], from);
+                        if (side) qsum[nt][i] = other;
+                    }
+                }
+                const int mine = nt * 4 + query;
+                limit[nt] = mine < cols ? d.start + by_group(a, d.ctile * COLS + mine) : -1;
             }
         }
-        if (d.flags & KI_FIRST) {
+        if (flags & KI_FIRST) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 m[nt] = -INFINITY;
                 l[nt] = factor[nt] * 0.f;
 #pragma unroll
-                for (int i = 0; i < NG; ++i) zsum[nt][i] = 0.f;
+                for (int i = 0; i < OWN; ++i) zsum[nt][i] = 0.f;
 #pragma unroll
-                for (int i = 0; i < 2 * NG; ++i) acc[nt][i][0] = acc[nt][i][1] = 0.f;
+                for (int i = 0; i < 2 * OWN; ++i) acc[nt][i][0] = acc[nt][i][1] = 0.f;
             }
         }
-        const int base = d.base + warp * (KT * KV4_TILE);
-        const int nk = min(KT, (d.hi - base + KV4_TILE - 1) / KV4_TILE);    // tiles that are there
-        if (nk > 0) {
-            const unsigned char* const mine = stage + warp * (KT * S::TILE);
-            const bool whole = base + KT * KV4_TILE - 1 <= d.start + d.ctile * COLS / a.group;   // every column sees all of them
+        if (left > 0) {
+            const unsigned char* const mine = stage + warp * S::TILE;
+            auto there = [&](int k2) { return k2 * (KA_WARPS * KV4_TILE) < left; };     // whether the warp has a tile number k2
             float sc[KT][NT][2];      // scores of keys g and g + 8 of every tile, then weights
 #pragma unroll
             for (int k2 = 0; k2 < KT; ++k2) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) sc[k2][nt][0] = sc[k2][nt][1] = 0.f;
-                if (k2 < nk) {
+                if (there(k2)) {
 #pragma unroll
-                    for (int i = 0; i < NG; ++i) {
-                        const unsigned char* p = mine + k2 * S::TILE + i * KV4_GT;
-                        const uint2 code = *reinterpret_cast<const uint2*>(p + lane * 8);
-                        const uint2 par = *reinterpret_cast<const uint2*>(p + KV4_KPAR + g * 8);
+                    for (int i = 0; i < OWN; ++i) {
+                        const unsigned char* const p = mine + k2 * NEXT + i * SIDES * KV4_GT;
+                        const uint2 par = *reinterpret_cast<const uint2*>(p + side * KV4_GT + KV4_KPAR + g * 8);
                         const float2 p0 = __half22float2(as_h2(par.x)), p1 = __half22float2(as_h2(par.y));     // scale, zero
-                        const uint32_t a0 = code.x & 0x0f0f0f0fu, a1 = code.y & 0x0f0f0f0fu;
-                        const uint32_t a2 = code.x >> 4 & 0x0f0f0f0fu, a3 = code.y >> 4 & 0x0f0f0f0fu;
+                        int x[NT][4];
+#pragma unroll
+                        for (int j = 0; j < SIDES; ++j) {
+                            const uint2 code = *reinterpret_cast<const uint2*>(p + j * KV4_GT + lane * 8);
+                            const uint32_t a0 = code.x & 0x0f0f0f0fu, a1 = code.y & 0x0f0f0f0fu;
+                            const uint32_t a2 = code.x >> 4 & 0x0f0f0f0fu, a3 = code.y >> 4 & 0x0f0f0f0fu;
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                const uint32_t* const q = qf[nt][i * SIDES + j];
+                                if (j == 0) mma16832<true>(x[nt], a0, a1, a2, a3, q[0], q[1], KA_ORIGIN, KA_ORIGIN, KA_ORIGIN, KA_ORIGIN);
+                                else mma16832<true>(x[nt], a0, a1, a2, a3, q[0], q[1], x[nt][0], x[nt][1], x[nt][2], x[nt][3]);
+                            }
+                        }
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            int x[4] = {KA_ORIGIN, KA_ORIGIN, KA_ORIGIN, KA_ORIGIN};
-                            mma16832<true>(x, a0, a1, a2, a3, qf[nt][i][0], qf[nt][i][1]);
-                            sc[k2][nt][0] = fmaf(p0.x, fmaf(from_origin(x[0]), 256.f, from_origin(x[1])), fmaf(p0.y, qsum[nt][i], sc[k2][nt][0]));
-                            sc[k2][nt][1] = fmaf(p1.x, fmaf(from_origin(x[2]), 256.f, from_origin(x[3])), fmaf(p1.y, qsum[nt][i], sc[k2][nt][1]));
+                            sc[k2][nt][0] = fmaf(p0.x, two_bytes(x[nt][0], x[nt][1]), fmaf(p0.y, qsum[nt][i], sc[k2][nt][0]));
+                            sc[k2][nt][1] = fmaf(p1.x, two_bytes(x[nt][2], x[nt][3]), fmaf(p1.y, qsum[nt][i], sc[k2][nt][1]));
                         }
+                    }
+                    if constexpr (HALVES) {
+                        sc[k2][0][0] += __shfl_xor_sync(0xffffffffu, sc[k2][0][0], 1);
+                        sc[k2][0][1] += __shfl_xor_sync(0xffffffffu, sc[k2][0][1], 1);
                     }
                 }
             }
@@ -670,8 +715,8 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn_few(const Kv4AttnA
                 for (int k2 = 0; k2 < KT; ++k2) {
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        if (base + k2 * 16 + g > limit[nt]) sc[k2][nt][0] = -INFINITY;
-                        if (base + k2 * 16 + g + 8 > limit[nt]) sc[k2][nt][1] = -INFINITY;
+                        if (base + k2 * (KA_WARPS * KV4_TILE) + g > limit[nt]) sc[k2][nt][0] = -INFINITY;
+                        if (base + k2 * (KA_WARPS * KV4_TILE) + g + 8 > limit[nt]) sc[k2][nt][1] = -INFINITY;
                     }
                 }
             }
@@ -683,16 +728,16 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn_few(const Kv4AttnA
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                 top *= factor[nt];
-                if (d.flags & KI_FIRST) {
+                if (flags & KI_FIRST) {
                     m[nt] = top;
                 } else if (__any_sync(0xffffffffu, top > m[nt])) {
                     const float best = fmaxf(m[nt], top), old = best == -INFINITY ? 1.f : ex2(m[nt] - best);
                     m[nt] = best;
                     l[nt] *= old;
 #pragma unroll
-                    for (int i = 0; i < NG; ++i) zsum[nt][i] *= old;
+                    for (int i = 0; i < OWN; ++i) zsum[nt][i] *= old;
 #pragma unroll
-                    for (int i = 0; i < 2 * NG; ++i) { acc[nt][i][0] *= old; acc[nt][i][1] *= old; }
+                    for (int i = 0; i < 2 * OWN; ++i) { acc[nt][i][0] *= old; acc[nt][i][1] *= old; }
                 }
                 const float less = m[nt] == -INFINITY ? 0.f : -m[nt];       // nothing seen yet: weights of exp(-inf) = 0
 #pragma unroll
@@ -705,16 +750,16 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn_few(const Kv4AttnA
                 }
             }
             // value scales, and the largest of each group
-            float vs[KT][NG][2], unit[NG];
+            float vs[KT][OWN][2], unit[OWN], units[OWN];
 #pragma unroll
-            for (int i = 0; i < NG; ++i) unit[i] = 0.f;
+            for (int i = 0; i < OWN; ++i) unit[i] = 0.f;
 #pragma unroll
             for (int k2 = 0; k2 < KT; ++k2) {
 #pragma unroll
-                for (int i = 0; i < NG; ++i) {
+                for (int i = 0; i < OWN; ++i) {
                     vs[k2][i][0] = vs[k2][i][1] = 0.f;
-                    if (k2 < nk) {
-                        const uint2 par = *reinterpret_cast<const uint2*>(mine + k2 * S::TILE + i * KV4_GT + KV4_VPAR + g * 8);
+                    if (there(k2)) {
+                        const uint2 par = *reinterpret_cast<const uint2*>(mine + k2 * NEXT + (i * SIDES + side) * KV4_GT + KV4_VPAR + g * 8);
                         const float2 p0 = __half22float2(as_h2(par.x)), p1 = __half22float2(as_h2(par.y));
                         vs[k2][i][0] = p0.x;
                         vs[k2][i][1] = p1.x;
@@ -724,43 +769,55 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn_few(const Kv4AttnA
                     }
                 }
             }
-            float units[NG];
 #pragma unroll
-            for (int i = 0; i < NG; ++i) {
-                unit[i] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(unit[i])));
+            for (int i = 0; i < OWN; ++i) {
+                if constexpr (HALVES) {
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) unit[i] = fmaxf(unit[i], __shfl_xor_sync(0xffffffffu, unit[i], o));
+                } else {
+                    unit[i] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(unit[i])));
+                }
                 units[i] = unit[i] > 0.f ? __fdividef(65280.f, unit[i]) : 0.f;
                 unit[i] *= 1.f / 65280.f;
             }
 #pragma unroll
             for (int k2 = 0; k2 < KT; ++k2) {
 #pragma unroll
-                for (int i = 0; i < NG; ++i) { vs[k2][i][0] *= units[i]; vs[k2][i][1] *= units[i]; }
+                for (int i = 0; i < OWN; ++i) { vs[k2][i][0] *= units[i]; vs[k2][i][1] *= units[i]; }
             }
 #pragma unroll
-            for (int i = 0; i < NG; ++i) {
-                int x[NT][2][4];
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) x[nt][0][j] = x[nt][1][j] = KA_ORIGIN;
-                }
+            for (int i = 0; i < OWN; ++i) {
+                int x[NT][SIDES][2][4];
 #pragma unroll
                 for (int k2 = 0; k2 < KT; k2 += 2) {
-                    if (k2 < nk) {       // of a second tile that is not there the weights are 0
-                        const uint2 first = *reinterpret_cast<const uint2*>(mine + k2 * S::TILE + i * KV4_GT + KV4_VCODE + lane * 8);
-                        const uint2 second = *reinterpret_cast<const uint2*>(mine + (k2 + 1) * S::TILE + i * KV4_GT + KV4_VCODE + lane * 8);
+                    if (k2 == 0 || there(k2)) {       // of a second tile that is not there the weights are 0
+                        uint32_t b[NT][2];
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            uint32_t b[2];
 #pragma unroll
                             for (int j = 0; j < 2; ++j) {
                                 // the nearest whole number in the low 16 bits, twice over, for the columns of both bytes
                                 const uint32_t w0 = __float_as_uint(fmaf(sc[k2 + j][nt][0], vs[k2 + j][i][0], 8388608.f));
                                 const uint32_t w8 = __float_as_uint(fmaf(sc[k2 + j][nt][1], vs[k2 + j][i][1], 8388608.f));
-                                b[j] = __byte_perm(movmatrix(__byte_perm(w0, 0, 0x1010)), movmatrix(__byte_perm(w8, 0, 0x1010)), pick);
+                                b[nt][j] = __byte_perm(movmatrix(__byte_perm(w0, 0, 0x1010)), movmatrix(__byte_perm(w8, 0, 0x1010)), pick);
                             }
-                            mma16832<false>(x[nt][0], first.x & 0x0f0f0f0fu, first.x >> 4 & 0x0f0f0f0fu, second.x & 0x0f0f0f0fu, second.x >> 4 & 0x0f0f0f0fu, b[0], b[1]);
-                            mma16832<false>(x[nt][1], first.y & 0x0f0f0f0fu, first.y >> 4 & 0x0f0f0f0fu, second.y & 0x0f0f0f0fu, second.y >> 4 & 0x0f0f0f0fu, b[0], b[1]);
+                        }
+#pragma unroll
+                        for (int j = 0; j < SIDES; ++j) {
+                            const unsigned char* const p = mine + k2 * NEXT + (i * SIDES + j) * KV4_GT + KV4_VCODE + lane * 8;
+                            const uint2 c0 = *reinterpret_cast<const uint2*>(p), c1 = *reinterpret_cast<const uint2*>(p + NEXT);
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                // elements in the high nibbles come out 16 times as large
+                                int(&y)[4] = x[nt][j][0], (&z)[4] = x[nt][j][1];
+                                if (k2 == 0) {
+                                    mma16832<false>(y, c0.x & 0x0f0f0f0fu, c0.x & 0xf0f0f0f0u, c1.x & 0x0f0f0f0fu, c1.x & 0xf0f0f0f0u, b[nt][0], b[nt][1], KA_ORIGIN, KA_ORIGIN, KA_ORIGIN, KA_ORIGIN);
+                                    mma16832<false>(z, c0.y & 0x0f0f0f0fu, c0.y & 0xf0f0f0f0u, c1.y & 0x0f0f0f0fu, c1.y & 0xf0f0f0f0u, b[nt][0], b[nt][1], KA_ORIGIN, KA_ORIGIN, KA_ORIGIN, KA_ORIGIN);
+                                } else {
+                                    mma16832<false>(y, c0.x & 0x0f0f0f0fu, c0.x & 0xf0f0f0f0u, c1.x & 0x0f0f0f0fu, c1.x & 0xf0f0f0f0u, b[nt][0], b[nt][1], y[0], y[1], y[2], y[3]);
+                                    mma16832<false>(z, c0.y & 0x0f0f0f0fu, c0.y & 0xf0f0f0f0u, c1.y & 0x0f0f0f0fu, c1.y & 0xf0f0f0f0u, b[nt][0], b[nt][1], z[0], z[1], z[2], z[3]);
+                                }
+                            }
                         }
                     }
                 }
@@ -768,37 +825,46 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn_few(const Kv4AttnA
                 for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        acc[nt][2 * i + j][0] = fmaf(unit[i], fmaf(from_origin(x[nt][j][0]), 256.f, from_origin(x[nt][j][1])), acc[nt][2 * i + j][0]);
-                        acc[nt][2 * i + j][1] = fmaf(unit[i], fmaf(from_origin(x[nt][j][2]), 256.f, from_origin(x[nt][j][3])), acc[nt][2 * i + j][1]);
+                        int y[4];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) y[r] = HALVES && side ? x[nt][SIDES - 1][j][r] : x[nt][0][j][r];
+                        acc[nt][2 * i + j][0] = fmaf(unit[i], two_bytes(y[0], y[1]), acc[nt][2 * i + j][0]);
+                        acc[nt][2 * i + j][1] = fmaf(unit[i] * 0.0625f, two_bytes(y[2], y[3]), acc[nt][2 * i + j][1]);
                     }
                 }
             }
         }
+        if (!(flags & KI_LAST)) {
+            __syncwarp();
+            if (lane == 0) bar_arrive(ring.empty(s));
+            continue;
+        }
+        const Kv4Item last = d;
         __syncwarp();
         if (lane == 0) bar_arrive(ring.empty(s));
-        if (!(d.flags & KI_LAST)) continue;
+        const int cols = last.rows * a.group - last.ctile * COLS;           // valid ones of this tile, if fewer than COLS
         if (merged && !bar_wait(ring.acc_empty(), (merged - 1) & 1)) { give_up(a.c.flag); return; }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const int col = nt * 4 + t;
+            const int col = nt * 4 + query;
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) {
                 l[nt] += __shfl_xor_sync(0xffffffffu, l[nt], o);
 #pragma unroll
-                for (int i = 0; i < NG; ++i) zsum[nt][i] += __shfl_xor_sync(0xffffffffu, zsum[nt][i], o);
+                for (int i = 0; i < OWN; ++i) zsum[nt][i] += __shfl_xor_sync(0xffffffffu, zsum[nt][i], o);
             }
             if (col < cols) {
-                if (g == 0) ring.ml[warp * COLS + col] = make_float2(m[nt], l[nt]);
+                if (g == 0 && side == 0) ring.ml[warp * COLS + col] = make_float2(m[nt], l[nt]);
 #pragma unroll
-                for (int i = 0; i < NG; ++i)
-                    *reinterpret_cast<float4*>(ring.acc + (warp * COLS + col) * (HD + 4) + i * KV4_GROUP + 4 * g) =
+                for (int i = 0; i < OWN; ++i)
+                    *reinterpret_cast<float4*>(ring.acc + (warp * COLS + col) * (HD + 4) + (i * SIDES + side) * KV4_GROUP + 4 * g) =
                         make_float4(acc[nt][2 * i][0] + zsum[nt][i], acc[nt][2 * i][1] + zsum[nt][i], acc[nt][2 * i + 1][0] + zsum[nt][i], acc[nt][2 * i + 1][1] + zsum[nt][i]);
             }
         }
         __syncwarp();
         if (lane == 0) bar_arrive(ring.acc_full());
         if (!bar_wait(ring.acc_full(), merged & 1)) { give_up(a.c.flag); return; }
-        ka_finish<NG, COLS>(a, ring, d, cols);
+        ka_finish<NG, COLS>(a, ring, last, cols);
         __syncwarp();
         if (lane == 0) bar_arrive(ring.acc_empty());
         ++merged;
@@ -823,9 +889,9 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) k_kv4_merge(con
     if (entry < 0) return;
     const int4 e = __ldcg(a.entries + entry);
     const long long unit = __ldcg(a.cu_units + entry);
-    const int all = (e.y + e.z + a.split - 1) / a.split;
+    const int all = a.split.parts((long long)e.y + e.z);
     if (all == 1) return;
-    const int own = (e.y + row - e.w) / a.split + 1;        // splits that the row sees
+    const int own = (e.y + row - e.w) / a.split.of((long long)e.y + e.z) + 1;        // splits that the row sees
     const int c = (row - e.w) * a.group + head % a.group;
     const long long w = unit * a.c.n_kv + ((long long)(c / cols) * a.c.n_kv + kv) * all;
     const float2* ml = a.ml + w * cols + c % cols;

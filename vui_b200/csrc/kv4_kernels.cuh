@@ -48,13 +48,24 @@ struct Kv4Cache {
     int n_kv, block_shift, n_blocks, max_seqs, max_blocks;
 };
 
+// Positions of a split of attention's work: by the length of the sequence alone, so that a row's bits do not depend on what else is there.
+struct Kv4Split {
+    int up_to_1024, beyond;
+    bool weigh;      // units count for what they cost: their positions by 64, and one more
+    __host__ __device__ int of(long long len) const { return len > 1024 ? beyond : up_to_1024; }
+    __host__ __device__ int parts(long long len) const { const int s = of(len); return (int)((len + s - 1) / s); }
+    __host__ __device__ int work(long long len) const { return parts(len) + (weigh ? (int)((len + 63) / 64) : 0); }     // of all parts
+    __host__ __device__ int work_of(int positions) const { return 1 + (weigh ? (positions + 63) / 64 : 0); }            // of one
+};
+
 // ------------------------------------------------------------------------------------------------ tables and maps
 struct Kv4PlanArgs {
     Kv4Cache c;
     const int32_t* slots; const int32_t* new_lens; const int32_t* at;
     int n, n_rows, max_new;
-    int group, cols, split;     // query heads a kv head, columns of a tile, positions of a split: attention's units are counted here
-    int4* entries; int32_t* cu_units; int32_t* cu_tiles; int32_t* row_entry;    // the plan's work array
+    int group, cols;            // query heads a kv head, columns of a tile: attention's units are counted here
+    Kv4Split split;
+    int4* entries; int32_t* cu_units; int32_t* cu_work; int32_t* cu_tiles; int32_t* row_entry;    // the plan's work array
     int32_t* cu_rows; int32_t* row_slot; int32_t* row_pos; long long* slot_map;
 };
 
@@ -120,7 +131,7 @@ __device__ __forceinline__ int find_in(const int* first, int n, int x) {
 // rows and blocks many.  Latency bound: three dependent reads (entry, length, table) and five barriers.
 __global__ void __launch_bounds__(1024) k_kv4_plan(const Kv4PlanArgs a) {
     extern __shared__ int sm[];
-    __shared__ int scan_a[1][32], scan_b[2][32], scan_c[4][32];
+    __shared__ int scan_a[1][32], scan_b[2][32], scan_c[5][32];
     const int n = a.n, per = (n + blockDim.x - 1) / blockDim.x;
     int* s_slot = sm;               // n each; slot -1: takes no part
     int* s_start = s_slot + n;
@@ -189,8 +200,10 @@ __global__ void __launch_bounds__(1024) k_kv4_plan(const Kv4PlanArgs a) {
     }
     block_scan<2>(blocks, scan_b, sum);
     const int dropped = sum[0], top = n_free + dropped;
-    int part[4] = {0, 0, 0, 0}, whole[4];   // blocks got, rows, units of attention (of a kv head), tiles of 16 positions written
-    auto units_of = [&](int i) { return s_new[i] ? (int)min(((long long)s_new[i] * a.group + a.cols - 1) / a.cols * ((s_start[i] + (long long)s_new[i] + a.split - 1) / a.split), (long long)KV4_MANY) : 0; };
+    int part[5] = {0, 0, 0, 0, 0}, whole[5];   // blocks got, rows, units of attention (of a kv head) and their work, tiles of 16 positions written
+    auto times_tiles = [&](int i, int of_one) { return (int)min(((long long)s_new[i] * a.group + a.cols - 1) / a.cols * of_one, (long long)KV4_MANY); };
+    auto units_of = [&](int i) { return s_new[i] ? times_tiles(i, a.split.parts(s_start[i] + (long long)s_new[i])) : 0; };
+    auto work_of = [&](int i) { return s_new[i] ? times_tiles(i, a.split.work(s_start[i] + (long long)s_new[i])) : 0; };
     auto tiles_of = [&](int i) { return s_new[i] ? ((s_start[i] + s_new[i] - 1) >> 4) - (s_start[i] >> 4) + 1 : 0; };
     for (int i = first; i < last; ++i) {
         s_drop[i] = blocks[0];
@@ -205,11 +218,12 @@ __global__ void __launch_bounds__(1024) k_kv4_plan(const Kv4PlanArgs a) {
         }
         part[1] += s_new[i];
         part[2] = min(part[2] + units_of(i), KV4_MANY);
-        part[3] += tiles_of(i);
+        part[3] = min(part[3] + work_of(i), KV4_MANY);
+        part[4] += tiles_of(i);
     }
-    block_scan<4>(part, scan_c, whole);
+    block_scan<5>(part, scan_c, whole);
     const int grown = whole[0], rows = whole[1];
-    int units = part[2], tiles = part[3];
+    int units = part[2], work = part[3], tiles = part[4];
     for (int i = first; i < last; ++i) {
         s_grow[i] = part[0];
         s_cu[i] = part[1];
@@ -225,12 +239,15 @@ __global__ void __launch_bounds__(1024) k_kv4_plan(const Kv4PlanArgs a) {
             *a.c.n_free = top - grown;
             a.cu_rows[n] = rows;
             a.cu_units[n] = whole[2];
-            a.cu_tiles[n] = whole[3];
+            a.cu_work[n] = whole[3];
+            a.cu_tiles[n] = whole[4];
         }
         for (int i = first; i < last; ++i) {
             a.cu_units[i] = units;
+            a.cu_work[i] = work;
             a.cu_tiles[i] = tiles;
             units = min(units + units_of(i), KV4_MANY);
+            work = min(work + work_of(i), KV4_MANY);
             tiles += tiles_of(i);
             a.cu_rows[i] = s_cu[i];
             a.entries[i] = make_int4(s_slot[i], s_start[i], s_new[i], s_cu[i]);

@@ -36,7 +36,7 @@ class Kv4Plan:
 
     def __init__(self, device, n_seqs: int, n_rows: int, max_new: int):
         self.n_seqs, self.n_rows, self.max_new = n_seqs, n_rows, max_new
-        work = (6 * n_seqs + 2 + n_rows + 3) & ~3          # the parts behind it: 16-byte aligned
+        work = (7 * n_seqs + 3 + n_rows + 3) & ~3          # the parts behind it: 16-byte aligned
         row = (n_rows + 3) & ~3
         # one allocation: work, slot_map (int64), row_slot, row_pos, cu_rows
         self._ints = ints = torch.empty(work + 4 * row + n_seqs + 1, dtype=torch.int32, device=device)
