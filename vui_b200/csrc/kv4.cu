@@ -77,10 +77,7 @@ Shape shape_of(const VuibKv4* c, const VuibKv4Plan* p) {
     s.nt = s.few ? (most <= 4 ? 1 : most <= 8 ? 2 : 4) : c->ng > 2 ? 2 : 4;
     s.halves = most <= 2 && c->ng != 3;
     s.cols = s.halves ? 2 : (s.few ? 4 : 8) * s.nt;
-#ifndef KV4_LONG
-#define KV4_LONG 512
-#endif
-    s.split = {256, KV4_LONG, true};
+    s.split = {256, 512, true};
     if (!s.few) {
         const long long tiles = ceil_div((long long)p->n_rows * group, s.cols) + p->n_seqs;
         const long long len = (long long)c->cfg.max_blocks << c->block_shift;

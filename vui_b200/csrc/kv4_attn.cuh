@@ -124,34 +124,50 @@ __device__ __forceinline__ void walk_next(const Kv4AttnArgs& a, Kv4Walk& u) {
     walk_range<COLS>(a, u);
 }
 
-// The first unit that has at least `at` work before it (at < the work of all), found by the whole warp, 32 sequences at a time.
+// A CTA's share [from, to) of all work, and the first unit that has at least `from` work before it, found by the whole warp, 32 sequences
+// at a time.  The sequences' places are read along with their work, so that n up to 32 take one read of the L2 and up to 1024 two.
 template <int COLS>
-__device__ __forceinline__ Kv4Walk walk_at(const Kv4AttnArgs& a, long long at, int lane) {
-    Kv4Walk u;
-    int lo = 0, hi = a.n;      // work before lo <= at < work before hi
-    long long before = 0;
-    while (hi - lo > 1) {
+__device__ __forceinline__ bool walk_begin(const Kv4AttnArgs& a, Kv4Walk& u, long long& to, int lane) {
+    long long from = 0, before = 0;
+    int lo = 0, hi = a.n, units = 0;      // work before lo <= from < work before hi
+    int4 e = make_int4(0, 0, 0, 0);
+    const int all = __ldcg(a.cu_work + a.n);
+    for (bool first = true; first || hi - lo > 1; first = false) {
         const int step = (hi - lo + 31) / 32, i = lo + lane * step;
-        const long long first = i < hi ? (long long)__ldcg(a.cu_work + i) * a.c.n_kv : 0x7fffffffffffffffll;
-        const int k = 31 - __clz(__ballot_sync(0xffffffffu, first <= at));
-        before = __shfl_sync(0xffffffffu, first, k);
+        const long long work = i < hi ? (long long)__ldcg(a.cu_work + i) * a.c.n_kv : 0x7fffffffffffffffll;
+        if (step == 1 && i < hi) {
+            e = __ldcg(a.entries + i);
+            units = __ldcg(a.cu_units + i);
+        }
+        if (first) {
+            const long long total = (long long)all * a.c.n_kv;
+            from = total * blockIdx.x / gridDim.x;
+            to = total * (blockIdx.x + 1) / gridDim.x;
+            if (from >= to) return false;
+        }
+        const int k = 31 - __clz(__ballot_sync(0xffffffffu, work <= from));
+        before = __shfl_sync(0xffffffffu, work, k);
+        if (step == 1) {
+            e.x = __shfl_sync(0xffffffffu, e.x, k); e.y = __shfl_sync(0xffffffffu, e.y, k);
+            e.z = __shfl_sync(0xffffffffu, e.z, k); e.w = __shfl_sync(0xffffffffu, e.w, k);
+            units = __shfl_sync(0xffffffffu, units, k);
+        }
         lo += k * step;
         hi = min(hi, lo + step);
     }
     u.entry = lo;
-    const int4 e = __ldcg(a.entries + lo);
-    walk_enter(a, u, e, __ldcg(a.cu_units + lo));
+    walk_enter(a, u, e, units);
     const int one = a.split.work((long long)e.y + e.z), full = a.split.work_of(u.size);     // of a (column tile, head), of a split
-    const long long turn = (at - before) / one;
-    const int into = (int)((at - before) % one);
+    const long long turn = (from - before) / one;
+    const int into = (int)((from - before) % one);
     u.split = min((into + full - 1) / full, u.splits - 1);
     u.head = (int)(turn % a.c.n_kv);
     u.ctile = (int)(turn / a.c.n_kv);
     u.w += turn * u.splits + u.split;
     u.at = before + turn * one + u.split * full;
     walk_range<COLS>(a, u);
-    if (u.at < at) walk_next<COLS>(a, u);
-    return u;
+    if (u.at < from) walk_next<COLS>(a, u);
+    return u.at < to && u.entry < a.n;
 }
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -232,20 +248,15 @@ __device__ __forceinline__ void ka_produce(const Kv4AttnArgs& a, const KaRing<NG
     using S = KaShared<NG, COLS>;
     constexpr int HD = NG * KV4_GROUP, KT = S::KT, D = S::STAGES;
     const int tiles = 1 << (a.c.block_shift - 4);     // of a block
-    const long long total = (long long)__ldcg(a.cu_work + a.n) * a.c.n_kv;
-    const long long from = total * blockIdx.x / gridDim.x, last = total * (blockIdx.x + 1) / gridDim.x;
     Kv4Walk u = {};
     int id = 0;     // the lane's tile's block
     auto block_of = [&]() {
         const int pos = u.base + lane * KV4_TILE;
         return lane < KA_WARPS * KT && pos < u.hi ? __ldcg(a.c.table + (size_t)u.e.x * a.c.max_blocks + (pos >> a.c.block_shift)) : 0;
     };
-    bool queries = true, begins = true, more = from < last;
-    if (more) {
-        u = walk_at<COLS>(a, from, lane);
-        more = u.at < last && u.entry < a.n;
-        if (more) id = block_of();
-    }
+    long long last = 0;
+    bool queries = true, begins = true, more = walk_begin<COLS>(a, u, last, lane);
+    if (more) id = block_of();
     const int run = min(tiles, KA_WARPS * KT);    // tiles that lie behind one another
     for (unsigned k = 0;; ++k) {
         const int s = k % D;
@@ -871,28 +882,27 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn_few(const Kv4AttnA
     }
 }
 
-// Adds up the splits of every row that has more than one: a CTA a (row, query head), WARPS warps.  Split i belongs to class i % 32; a class
-// adds its splits in order, and the classes are added in order, so that a row's bits do not depend on WARPS, which goes by the
-// cache's size: with up to 32 splits one warp, as each class then has one member at most.
+// Adds up the splits of every row that has more than one: a warp, or 8, a (row, query head).  Split i belongs to class i % 32; a class adds
+// its splits in order, and the classes are added in order, so that a row's bits do not depend on the number of warps, which goes by
+// the cache's size: with up to 32 splits one warp, as each class then has one member at most.
+// Where a row's parts lie is read from the plan before the kernel in front, the attention, has ended: that one starts its successors when
+// the plan is done.  Every way out waits for it, because what comes next waits for this kernel alone.
 template <int NG, int WARPS>
 __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) k_kv4_merge(const Kv4AttnArgs a, const int cols) {
     constexpr int HD = NG * KV4_GROUP, CLASSES = 32 / WARPS;
     __shared__ float part_acc[WARPS == 1 ? 1 : 32][HD];
-    __shared__ float part_sum[WARPS == 1 ? 1 : 32];
+    __shared__ float2 part_ml[WARPS == 1 ? 1 : 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, heads = a.c.n_kv * a.group;
     const long long id = WARPS == 1 ? (long long)blockIdx.x * 4 + warp : blockIdx.x;
-    pdl_wait();
     pdl_launch();
-    const int row = (int)(id / heads), head = (int)(id % heads), kv = head / a.group;
-    if (row >= a.n_rows) return;
-    const int entry = __ldcg(a.row_entry + row);
-    if (entry < 0) return;
-    const int4 e = __ldcg(a.entries + entry);
-    const long long unit = __ldcg(a.cu_units + entry);
+    const int row = (int)(id / heads), head = (int)(id % heads), kv = by_group(a, head);
+    const int entry = row < a.n_rows ? __ldcg(a.row_entry + row) : -1;
+    const int4 e = entry >= 0 ? __ldcg(a.entries + entry) : make_int4(0, 0, 0, 0);
+    const long long unit = entry >= 0 ? __ldcg(a.cu_units + entry) : 0;
     const int all = a.split.parts((long long)e.y + e.z);
-    if (all == 1) return;
+    if (all <= 1) return pdl_wait();
     const int own = (e.y + row - e.w) / a.split.of((long long)e.y + e.z) + 1;        // splits that the row sees
-    const int c = (row - e.w) * a.group + head % a.group;
+    const int c = (row - e.w) * a.group + head - kv * a.group;
     const long long w = unit * a.c.n_kv + ((long long)(c / cols) * a.c.n_kv + kv) * all;
     const float2* ml = a.ml + w * cols + c % cols;
     const float* acc = a.acc + (size_t)(w * cols + c % cols) * HD + lane * NG;
@@ -901,19 +911,20 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) k_kv4_merge(con
     float best = -INFINITY, sum = 0.f, out[NG];
 #pragma unroll
     for (int j = 0; j < NG; ++j) out[j] = 0.f;
+    pdl_wait();
     if constexpr (WARPS == 1) {
         const float2 mine = lane < own ? __ldcg(ml + (size_t)lane * cols) : make_float2(-INFINITY, 0.f);
+        float v[8][NG];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+#pragma unroll
+            for (int j = 0; j < NG; ++j) v[k][j] = k < own ? __ldcg(acc + k * step + j) : 0.f;
+        }
         best = mine.x;
 #pragma unroll
         for (int o = 16; o; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
-        const float f = ex2(mine.x - (best == -INFINITY ? 0.f : best)), l = f * mine.y;
+        const float f = ex2(mine.x - (best == -INFINITY ? 0.f : best)), l = __fmul_rn(f, mine.y);
         for (int i = 0; i < own; i += 8) {
-            float v[8][NG];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-#pragma unroll
-                for (int j = 0; j < NG; ++j) v[k][j] = i + k < own ? __ldcg(acc + (i + k) * step + j) : 0.f;
-            }
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 const float fk = __shfl_sync(0xffffffffu, f, i + k);
@@ -921,48 +932,61 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) k_kv4_merge(con
 #pragma unroll
                 for (int j = 0; j < NG; ++j) out[j] = __fadd_rn(out[j], __fmul_rn(fk, v[k][j]));
             }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+#pragma unroll
+                for (int j = 0; j < NG; ++j) v[k][j] = i + 8 + k < own ? __ldcg(acc + (i + 8 + k) * step + j) : 0.f;
+            }
         }
     } else {
-        for (int i = lane; i < own; i += 32) best = fmaxf(best, __ldcg(&ml[(size_t)i * cols].x));
-#pragma unroll
-        for (int o = 16; o; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
-        const float now = best == -INFINITY ? 0.f : best;
-        float s[CLASSES], o[CLASSES][NG];
+        float2 st[CLASSES];     // of a class: maximum and sum
+        float o[CLASSES][NG];
 #pragma unroll
         for (int k = 0; k < CLASSES; ++k) {
-            s[k] = 0.f;
+            const int i = warp * CLASSES + k;
+            st[k] = i < own ? __ldcg(ml + (size_t)i * cols) : make_float2(-INFINITY, 0.f);
 #pragma unroll
-            for (int j = 0; j < NG; ++j) o[k][j] = 0.f;
+            for (int j = 0; j < NG; ++j) o[k][j] = i < own ? __ldcg(acc + i * step + j) : 0.f;
         }
-        for (int i = warp * CLASSES; i < own; i += 32) {
+#pragma unroll 2
+        for (int first = warp * CLASSES + 32; first < own; first += 32) {
             float2 p[CLASSES];
             float v[CLASSES][NG];
 #pragma unroll
             for (int k = 0; k < CLASSES; ++k) {
-                p[k] = i + k < own ? __ldcg(ml + (size_t)(i + k) * cols) : make_float2(-INFINITY, 0.f);
+                const int i = first + k;
+                p[k] = i < own ? __ldcg(ml + (size_t)i * cols) : make_float2(-INFINITY, 0.f);
 #pragma unroll
-                for (int j = 0; j < NG; ++j) v[k][j] = i + k < own ? __ldcg(acc + (i + k) * step + j) : 0.f;
+                for (int j = 0; j < NG; ++j) v[k][j] = i < own ? __ldcg(acc + i * step + j) : 0.f;
             }
 #pragma unroll
             for (int k = 0; k < CLASSES; ++k) {
-                const float f = ex2(p[k].x - now);
-                s[k] = __fadd_rn(s[k], f * p[k].y);
+                const float top = fmaxf(st[k].x, p[k].x), now = top == -INFINITY ? 0.f : top;
+                const float f0 = ex2(st[k].x - now), f1 = ex2(p[k].x - now);
+                st[k] = make_float2(top, f0 * st[k].y + f1 * p[k].y);
 #pragma unroll
-                for (int j = 0; j < NG; ++j) o[k][j] = __fadd_rn(o[k][j], __fmul_rn(f, v[k][j]));
+                for (int j = 0; j < NG; ++j) o[k][j] = f0 * o[k][j] + f1 * v[k][j];
             }
         }
 #pragma unroll
         for (int k = 0; k < CLASSES; ++k) {
-            if (lane == 0) part_sum[warp * CLASSES + k] = s[k];
+            if (lane == 0) part_ml[warp * CLASSES + k] = st[k];
 #pragma unroll
             for (int j = 0; j < NG; ++j) part_acc[warp * CLASSES + k][lane * NG + j] = o[k][j];
         }
         __syncthreads();
         if (warp) return;
-        for (int k = 0; k < 32; ++k) {
-            sum = __fadd_rn(sum, part_sum[k]);
+        const float2 mine = part_ml[lane];
+        best = mine.x;
 #pragma unroll
-            for (int j = 0; j < NG; ++j) out[j] = __fadd_rn(out[j], part_acc[k][lane * NG + j]);
+        for (int k = 16; k; k >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, k));
+        const float f = ex2(mine.x - (best == -INFINITY ? 0.f : best)), l = __fmul_rn(f, mine.y);
+#pragma unroll 8
+        for (int k = 0; k < 32; ++k) {
+            const float fk = __shfl_sync(0xffffffffu, f, k);
+            sum = __fadd_rn(sum, __shfl_sync(0xffffffffu, l, k));
+#pragma unroll
+            for (int j = 0; j < NG; ++j) out[j] = __fadd_rn(out[j], __fmul_rn(fk, part_acc[k][lane * NG + j]));
         }
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;

@@ -27,6 +27,8 @@ from torch import Tensor
 from . import _lib
 
 _NOTHING = contextlib.nullcontext()
+# the current stream's handle; torch's public call builds a stream object first (2 us of a call that takes 15)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
 class Kv4Plan:
@@ -39,16 +41,28 @@ class Kv4Plan:
         work = (7 * n_seqs + 3 + n_rows + 3) & ~3          # the parts behind it: 16-byte aligned
         row = (n_rows + 3) & ~3
         # one allocation: work, slot_map (int64), row_slot, row_pos, cu_rows
-        self._ints = ints = torch.empty(work + 4 * row + n_seqs + 1, dtype=torch.int32, device=device)
-        self.slot_map = ints[work:work + 2 * n_rows].view(torch.int64)
-        self.row_slot = ints[work + 2 * row:work + 2 * row + n_rows]
-        self.row_pos = ints[work + 3 * row:work + 3 * row + n_rows]
-        self.cu_rows = ints[work + 4 * row:]
-        at = ints.data_ptr()
-        self._c = _lib.VuibKv4Plan(n_seqs, n_rows, max_new, at, at + 4 * (work + 4 * row), at + 4 * (work + 2 * row), at + 4 * (work + 3 * row),
-                                   at + 4 * work)
+        self._ints = torch.empty(work + 4 * row + n_seqs + 1, dtype=torch.int32, device=device)
+        self._at = (work, work + 2 * row, work + 3 * row, work + 4 * row)
+        at = self._ints.data_ptr()
+        self._c = _lib.VuibKv4Plan(n_seqs, n_rows, max_new, at, at + 4 * self._at[3], at + 4 * self._at[1], at + 4 * self._at[2], at + 4 * work)
         self._ref = C.byref(self._c)
         self._ws_bytes = -1        # of its attention calls, asked for once
+
+    @property
+    def slot_map(self) -> Tensor:
+        return self._ints[self._at[0]:self._at[0] + 2 * self.n_rows].view(torch.int64)
+
+    @property
+    def row_slot(self) -> Tensor:
+        return self._ints[self._at[1]:self._at[1] + self.n_rows]
+
+    @property
+    def row_pos(self) -> Tensor:
+        return self._ints[self._at[2]:self._at[2] + self.n_rows]
+
+    @property
+    def cu_rows(self) -> Tensor:
+        return self._ints[self._at[3]:]
 
 
 class Kv4Cache:
@@ -102,7 +116,7 @@ class Kv4Cache:
 
     @property
     def _stream(self):
-        return torch.cuda.current_stream(self.device).cuda_stream
+        return _raw_stream(self._index)
 
     def _here(self):
         """Makes the cache's device the current one, where it is not."""
@@ -185,9 +199,12 @@ class Kv4Cache:
         """Stores the plan's rows: k, v (n_rows, n_kv_heads, head_dim), keys with RoPE applied.  NaN is stored as 0 and
         magnitudes beyond 60000 as 60000, which ``check_device`` reports."""
         with self._here():
-            k, v = (self._rows(t, name, plan.n_rows, self.n_kv_heads) for t, name in ((k, "k"), (v, "v")))
-            self._ck(self._lib.vuib_kv4_append(self._h, layer, plan._ref, k.data_ptr(), self._step(k, self.n_kv_heads),
-                                               v.data_ptr(), self._step(v, self.n_kv_heads), self._stream))
+            n, heads = plan.n_rows, self.n_kv_heads
+            k, v = self._rows(k, "k", n, heads), self._rows(v, "v", n, heads)
+            rc = self._lib.vuib_kv4_append(self._h, layer, plan._ref, k.data_ptr(), self._step(k, heads), v.data_ptr(), self._step(v, heads),
+                                           _raw_stream(self._index))
+            if rc:
+                self._ck(rc)
 
     def read(self, layer: int, row_slot, row_pos, *, k_out: Tensor | None = None, v_out: Tensor | None = None) -> tuple[Tensor, Tensor]:
         """The keys and values stored for position ``row_pos[i]`` of sequence ``row_slot[i]``: (n, n_kv_heads, head_dim) bf16,
