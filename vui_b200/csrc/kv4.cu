@@ -9,6 +9,7 @@
 
 #include "../../include/vuib200.h"
 #include "kv4_attn.cuh"
+#include "kv4_chunk.cuh"
 #include "kv4_kernels.cuh"
 
 using namespace vuik;
@@ -68,31 +69,32 @@ long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 // What a plan's shape decides for attention: columns of a tile (rows x query heads of a kv head) and positions of a split.
 // A few columns: splits of 256 positions in sequences of up to 1024, 512 beyond, whatever the batch.
 // Up to 16 columns the form for a few (2, 4, 8 or 16 columns a tile), else the one for many.
-struct Shape { bool few, halves; int nt, cols; Kv4Split split; };
+enum Form { FEW_HALVES, FEW_4, FEW_8, FEW_16, MANY, CHUNK };
+#ifndef KV4_CHUNK
+#define KV4_CHUNK 64
+#endif
+struct Shape { Form form; int cols; Kv4Split split; };
 Shape shape_of(const VuibKv4* c, const VuibKv4Plan* p) {
-    Shape s;
     const int group = c->cfg.n_heads / c->cfg.n_kv_heads;
     const long long most = (long long)p->max_new * group;       // columns of one sequence
-    s.few = most <= 16;
-    s.nt = s.few ? (most <= 4 ? 1 : most <= 8 ? 2 : 4) : c->ng > 2 ? 2 : 4;
-    s.halves = most <= 2 && c->ng != 3;
-    s.cols = s.halves ? 2 : (s.few ? 4 : 8) * s.nt;
-    s.split = {256, 512, true};
-    if (!s.few) {
-        const long long tiles = ceil_div((long long)p->n_rows * group, s.cols) + p->n_seqs;
-        const long long len = (long long)c->cfg.max_blocks << c->block_shift;
-        int split = 512;
-        while ((long long)split * 32 < len) split *= 2;
-        if (tiles * c->cfg.n_kv_heads >= 2 * c->sms) split = 1 << 30;
-        s.split = {split, split, false};
+    if (most <= 16) {
+        const Form f = most <= 2 && c->ng != 3 ? FEW_HALVES : most <= 4 ? FEW_4 : most <= 8 ? FEW_8 : FEW_16;
+        return {f, f == FEW_HALVES ? 2 : f == FEW_4 ? 4 : f == FEW_8 ? 8 : 16, {256, 512, 1 << 30, true}};
     }
+    Shape s = {MANY, c->ng > 2 ? 16 : 32, {}};
+    if (most >= KV4_CHUNK) s = {CHUNK, KC_COLS, {}};
+    const long long tiles = ceil_div((long long)p->n_rows * group, s.cols) + p->n_seqs;
+    // enough tiles for the SMs: no splits; else at most 8 of a sequence, so that their sums stay a few megabytes
+    const long long len = (long long)c->cfg.max_blocks << c->block_shift;
+    const bool enough = tiles * c->cfg.n_kv_heads >= (s.form == CHUNK ? 1 : 2) * c->sms;
+    s.split = {enough ? 1 << 30 : 512, enough ? 1 << 30 : 512, 8, tiles * (len / 64 + 16) < 1 << 29};
     return s;
 }
 
 // Most splits of one sequence.
 long long most_parts(const VuibKv4* c, const Shape& s) {
     const long long len = (long long)c->cfg.max_blocks << c->block_shift;
-    return max(s.split.parts(min(len, 1024ll)), s.split.parts(len));
+    return min((long long)s.split.most, max(ceil_div(min(len, 1024ll), s.split.up_to_1024), ceil_div(len, s.split.beyond)));
 }
 
 // Most units (of one kv head) that a plan of this shape can have.  Sequences share no blocks, so their lengths sum up to the pool's.
@@ -133,37 +135,41 @@ int32_t check_rows(VuibKv4* c, const char* name, const void* p, int64_t stride, 
     return VUIB_OK;
 }
 
-template <int NG, int COLS>
-cudaError_t launch_attn(VuibKv4* c, const Shape& s, void (*kern)(Kv4AttnArgs), int& resident, const Kv4AttnArgs& a, long long items, bool merge, void* stream) {
-    constexpr int smem = KaShared<NG, COLS>::TOTAL;
+template <int NG>
+cudaError_t launch_attn(VuibKv4* c, const Shape& s, void (*kern)(Kv4AttnArgs), int threads, int smem, Kv4AttnArgs a, long long items, bool merge, void* stream) {
+    int& resident = c->resident[s.form];
     cudaError_t e = cudaSuccess;
     if (!resident) {     // as many CTAs as fit the SMs: asked for, and attributes set, once a handle and form
         e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-        if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kern, KA_THREADS + 32, smem);
+        if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kern, threads, smem);
         if (e != cudaSuccess) return e;
-        if (resident < 1) resident = 1;
+        if (resident < 1 || s.form == CHUNK) resident = 1;      // CHUNK: a CTA takes all of an SM's tensor memory
     }
-    e = launch(c, kern, dim3((unsigned)min(items, (long long)c->sms * resident)), KA_THREADS + 32, smem, 1, stream, a);
+    const long long room = (long long)c->sms * resident;
+    // A kernel that starts beside the merge finds its SMs partly taken, and one that fills them all then has late CTAs: 256 sequences of
+    // 512 to 2048 positions call after call 61.0 us with an early start and 53.0 without, one sequence of 300 6.3 and 6.7.
+    a.early = 2 * items < room;
+    e = launch(c, kern, dim3((unsigned)min(items, room)), threads, smem, 1, stream, a);
     if (e != cudaSuccess || !merge) return e;
     const long long rows = (long long)a.n_rows * c->cfg.n_heads;
     if (most_parts(c, s) <= 32)
-        return launch(c, k_kv4_merge<NG, 1>, dim3((unsigned)ceil_div(rows, 4)), 128, 0, 1, stream, a, COLS);
-    return launch(c, k_kv4_merge<NG, 8>, dim3((unsigned)rows), 256, 0, 1, stream, a, COLS);
+        return launch(c, k_kv4_merge<NG, 1>, dim3((unsigned)ceil_div(rows, 4)), 128, 0, 1, stream, a, s.cols);
+    return launch(c, k_kv4_merge<NG, 8>, dim3((unsigned)rows), 256, 0, 1, stream, a, s.cols);
 }
 
 template <int NG>
 cudaError_t launch_form(VuibKv4* c, const Shape& s, const Kv4AttnArgs& a, long long items, bool merge, void* stream) {
-    int* resident = c->resident;
-    if (s.few) {
-        if constexpr (NG != 3)
-            if (s.halves) return launch_attn<NG, 2>(c, s, k_kv4_attn_few<NG, 1, true>, resident[5], a, items, merge, stream);
-        if (s.nt == 1) return launch_attn<NG, 4>(c, s, k_kv4_attn_few<NG, 1, false>, resident[0], a, items, merge, stream);
-        if (s.nt == 2) return launch_attn<NG, 8>(c, s, k_kv4_attn_few<NG, 2, false>, resident[1], a, items, merge, stream);
-        return launch_attn<NG, 16>(c, s, k_kv4_attn_few<NG, 4, false>, resident[2], a, items, merge, stream);
+    constexpr int T = KA_THREADS + 32, MANY_NT = NG == 2 ? 4 : 2;
+    switch (s.form) {
+        case FEW_HALVES:
+            if constexpr (NG != 3) return launch_attn<NG>(c, s, k_kv4_attn_few<NG, 1, true>, T, KaShared<NG, 2>::TOTAL, a, items, merge, stream);
+        case FEW_4: return launch_attn<NG>(c, s, k_kv4_attn_few<NG, 1, false>, T, KaShared<NG, 4>::TOTAL, a, items, merge, stream);
+        case FEW_8: return launch_attn<NG>(c, s, k_kv4_attn_few<NG, 2, false>, T, KaShared<NG, 8>::TOTAL, a, items, merge, stream);
+        case FEW_16: return launch_attn<NG>(c, s, k_kv4_attn_few<NG, 4, false>, T, KaShared<NG, 16>::TOTAL, a, items, merge, stream);
+        case MANY: return launch_attn<NG>(c, s, k_kv4_attn<NG, MANY_NT>, T, KaShared<NG, 8 * MANY_NT>::TOTAL, a, items, merge, stream);
+        default: return launch_attn<NG>(c, s, k_kv4_attn_chunk<NG>, KC_THREADS, KcShared<NG>::TOTAL, a, items, merge, stream);
     }
-    if constexpr (NG == 2) return launch_attn<NG, 32>(c, s, k_kv4_attn<NG, 4>, resident[3], a, items, merge, stream);
-    else return launch_attn<NG, 16>(c, s, k_kv4_attn<NG, 2>, resident[4], a, items, merge, stream);
 }
 
 }  // namespace

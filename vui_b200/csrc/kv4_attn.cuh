@@ -16,6 +16,7 @@ struct Kv4AttnArgs {
     const __nv_bfloat16* q; long long q_stride;
     __nv_bfloat16* out; long long out_stride;
     float scale_log2;                          // scale * log2(e)
+    bool early;                                // whether the merge lets its successor start beside it
     float* acc;                                // partial sums: (unit, column, dim), where a sequence has more than one split
     float2* ml;                                // maximum (of log2 scores) and sum: (unit, column)
 };
@@ -894,7 +895,7 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) k_kv4_merge(con
     __shared__ float2 part_ml[WARPS == 1 ? 1 : 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, heads = a.c.n_kv * a.group;
     const long long id = WARPS == 1 ? (long long)blockIdx.x * 4 + warp : blockIdx.x;
-    pdl_launch();
+    if (a.early) pdl_launch();
     const int row = (int)(id / heads), head = (int)(id % heads), kv = by_group(a, head);
     const int entry = row < a.n_rows ? __ldcg(a.row_entry + row) : -1;
     const int4 e = entry >= 0 ? __ldcg(a.entries + entry) : make_int4(0, 0, 0, 0);

@@ -1,0 +1,538 @@
+// Attention of many columns (chunks of prompts) over the paged 4-bit cache, on the 5th-generation tensor cores.
+//
+// A CTA takes 256 columns (a sequence's rows times the query heads of a kv head) of one kv head as two tiles of 128, and walks the
+// positions 128 at a time:
+//   * 4 warps read codes from the cache (a step ahead, in registers) and write keys and values as f16 into a ring of shared-memory tiles
+//     that both tiles of columns share: keys [position][dim], values [dim][position], both K-major with the 128-byte swizzle;
+//   * one thread issues tcgen05.mma: S = Q K^T (128 x 128, K = head_dim) and O += P V (A = P from tensor memory, K = 128 positions);
+//   * 4 warps a tile, one thread a column: maximum, exponentials, P as f16 back into tensor memory over S, and, where the maximum has grown
+//     by more than 2^8 since the reference was set, the correction of O.
+// While one tile's softmax runs, the tensor cores work on the other.  Per step of 128 positions and two tiles at head_dim 128 the tensor
+// cores take 2048 cycles, the exponentials (16 a clock) 2048, the issue slots about 1700.
+// Every wait is bounded; a role that gives up leaves its loop, and all warps meet before tensor memory is freed.
+#pragma once
+#include "kv4_attn.cuh"
+
+namespace vuik {
+
+constexpr int KC_COLS = 256, KC_TILE = 128, KC_STEP = 128;
+constexpr int KC_FILL = 4, KC_WARPS = 13, KC_THREADS = KC_WARPS * 32;      // warps 0-3 fill, 4-7 and 8-11 softmax, 12 MMA
+
+template <int NG>
+struct KcShared {
+    static constexpr int HD = NG * KV4_GROUP, NB = (HD + 63) / 64;
+    static constexpr int BLOCK = 128 * 128;                // 128 rows of 128 bytes
+    static constexpr int Q = NB * BLOCK, SLOT = NB * BLOCK; // of a tile of columns; of a tile of keys or values
+    static constexpr int SLOTS = 4;
+    static constexpr int BARS = 2 * Q + SLOTS * SLOT;
+    static constexpr int TOTAL = BARS + 256 + 1024;        // and room to start at a multiple of 1024
+};
+
+// Steps of 128 positions that the two tiles of a unit take; 0: a tile without columns, or one that does not see this split.
+__device__ __forceinline__ void kc_steps(const Kv4AttnArgs& a, const Kv4Walk& u, int (&n)[2]) {
+    const int all = u.e.z * a.group, first = u.ctile * KC_COLS;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const int end = min(first + (x + 1) * KC_TILE, all);          // one past the tile's last column
+        const int hi = min(u.hi, u.e.y + by_group(a, max(end - 1, 0)) + 1);
+        n[x] = end > first + x * KC_TILE ? max(0, (hi - u.base + KC_STEP - 1) / KC_STEP) : 0;
+    }
+}
+
+struct KcBars {
+    uint32_t at;
+    __device__ __forceinline__ uint32_t q_full(int x) const { return at + 8 * x; }
+    __device__ __forceinline__ uint32_t s_full(int x) const { return at + 16 + 8 * x; }
+    __device__ __forceinline__ uint32_t p_full(int x) const { return at + 32 + 8 * x; }
+    __device__ __forceinline__ uint32_t o_full(int x) const { return at + 48 + 8 * x; }
+    __device__ __forceinline__ uint32_t pv_done(int x) const { return at + 64 + 8 * x; }
+    __device__ __forceinline__ uint32_t kv_full(int s) const { return at + 80 + 8 * s; }
+    __device__ __forceinline__ uint32_t kv_empty(int s) const { return at + 112 + 8 * s; }
+    __device__ __forceinline__ uint32_t tmem() const { return at + 144; }
+};
+
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+// Descriptor of a K-major tile with the 128-byte swizzle (rows 128 bytes apart, groups of 8 rows 1024).
+__device__ __forceinline__ uint64_t tile_desc(uint32_t addr) {
+    return (uint64_t)((1024u >> 4) | 1u << 14 | 2u << 29) << 32 | ((addr >> 4 & 0x3FFF) | 1u << 16);
+}
+// f16 operands, fp32 sums, both K-major, 128 rows, n columns.
+__host__ __device__ constexpr uint32_t kc_idesc(int n) { return 1u << 4 | (uint32_t)(n >> 3) << 17 | 8u << 24; }
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, int add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+}
+#define KC_R32(r) "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), \
+    "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),     \
+    "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+// 32 columns of this thread's lane; they are there behind tm_wait().
+__device__ __forceinline__ void tm_load32(uint32_t at, uint32_t (&r)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,"
+                 "%27,%28,%29,%30,%31}, [%32];" : KC_R32(r) : "r"(at));
+}
+// The wait names the registers, so that nothing that reads them moves in front of it.
+#define KC_RW32(r) "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), \
+    "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),      \
+    "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+__device__ __forceinline__ void tm_wait(uint32_t (&r)[32]) { asm volatile("tcgen05.wait::ld.sync.aligned;" : KC_RW32(r)::"memory"); }
+__device__ __forceinline__ void tm_store32(uint32_t at, const uint32_t (&r)[32]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,"
+                 "%27,%28,%29,%30,%31,%32};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+                 "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+                 "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+}
+__device__ __forceinline__ void tm_store16(uint32_t at, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+                 "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void tm_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void sts128(uint32_t at, const uint32_t (&r)[4]) {
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
+// Four 8 x 8 matrices of 16-bit elements in fragment order; lane l says where row l % 8 of matrix l / 8 goes (16 bytes).
+__device__ __forceinline__ void stmatrix4(uint32_t at, const uint32_t (&r)[4]) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
+
+// ---- the filling warps: warp w takes tiles w and w + 4 of every 8 (of 16 positions)
+template <int NG>
+__device__ __forceinline__ void kc_fill(const Kv4AttnArgs& a, uint32_t ring, const KcBars bars, int w, int lane) {
+    using S = KcShared<NG>;
+    const int g = lane >> 2, t = lane & 3, tiles = 1 << (a.c.block_shift - 4);
+    Kv4Walk u = {};
+    long long to = 0;
+    unsigned n = 0;        // tiles written: keys and values in turn
+    bool more = walk_begin<KC_COLS>(a, u, to, lane);
+    while (more) {
+        int steps[2];
+        kc_steps(a, u, steps);
+        const int last = max(steps[0], steps[1]);
+        int id[2] = {0, 0};
+        auto read_ids = [&](int j) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int pos = u.base + j * KC_STEP + (k * KC_FILL + w) * KV4_TILE;
+                id[k] = pos < u.hi ? __ldcg(a.c.table + (size_t)u.e.x * a.c.max_blocks + (pos >> a.c.block_shift)) : -1;
+            }
+        };
+        const unsigned char* at[2];
+        auto place = [&](int j) {       // of the step whose blocks are in id
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int pos = u.base + j * KC_STEP + (k * KC_FILL + w) * KV4_TILE;
+                at[k] = nullptr;
+                if (pos < u.hi) {
+                    int b = id[k];
+                    if ((unsigned)b >= (unsigned)a.c.n_blocks) {
+                        if (lane == 0) atomicOr(a.c.flag, KV4_BAD_BLOCK);
+                        b = 0;
+                    }
+                    at[k] = a.c.pool + ((size_t)((long long)b * a.c.n_kv + u.head) * tiles + ((pos & ((1 << a.c.block_shift) - 1)) >> 4)) * (NG * KV4_GT);
+                }
+            }
+        };
+        // what is not there is zeros: codes, scales and values
+        uint2 kc[2][NG], kp[2][NG], vc[2][NG];
+        uint4 vp[2][NG];
+        auto read_keys = [&]() {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+#pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    kc[k][i] = kp[k][i] = make_uint2(0, 0);
+                    if (at[k]) {
+                        kc[k][i] = __ldcg(reinterpret_cast<const uint2*>(at[k] + i * KV4_GT + lane * 8));
+                        kp[k][i] = __ldcg(reinterpret_cast<const uint2*>(at[k] + i * KV4_GT + KV4_KPAR + g * 8));
+                    }
+                }
+            }
+        };
+        auto read_values = [&]() {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+#pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    vc[k][i] = make_uint2(0, 0);
+                    vp[k][i] = make_uint4(0, 0, 0, 0);
+                    if (at[k]) {
+                        vc[k][i] = __ldcg(reinterpret_cast<const uint2*>(at[k] + i * KV4_GT + KV4_VCODE + lane * 8));
+                        vp[k][i] = __ldcg(reinterpret_cast<const uint4*>(at[k] + i * KV4_GT + KV4_VPAR + t * 16));   // of keys 2t, 2t+8, 2t+1, 2t+9
+                    }
+                }
+            }
+        };
+        auto done = [&]() {
+            fence_async();
+            __syncwarp();
+            if (lane == 0) bar_arrive(bars.kv_full(n % S::SLOTS));
+            ++n;
+        };
+        if (last > 0) {
+            read_ids(0);
+            place(0);
+            read_keys();
+        }
+        for (int j = 0; j < last; ++j) {
+            if (j + 1 < last) read_ids(j + 1);
+            read_values();
+            if (n >= S::SLOTS && !bar_wait(bars.kv_empty(n % S::SLOTS), (n / S::SLOTS - 1) & 1)) return give_up(a.c.flag);
+            uint32_t slot = ring + (n % S::SLOTS) * S::SLOT;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+#pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    const int key = (k * KC_FILL + w) * KV4_TILE + g;       // and key + 8, which has the same low three bits
+                    const uint32_t row = slot + (i >> 1) * S::BLOCK + key * 128 + ((((i & 1) * 4 + t) ^ (key & 7)) << 4);
+                    const __half2 s0 = __low2half2(as_h2(kp[k][i].x)), z0 = __high2half2(as_h2(kp[k][i].x));
+                    const __half2 s1 = __low2half2(as_h2(kp[k][i].y)), z1 = __high2half2(as_h2(kp[k][i].y));
+                    uint32_t r[4];
+                    kv4_values(kc[k][i].x, s0, z0, s0, z0, r);
+                    sts128(row, r);
+                    kv4_values(kc[k][i].y, s1, z1, s1, z1, r);
+                    sts128(row + 8 * 128, r);
+                }
+            }
+            done();
+            if (j + 1 < last) {
+                place(j + 1);
+                read_keys();
+            }
+            if (n >= S::SLOTS && !bar_wait(bars.kv_empty(n % S::SLOTS), (n / S::SLOTS - 1) & 1)) return give_up(a.c.flag);
+            slot = ring + (n % S::SLOTS) * S::SLOT;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int tile = k * KC_FILL + w, chunk = (tile & 3) * 2 + (lane >> 4);      // matrices 2 and 3: keys 8 to 15 of the tile
+#pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    // element 4 g + j of the group is row 8 j + g, so that a matrix's eight rows lie in eight different banks
+                    const int rho = i * 32 + (lane >> 3 & 1) * 8 + (lane & 7);
+                    const uint32_t row = slot + (tile >> 2) * (S::HD * 128) + rho * 128 + ((chunk ^ (lane & 7)) << 4);
+                    const __half2 s0 = as_h2(__byte_perm(vp[k][i].x, vp[k][i].z, 0x5410)), z0 = as_h2(__byte_perm(vp[k][i].x, vp[k][i].z, 0x7632));
+                    const __half2 s8 = as_h2(__byte_perm(vp[k][i].y, vp[k][i].w, 0x5410)), z8 = as_h2(__byte_perm(vp[k][i].y, vp[k][i].w, 0x7632));
+                    uint32_t r[4];
+                    kv4_values(vc[k][i].x, s0, z0, s8, z8, r);
+                    stmatrix4(row, r);
+                    kv4_values(vc[k][i].y, s0, z0, s8, z8, r);
+                    stmatrix4(row + 16 * 128, r);
+                }
+            }
+            done();
+        }
+        walk_next<KC_COLS>(a, u);
+        more = u.at < to && u.entry < a.n;
+    }
+}
+
+// ---- the issuing warp
+template <int NG>
+__device__ __forceinline__ void kc_issue(const Kv4AttnArgs& a, uint32_t smem, const KcBars bars, uint32_t tmem, int lane) {
+    using S = KcShared<NG>;
+    const uint32_t ring = smem + 2 * S::Q;
+    Kv4Walk u = {};
+    long long to = 0;
+    unsigned n = 0, units[2] = {0, 0}, steps_done[2] = {0, 0};
+#ifdef KC_WAIT
+    unsigned pv[2] = {0, 0};
+#endif
+    bool more = walk_begin<KC_COLS>(a, u, to, lane);
+    auto scores = [&](int x, unsigned slot) {       // S of tile x
+        const uint64_t q = tile_desc(smem + x * S::Q), k = tile_desc(ring + slot * S::SLOT);
+#pragma unroll
+        for (int i = 0; i < S::HD / 16; ++i) {
+            const uint64_t off = (i >> 2) * (S::BLOCK >> 4) + (i & 3) * 2;
+            mma_ss(tmem + x * KC_TILE, q + off, k + off, kc_idesc(KC_STEP), i > 0);
+        }
+        tc_commit(bars.s_full(x));
+    };
+    auto sums = [&](int x, unsigned slot, bool add) {
+        const uint64_t v = tile_desc(ring + slot * S::SLOT);
+#pragma unroll
+        for (int i = 0; i < KC_STEP / 16; ++i)
+            mma_ts(tmem + 256 + x * S::HD, tmem + x * KC_TILE + i * 8, v + (i >> 2) * (S::HD * 128 >> 4) + (i & 3) * 2, kc_idesc(S::HD), add || i > 0);
+    };
+    while (more) {
+        int steps[2];
+        kc_steps(a, u, steps);
+        const int last = max(steps[0], steps[1]);
+        if (last > 0) {
+            if (!bar_wait(bars.kv_full(n % S::SLOTS), (n / S::SLOTS) & 1)) return give_up(a.c.flag);
+            for (int x = 0; x < 2; ++x) {
+                if (!steps[x]) continue;
+                if (!bar_wait(bars.q_full(x), units[x] & 1)) return give_up(a.c.flag);
+                ++units[x];
+                tc_after();
+                if (elect_one()) scores(x, n % S::SLOTS);
+                __syncwarp();
+            }
+            if (elect_one()) tc_commit(bars.kv_empty(n % S::SLOTS));
+            __syncwarp();
+            ++n;
+            for (int j = 0; j < last; ++j) {
+                const unsigned vslot = n % S::SLOTS, kslot = (n + 1) % S::SLOTS;
+                if (!bar_wait(bars.kv_full(vslot), (n / S::SLOTS) & 1)) return give_up(a.c.flag);
+                if (j + 1 < last && !bar_wait(bars.kv_full(kslot), ((n + 1) / S::SLOTS) & 1)) return give_up(a.c.flag);
+                for (int x = 0; x < 2; ++x) {
+                    if (j >= steps[x]) continue;
+                    if (!bar_wait(bars.p_full(x), steps_done[x] & 1)) return give_up(a.c.flag);
+                    tc_after();
+                    if (elect_one()) {
+                        sums(x, vslot, j > 0);
+                        if (j + 1 == steps[x]) tc_commit(bars.o_full(x));
+#ifdef KC_WAIT
+                        else tc_commit(bars.pv_done(x));
+#endif
+                    }
+                    __syncwarp();
+                    if (j + 1 < steps[x]) {
+#ifdef KC_WAIT
+                        if (!bar_wait(bars.pv_done(x), pv[x]++ & 1)) return give_up(a.c.flag);
+                        tc_after();
+#endif
+                        if (elect_one()) scores(x, kslot);
+                        __syncwarp();
+                    }
+                    ++steps_done[x];
+                }
+                if (elect_one()) {
+                    tc_commit(bars.kv_empty(vslot));
+                    if (j + 1 < last) tc_commit(bars.kv_empty(kslot));
+                }
+                __syncwarp();
+                n += j + 1 < last ? 2 : 1;
+            }
+        }
+        walk_next<KC_COLS>(a, u);
+        more = u.at < to && u.entry < a.n;
+    }
+}
+
+// ---- the softmax warps of tile x: thread r of 128 has column r, which is its lane of tensor memory
+template <int NG>
+__device__ __forceinline__ void kc_softmax(const Kv4AttnArgs& a, uint32_t smem, const KcBars bars, uint32_t tmem, int x, int r, int lane) {
+    using S = KcShared<NG>;
+    constexpr int HD = S::HD;
+    const uint32_t lanes = tmem + ((uint32_t)(r & ~31) << 16), scores = lanes + x * KC_TILE, sums = lanes + 256 + x * HD;
+    Kv4Walk u = {};
+    long long to = 0;
+    unsigned n = 0, units = 0;       // steps, units with steps
+    bool more = walk_begin<KC_COLS>(a, u, to, lane);
+    while (more) {
+        int steps[2];
+        kc_steps(a, u, steps);
+        const int mine = steps[x], col = u.ctile * KC_COLS + x * KC_TILE + r;
+        const bool there = col < u.e.z * a.group;
+        const int row = there ? by_group(a, col) : 0, head = u.head * a.group + (there ? col - row * a.group : 0);
+        const int limit = there ? u.e.y + row : -1, all = u.e.y + by_group(a, u.ctile * KC_COLS + x * KC_TILE);
+        float m = -INFINITY, l = 0.f;
+        if (mine > 0) {
+            // the query times a power of two, so that its largest element lies in [1, 2): exact in f16 but for elements 2^14 times smaller
+            const uint4* src = reinterpret_cast<const uint4*>(a.q + (long long)(u.e.w + row) * a.q_stride + head * HD);
+            uint4 raw[HD / 8];
+            uint32_t big = 0;
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i) {
+                raw[i] = there ? __ldcg(src + i) : make_uint4(0, 0, 0, 0);
+                big = max(big, most_bits(raw[i]));
+            }
+            const int e = min(max((int)(big >> 7), 1), 253);
+            const float down = __int_as_float((254 - e) << 23), up = __int_as_float(e << 23);
+            const float factor = fmaxf(a.scale_log2 * up, 1e-37f);       // not 0, which would make NaN of masked scores
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i) {
+                const uint32_t v[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                uint32_t h[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) h[j] = pack_h2(__uint_as_float(v[j] << 16) * down, __uint_as_float(v[j] & 0xffff0000u) * down);
+                sts128(smem + x * S::Q + (i >> 3) * S::BLOCK + r * 128 + (((i & 7) ^ (r & 7)) << 4), h);
+            }
+            fence_async();
+            __syncwarp();
+            if (lane == 0) bar_arrive(bars.q_full(x));
+
+            for (int j = 0; j < mine; ++j, ++n) {
+                if (!bar_wait(bars.s_full(x), n & 1)) return give_up(a.c.flag);
+                tc_after();
+                const int base = u.base + j * KC_STEP;
+                const bool whole = base + KC_STEP - 1 <= all;        // every column sees all of the step
+                uint32_t s0[32], s1[32];
+                auto mask = [&](uint32_t (&s)[32], int first) {
+                    if (!whole) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (base + first + i > limit) s[i] = 0xff800000u;
+                    }
+                };
+                float top = -INFINITY;
+                auto most = [&](const uint32_t (&s)[32]) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) top = fmaxf(fmaxf(top, __uint_as_float(s[i])), __uint_as_float(s[i + 1]));
+                };
+                tm_load32(scores, s0);
+                tm_wait(s0);
+                tm_load32(scores + 32, s1);
+                mask(s0, 0);
+                most(s0);
+                tm_wait(s1);
+                tm_load32(scores + 64, s0);
+                mask(s1, 32);
+                most(s1);
+                tm_wait(s0);
+                tm_load32(scores + 96, s1);
+                mask(s0, 64);
+                most(s0);
+                tm_wait(s1);
+                tm_load32(scores, s0);
+                mask(s1, 96);
+                most(s1);
+                top *= factor;
+                if (j == 0) {
+                    m = top;
+                } else {
+                    // the reference stays while weights remain below 2^8; each column decides for itself
+                    const bool far = top > m + 8.f || (m == -INFINITY && top > m);
+                    if (__any_sync(0xffffffffu, far)) {
+                        const float old = far ? (m == -INFINITY ? 0.f : ex2(m - top)) : 1.f;
+                        if (far) m = top;
+                        l *= old;
+                        tm_wait(s0);
+#pragma unroll
+                        for (int i = 0; i < HD; i += 32) {
+                            tm_load32(sums + i, s1);
+                            tm_wait(s1);
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) s1[k] = __float_as_uint(__uint_as_float(s1[k]) * old);
+                            tm_store32(sums + i, s1);
+                        }
+                    }
+                }
+                const float less = m == -INFINITY ? 0.f : -m;        // nothing seen yet: weights of exp(-inf) = 0
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
+                auto weigh = [&](uint32_t (&s)[32], int first) {
+                    uint32_t p[16];
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        const float w0 = ex2(fmaf(__uint_as_float(s[i]), factor, less)), w1 = ex2(fmaf(__uint_as_float(s[i + 1]), factor, less));
+                        part[i & 2] += w0;
+                        part[(i & 2) + 1] += w1;
+                        p[i >> 1] = pack_h2(w0, w1);
+                    }
+                    tm_store16(scores + (first >> 1), p);       // over scores that have been read
+                };
+                tm_wait(s0);
+                tm_load32(scores + 32, s1);
+                mask(s0, 0);
+                weigh(s0, 0);
+                tm_wait(s1);
+                tm_load32(scores + 64, s0);
+                mask(s1, 32);
+                weigh(s1, 32);
+                tm_wait(s0);
+                tm_load32(scores + 96, s1);
+                mask(s0, 64);
+                weigh(s0, 64);
+                tm_wait(s1);
+                mask(s1, 96);
+                weigh(s1, 96);
+                l += (part[0] + part[1]) + (part[2] + part[3]);
+                tm_stored();
+                tc_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(bars.p_full(x));
+            }
+            if (!bar_wait(bars.o_full(x), units & 1)) return give_up(a.c.flag);
+            ++units;
+            tc_after();
+        }
+        if (u.splits > 1 && there) a.ml[u.w * KC_COLS + x * KC_TILE + r] = make_float2(m, l);
+        if (mine > 0) {
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            __nv_bfloat16* dst = a.out + (long long)(u.e.w + row) * a.out_stride + head * HD;
+            float* part = a.acc + (size_t)(u.w * KC_COLS + x * KC_TILE + r) * HD;
+#pragma unroll
+            for (int i = 0; i < HD; i += 32) {
+                uint32_t v[32];
+                tm_load32(sums + i, v);
+                tm_wait(v);
+                if (!there) continue;
+                // element 4 g + k of the group is column 8 k + g
+                if (u.splits == 1) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int d = k * 8 + 2 * j;
+                            const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(v[(d & 3) * 8 + (d >> 2)]) * inv, __uint_as_float(v[((d + 1) & 3) * 8 + (d >> 2)]) * inv);
+                            w[j] = *reinterpret_cast<const uint32_t*>(&h);
+                        }
+                        reinterpret_cast<uint4*>(dst + i)[k] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        reinterpret_cast<uint4*>(part + i)[k] = make_uint4(v[k], v[8 + k], v[16 + k], v[24 + k]);
+                }
+            }
+        }
+        walk_next<KC_COLS>(a, u);
+        more = u.at < to && u.entry < a.n;
+    }
+}
+
+template <int NG>
+__global__ void __launch_bounds__(KC_THREADS, 1) k_kv4_attn_chunk(const Kv4AttnArgs a) {
+    using S = KcShared<NG>;
+    extern __shared__ unsigned char smem_raw[];
+    const uint32_t smem = (smem_addr(smem_raw) + 1023) & ~1023u;
+    const KcBars bars = {smem + S::BARS};
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (threadIdx.x == 0) {
+        for (int x = 0; x < 2; ++x) {
+            bar_init(bars.q_full(x), 4);
+            bar_init(bars.s_full(x), 1);
+            bar_init(bars.p_full(x), 4);
+            bar_init(bars.o_full(x), 1);
+            bar_init(bars.pv_done(x), 1);
+        }
+        for (int s = 0; s < S::SLOTS; ++s) {
+            bar_init(bars.kv_full(s), KC_FILL);
+            bar_init(bars.kv_empty(s), 1);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    pdl_wait();
+    pdl_launch();
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(bars.tmem()) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    uint32_t tmem;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(bars.tmem()));
+    if (warp < KC_FILL) kc_fill<NG>(a, smem + 2 * S::Q, bars, warp, lane);
+    else if (warp < 12) kc_softmax<NG>(a, smem, bars, tmem, warp >= 8, threadIdx.x & 127, lane);
+    else kc_issue<NG>(a, smem, bars, tmem, lane);
+    tc_before();
+    __syncthreads();
+    tc_after();
+    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+}  // namespace vuik
