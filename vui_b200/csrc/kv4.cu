@@ -82,12 +82,12 @@ Shape shape_of(const VuibKv4* c, const VuibKv4Plan* p) {
         return {f, f == FEW_HALVES ? 2 : f == FEW_4 ? 4 : f == FEW_8 ? 8 : 16, {256, 512, 1 << 30, true}};
     }
     Shape s = {MANY, c->ng > 2 ? 16 : 32, {}};
-    if (most >= KV4_CHUNK) s = {CHUNK, KC_COLS, {}};
+    if (most >= KV4_CHUNK) return {CHUNK, KC_COLS, {1 << 30, 1 << 30, 1, false}};
     const long long tiles = ceil_div((long long)p->n_rows * group, s.cols) + p->n_seqs;
     // enough tiles for the SMs: no splits; else at most 8 of a sequence, so that their sums stay a few megabytes
     const long long len = (long long)c->cfg.max_blocks << c->block_shift;
-    const bool enough = tiles * c->cfg.n_kv_heads >= (s.form == CHUNK ? 1 : 2) * c->sms;
-    s.split = {enough ? 1 << 30 : 512, enough ? 1 << 30 : 512, 8, tiles * (len / 64 + 16) < 1 << 29};
+    const bool enough = tiles * c->cfg.n_kv_heads >= 2 * c->sms;
+    s.split = {enough ? 1 << 30 : 512, enough ? 1 << 30 : 512, 8, tiles * (len / 64 + 16) < KV4_MANY};
     return s;
 }
 
@@ -104,6 +104,11 @@ long long most_units(const VuibKv4* c, const VuibKv4Plan* p, const Shape& s) {
     const long long a_seq = ceil_div((long long)p->max_new * group, s.cols);
     const long long tiles = min((long long)p->n_seqs * a_seq, ceil_div((long long)p->n_rows * group, s.cols) + p->n_seqs);
     return min(tiles * most_parts(c, s), a_seq * (p->n_seqs + pool / s.split.up_to_1024));
+}
+
+// Units whose sums may have to be kept: of the form for chunks, two a CTA.
+long long most_items(const VuibKv4* c, const VuibKv4Plan* p, const Shape& s) {
+    return s.form == CHUNK ? 2ll * c->sms : most_units(c, p, s) * c->cfg.n_kv_heads;
 }
 
 size_t acc_bytes(const VuibKv4* c, long long items, int cols) { return ((size_t)items * cols * c->cfg.head_dim * 4 + 255) & ~size_t(255); }
@@ -150,9 +155,10 @@ cudaError_t launch_attn(VuibKv4* c, const Shape& s, void (*kern)(Kv4AttnArgs), i
     // A kernel that starts beside the merge finds its SMs partly taken, and one that fills them all then has late CTAs: 256 sequences of
     // 512 to 2048 positions call after call 61.0 us with an early start and 53.0 without, one sequence of 300 6.3 and 6.7.
     a.early = 2 * items < room;
-    e = launch(c, kern, dim3((unsigned)min(items, room)), threads, smem, 1, stream, a);
+    const long long grid = s.form == CHUNK ? c->sms : min(items, room), rows = (long long)a.n_rows * c->cfg.n_heads;
+    e = launch(c, kern, dim3((unsigned)grid), threads, smem, 1, stream, a);
     if (e != cudaSuccess || !merge) return e;
-    const long long rows = (long long)a.n_rows * c->cfg.n_heads;
+    if (s.form == CHUNK) return launch(c, k_kv4_chunk_merge<NG>, dim3((unsigned)ceil_div(rows, 4)), 128, 0, 1, stream, a, (int)grid);
     if (most_parts(c, s) <= 32)
         return launch(c, k_kv4_merge<NG, 1>, dim3((unsigned)ceil_div(rows, 4)), 128, 0, 1, stream, a, s.cols);
     return launch(c, k_kv4_merge<NG, 8>, dim3((unsigned)rows), 256, 0, 1, stream, a, s.cols);
@@ -247,12 +253,14 @@ extern "C" int32_t vuib_kv4_plan(VuibKv4* c, const VuibKv4Plan* p, const int32_t
     if (!slots_dev) return fail(c, VUIB_ERR_NULL, "slots is NULL");
     if (!new_dev && p->max_new < 1) return fail(c, VUIB_ERR_RANGE, "one new row each, but max_new is %d", p->max_new);
     const Shape s = shape_of(c, p);
-    if (most_units(c, p, s) > 0x7fffffffll / 2) return fail(c, VUIB_ERR_RANGE, "too many units of work for one plan");
+    const long long len = (long long)c->cfg.max_blocks << c->block_shift;
+    const long long tiles = ceil_div((long long)p->n_rows * (c->cfg.n_heads / c->cfg.n_kv_heads), s.cols) + p->n_seqs;
+    if (s.form == CHUNK ? tiles * (len / KC_STEP + 1) >= KV4_MANY : most_units(c, p, s) >= KV4_MANY) return fail(c, VUIB_ERR_RANGE, "too many units of work for one plan");
     Kv4PlanArgs a = {};
     a.c = c->cache;
     a.slots = slots_dev; a.new_lens = new_dev; a.at = at_dev;
     a.n = p->n_seqs; a.n_rows = p->n_rows; a.max_new = p->max_new;
-    a.group = c->cfg.n_heads / c->cfg.n_kv_heads; a.cols = s.cols; a.split = s.split;
+    a.group = c->cfg.n_heads / c->cfg.n_kv_heads; a.cols = s.cols; a.split = s.split; a.steps = s.form == CHUNK;
     a.entries = plan_entries(p); a.cu_units = plan_units(p); a.cu_work = plan_work(p); a.cu_tiles = plan_tiles(p); a.row_entry = plan_row_entry(p);
     a.cu_rows = p->cu_rows;
     a.row_slot = p->row_slot; a.row_pos = p->row_pos; a.slot_map = reinterpret_cast<long long*>(p->slot_map);
@@ -318,8 +326,8 @@ extern "C" int32_t vuib_kv4_attention_workspace(VuibKv4* c, const VuibKv4Plan* p
     *bytes = 0;
     if (!p->n_rows || !p->max_new) return VUIB_OK;
     const Shape s = shape_of(c, p);
-    if (most_parts(c, s) <= 1) return VUIB_OK;
-    const long long items = most_units(c, p, s) * c->cfg.n_kv_heads;
+    if (s.form != CHUNK && most_parts(c, s) <= 1) return VUIB_OK;
+    const long long items = most_items(c, p, s);
     *bytes = acc_bytes(c, items, s.cols) + (size_t)items * s.cols * 8;
     return VUIB_OK;
 }
@@ -339,7 +347,7 @@ extern "C" int32_t vuib_kv4_attention(VuibKv4* c, int32_t layer, const VuibKv4Pl
     if (need && (!ws_dev || ws_bytes < need || reinterpret_cast<uintptr_t>(ws_dev) & 255))
         return fail(c, VUIB_ERR_WORKSPACE, "workspace of %zu bytes, 256-byte aligned, needed", need);
     const Shape s = shape_of(c, p);
-    const long long items = most_units(c, p, s) * c->cfg.n_kv_heads;
+    const long long items = most_items(c, p, s);
     Kv4AttnArgs a = {};
     a.c = c->cache;
     a.c.pool += c->layer_bytes * layer;

@@ -15,7 +15,7 @@
 
 namespace vuik {
 
-constexpr int KC_COLS = 256, KC_TILE = 128, KC_STEP = 128;
+constexpr int KC_TILE = 128;
 constexpr int KC_FILL = 4, KC_WARPS = 13, KC_THREADS = KC_WARPS * 32;      // warps 0-3 fill, 4-7 and 8-11 softmax, 12 MMA
 
 template <int NG>
@@ -28,15 +28,86 @@ struct KcShared {
     static constexpr int TOTAL = BARS + 256 + 1024;        // and room to start at a multiple of 1024
 };
 
-// Steps of 128 positions that the two tiles of a unit take; 0: a tile without columns, or one that does not see this split.
-__device__ __forceinline__ void kc_steps(const Kv4AttnArgs& a, const Kv4Walk& u, int (&n)[2]) {
+// The CTAs share out all steps of all column tiles and kv heads evenly, in the order sequence, column tile, kv head, step.  A run is what a
+// CTA has of one (column tile, kv head): all its steps, and the output is written; or a part, and its sums go to one of the CTA's two places
+// for parts (the first if the run goes on from the CTA before, the second if it begins here).
+struct KcRun {
+    int entry, ctile, head, cost, from, to, steps[2];   // of the tiles: steps to take; cost: steps of the whole (tile, head)
+    int4 e;
+    long long at, end;      // work before the run, and where the CTA's share ends
+};
+
+__device__ __forceinline__ void kc_enter(const Kv4AttnArgs& a, KcRun& u, int from) {
+    u.cost = kc_cost(u.e.y, u.e.z, a.group, u.ctile);
+    u.from = from;
+    u.to = (int)min((long long)u.cost, from + u.end - u.at);
     const int all = u.e.z * a.group, first = u.ctile * KC_COLS;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
         const int end = min(first + (x + 1) * KC_TILE, all);          // one past the tile's last column
-        const int hi = min(u.hi, u.e.y + by_group(a, max(end - 1, 0)) + 1);
-        n[x] = end > first + x * KC_TILE ? max(0, (hi - u.base + KC_STEP - 1) / KC_STEP) : 0;
+        const int sees = end > first + x * KC_TILE ? (u.e.y + by_group(a, end - 1) + KC_STEP) / KC_STEP : 0;
+        u.steps[x] = max(min(u.to, sees) - u.from, 0);
     }
+}
+
+__device__ __forceinline__ bool kc_begin(const Kv4AttnArgs& a, KcRun& u, int lane) {
+    const long long total = (long long)__ldcg(a.cu_work + a.n) * a.c.n_kv;
+    u.at = total * blockIdx.x / gridDim.x;
+    u.end = total * (blockIdx.x + 1) / gridDim.x;
+    if (u.at >= u.end) return false;
+    int lo = 0, hi = a.n;      // work before lo <= at < work before hi
+    long long before = 0;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, i = lo + lane * step;
+        const long long work = i < hi ? (long long)__ldcg(a.cu_work + i) * a.c.n_kv : 0x7fffffffffffffffll;
+        const int k = 31 - __clz(__ballot_sync(0xffffffffu, work <= u.at));
+        before = __shfl_sync(0xffffffffu, work, k);
+        lo += k * step;
+        hi = min(hi, lo + step);
+    }
+    u.entry = lo;
+    u.e = __ldcg(a.entries + lo);
+    long long into = u.at - before;      // and now the column tile, 32 at a time
+    for (u.ctile = 0;; u.ctile += 32) {
+        const int t = u.ctile + lane;
+        const long long mine = t * KC_COLS < u.e.z * a.group ? (long long)kc_cost(u.e.y, u.e.z, a.group, t) * a.c.n_kv : 0;
+        long long sum = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += y;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, sum > into);
+        if (past) {
+            const int k = __ffs(past) - 1;
+            into -= __shfl_sync(0xffffffffu, sum - mine, k);
+            u.ctile += k;
+            break;
+        }
+        into -= __shfl_sync(0xffffffffu, sum, 31);
+        if ((u.ctile + 32) * KC_COLS >= u.e.z * a.group) return false;      // not reached: the entry's work is the sum of its tiles'
+    }
+    const int cost = kc_cost(u.e.y, u.e.z, a.group, u.ctile);
+    u.head = (int)(into / cost);
+    kc_enter(a, u, (int)(into % cost));
+    return true;
+}
+
+__device__ __forceinline__ bool kc_next(const Kv4AttnArgs& a, KcRun& u) {
+    u.at += u.to - u.from;
+    if (u.at >= u.end) return false;
+    if (++u.head == a.c.n_kv) {
+        u.head = 0;
+        if (++u.ctile * KC_COLS >= u.e.z * a.group) {
+            u.ctile = 0;
+            do {
+                if (++u.entry >= a.n) return false;
+                u.e = __ldcg(a.entries + u.entry);
+            } while (u.e.z == 0);
+        }
+    }
+    kc_enter(a, u, 0);
+    return true;
 }
 
 struct KcBars {
@@ -45,10 +116,9 @@ struct KcBars {
     __device__ __forceinline__ uint32_t s_full(int x) const { return at + 16 + 8 * x; }
     __device__ __forceinline__ uint32_t p_full(int x) const { return at + 32 + 8 * x; }
     __device__ __forceinline__ uint32_t o_full(int x) const { return at + 48 + 8 * x; }
-    __device__ __forceinline__ uint32_t pv_done(int x) const { return at + 64 + 8 * x; }
-    __device__ __forceinline__ uint32_t kv_full(int s) const { return at + 80 + 8 * s; }
-    __device__ __forceinline__ uint32_t kv_empty(int s) const { return at + 112 + 8 * s; }
-    __device__ __forceinline__ uint32_t tmem() const { return at + 144; }
+    __device__ __forceinline__ uint32_t kv_full(int s) const { return at + 64 + 8 * s; }
+    __device__ __forceinline__ uint32_t kv_empty(int s) const { return at + 96 + 8 * s; }
+    __device__ __forceinline__ uint32_t tmem() const { return at + 128; }
 };
 
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -84,11 +154,20 @@ __device__ __forceinline__ void tm_load32(uint32_t at, uint32_t (&r)[32]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,"
                  "%27,%28,%29,%30,%31}, [%32];" : KC_R32(r) : "r"(at));
 }
+__device__ __forceinline__ void tm_load16(uint32_t at, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                   "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(at));
+}
 // The wait names the registers, so that nothing that reads them moves in front of it.
 #define KC_RW32(r) "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), \
     "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),      \
     "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
 __device__ __forceinline__ void tm_wait(uint32_t (&r)[32]) { asm volatile("tcgen05.wait::ld.sync.aligned;" : KC_RW32(r)::"memory"); }
+__device__ __forceinline__ void tm_wait(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+}
 __device__ __forceinline__ void tm_store32(uint32_t at, const uint32_t (&r)[32]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,"
                  "%27,%28,%29,%30,%31,%32};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
@@ -114,29 +193,25 @@ template <int NG>
 __device__ __forceinline__ void kc_fill(const Kv4AttnArgs& a, uint32_t ring, const KcBars bars, int w, int lane) {
     using S = KcShared<NG>;
     const int g = lane >> 2, t = lane & 3, tiles = 1 << (a.c.block_shift - 4);
-    Kv4Walk u = {};
-    long long to = 0;
+    KcRun u;
     unsigned n = 0;        // tiles written: keys and values in turn
-    bool more = walk_begin<KC_COLS>(a, u, to, lane);
-    while (more) {
-        int steps[2];
-        kc_steps(a, u, steps);
-        const int last = max(steps[0], steps[1]);
+    for (bool more = kc_begin(a, u, lane); more; more = kc_next(a, u)) {
+        const int last = max(u.steps[0], u.steps[1]), base = u.from * KC_STEP, len = u.e.y + u.e.z;
         int id[2] = {0, 0};
         auto read_ids = [&](int j) {
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const int pos = u.base + j * KC_STEP + (k * KC_FILL + w) * KV4_TILE;
-                id[k] = pos < u.hi ? __ldcg(a.c.table + (size_t)u.e.x * a.c.max_blocks + (pos >> a.c.block_shift)) : -1;
+                const int pos = base + j * KC_STEP + (k * KC_FILL + w) * KV4_TILE;
+                id[k] = pos < len ? __ldcg(a.c.table + (size_t)u.e.x * a.c.max_blocks + (pos >> a.c.block_shift)) : -1;
             }
         };
         const unsigned char* at[2];
         auto place = [&](int j) {       // of the step whose blocks are in id
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const int pos = u.base + j * KC_STEP + (k * KC_FILL + w) * KV4_TILE;
+                const int pos = base + j * KC_STEP + (k * KC_FILL + w) * KV4_TILE;
                 at[k] = nullptr;
-                if (pos < u.hi) {
+                if (pos < len) {
                     int b = id[k];
                     if ((unsigned)b >= (unsigned)a.c.n_blocks) {
                         if (lane == 0) atomicOr(a.c.flag, KV4_BAD_BLOCK);
@@ -233,8 +308,6 @@ __device__ __forceinline__ void kc_fill(const Kv4AttnArgs& a, uint32_t ring, con
             }
             done();
         }
-        walk_next<KC_COLS>(a, u);
-        more = u.at < to && u.entry < a.n;
     }
 }
 
@@ -243,13 +316,8 @@ template <int NG>
 __device__ __forceinline__ void kc_issue(const Kv4AttnArgs& a, uint32_t smem, const KcBars bars, uint32_t tmem, int lane) {
     using S = KcShared<NG>;
     const uint32_t ring = smem + 2 * S::Q;
-    Kv4Walk u = {};
-    long long to = 0;
+    KcRun u;
     unsigned n = 0, units[2] = {0, 0}, steps_done[2] = {0, 0};
-#ifdef KC_WAIT
-    unsigned pv[2] = {0, 0};
-#endif
-    bool more = walk_begin<KC_COLS>(a, u, to, lane);
     auto scores = [&](int x, unsigned slot) {       // S of tile x
         const uint64_t q = tile_desc(smem + x * S::Q), k = tile_desc(ring + slot * S::SLOT);
 #pragma unroll
@@ -265,9 +333,8 @@ __device__ __forceinline__ void kc_issue(const Kv4AttnArgs& a, uint32_t smem, co
         for (int i = 0; i < KC_STEP / 16; ++i)
             mma_ts(tmem + 256 + x * S::HD, tmem + x * KC_TILE + i * 8, v + (i >> 2) * (S::HD * 128 >> 4) + (i & 3) * 2, kc_idesc(S::HD), add || i > 0);
     };
-    while (more) {
-        int steps[2];
-        kc_steps(a, u, steps);
+    for (bool more = kc_begin(a, u, lane); more; more = kc_next(a, u)) {
+        const int(&steps)[2] = u.steps;
         const int last = max(steps[0], steps[1]);
         if (last > 0) {
             if (!bar_wait(bars.kv_full(n % S::SLOTS), (n / S::SLOTS) & 1)) return give_up(a.c.flag);
@@ -293,16 +360,9 @@ __device__ __forceinline__ void kc_issue(const Kv4AttnArgs& a, uint32_t smem, co
                     if (elect_one()) {
                         sums(x, vslot, j > 0);
                         if (j + 1 == steps[x]) tc_commit(bars.o_full(x));
-#ifdef KC_WAIT
-                        else tc_commit(bars.pv_done(x));
-#endif
                     }
                     __syncwarp();
                     if (j + 1 < steps[x]) {
-#ifdef KC_WAIT
-                        if (!bar_wait(bars.pv_done(x), pv[x]++ & 1)) return give_up(a.c.flag);
-                        tc_after();
-#endif
                         if (elect_one()) scores(x, kslot);
                         __syncwarp();
                     }
@@ -316,8 +376,6 @@ __device__ __forceinline__ void kc_issue(const Kv4AttnArgs& a, uint32_t smem, co
                 n += j + 1 < last ? 2 : 1;
             }
         }
-        walk_next<KC_COLS>(a, u);
-        more = u.at < to && u.entry < a.n;
     }
 }
 
@@ -327,14 +385,10 @@ __device__ __forceinline__ void kc_softmax(const Kv4AttnArgs& a, uint32_t smem, 
     using S = KcShared<NG>;
     constexpr int HD = S::HD;
     const uint32_t lanes = tmem + ((uint32_t)(r & ~31) << 16), scores = lanes + x * KC_TILE, sums = lanes + 256 + x * HD;
-    Kv4Walk u = {};
-    long long to = 0;
-    unsigned n = 0, units = 0;       // steps, units with steps
-    bool more = walk_begin<KC_COLS>(a, u, to, lane);
-    while (more) {
-        int steps[2];
-        kc_steps(a, u, steps);
-        const int mine = steps[x], col = u.ctile * KC_COLS + x * KC_TILE + r;
+    KcRun u;
+    unsigned n = 0, units = 0;       // steps, runs with steps
+    for (bool more = kc_begin(a, u, lane); more; more = kc_next(a, u)) {
+        const int mine = u.steps[x], col = u.ctile * KC_COLS + x * KC_TILE + r;
         const bool there = col < u.e.z * a.group;
         const int row = there ? by_group(a, col) : 0, head = u.head * a.group + (there ? col - row * a.group : 0);
         const int limit = there ? u.e.y + row : -1, all = u.e.y + by_group(a, u.ctile * KC_COLS + x * KC_TILE);
@@ -367,87 +421,91 @@ __device__ __forceinline__ void kc_softmax(const Kv4AttnArgs& a, uint32_t smem, 
             for (int j = 0; j < mine; ++j, ++n) {
                 if (!bar_wait(bars.s_full(x), n & 1)) return give_up(a.c.flag);
                 tc_after();
-                const int base = u.base + j * KC_STEP;
+                const int base = (u.from + j) * KC_STEP;
                 const bool whole = base + KC_STEP - 1 <= all;        // every column sees all of the step
-                uint32_t s0[32], s1[32];
-                auto mask = [&](uint32_t (&s)[32], int first) {
+                uint32_t s0[16], s1[16];
+                auto mask = [&](uint32_t (&s)[16], int first) {
                     if (!whole) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
+                        for (int i = 0; i < 16; ++i)
                             if (base + first + i > limit) s[i] = 0xff800000u;
                     }
                 };
+                // Weights are taken against a reference, the first step's maximum: below 2^14 of it they fit f16 and the sums all the same, so
+                // a step looks for its own maximum while it weighs.  Only a column that has seen nothing yet, or that this step carries beyond
+                // 2^14, has to find the maximum first; each column decides for itself, so that its bits are its own.
                 float top = -INFINITY;
-                auto most = [&](const uint32_t (&s)[32]) {
+                auto most = [&](const uint32_t (&s)[16]) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) top = fmaxf(fmaxf(top, __uint_as_float(s[i])), __uint_as_float(s[i + 1]));
+                    for (int i = 0; i < 16; i += 2) top = fmaxf(fmaxf(top, __uint_as_float(s[i])), __uint_as_float(s[i + 1]));
                 };
-                tm_load32(scores, s0);
-                tm_wait(s0);
-                tm_load32(scores + 32, s1);
-                mask(s0, 0);
-                most(s0);
-                tm_wait(s1);
-                tm_load32(scores + 64, s0);
-                mask(s1, 32);
-                most(s1);
-                tm_wait(s0);
-                tm_load32(scores + 96, s1);
-                mask(s0, 64);
-                most(s0);
-                tm_wait(s1);
-                tm_load32(scores, s0);
-                mask(s1, 96);
-                most(s1);
-                top *= factor;
-                if (j == 0) {
-                    m = top;
-                } else {
-                    // the reference stays while weights remain below 2^8; each column decides for itself
-                    const bool far = top > m + 8.f || (m == -INFINITY && top > m);
-                    if (__any_sync(0xffffffffu, far)) {
-                        const float old = far ? (m == -INFINITY ? 0.f : ex2(m - top)) : 1.f;
-                        if (far) m = top;
-                        l *= old;
+                auto look = [&]() {         // the step's maximum, times the factor
+                    top = -INFINITY;
+#pragma unroll 1
+                    for (int i = 0; i < KC_STEP; i += 16) {
+                        tm_load16(scores + i, s0);
                         tm_wait(s0);
-#pragma unroll
-                        for (int i = 0; i < HD; i += 32) {
-                            tm_load32(sums + i, s1);
-                            tm_wait(s1);
-#pragma unroll
-                            for (int k = 0; k < 32; ++k) s1[k] = __float_as_uint(__uint_as_float(s1[k]) * old);
-                            tm_store32(sums + i, s1);
-                        }
+                        mask(s0, i);
+                        most(s0);
                     }
+                    top *= factor;
+                };
+                if (__any_sync(0xffffffffu, m == -INFINITY)) {
+                    look();
+                    if (m == -INFINITY) m = top;      // its sums are zeros so far
+                    top = -INFINITY;
                 }
-                const float less = m == -INFINITY ? 0.f : -m;        // nothing seen yet: weights of exp(-inf) = 0
-                float part[4] = {0.f, 0.f, 0.f, 0.f};
-                auto weigh = [&](uint32_t (&s)[32], int first) {
-                    uint32_t p[16];
+                float part[4];
+                uint32_t p[64];
+                auto weigh = [&](uint32_t (&s)[16], int first, float less) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
+                    for (int i = 0; i < 16; i += 2) {
                         const float w0 = ex2(fmaf(__uint_as_float(s[i]), factor, less)), w1 = ex2(fmaf(__uint_as_float(s[i + 1]), factor, less));
                         part[i & 2] += w0;
                         part[(i & 2) + 1] += w1;
-                        p[i >> 1] = pack_h2(w0, w1);
+                        p[(first + i) >> 1] = pack_h2(w0, w1);
                     }
-                    tm_store16(scores + (first >> 1), p);       // over scores that have been read
                 };
-                tm_wait(s0);
-                tm_load32(scores + 32, s1);
-                mask(s0, 0);
-                weigh(s0, 0);
-                tm_wait(s1);
-                tm_load32(scores + 64, s0);
-                mask(s1, 32);
-                weigh(s1, 32);
-                tm_wait(s0);
-                tm_load32(scores + 96, s1);
-                mask(s0, 64);
-                weigh(s0, 64);
-                tm_wait(s1);
-                mask(s1, 96);
-                weigh(s1, 96);
+                auto pass = [&]() {
+                    const float less = m == -INFINITY ? 0.f : -m;        // nothing seen yet: weights of exp(-inf) = 0
+                    part[0] = part[1] = part[2] = part[3] = 0.f;
+                    tm_load16(scores, s0);
+#pragma unroll
+                    for (int i = 0; i < KC_STEP; i += 32) {
+                        tm_wait(s0);
+                        tm_load16(scores + i + 16, s1);
+                        mask(s0, i);
+                        most(s0);
+                        weigh(s0, i, less);
+                        tm_wait(s1);
+                        if (i + 32 < KC_STEP) tm_load16(scores + i + 32, s0);
+                        mask(s1, i + 16);
+                        most(s1);
+                        weigh(s1, i + 16, less);
+                    }
+                };
+                pass();
+                top *= factor;
+                if (__any_sync(0xffffffffu, top > m + 14.f)) {
+                    const bool far = top > m + 14.f;
+                    const float old = far ? ex2(m - top) : 1.f;
+                    if (far) m = top;
+                    l *= old;
+                    if (j > 0) {
+#pragma unroll 1
+                        for (int i = 0; i < HD; i += 16) {
+                            tm_load16(sums + i, s0);
+                            tm_wait(s0);
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) s0[k] = __float_as_uint(__uint_as_float(s0[k]) * old);
+                            tm_store16(sums + i, s0);
+                        }
+                    }
+                    pass();
+                }
+                // over the scores, which have been read
+                tm_store32(scores, reinterpret_cast<uint32_t(&)[32]>(p[0]));
+                tm_store32(scores + 32, reinterpret_cast<uint32_t(&)[32]>(p[32]));
                 l += (part[0] + part[1]) + (part[2] + part[3]);
                 tm_stored();
                 tc_before();
@@ -458,11 +516,13 @@ __device__ __forceinline__ void kc_softmax(const Kv4AttnArgs& a, uint32_t smem, 
             ++units;
             tc_after();
         }
-        if (u.splits > 1 && there) a.ml[u.w * KC_COLS + x * KC_TILE + r] = make_float2(m, l);
+        const bool entire = u.to - u.from == u.cost;
+        const size_t place = (size_t)(2 * blockIdx.x + (u.from == 0)) * KC_COLS + x * KC_TILE + r;
+        if (!entire && there) a.ml[place] = make_float2(m, l);
         if (mine > 0) {
             const float inv = l == 0.f ? 0.f : 1.f / l;
             __nv_bfloat16* dst = a.out + (long long)(u.e.w + row) * a.out_stride + head * HD;
-            float* part = a.acc + (size_t)(u.w * KC_COLS + x * KC_TILE + r) * HD;
+            float* part = a.acc + place * HD;
 #pragma unroll
             for (int i = 0; i < HD; i += 32) {
                 uint32_t v[32];
@@ -470,7 +530,7 @@ __device__ __forceinline__ void kc_softmax(const Kv4AttnArgs& a, uint32_t smem, 
                 tm_wait(v);
                 if (!there) continue;
                 // element 4 g + k of the group is column 8 k + g
-                if (u.splits == 1) {
+                if (entire) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         uint32_t w[4];
@@ -489,8 +549,6 @@ __device__ __forceinline__ void kc_softmax(const Kv4AttnArgs& a, uint32_t smem, 
                 }
             }
         }
-        walk_next<KC_COLS>(a, u);
-        more = u.at < to && u.entry < a.n;
     }
 }
 
@@ -507,7 +565,6 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv4_attn_chunk(const Kv4AttnA
             bar_init(bars.s_full(x), 1);
             bar_init(bars.p_full(x), 4);
             bar_init(bars.o_full(x), 1);
-            bar_init(bars.pv_done(x), 1);
         }
         for (int s = 0; s < S::SLOTS; ++s) {
             bar_init(bars.kv_full(s), KC_FILL);
@@ -533,6 +590,56 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv4_attn_chunk(const Kv4AttnA
     __syncthreads();
     tc_after();
     if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+// Adds up the parts of the (column tile, kv head)s that several CTAs had, in the order of the positions: a warp a (row, query head).  Where a row
+// belongs is read from the plan before the attention has ended, as in k_kv4_merge; `ctas` is the attention's grid.
+template <int NG>
+__global__ void __launch_bounds__(128) k_kv4_chunk_merge(const Kv4AttnArgs a, const int ctas) {
+    constexpr int HD = NG * KV4_GROUP;
+    const int lane = threadIdx.x & 31, heads = a.c.n_kv * a.group;
+    const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (a.early) pdl_launch();
+    const int row = (int)(id / heads), head = (int)(id % heads), kv = by_group(a, head);
+    const int entry = row < a.n_rows ? __ldcg(a.row_entry + row) : -1;
+    if (entry < 0) return pdl_wait();
+    const int4 e = __ldcg(a.entries + entry);
+    const long long total = (long long)__ldcg(a.cu_work + a.n) * a.c.n_kv;
+    long long at = 0;
+    const int col = (row - e.w) * a.group + head - kv * a.group, ctile = col / KC_COLS;
+    for (int t = lane; t < ctile; t += 32) at += kc_cost(e.y, e.z, a.group, t);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) at += __shfl_xor_sync(0xffffffffu, at, o);
+    const int cost = kc_cost(e.y, e.z, a.group, ctile);
+    at = (at + __ldcg(a.cu_work + entry)) * a.c.n_kv + (long long)kv * cost;
+    // the CTAs that had steps [at, at + cost): CTA b has [total b / ctas, total (b + 1) / ctas)
+    const int first = (int)(((at + 1) * ctas - 1) / total), last = (int)(((at + cost) * ctas - 1) / total);
+    if (first == last) return pdl_wait();
+    auto place = [&](int b) { return (size_t)(2 * b + (b == first)) * KC_COLS + col % KC_COLS; };
+    auto idle = [&](int b) { return total * b / ctas == total * (b + 1) / ctas; };      // fewer steps than CTAs: some have none
+    pdl_wait();
+    float best = -INFINITY, sum = 0.f, out[NG];
+    for (int b = first + lane; b <= last; b += 32)
+        if (!idle(b)) best = fmaxf(best, __ldcg(&a.ml[place(b)].x));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+    const float now = best == -INFINITY ? 0.f : best;
+#pragma unroll
+    for (int j = 0; j < NG; ++j) out[j] = 0.f;
+#pragma unroll 4
+    for (int b = first; b <= last; ++b) {
+        if (idle(b)) continue;
+        const float2 part = __ldcg(a.ml + place(b));
+        if (part.y == 0.f) continue;      // nothing seen there: no sums were written
+        const float f = ex2(part.x - now);
+        sum += f * part.y;
+#pragma unroll
+        for (int j = 0; j < NG; ++j) out[j] += f * __ldcg(a.acc + place(b) * HD + lane * NG + j);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    __nv_bfloat16* dst = a.out + (long long)row * a.out_stride + head * HD + lane * NG;
+#pragma unroll
+    for (int j = 0; j < NG; ++j) dst[j] = __float2bfloat16_rn(out[j] * inv);
 }
 
 }  // namespace vuik

@@ -62,6 +62,14 @@ struct Kv4Split {
     __host__ __device__ int work_of(int positions) const { return 1 + (weigh ? (positions + 63) / 64 : 0); }            // of one
 };
 
+// Work of attention in the form for chunks: steps of 128 positions that a tile of 256 columns (rows x query heads of a kv head) takes, from
+// the sequence's first position to the last that any of its rows sees.
+constexpr int KC_COLS = 256, KC_STEP = 128;
+__device__ __forceinline__ int kc_cost(int start, int rows, int group, int ctile) {
+    const int last = (min((ctile + 1) * KC_COLS, rows * group) - 1) / group;
+    return (start + last + KC_STEP) / KC_STEP;
+}
+
 // ------------------------------------------------------------------------------------------------ tables and maps
 struct Kv4PlanArgs {
     Kv4Cache c;
@@ -69,6 +77,7 @@ struct Kv4PlanArgs {
     int n, n_rows, max_new;
     int group, cols;            // query heads a kv head, columns of a tile: attention's units are counted here
     Kv4Split split;
+    bool steps;                 // work is counted in steps of tiles (kc_cost)
     int4* entries; int32_t* cu_units; int32_t* cu_work; int32_t* cu_tiles; int32_t* row_entry;    // the plan's work array
     int32_t* cu_rows; int32_t* row_slot; int32_t* row_pos; long long* slot_map;
 };
@@ -207,7 +216,14 @@ __global__ void __launch_bounds__(1024) k_kv4_plan(const Kv4PlanArgs a) {
     int part[5] = {0, 0, 0, 0, 0}, whole[5];   // blocks got, rows, units of attention (of a kv head) and their work, tiles of 16 positions written
     auto times_tiles = [&](int i, int of_one) { return (int)min(((long long)s_new[i] * a.group + a.cols - 1) / a.cols * of_one, (long long)KV4_MANY); };
     auto units_of = [&](int i) { return s_new[i] ? times_tiles(i, a.split.parts(s_start[i] + (long long)s_new[i])) : 0; };
-    auto work_of = [&](int i) { return s_new[i] ? times_tiles(i, a.split.work(s_start[i] + (long long)s_new[i])) : 0; };
+    auto work_of = [&](int i) {
+        if (a.steps) {
+            int sum = 0;
+            for (int t = 0; t * KC_COLS < s_new[i] * a.group; ++t) sum = min(sum + kc_cost(s_start[i], s_new[i], a.group, t), KV4_MANY);
+            return sum;
+        }
+        return s_new[i] ? times_tiles(i, a.split.work(s_start[i] + (long long)s_new[i])) : 0;
+    };
     auto tiles_of = [&](int i) { return s_new[i] ? ((s_start[i] + s_new[i] - 1) >> 4) - (s_start[i] >> 4) + 1 : 0; };
     for (int i = first; i < last; ++i) {
         s_drop[i] = blocks[0];
