@@ -158,7 +158,7 @@ cudaError_t launch_attn(VuibKv4* c, const Shape& s, void (*kern)(Kv4AttnArgs), i
     const long long grid = s.form == CHUNK ? c->sms : min(items, room), rows = (long long)a.n_rows * c->cfg.n_heads;
     e = launch(c, kern, dim3((unsigned)grid), threads, smem, 1, stream, a);
     if (e != cudaSuccess || !merge) return e;
-    if (s.form == CHUNK) return launch(c, k_kv4_chunk_merge<NG>, dim3((unsigned)ceil_div(rows, 4)), 128, 0, 1, stream, a, (int)grid);
+    if (s.form == CHUNK) return launch(c, k_kv4_chunk_merge<NG>, dim3((unsigned)grid), 1024, 0, 1, stream, a);
     if (most_parts(c, s) <= 32)
         return launch(c, k_kv4_merge<NG, 1>, dim3((unsigned)ceil_div(rows, 4)), 128, 0, 1, stream, a, s.cols);
     return launch(c, k_kv4_merge<NG, 8>, dim3((unsigned)rows), 256, 0, 1, stream, a, s.cols);

@@ -50,11 +50,10 @@ __device__ __forceinline__ void kc_enter(const Kv4AttnArgs& a, KcRun& u, int fro
     }
 }
 
-__device__ __forceinline__ bool kc_begin(const Kv4AttnArgs& a, KcRun& u, int lane) {
-    const long long total = (long long)__ldcg(a.cu_work + a.n) * a.c.n_kv;
-    u.at = total * blockIdx.x / gridDim.x;
-    u.end = total * (blockIdx.x + 1) / gridDim.x;
-    if (u.at >= u.end) return false;
+// The run that begins with step number `at` of all, found by the whole warp.
+__device__ __forceinline__ bool kc_find(const Kv4AttnArgs& a, KcRun& u, long long at, long long end, int lane) {
+    u.at = at;
+    u.end = end;
     int lo = 0, hi = a.n;      // work before lo <= at < work before hi
     long long before = 0;
     while (hi - lo > 1) {
@@ -91,6 +90,12 @@ __device__ __forceinline__ bool kc_begin(const Kv4AttnArgs& a, KcRun& u, int lan
     u.head = (int)(into / cost);
     kc_enter(a, u, (int)(into % cost));
     return true;
+}
+
+__device__ __forceinline__ bool kc_begin(const Kv4AttnArgs& a, KcRun& u, int lane) {
+    const long long total = (long long)__ldcg(a.cu_work + a.n) * a.c.n_kv;
+    const long long at = total * blockIdx.x / gridDim.x, end = total * (blockIdx.x + 1) / gridDim.x;
+    return at < end && kc_find(a, u, at, end, lane);
 }
 
 __device__ __forceinline__ bool kc_next(const Kv4AttnArgs& a, KcRun& u) {
@@ -132,19 +137,32 @@ __device__ __forceinline__ bool elect_one() {
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
     return p != 0;
 }
-// Descriptor of a K-major tile with the 128-byte swizzle (rows 128 bytes apart, groups of 8 rows 1024).
-__device__ __forceinline__ uint64_t tile_desc(uint32_t addr) {
-    return (uint64_t)((1024u >> 4) | 1u << 14 | 2u << 29) << 32 | ((addr >> 4 & 0x3FFF) | 1u << 16);
-}
+// Low word of the descriptor of a K-major tile with the 128-byte swizzle (rows 128 bytes apart, groups of 8 rows 1024); the high word is the
+// same for all.  The tensor pipe has next to no queue, so what the issuing thread spends on descriptors the pipe waits for: four MMAs (64 of
+// K) are one block that adds to 32-bit words.
+__device__ __forceinline__ uint32_t tile_desc(uint32_t addr) { return (addr >> 4 & 0x3FFF) | 1u << 16; }
+constexpr uint32_t KC_DESC_HI = (1024u >> 4) | 1u << 14 | 2u << 29;
 // f16 operands, fp32 sums, both K-major, 128 rows, n columns.
 __host__ __device__ constexpr uint32_t kc_idesc(int n) { return 1u << 4 | (uint32_t)(n >> 3) << 17 | 8u << 24; }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+// N (4 or 2) MMAs of 16 of K with A from shared memory; the first adds to D unless FIRST.
+template <int N, bool FIRST>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+#define KC_SS(off, p) "add.u32 t, %1, " off ";\n\tadd.u32 u, %2, " off ";\n\tmov.b64 x, {t, %3};\n\tmov.b64 y, {u, %3};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %4, " p ";\n\t"
+    if constexpr (N == 4)
+        asm volatile("{\n\t.reg .b64 x, y;\n\t.reg .b32 t, u;\n\t" KC_SS("0", "%5") KC_SS("2", "1") KC_SS("4", "1") KC_SS("6", "1") "}"
+                     ::"r"(d), "r"(a), "r"(b), "r"(KC_DESC_HI), "r"(idesc), "n"(FIRST ? 0 : 1) : "memory");
+    else
+        asm volatile("{\n\t.reg .b64 x, y;\n\t.reg .b32 t, u;\n\t" KC_SS("0", "%5") KC_SS("2", "1") "}"
+                     ::"r"(d), "r"(a), "r"(b), "r"(KC_DESC_HI), "r"(idesc), "n"(FIRST ? 0 : 1) : "memory");
+#undef KC_SS
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, int add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+// Four MMAs of 16 of K with A from tensor memory (two f16 a column).
+template <bool FIRST>
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+#define KC_TS(aoff, boff, p) "add.u32 t, %1, " aoff ";\n\tadd.u32 u, %2, " boff ";\n\tmov.b64 y, {u, %3};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [t], y, %4, " p ";\n\t"
+    asm volatile("{\n\t.reg .b64 y;\n\t.reg .b32 t, u;\n\t" KC_TS("0", "0", "%5") KC_TS("8", "2", "1") KC_TS("16", "4", "1") KC_TS("24", "6", "1") "}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(KC_DESC_HI), "r"(idesc), "n"(FIRST ? 0 : 1) : "memory");
+#undef KC_TS
 }
 #define KC_R32(r) "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), \
     "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),     \
@@ -319,19 +337,16 @@ __device__ __forceinline__ void kc_issue(const Kv4AttnArgs& a, uint32_t smem, co
     KcRun u;
     unsigned n = 0, units[2] = {0, 0}, steps_done[2] = {0, 0};
     auto scores = [&](int x, unsigned slot) {       // S of tile x
-        const uint64_t q = tile_desc(smem + x * S::Q), k = tile_desc(ring + slot * S::SLOT);
-#pragma unroll
-        for (int i = 0; i < S::HD / 16; ++i) {
-            const uint64_t off = (i >> 2) * (S::BLOCK >> 4) + (i & 3) * 2;
-            mma_ss(tmem + x * KC_TILE, q + off, k + off, kc_idesc(KC_STEP), i > 0);
-        }
+        const uint32_t q = tile_desc(smem + x * S::Q), k = tile_desc(ring + slot * S::SLOT), d = tmem + x * KC_TILE;
+        mma_ss<4, true>(d, q, k, kc_idesc(KC_STEP));
+        if constexpr (NG > 2) mma_ss<NG == 4 ? 4 : 2, false>(d, q + (S::BLOCK >> 4), k + (S::BLOCK >> 4), kc_idesc(KC_STEP));
         tc_commit(bars.s_full(x));
     };
     auto sums = [&](int x, unsigned slot, bool add) {
-        const uint64_t v = tile_desc(ring + slot * S::SLOT);
-#pragma unroll
-        for (int i = 0; i < KC_STEP / 16; ++i)
-            mma_ts(tmem + 256 + x * S::HD, tmem + x * KC_TILE + i * 8, v + (i >> 2) * (S::HD * 128 >> 4) + (i & 3) * 2, kc_idesc(S::HD), add || i > 0);
+        const uint32_t v = tile_desc(ring + slot * S::SLOT), p = tmem + x * KC_TILE, d = tmem + 256 + x * S::HD;
+        if (add) mma_ts<false>(d, p, v, kc_idesc(S::HD));
+        else mma_ts<true>(d, p, v, kc_idesc(S::HD));
+        mma_ts<false>(d, p + 32, v + (S::HD * 128 >> 4), kc_idesc(S::HD));
     };
     for (bool more = kc_begin(a, u, lane); more; more = kc_next(a, u)) {
         const int(&steps)[2] = u.steps;
@@ -592,54 +607,68 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv4_attn_chunk(const Kv4AttnA
     if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
-// Adds up the parts of the (column tile, kv head)s that several CTAs had, in the order of the positions: a warp a (row, query head).  Where a row
-// belongs is read from the plan before the attention has ended, as in k_kv4_merge; `ctas` is the attention's grid.
+// Adds up the parts of the (column tile, kv head)s that several CTAs had, in the order of the positions.  CTA b of `ctas` does it for the one
+// whose steps begin in CTA b's share of the attention and go on behind it, if there is one; its place is found in the plan before the
+// attention has ended, as in k_kv4_merge.
 template <int NG>
-__global__ void __launch_bounds__(128) k_kv4_chunk_merge(const Kv4AttnArgs a, const int ctas) {
-    constexpr int HD = NG * KV4_GROUP;
-    const int lane = threadIdx.x & 31, heads = a.c.n_kv * a.group;
-    const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+__global__ void __launch_bounds__(1024) k_kv4_chunk_merge(const Kv4AttnArgs a) {
+    constexpr int HD = NG * KV4_GROUP, D4 = HD / 4;
+    __shared__ float2 whole[KC_COLS];       // of a column: reference, 1 / sum
+    const int lane = threadIdx.x & 31, ctas = gridDim.x, b = blockIdx.x;
     if (a.early) pdl_launch();
-    const int row = (int)(id / heads), head = (int)(id % heads), kv = by_group(a, head);
-    const int entry = row < a.n_rows ? __ldcg(a.row_entry + row) : -1;
-    if (entry < 0) return pdl_wait();
-    const int4 e = __ldcg(a.entries + entry);
+    KcRun u;
     const long long total = (long long)__ldcg(a.cu_work + a.n) * a.c.n_kv;
-    long long at = 0;
-    const int col = (row - e.w) * a.group + head - kv * a.group, ctile = col / KC_COLS;
-    for (int t = lane; t < ctile; t += 32) at += kc_cost(e.y, e.z, a.group, t);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) at += __shfl_xor_sync(0xffffffffu, at, o);
-    const int cost = kc_cost(e.y, e.z, a.group, ctile);
-    at = (at + __ldcg(a.cu_work + entry)) * a.c.n_kv + (long long)kv * cost;
-    // the CTAs that had steps [at, at + cost): CTA b has [total b / ctas, total (b + 1) / ctas)
-    const int first = (int)(((at + 1) * ctas - 1) / total), last = (int)(((at + cost) * ctas - 1) / total);
-    if (first == last) return pdl_wait();
-    auto place = [&](int b) { return (size_t)(2 * b + (b == first)) * KC_COLS + col % KC_COLS; };
-    auto idle = [&](int b) { return total * b / ctas == total * (b + 1) / ctas; };      // fewer steps than CTAs: some have none
+    auto share = [&](int i) { return total * i / ctas; };
+    const long long end = share(b + 1);
+    bool mine = share(b) < end && kc_find(a, u, end - 1, total, lane);
+    mine = mine && u.from + 1 < u.cost && end - 1 - u.from >= share(b);     // more steps behind, and the first is this CTA's
+    if (!mine) return pdl_wait();
+    // the CTA that has the last step, and of those between the ones that have any (with fewer steps than CTAs some have none)
+    const int last = (int)(((end - 1 - u.from + u.cost) * ctas - 1) / total);
+    __shared__ int parts[1024], n_parts;
+    if (threadIdx.x == 0) n_parts = 0;
+    __syncthreads();
+    if (threadIdx.x < 32)
+        for (int i = b + lane; i - lane <= last; i += 32) {
+            const bool has = i <= last && share(i) < share(i + 1);
+            const unsigned all = __ballot_sync(0xffffffffu, has);
+            if (has) parts[n_parts + __popc(all & ((1u << lane) - 1))] = (2 * i + (i == b)) * KC_COLS;
+            __syncwarp();
+            if (lane == 0) n_parts += __popc(all);
+            __syncwarp();
+        }
+    __syncthreads();
+    const int cols = min(u.e.z * a.group - u.ctile * KC_COLS, KC_COLS), n = n_parts;
     pdl_wait();
-    float best = -INFINITY, sum = 0.f, out[NG];
-    for (int b = first + lane; b <= last; b += 32)
-        if (!idle(b)) best = fmaxf(best, __ldcg(&a.ml[place(b)].x));
-#pragma unroll
-    for (int o = 16; o; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
-    const float now = best == -INFINITY ? 0.f : best;
-#pragma unroll
-    for (int j = 0; j < NG; ++j) out[j] = 0.f;
+    if (threadIdx.x < cols) {
+        float best = -INFINITY, sum = 0.f;
 #pragma unroll 4
-    for (int b = first; b <= last; ++b) {
-        if (idle(b)) continue;
-        const float2 part = __ldcg(a.ml + place(b));
-        if (part.y == 0.f) continue;      // nothing seen there: no sums were written
-        const float f = ex2(part.x - now);
-        sum += f * part.y;
-#pragma unroll
-        for (int j = 0; j < NG; ++j) out[j] += f * __ldcg(a.acc + place(b) * HD + lane * NG + j);
+        for (int i = 0; i < n; ++i) {
+            const float2 part = __ldcg(a.ml + parts[i] + threadIdx.x);
+            const float top = fmaxf(best, part.x), now = top == -INFINITY ? 0.f : top;
+            sum = sum * ex2(best - now) + part.y * ex2(part.x - now);
+            best = top;
+        }
+        whole[threadIdx.x] = make_float2(best == -INFINITY ? 0.f : best, sum == 0.f ? 0.f : 1.f / sum);
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    __nv_bfloat16* dst = a.out + (long long)row * a.out_stride + head * HD + lane * NG;
-#pragma unroll
-    for (int j = 0; j < NG; ++j) dst[j] = __float2bfloat16_rn(out[j] * inv);
+    __syncthreads();
+#pragma unroll 2
+    for (int k = threadIdx.x; k < cols * D4; k += 1024) {
+        const int col = k / D4, d = k % D4, c = u.ctile * KC_COLS + col, row = by_group(a, c);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) {
+            const float2 part = __ldcg(a.ml + parts[i] + col);
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(a.acc + (size_t)(parts[i] + col) * HD) + d);
+            if (part.y == 0.f) continue;        // nothing seen there: no sums were written
+            const float f = ex2(part.x - whole[col].x);
+            o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
+        }
+        const float inv = whole[col].y;
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(o.x * inv, o.y * inv), hi = __floats2bfloat162_rn(o.z * inv, o.w * inv);
+        *reinterpret_cast<uint2*>(a.out + (long long)(u.e.w + row) * a.out_stride + (u.head * a.group + c - row * a.group) * HD + d * 4) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    }
 }
 
 }  // namespace vuik
