@@ -79,22 +79,24 @@ Shape shape_of(const VuibKv4* c, const VuibKv4Plan* p) {
     const long long most = (long long)p->max_new * group;       // columns of one sequence
     if (most <= 16) {
         const Form f = most <= 2 && c->ng != 3 ? FEW_HALVES : most <= 4 ? FEW_4 : most <= 8 ? FEW_8 : FEW_16;
-        return {f, f == FEW_HALVES ? 2 : f == FEW_4 ? 4 : f == FEW_8 ? 8 : 16, {256, 512, 1 << 30, true}};
+        return {f, f == FEW_HALVES ? 2 : f == FEW_4 ? 4 : f == FEW_8 ? 8 : 16, {512, 256, 512, 1 << 30, true}};
     }
     Shape s = {MANY, c->ng > 2 ? 16 : 32, {}};
-    if (most >= KV4_CHUNK) return {CHUNK, KC_COLS, {1 << 30, 1 << 30, 1, false}};
+    if (most >= KV4_CHUNK) return {CHUNK, KC_COLS, {1 << 30, 1 << 30, 1 << 30, 1, false}};
     const long long tiles = ceil_div((long long)p->n_rows * group, s.cols) + p->n_seqs;
     // enough tiles for the SMs: no splits; else at most 8 of a sequence, so that their sums stay a few megabytes
     const long long len = (long long)c->cfg.max_blocks << c->block_shift;
     const bool enough = tiles * c->cfg.n_kv_heads >= 2 * c->sms;
-    s.split = {enough ? 1 << 30 : 512, enough ? 1 << 30 : 512, 8, tiles * (len / 64 + 16) < KV4_MANY};
+    const int split = enough ? 1 << 30 : 512;
+    s.split = {split, split, split, 8, tiles * (len / 64 + 16) < KV4_MANY};
     return s;
 }
 
 // Most splits of one sequence.
 long long most_parts(const VuibKv4* c, const Shape& s) {
     const long long len = (long long)c->cfg.max_blocks << c->block_shift;
-    return min((long long)s.split.most, max(ceil_div(min(len, 1024ll), s.split.up_to_1024), ceil_div(len, s.split.beyond)));
+    return min((long long)s.split.most, max(ceil_div(min(len, 512ll), s.split.up_to_512),
+                                            max(len > 512 ? ceil_div(min(len, 1024ll), s.split.up_to_1024) : 0, ceil_div(len, s.split.beyond))));
 }
 
 // Most units (of one kv head) that a plan of this shape can have.  Sequences share no blocks, so their lengths sum up to the pool's.
@@ -103,7 +105,7 @@ long long most_units(const VuibKv4* c, const VuibKv4Plan* p, const Shape& s) {
     const int group = c->cfg.n_heads / c->cfg.n_kv_heads;
     const long long a_seq = ceil_div((long long)p->max_new * group, s.cols);
     const long long tiles = min((long long)p->n_seqs * a_seq, ceil_div((long long)p->n_rows * group, s.cols) + p->n_seqs);
-    return min(tiles * most_parts(c, s), a_seq * (p->n_seqs + pool / s.split.up_to_1024));
+    return min(tiles * most_parts(c, s), a_seq * (p->n_seqs + pool / min(s.split.up_to_512, s.split.up_to_1024)));
 }
 
 // Units whose sums may have to be kept: of the form for chunks, two a CTA.
@@ -158,7 +160,7 @@ cudaError_t launch_attn(VuibKv4* c, const Shape& s, void (*kern)(Kv4AttnArgs), i
     const long long grid = s.form == CHUNK ? c->sms : min(items, room), rows = (long long)a.n_rows * c->cfg.n_heads;
     e = launch(c, kern, dim3((unsigned)grid), threads, smem, 1, stream, a);
     if (e != cudaSuccess || !merge) return e;
-    if (s.form == CHUNK) return launch(c, k_kv4_chunk_merge<NG>, dim3((unsigned)grid), 1024, 0, 1, stream, a);
+    if (s.form == CHUNK) return launch(c, k_kv4_chunk_merge<NG>, dim3((unsigned)grid, KC_COLS / KC_MERGE), 256, 0, 1, stream, a);
     if (most_parts(c, s) <= 32)
         return launch(c, k_kv4_merge<NG, 1>, dim3((unsigned)ceil_div(rows, 4)), 128, 0, 1, stream, a, s.cols);
     return launch(c, k_kv4_merge<NG, 8>, dim3((unsigned)rows), 256, 0, 1, stream, a, s.cols);

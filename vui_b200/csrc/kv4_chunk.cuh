@@ -607,14 +607,16 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv4_attn_chunk(const Kv4AttnA
     if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
-// Adds up the parts of the (column tile, kv head)s that several CTAs had, in the order of the positions.  CTA b of `ctas` does it for the one
-// whose steps begin in CTA b's share of the attention and go on behind it, if there is one; its place is found in the plan before the
-// attention has ended, as in k_kv4_merge.
+// Adds up the parts of the (column tile, kv head)s that several CTAs had, in the order of the positions.  CTA (b, i) does it for 32 columns of
+// the one whose steps begin in CTA b's share of the attention and go on behind it, if there is one; its place is found in the plan
+// before the attention has ended, as in k_kv4_merge.
+constexpr int KC_MERGE = 32;
 template <int NG>
-__global__ void __launch_bounds__(1024) k_kv4_chunk_merge(const Kv4AttnArgs a) {
+__global__ void __launch_bounds__(256) k_kv4_chunk_merge(const Kv4AttnArgs a) {
     constexpr int HD = NG * KV4_GROUP, D4 = HD / 4;
-    __shared__ float2 whole[KC_COLS];       // of a column: reference, 1 / sum
-    const int lane = threadIdx.x & 31, ctas = gridDim.x, b = blockIdx.x;
+    __shared__ float2 whole[KC_MERGE];       // of a column: reference, 1 / sum
+    __shared__ int parts[1024], n_parts;
+    const int lane = threadIdx.x & 31, ctas = gridDim.x, b = blockIdx.x, from = blockIdx.y * KC_MERGE;
     if (a.early) pdl_launch();
     KcRun u;
     const long long total = (long long)__ldcg(a.cu_work + a.n) * a.c.n_kv;
@@ -622,10 +624,10 @@ __global__ void __launch_bounds__(1024) k_kv4_chunk_merge(const Kv4AttnArgs a) {
     const long long end = share(b + 1);
     bool mine = share(b) < end && kc_find(a, u, end - 1, total, lane);
     mine = mine && u.from + 1 < u.cost && end - 1 - u.from >= share(b);     // more steps behind, and the first is this CTA's
-    if (!mine) return pdl_wait();
+    const int cols = mine ? min(u.e.z * a.group - u.ctile * KC_COLS - from, KC_MERGE) : 0;
+    if (cols <= 0) return pdl_wait();
     // the CTA that has the last step, and of those between the ones that have any (with fewer steps than CTAs some have none)
     const int last = (int)(((end - 1 - u.from + u.cost) * ctas - 1) / total);
-    __shared__ int parts[1024], n_parts;
     if (threadIdx.x == 0) n_parts = 0;
     __syncthreads();
     if (threadIdx.x < 32)
@@ -638,13 +640,13 @@ __global__ void __launch_bounds__(1024) k_kv4_chunk_merge(const Kv4AttnArgs a) {
             __syncwarp();
         }
     __syncthreads();
-    const int cols = min(u.e.z * a.group - u.ctile * KC_COLS, KC_COLS), n = n_parts;
+    const int n = n_parts;
     pdl_wait();
     if (threadIdx.x < cols) {
         float best = -INFINITY, sum = 0.f;
 #pragma unroll 4
         for (int i = 0; i < n; ++i) {
-            const float2 part = __ldcg(a.ml + parts[i] + threadIdx.x);
+            const float2 part = __ldcg(a.ml + parts[i] + from + threadIdx.x);
             const float top = fmaxf(best, part.x), now = top == -INFINITY ? 0.f : top;
             sum = sum * ex2(best - now) + part.y * ex2(part.x - now);
             best = top;
@@ -653,13 +655,13 @@ __global__ void __launch_bounds__(1024) k_kv4_chunk_merge(const Kv4AttnArgs a) {
     }
     __syncthreads();
 #pragma unroll 2
-    for (int k = threadIdx.x; k < cols * D4; k += 1024) {
-        const int col = k / D4, d = k % D4, c = u.ctile * KC_COLS + col, row = by_group(a, c);
+    for (int k = threadIdx.x; k < cols * D4; k += 256) {
+        const int col = k / D4, d = k % D4, c = u.ctile * KC_COLS + from + col, row = by_group(a, c);
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
         for (int i = 0; i < n; ++i) {
-            const float2 part = __ldcg(a.ml + parts[i] + col);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(a.acc + (size_t)(parts[i] + col) * HD) + d);
+            const float2 part = __ldcg(a.ml + parts[i] + from + col);
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(a.acc + (size_t)(parts[i] + from + col) * HD) + d);
             if (part.y == 0.f) continue;        // nothing seen there: no sums were written
             const float f = ex2(part.x - whole[col].x);
             o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;

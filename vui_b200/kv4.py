@@ -47,6 +47,7 @@ class Kv4Plan:
         self._c = _lib.VuibKv4Plan(n_seqs, n_rows, max_new, at, at + 4 * self._at[3], at + 4 * self._at[1], at + 4 * self._at[2], at + 4 * work)
         self._ref = C.byref(self._c)
         self._ws_bytes = -1        # of its attention calls, asked for once
+        self._ws: dict[int, Tensor] = {}      # by stream
 
     @property
     def slot_map(self) -> Tensor:
@@ -227,18 +228,34 @@ class Kv4Cache:
         Rows behind the plan's last are not written."""
         if scale is not None and not 0 < scale <= 1e30:
             raise ValueError("scale must be positive")
-        with self._here():
-            q = self._rows(q, "q", plan.n_rows, self.n_heads)
-            out = torch.empty(q.shape, dtype=torch.bfloat16, device=self.device) if out is None else self._rows(out, "out", plan.n_rows, self.n_heads, out=True)
-            if plan._ws_bytes < 0:
-                n = C.c_size_t()
-                self._ck(self._lib.vuib_kv4_attention_workspace(self._h, plan._ref, C.byref(n)))
-                plan._ws_bytes = n.value
-            n = plan._ws_bytes
-            ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None     # the call's own: calls may overlap
-            self._ck(self._lib.vuib_kv4_attention(self._h, layer, plan._ref, q.data_ptr(), self._step(q, self.n_heads), out.data_ptr(),
-                                                  self._step(out, self.n_heads), float(scale or 0.0), None if ws is None else ws.data_ptr(), n,
-                                                  self._stream))
+        if torch.cuda.current_device() != self._index:
+            with torch.cuda.device(self._index):
+                return self.attention(layer, q, plan, scale=scale, out=out)
+        rows, heads, width = plan.n_rows, self.n_heads, self.n_heads * self.head_dim
+        q = self._rows(q, "q", rows, heads)
+        if out is None:
+            out = torch.empty(q.shape, dtype=torch.bfloat16, device=self.device)
+            step = width
+        else:
+            out = self._rows(out, "out", rows, heads, out=True)
+            step = self._step(out, heads)
+        stream = _raw_stream(self._index)
+        if plan._ws_bytes < 0:
+            n = C.c_size_t()
+            self._ck(self._lib.vuib_kv4_attention_workspace(self._h, plan._ref, C.byref(n)))
+            plan._ws_bytes = n.value
+        ws = None
+        if plan._ws_bytes:
+            # calls on one stream follow one another and share the plan's workspace; a captured call has its own, which its graph keeps
+            ws = plan._ws.get(stream)
+            if ws is None or torch.cuda.is_current_stream_capturing():
+                ws = torch.empty(plan._ws_bytes, dtype=torch.uint8, device=self.device)
+                if not torch.cuda.is_current_stream_capturing():
+                    plan._ws[stream] = ws
+        rc = self._lib.vuib_kv4_attention(self._h, layer, plan._ref, q.data_ptr(), self._step(q, heads), out.data_ptr(), step, scale or 0.0,
+                                          None if ws is None else ws.data_ptr(), plan._ws_bytes, stream)
+        if rc:
+            self._ck(rc)
         return out
 
     # ------------------------------------------------------------- diagnostics
