@@ -382,6 +382,35 @@ def test_peaked_scores():
     close(f.cache.attention(0, q, plan), (ref, 2 * mag, more))
 
 
+@pytest.mark.parametrize("heads, kv, dim, grow", [(16, 8, 64, False), (8, 2, 128, True), (6, 2, 96, True), (16, 8, 64, True)])
+def test_peaked_chunks(heads, kv, dim, grow):
+    """The same for chunks of prompts; with keys that grow along the sequence, so that a column's maximum keeps leaving the weights' range.
+    Scores as above, of up to 450."""
+    f = Filled([1], heads, kv, dim, 64, spare=1800, key_scale=30.0, max_blocks=40)
+    for part in range(6):
+        f.key_scale = 30.0 * (2.0 ** (part - 5) if grow else 1.0)
+        plan = f.add([250])
+        q = torch.randn(250, heads, dim, device="cuda", generator=f.g).bfloat16()
+        ref, mag, more = f.want(q, [250])
+        out = f.cache.attention(0, q, plan)
+        close(out, (ref, 2 * mag, more))
+        assert torch.equal(out, f.cache.attention(0, q, plan))
+    f.cache.check_device()
+
+
+def test_a_row_of_nan_in_a_chunk():
+    f = Filled([700], 16, 8, 64, 64, spare=100)
+    plan = f.add([100])
+    q = torch.randn(100, 16, 64, device="cuda", generator=f.g).bfloat16()
+    want = f.want(q, [100])
+    bad = q.clone()
+    bad[31, 7, 5], bad[90, 2, 0] = float("nan"), float("inf")
+    out = f.cache.attention(0, bad, plan)
+    assert out[31, 7].isnan().all() and out[90, 2].isnan().all()
+    out[31, 7], out[90, 2] = want[0][31, 7].bfloat16(), want[0][90, 2].bfloat16()
+    close(out, want)
+
+
 def test_a_row_of_nan_stays_its_own():
     f = Filled([100, 400, 30], 16, 8, 64, 64)
     plan = f.add([2, 2, 2])

@@ -2,11 +2,14 @@
 //
 // A CTA takes 256 columns (a sequence's rows times the query heads of a kv head) of one kv head as two tiles of 128, and walks the
 // positions 128 at a time:
-//   * 4 warps read codes from the cache (a step ahead, in registers) and write keys and values as f16 into a ring of shared-memory tiles
-//     that both tiles of columns share: keys [position][dim], values [dim][position], both K-major with the 128-byte swizzle;
+//   * 8 warps read codes from the cache (half a step ahead, in registers) and write keys and values as f16 into a ring of shared-memory
+//     tiles that both tiles of columns share: keys [position][dim], values [dim][position], both K-major with the 128-byte swizzle;
 //   * one thread issues tcgen05.mma: S = Q K^T (128 x 128, K = head_dim) and O += P V (A = P from tensor memory, K = 128 positions);
-//   * 4 warps a tile, one thread a column: maximum, exponentials, P as f16 back into tensor memory over S, and, where the maximum has grown
-//     by more than 2^8 since the reference was set, the correction of O.
+//   * 4 warps a tile, one thread a column: exponentials, their sum, and P as f16 back into tensor memory over S.
+// Weights are taken against a reference, the first maximum that a column meets: below 2^14 of it they fit f16 and the sums all the same, so
+// that a step needs no maximum before it weighs; it looks for it meanwhile.  A step that carries a column beyond 2^14 is taken again: the
+// scores are computed anew (the keys are kept until the step is accepted), the column's sums corrected, each column's by its own maximum, so
+// that its bits are its own.
 // While one tile's softmax runs, the tensor cores work on the other.  Per step of 128 positions and two tiles at head_dim 128 the tensor
 // cores take 2048 cycles, the exponentials (16 a clock) 2048, the issue slots about 1700.
 // Every wait is bounded; a role that gives up leaves its loop, and all warps meet before tensor memory is freed.
@@ -16,7 +19,7 @@
 namespace vuik {
 
 constexpr int KC_TILE = 128;
-constexpr int KC_FILL = 4, KC_WARPS = 13, KC_THREADS = KC_WARPS * 32;      // warps 0-3 fill, 4-7 and 8-11 softmax, 12 MMA
+constexpr int KC_FILL = 8, KC_WARPS = 17, KC_THREADS = KC_WARPS * 32;      // warps 0-7 fill, 8-11 and 12-15 softmax, 16 MMA
 
 template <int NG>
 struct KcShared {
@@ -120,10 +123,10 @@ struct KcBars {
     __device__ __forceinline__ uint32_t q_full(int x) const { return at + 8 * x; }
     __device__ __forceinline__ uint32_t s_full(int x) const { return at + 16 + 8 * x; }
     __device__ __forceinline__ uint32_t p_full(int x) const { return at + 32 + 8 * x; }
-    __device__ __forceinline__ uint32_t o_full(int x) const { return at + 48 + 8 * x; }
-    __device__ __forceinline__ uint32_t kv_full(int s) const { return at + 64 + 8 * s; }
-    __device__ __forceinline__ uint32_t kv_empty(int s) const { return at + 96 + 8 * s; }
-    __device__ __forceinline__ uint32_t tmem() const { return at + 128; }
+    __device__ __forceinline__ uint32_t kv_full(int s) const { return at + 48 + 8 * s; }
+    __device__ __forceinline__ uint32_t kv_empty(int s) const { return at + 80 + 8 * s; }
+    __device__ __forceinline__ uint32_t tmem() const { return at + 112; }
+    __device__ __forceinline__ uint32_t again(int x) const { return at + 116 + 4 * x; }     // the round of P whose step is to be taken again
 };
 
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -192,12 +195,22 @@ __device__ __forceinline__ void tm_store32(uint32_t at, const uint32_t (&r)[32])
                  "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
                  "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
 }
+__device__ __forceinline__ void tm_store8(uint32_t at, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
+                 "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
 __device__ __forceinline__ void tm_store16(uint32_t at, const uint32_t (&r)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at), "r"(r[0]), "r"(r[1]),
                  "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
                  "r"(r[14]), "r"(r[15]) : "memory");
 }
 __device__ __forceinline__ void tm_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void sts32(uint32_t at, uint32_t v) { asm volatile("st.volatile.shared.b32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
+__device__ __forceinline__ uint32_t lds32(uint32_t at) {
+    uint32_t v;
+    asm volatile("ld.volatile.shared.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
 __device__ __forceinline__ void sts128(uint32_t at, const uint32_t (&r)[4]) {
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
 }
@@ -206,66 +219,54 @@ __device__ __forceinline__ void stmatrix4(uint32_t at, const uint32_t (&r)[4]) {
     asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
 }
 
-// ---- the filling warps: warp w takes tiles w and w + 4 of every 8 (of 16 positions)
+// ---- the filling warps: warp w takes tile w of every 8 (of 16 positions)
 template <int NG>
 __device__ __forceinline__ void kc_fill(const Kv4AttnArgs& a, uint32_t ring, const KcBars bars, int w, int lane) {
     using S = KcShared<NG>;
     const int g = lane >> 2, t = lane & 3, tiles = 1 << (a.c.block_shift - 4);
+    // keys: row 16 w + g of the tile (and + 8, with the same low three bits); values: element 4 g + j of a group is row 8 j + g, so that the
+    // eight rows of a matrix lie in eight different banks; lane l names row l % 8 of matrix l / 8: (j = 0, keys 0-7), (1, 0-7), (0, 8-15), (1, 8-15)
+    const uint32_t key_row = (w * KV4_TILE + g) * 128, key_sw = g, val_sw = ((w & 3) * 2 + (lane >> 4)) ^ (lane & 7);
+    const uint32_t val_row = (w >> 2) * (S::HD * 128) + ((lane >> 3 & 1) * 8 + (lane & 7)) * 128 + (val_sw << 4);
     KcRun u;
     unsigned n = 0;        // tiles written: keys and values in turn
     for (bool more = kc_begin(a, u, lane); more; more = kc_next(a, u)) {
-        const int last = max(u.steps[0], u.steps[1]), base = u.from * KC_STEP, len = u.e.y + u.e.z;
-        int id[2] = {0, 0};
-        auto read_ids = [&](int j) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int pos = base + j * KC_STEP + (k * KC_FILL + w) * KV4_TILE;
-                id[k] = pos < len ? __ldcg(a.c.table + (size_t)u.e.x * a.c.max_blocks + (pos >> a.c.block_shift)) : -1;
-            }
+        const int last = max(u.steps[0], u.steps[1]), base = u.from * KC_STEP + w * KV4_TILE, len = u.e.y + u.e.z;
+        const int32_t* const table = a.c.table + (size_t)u.e.x * a.c.max_blocks;
+        auto block_of = [&](int j) {
+            const int pos = base + j * KC_STEP;
+            return j < last && pos < len ? __ldcg(table + (pos >> a.c.block_shift)) : -1;
         };
-        const unsigned char* at[2];
-        auto place = [&](int j) {       // of the step whose blocks are in id
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int pos = base + j * KC_STEP + (k * KC_FILL + w) * KV4_TILE;
-                at[k] = nullptr;
-                if (pos < len) {
-                    int b = id[k];
-                    if ((unsigned)b >= (unsigned)a.c.n_blocks) {
-                        if (lane == 0) atomicOr(a.c.flag, KV4_BAD_BLOCK);
-                        b = 0;
-                    }
-                    at[k] = a.c.pool + ((size_t)((long long)b * a.c.n_kv + u.head) * tiles + ((pos & ((1 << a.c.block_shift) - 1)) >> 4)) * (NG * KV4_GT);
-                }
+        auto place = [&](int j, int b) -> const unsigned char* {
+            const int pos = base + j * KC_STEP;
+            if (j >= last || pos >= len) return nullptr;
+            if ((unsigned)b >= (unsigned)a.c.n_blocks) {
+                if (lane == 0) atomicOr(a.c.flag, KV4_BAD_BLOCK);
+                b = 0;
             }
+            return a.c.pool + ((size_t)((long long)b * a.c.n_kv + u.head) * tiles + ((pos & ((1 << a.c.block_shift) - 1)) >> 4)) * (NG * KV4_GT);
         };
         // what is not there is zeros: codes, scales and values
-        uint2 kc[2][NG], kp[2][NG], vc[2][NG];
-        uint4 vp[2][NG];
-        auto read_keys = [&]() {
+        uint2 kc[NG], kp[NG], vc[NG];
+        uint4 vp[NG];
+        auto read_keys = [&](const unsigned char* at) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-#pragma unroll
-                for (int i = 0; i < NG; ++i) {
-                    kc[k][i] = kp[k][i] = make_uint2(0, 0);
-                    if (at[k]) {
-                        kc[k][i] = __ldcg(reinterpret_cast<const uint2*>(at[k] + i * KV4_GT + lane * 8));
-                        kp[k][i] = __ldcg(reinterpret_cast<const uint2*>(at[k] + i * KV4_GT + KV4_KPAR + g * 8));
-                    }
+            for (int i = 0; i < NG; ++i) {
+                kc[i] = kp[i] = make_uint2(0, 0);
+                if (at) {
+                    kc[i] = __ldcg(reinterpret_cast<const uint2*>(at + i * KV4_GT + lane * 8));
+                    kp[i] = __ldcg(reinterpret_cast<const uint2*>(at + i * KV4_GT + KV4_KPAR + g * 8));
                 }
             }
         };
-        auto read_values = [&]() {
+        auto read_values = [&](const unsigned char* at) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-#pragma unroll
-                for (int i = 0; i < NG; ++i) {
-                    vc[k][i] = make_uint2(0, 0);
-                    vp[k][i] = make_uint4(0, 0, 0, 0);
-                    if (at[k]) {
-                        vc[k][i] = __ldcg(reinterpret_cast<const uint2*>(at[k] + i * KV4_GT + KV4_VCODE + lane * 8));
-                        vp[k][i] = __ldcg(reinterpret_cast<const uint4*>(at[k] + i * KV4_GT + KV4_VPAR + t * 16));   // of keys 2t, 2t+8, 2t+1, 2t+9
-                    }
+            for (int i = 0; i < NG; ++i) {
+                vc[i] = make_uint2(0, 0);
+                vp[i] = make_uint4(0, 0, 0, 0);
+                if (at) {
+                    vc[i] = __ldcg(reinterpret_cast<const uint2*>(at + i * KV4_GT + KV4_VCODE + lane * 8));
+                    vp[i] = __ldcg(reinterpret_cast<const uint4*>(at + i * KV4_GT + KV4_VPAR + t * 16));   // of keys 2t, 2t+8, 2t+1, 2t+9
                 }
             }
         };
@@ -275,54 +276,40 @@ __device__ __forceinline__ void kc_fill(const Kv4AttnArgs& a, uint32_t ring, con
             if (lane == 0) bar_arrive(bars.kv_full(n % S::SLOTS));
             ++n;
         };
-        if (last > 0) {
-            read_ids(0);
-            place(0);
-            read_keys();
-        }
+        const unsigned char* at = place(0, block_of(0));
+        int id = block_of(1);
+        if (last > 0) read_keys(at);
         for (int j = 0; j < last; ++j) {
-            if (j + 1 < last) read_ids(j + 1);
-            read_values();
+            read_values(at);
+            at = place(j + 1, id);
+            id = block_of(j + 2);
             if (n >= S::SLOTS && !bar_wait(bars.kv_empty(n % S::SLOTS), (n / S::SLOTS - 1) & 1)) return give_up(a.c.flag);
             uint32_t slot = ring + (n % S::SLOTS) * S::SLOT;
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-#pragma unroll
-                for (int i = 0; i < NG; ++i) {
-                    const int key = (k * KC_FILL + w) * KV4_TILE + g;       // and key + 8, which has the same low three bits
-                    const uint32_t row = slot + (i >> 1) * S::BLOCK + key * 128 + ((((i & 1) * 4 + t) ^ (key & 7)) << 4);
-                    const __half2 s0 = __low2half2(as_h2(kp[k][i].x)), z0 = __high2half2(as_h2(kp[k][i].x));
-                    const __half2 s1 = __low2half2(as_h2(kp[k][i].y)), z1 = __high2half2(as_h2(kp[k][i].y));
-                    uint32_t r[4];
-                    kv4_values(kc[k][i].x, s0, z0, s0, z0, r);
-                    sts128(row, r);
-                    kv4_values(kc[k][i].y, s1, z1, s1, z1, r);
-                    sts128(row + 8 * 128, r);
-                }
+            for (int i = 0; i < NG; ++i) {
+                const uint32_t row = slot + (i >> 1) * S::BLOCK + key_row + ((((i & 1) * 4 + t) ^ key_sw) << 4);
+                const __half2 s0 = __low2half2(as_h2(kp[i].x)), z0 = __high2half2(as_h2(kp[i].x));
+                const __half2 s1 = __low2half2(as_h2(kp[i].y)), z1 = __high2half2(as_h2(kp[i].y));
+                uint32_t r[4];
+                kv4_values(kc[i].x, s0, z0, s0, z0, r);
+                sts128(row, r);
+                kv4_values(kc[i].y, s1, z1, s1, z1, r);
+                sts128(row + 8 * 128, r);
             }
             done();
-            if (j + 1 < last) {
-                place(j + 1);
-                read_keys();
-            }
+            read_keys(at);
             if (n >= S::SLOTS && !bar_wait(bars.kv_empty(n % S::SLOTS), (n / S::SLOTS - 1) & 1)) return give_up(a.c.flag);
             slot = ring + (n % S::SLOTS) * S::SLOT;
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int tile = k * KC_FILL + w, chunk = (tile & 3) * 2 + (lane >> 4);      // matrices 2 and 3: keys 8 to 15 of the tile
-#pragma unroll
-                for (int i = 0; i < NG; ++i) {
-                    // element 4 g + j of the group is row 8 j + g, so that a matrix's eight rows lie in eight different banks
-                    const int rho = i * 32 + (lane >> 3 & 1) * 8 + (lane & 7);
-                    const uint32_t row = slot + (tile >> 2) * (S::HD * 128) + rho * 128 + ((chunk ^ (lane & 7)) << 4);
-                    const __half2 s0 = as_h2(__byte_perm(vp[k][i].x, vp[k][i].z, 0x5410)), z0 = as_h2(__byte_perm(vp[k][i].x, vp[k][i].z, 0x7632));
-                    const __half2 s8 = as_h2(__byte_perm(vp[k][i].y, vp[k][i].w, 0x5410)), z8 = as_h2(__byte_perm(vp[k][i].y, vp[k][i].w, 0x7632));
-                    uint32_t r[4];
-                    kv4_values(vc[k][i].x, s0, z0, s8, z8, r);
-                    stmatrix4(row, r);
-                    kv4_values(vc[k][i].y, s0, z0, s8, z8, r);
-                    stmatrix4(row + 16 * 128, r);
-                }
+            for (int i = 0; i < NG; ++i) {
+                const uint32_t row = slot + val_row + i * (32 * 128);
+                const __half2 s0 = as_h2(__byte_perm(vp[i].x, vp[i].z, 0x5410)), z0 = as_h2(__byte_perm(vp[i].x, vp[i].z, 0x7632));
+                const __half2 s8 = as_h2(__byte_perm(vp[i].y, vp[i].w, 0x5410)), z8 = as_h2(__byte_perm(vp[i].y, vp[i].w, 0x7632));
+                uint32_t r[4];
+                kv4_values(vc[i].x, s0, z0, s8, z8, r);
+                stmatrix4(row, r);
+                kv4_values(vc[i].y, s0, z0, s8, z8, r);
+                stmatrix4(row + 16 * 128, r);
             }
             done();
         }
@@ -335,7 +322,7 @@ __device__ __forceinline__ void kc_issue(const Kv4AttnArgs& a, uint32_t smem, co
     using S = KcShared<NG>;
     const uint32_t ring = smem + 2 * S::Q;
     KcRun u;
-    unsigned n = 0, units[2] = {0, 0}, steps_done[2] = {0, 0};
+    unsigned n = 0, runs[2] = {0, 0}, rounds[2] = {0, 0};     // tiles of keys and values, runs with steps, rounds of P
     auto scores = [&](int x, unsigned slot) {       // S of tile x
         const uint32_t q = tile_desc(smem + x * S::Q), k = tile_desc(ring + slot * S::SLOT), d = tmem + x * KC_TILE;
         mma_ss<4, true>(d, q, k, kc_idesc(KC_STEP));
@@ -351,45 +338,41 @@ __device__ __forceinline__ void kc_issue(const Kv4AttnArgs& a, uint32_t smem, co
     for (bool more = kc_begin(a, u, lane); more; more = kc_next(a, u)) {
         const int(&steps)[2] = u.steps;
         const int last = max(steps[0], steps[1]);
-        if (last > 0) {
-            if (!bar_wait(bars.kv_full(n % S::SLOTS), (n / S::SLOTS) & 1)) return give_up(a.c.flag);
-            for (int x = 0; x < 2; ++x) {
-                if (!steps[x]) continue;
-                if (!bar_wait(bars.q_full(x), units[x] & 1)) return give_up(a.c.flag);
-                ++units[x];
-                tc_after();
-                if (elect_one()) scores(x, n % S::SLOTS);
-                __syncwarp();
-            }
-            if (elect_one()) tc_commit(bars.kv_empty(n % S::SLOTS));
+        if (last == 0) continue;
+        if (!bar_wait(bars.kv_full(n % S::SLOTS), (n / S::SLOTS) & 1)) return give_up(a.c.flag);
+        for (int x = 0; x < 2; ++x) {
+            if (!steps[x]) continue;
+            if (!bar_wait(bars.q_full(x), runs[x] & 1)) return give_up(a.c.flag);
+            ++runs[x];
+            tc_after();
+            if (elect_one()) scores(x, n % S::SLOTS);
             __syncwarp();
-            ++n;
-            for (int j = 0; j < last; ++j) {
-                const unsigned vslot = n % S::SLOTS, kslot = (n + 1) % S::SLOTS;
-                if (!bar_wait(bars.kv_full(vslot), (n / S::SLOTS) & 1)) return give_up(a.c.flag);
-                if (j + 1 < last && !bar_wait(bars.kv_full(kslot), ((n + 1) / S::SLOTS) & 1)) return give_up(a.c.flag);
-                for (int x = 0; x < 2; ++x) {
-                    if (j >= steps[x]) continue;
-                    if (!bar_wait(bars.p_full(x), steps_done[x] & 1)) return give_up(a.c.flag);
+        }
+        for (int j = 0; j < last; ++j, n += 2) {
+            const unsigned kslot = n % S::SLOTS, vslot = (n + 1) % S::SLOTS, next = (n + 2) % S::SLOTS;
+            if (!bar_wait(bars.kv_full(vslot), ((n + 1) / S::SLOTS) & 1)) return give_up(a.c.flag);
+            if (j + 1 < last && !bar_wait(bars.kv_full(next), ((n + 2) / S::SLOTS) & 1)) return give_up(a.c.flag);
+            for (int x = 0; x < 2; ++x) {
+                if (j >= steps[x]) continue;
+                for (;;) {
+                    if (!bar_wait(bars.p_full(x), rounds[x] & 1)) return give_up(a.c.flag);
                     tc_after();
-                    if (elect_one()) {
-                        sums(x, vslot, j > 0);
-                        if (j + 1 == steps[x]) tc_commit(bars.o_full(x));
-                    }
+                    if (lds32(bars.again(x)) != rounds[x]++) break;
+                    if (elect_one()) scores(x, kslot);
                     __syncwarp();
-                    if (j + 1 < steps[x]) {
-                        if (elect_one()) scores(x, kslot);
-                        __syncwarp();
-                    }
-                    ++steps_done[x];
                 }
                 if (elect_one()) {
-                    tc_commit(bars.kv_empty(vslot));
-                    if (j + 1 < last) tc_commit(bars.kv_empty(kslot));
+                    sums(x, vslot, j > 0);
+                    if (j + 1 < steps[x]) scores(x, next);
+                    else tc_commit(bars.s_full(x));
                 }
                 __syncwarp();
-                n += j + 1 < last ? 2 : 1;
             }
+            if (elect_one()) {
+                tc_commit(bars.kv_empty(kslot));
+                tc_commit(bars.kv_empty(vslot));
+            }
+            __syncwarp();
         }
     }
 }
@@ -401,13 +384,13 @@ __device__ __forceinline__ void kc_softmax(const Kv4AttnArgs& a, uint32_t smem, 
     constexpr int HD = S::HD;
     const uint32_t lanes = tmem + ((uint32_t)(r & ~31) << 16), scores = lanes + x * KC_TILE, sums = lanes + 256 + x * HD;
     KcRun u;
-    unsigned n = 0, units = 0;       // steps, runs with steps
+    unsigned ns = 0, np = 0;       // rounds of S and of P
     for (bool more = kc_begin(a, u, lane); more; more = kc_next(a, u)) {
         const int mine = u.steps[x], col = u.ctile * KC_COLS + x * KC_TILE + r;
         const bool there = col < u.e.z * a.group;
         const int row = there ? by_group(a, col) : 0, head = u.head * a.group + (there ? col - row * a.group : 0);
         const int limit = there ? u.e.y + row : -1, all = u.e.y + by_group(a, u.ctile * KC_COLS + x * KC_TILE);
-        float m = -INFINITY, l = 0.f;
+        float m = there ? -INFINITY : 0.f, l = 0.f;       // reference, sum
         if (mine > 0) {
             // the query times a power of two, so that its largest element lies in [1, 2): exact in f16 but for elements 2^14 times smaller
             const uint4* src = reinterpret_cast<const uint4*>(a.q + (long long)(u.e.w + row) * a.q_stride + head * HD);
@@ -433,103 +416,90 @@ __device__ __forceinline__ void kc_softmax(const Kv4AttnArgs& a, uint32_t smem, 
             __syncwarp();
             if (lane == 0) bar_arrive(bars.q_full(x));
 
-            for (int j = 0; j < mine; ++j, ++n) {
-                if (!bar_wait(bars.s_full(x), n & 1)) return give_up(a.c.flag);
+            float top = -INFINITY, step = 0.f;      // of the step last weighed: maximum, and the sum that counts once it is accepted
+            for (int j = 0;; ++j) {
+                if (!bar_wait(bars.s_full(x), ns & 1)) return give_up(a.c.flag);
+                ++ns;
                 tc_after();
+                if (j > 0) {
+                    if (lds32(bars.again(x)) == np - 1) {       // the same step once more
+                        --j;
+                        const bool far = top > m + 14.f;
+                        const float old = far ? ex2(m - top) : 1.f;
+                        if (far) m = top;
+                        l *= old;
+                        if (j > 0) {
+#pragma unroll 1
+                            for (int i = 0; i < HD; i += 16) {
+                                uint32_t v[16];
+                                tm_load16(sums + i, v);
+                                tm_wait(v);
+#pragma unroll
+                                for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * old);
+                                tm_store16(sums + i, v);
+                            }
+                        }
+                    } else {
+                        l += step;
+                        if (j == mine) break;
+                    }
+                }
                 const int base = (u.from + j) * KC_STEP;
                 const bool whole = base + KC_STEP - 1 <= all;        // every column sees all of the step
-                uint32_t s0[16], s1[16];
-                auto mask = [&](uint32_t (&s)[16], int first) {
+                top = -INFINITY;
+                auto look = [&](uint32_t (&s)[16], int first) {
                     if (!whole) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
                             if (base + first + i > limit) s[i] = 0xff800000u;
                     }
-                };
-                // Weights are taken against a reference, the first step's maximum: below 2^14 of it they fit f16 and the sums all the same, so
-                // a step looks for its own maximum while it weighs.  Only a column that has seen nothing yet, or that this step carries beyond
-                // 2^14, has to find the maximum first; each column decides for itself, so that its bits are its own.
-                float top = -INFINITY;
-                auto most = [&](const uint32_t (&s)[16]) {
 #pragma unroll
                     for (int i = 0; i < 16; i += 2) top = fmaxf(fmaxf(top, __uint_as_float(s[i])), __uint_as_float(s[i + 1]));
                 };
-                auto look = [&]() {         // the step's maximum, times the factor
-                    top = -INFINITY;
+                uint32_t s0[16], s1[16];
+                if (__any_sync(0xffffffffu, m == -INFINITY)) {       // a column has no reference yet
 #pragma unroll 1
                     for (int i = 0; i < KC_STEP; i += 16) {
                         tm_load16(scores + i, s0);
                         tm_wait(s0);
-                        mask(s0, i);
-                        most(s0);
+                        look(s0, i);
                     }
-                    top *= factor;
-                };
-                if (__any_sync(0xffffffffu, m == -INFINITY)) {
-                    look();
-                    if (m == -INFINITY) m = top;      // its sums are zeros so far
+                    if (m == -INFINITY) m = top * factor;            // its sums are zeros so far
                     top = -INFINITY;
                 }
-                float part[4];
-                uint32_t p[64];
-                auto weigh = [&](uint32_t (&s)[16], int first, float less) {
+                const float less = m == -INFINITY ? 0.f : -m;        // still nothing seen: weights of exp(-inf) = 0
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
+                auto weigh = [&](uint32_t (&s)[16], int first) {
+                    look(s, first);
+                    uint32_t p[8];
 #pragma unroll
                     for (int i = 0; i < 16; i += 2) {
                         const float w0 = ex2(fmaf(__uint_as_float(s[i]), factor, less)), w1 = ex2(fmaf(__uint_as_float(s[i + 1]), factor, less));
                         part[i & 2] += w0;
                         part[(i & 2) + 1] += w1;
-                        p[(first + i) >> 1] = pack_h2(w0, w1);
+                        p[i >> 1] = pack_h2(w0, w1);
                     }
+                    tm_store8(scores + (first >> 1), p);             // over scores that have been read
                 };
-                auto pass = [&]() {
-                    const float less = m == -INFINITY ? 0.f : -m;        // nothing seen yet: weights of exp(-inf) = 0
-                    part[0] = part[1] = part[2] = part[3] = 0.f;
-                    tm_load16(scores, s0);
+                tm_load16(scores, s0);
 #pragma unroll
-                    for (int i = 0; i < KC_STEP; i += 32) {
-                        tm_wait(s0);
-                        tm_load16(scores + i + 16, s1);
-                        mask(s0, i);
-                        most(s0);
-                        weigh(s0, i, less);
-                        tm_wait(s1);
-                        if (i + 32 < KC_STEP) tm_load16(scores + i + 32, s0);
-                        mask(s1, i + 16);
-                        most(s1);
-                        weigh(s1, i + 16, less);
-                    }
-                };
-                pass();
-                top *= factor;
-                if (__any_sync(0xffffffffu, top > m + 14.f)) {
-                    const bool far = top > m + 14.f;
-                    const float old = far ? ex2(m - top) : 1.f;
-                    if (far) m = top;
-                    l *= old;
-                    if (j > 0) {
-#pragma unroll 1
-                        for (int i = 0; i < HD; i += 16) {
-                            tm_load16(sums + i, s0);
-                            tm_wait(s0);
-#pragma unroll
-                            for (int k = 0; k < 16; ++k) s0[k] = __float_as_uint(__uint_as_float(s0[k]) * old);
-                            tm_store16(sums + i, s0);
-                        }
-                    }
-                    pass();
+                for (int i = 0; i < KC_STEP; i += 32) {
+                    tm_wait(s0);
+                    tm_load16(scores + i + 16, s1);
+                    weigh(s0, i);
+                    tm_wait(s1);
+                    if (i + 32 < KC_STEP) tm_load16(scores + i + 32, s0);
+                    weigh(s1, i + 16);
                 }
-                // over the scores, which have been read
-                tm_store32(scores, reinterpret_cast<uint32_t(&)[32]>(p[0]));
-                tm_store32(scores + 32, reinterpret_cast<uint32_t(&)[32]>(p[32]));
-                l += (part[0] + part[1]) + (part[2] + part[3]);
+                step = (part[0] + part[1]) + (part[2] + part[3]);
+                top *= factor;
+                if (__any_sync(0xffffffffu, top > m + 14.f) && lane == 0) sts32(bars.again(x), np);
+                ++np;
                 tm_stored();
                 tc_before();
                 __syncwarp();
                 if (lane == 0) bar_arrive(bars.p_full(x));
             }
-            if (!bar_wait(bars.o_full(x), units & 1)) return give_up(a.c.flag);
-            ++units;
-            tc_after();
         }
         const bool entire = u.to - u.from == u.cost;
         const size_t place = (size_t)(2 * blockIdx.x + (u.from == 0)) * KC_COLS + x * KC_TILE + r;
@@ -579,7 +549,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv4_attn_chunk(const Kv4AttnA
             bar_init(bars.q_full(x), 4);
             bar_init(bars.s_full(x), 1);
             bar_init(bars.p_full(x), 4);
-            bar_init(bars.o_full(x), 1);
+            sts32(bars.again(x), 0xffffffffu);
         }
         for (int s = 0; s < S::SLOTS; ++s) {
             bar_init(bars.kv_full(s), KC_FILL);
@@ -589,7 +559,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv4_attn_chunk(const Kv4AttnA
     }
     pdl_wait();
     pdl_launch();
-    if (warp == 12) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(bars.tmem()) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -599,12 +569,12 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv4_attn_chunk(const Kv4AttnA
     uint32_t tmem;
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(bars.tmem()));
     if (warp < KC_FILL) kc_fill<NG>(a, smem + 2 * S::Q, bars, warp, lane);
-    else if (warp < 12) kc_softmax<NG>(a, smem, bars, tmem, warp >= 8, threadIdx.x & 127, lane);
+    else if (warp < 16) kc_softmax<NG>(a, smem, bars, tmem, warp >= 12, threadIdx.x & 127, lane);
     else kc_issue<NG>(a, smem, bars, tmem, lane);
     tc_before();
     __syncthreads();
     tc_after();
-    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
 // Adds up the parts of the (column tile, kv head)s that several CTAs had, in the order of the positions.  CTA (b, i) does it for 32 columns of
