@@ -351,7 +351,6 @@ __device__ __forceinline__ void kc_issue(const Kv4AttnArgs& a, uint32_t smem, co
         for (int j = 0; j < last; ++j, n += 2) {
             const unsigned kslot = n % S::SLOTS, vslot = (n + 1) % S::SLOTS, next = (n + 2) % S::SLOTS;
             if (!bar_wait(bars.kv_full(vslot), ((n + 1) / S::SLOTS) & 1)) return give_up(a.c.flag);
-            if (j + 1 < last && !bar_wait(bars.kv_full(next), ((n + 2) / S::SLOTS) & 1)) return give_up(a.c.flag);
             for (int x = 0; x < 2; ++x) {
                 if (j >= steps[x]) continue;
                 for (;;) {
@@ -363,9 +362,13 @@ __device__ __forceinline__ void kc_issue(const Kv4AttnArgs& a, uint32_t smem, co
                 }
                 if (elect_one()) {
                     sums(x, vslot, j > 0);
-                    if (j + 1 < steps[x]) scores(x, next);
-                    else tc_commit(bars.s_full(x));
+                    if (j + 1 == steps[x]) tc_commit(bars.s_full(x));
                 }
+                __syncwarp();
+                if (j + 1 == steps[x]) continue;
+                if (!bar_wait(bars.kv_full(next), ((n + 2) / S::SLOTS) & 1)) return give_up(a.c.flag);
+                tc_after();
+                if (elect_one()) scores(x, next);
                 __syncwarp();
             }
             if (elect_one()) {
@@ -469,9 +472,8 @@ __device__ __forceinline__ void kc_softmax(const Kv4AttnArgs& a, uint32_t smem, 
                 }
                 const float less = m == -INFINITY ? 0.f : -m;        // still nothing seen: weights of exp(-inf) = 0
                 float part[4] = {0.f, 0.f, 0.f, 0.f};
-                auto weigh = [&](uint32_t (&s)[16], int first) {
+                auto weigh = [&](uint32_t (&s)[16], int first, uint32_t (&p)[8]) {
                     look(s, first);
-                    uint32_t p[8];
 #pragma unroll
                     for (int i = 0; i < 16; i += 2) {
                         const float w0 = ex2(fmaf(__uint_as_float(s[i]), factor, less)), w1 = ex2(fmaf(__uint_as_float(s[i + 1]), factor, less));
@@ -479,18 +481,22 @@ __device__ __forceinline__ void kc_softmax(const Kv4AttnArgs& a, uint32_t smem, 
                         part[(i & 2) + 1] += w1;
                         p[i >> 1] = pack_h2(w0, w1);
                     }
-                    tm_store8(scores + (first >> 1), p);             // over scores that have been read
                 };
+                // P goes over scores that have been read, a piece behind, so that a store does not wait for the exponentials under way
+                uint32_t p0[8], p1[8];
                 tm_load16(scores, s0);
 #pragma unroll
                 for (int i = 0; i < KC_STEP; i += 32) {
                     tm_wait(s0);
                     tm_load16(scores + i + 16, s1);
-                    weigh(s0, i);
+                    weigh(s0, i, p0);
+                    if (i > 0) tm_store8(scores + (i >> 1) - 8, p1);
                     tm_wait(s1);
                     if (i + 32 < KC_STEP) tm_load16(scores + i + 32, s0);
-                    weigh(s1, i + 16);
+                    weigh(s1, i + 16, p1);
+                    tm_store8(scores + (i >> 1), p0);
                 }
+                tm_store8(scores + KC_STEP / 2 - 8, p1);
                 step = (part[0] + part[1]) + (part[2] + part[3]);
                 top *= factor;
                 if (__any_sync(0xffffffffu, top > m + 14.f) && lane == 0) sts32(bars.again(x), np);
