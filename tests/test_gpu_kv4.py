@@ -240,6 +240,21 @@ def test_rows_that_lie_anywhere():
 
 
 # -------------------------------------------------------------------------------------------------------- attention
+def fixed(x, k, v, p, mag, scale):
+    """What fixed-point queries and weights may add to an error: x (rows, heads, dim), k and v (n, heads, dim), p (heads, rows, n).
+
+    Queries enter as whole numbers of 2^-13 of the power of two below their largest element: exact (8 digits) but for elements below
+    2^-6 of it, each half a unit off at most.  Weights times value scales enter in units of 2^-16 of the largest scale R, half a unit off at
+    most, against codes up to 15.  Both kinds of errors are independent of one another: six standard deviations (a unit's over the
+    square root of 12)."""
+    unit = torch.exp2(x.abs().amax(-1).clamp(min=1e-300).log2().floor())                # (rows, heads)
+    small = (x.abs() < unit[..., None] / 64).double()
+    score = torch.einsum("rhd,nhd->rhn", small, k * k).amax(-1).sqrt() * unit * scale * 2.0 ** -13 / 12 ** 0.5 * 6
+    span = (v.unflatten(-1, (-1, 32)).amax(-1) - v.unflatten(-1, (-1, 32)).amin(-1)).amax() / 15 * 1.001
+    sums = k.shape[0] ** 0.5 * span * 15 * 2.0 ** -16 / 12 ** 0.5 * 6 * p.amax(-1).T     # the largest weight is 1 of the sum
+    return 2 * score[..., None] * mag + sums[..., None]
+
+
 class Filled:
     """A cache with sequences of the given lengths, stored in rounds so that their blocks lie in turn, and its contents in fp64."""
 
@@ -272,12 +287,7 @@ class Filled:
         return plan
 
     def want(self, q, new, scale=None):
-        """Softmax attention in 64 bits, the same of the values' magnitudes, and what fixed-point queries and weights may add to an error.
-
-        Queries enter as whole numbers of 2^-13 of the power of two below their largest element: exact (8 digits) but for elements below
-        2^-6 of it, each half a unit off at most.  Weights times value scales enter in units of 2^-16 of the largest scale R, half a unit off at
-        most, against codes up to 15.  Both kinds of errors are independent of one another: six standard deviations (a unit's over the
-        square root of 12)."""
+        """Softmax attention in 64 bits, the same of the values' magnitudes, and what fixed() says."""
         outs, mags, more, a = [], [], [], 0
         scale = self.dim ** -0.5 if scale is None else scale
         for i, m in enumerate(new):
@@ -289,15 +299,7 @@ class Filled:
             p = s.masked_fill(late, float("-inf")).softmax(-1)
             outs.append(torch.einsum("hrn,nhd->rhd", p, v))
             mags.append(torch.einsum("hrn,nhd->rhd", p, v.abs()))
-            if m and n:
-                unit = torch.exp2(x.abs().amax(-1).clamp(min=1e-300).log2().floor())                # (rows, heads)
-                small = (x.abs() < unit[..., None] / 64).double()
-                score = torch.einsum("rhd,nhd->rhn", small, k * k).amax(-1).sqrt() * unit * scale * 2.0 ** -13 / 12 ** 0.5 * 6
-                span = (v.unflatten(-1, (-1, 32)).amax(-1) - v.unflatten(-1, (-1, 32)).amin(-1)).amax() / 15 * 1.001
-                sums = n ** 0.5 * span * 15 * 2.0 ** -16 / 12 ** 0.5 * 6 * p.amax(-1).T               # the largest weight is 1 of the sum
-                more.append(2 * score[..., None] * mags[-1] + sums[..., None])
-            else:
-                more.append(torch.zeros_like(mags[-1]))
+            more.append(fixed(x, k, v, p, mags[-1], scale) if m and n else torch.zeros_like(mags[-1]))
             a += m
         return torch.cat(outs), torch.cat(mags), torch.cat(more)
 
@@ -337,6 +339,17 @@ def test_single_tokens(heads, kv, dim, block):
     (4, 4, 64, 64, [2000], [2]),
     (2, 2, 96, 256, [0, 40, 1], [600, 500, 700]),
     (16, 8, 64, 64, [20] * 40, [0] * 13 + [64] * 20 + [33] * 7),
+    # 4096 query heads of rows and more, and 128 of a kv head: whole and partial tiles of 128, groups that do not divide them, sequences
+    # without rows, more tiles than SMs and fewer
+    (16, 8, 64, 16, [0], [256]),
+    (16, 8, 64, 64, [1000, 0, 3, 40], [64, 0, 200, 1]),
+    (28, 4, 64, 32, [0, 129, 700], [101, 19, 55]),
+    (24, 8, 96, 64, [0, 300], [171, 43]),
+    (32, 2, 96, 128, [1500], [131]),
+    (15, 5, 128, 16, [127, 1, 0], [129, 128, 127]),
+    (64, 4, 128, 256, [0, 0, 2000], [1, 8, 64]),
+    (16, 16, 64, 64, [100, 5], [1100, 7]),
+    (32, 8, 128, 32, [0, 0, 0, 900], [380, 257, 128, 5]),
 ])
 def test_chunks_of_prompts(heads, kv, dim, block, before, new):
     f = Filled([max(x, 1) for x in before], heads, kv, dim, block, spare=max(new))
@@ -382,27 +395,30 @@ def test_peaked_scores():
     close(f.cache.attention(0, q, plan), (ref, 2 * mag, more))
 
 
-@pytest.mark.parametrize("heads, kv, dim, grow", [(16, 8, 64, False), (8, 2, 128, True), (6, 2, 96, True), (16, 8, 64, True)])
-def test_peaked_chunks(heads, kv, dim, grow):
+@pytest.mark.parametrize("heads, kv, dim, grow, new", [
+    (16, 8, 64, False, 250), (8, 2, 128, True, 250), (6, 2, 96, True, 250), (16, 8, 64, True, 250),
+    (16, 8, 64, False, 270), (16, 2, 64, True, 270), (32, 4, 128, True, 270), (24, 8, 96, True, 270), (32, 2, 128, False, 257)])
+def test_peaked_chunks(heads, kv, dim, grow, new):
     """The same for chunks of prompts; with keys that grow along the sequence, so that a column's maximum keeps leaving the weights' range.
     Scores as above, of up to 450."""
     f = Filled([1], heads, kv, dim, 64, spare=1800, key_scale=30.0, max_blocks=40)
     for part in range(6):
         f.key_scale = 30.0 * (2.0 ** (part - 5) if grow else 1.0)
-        plan = f.add([250])
-        q = torch.randn(250, heads, dim, device="cuda", generator=f.g).bfloat16()
-        ref, mag, more = f.want(q, [250])
+        plan = f.add([new])
+        q = torch.randn(new, heads, dim, device="cuda", generator=f.g).bfloat16()
+        ref, mag, more = f.want(q, [new])
         out = f.cache.attention(0, q, plan)
         close(out, (ref, 2 * mag, more))
         assert torch.equal(out, f.cache.attention(0, q, plan))
     f.cache.check_device()
 
 
-def test_a_row_of_nan_in_a_chunk():
-    f = Filled([700], 16, 8, 64, 64, spare=100)
-    plan = f.add([100])
-    q = torch.randn(100, 16, 64, device="cuda", generator=f.g).bfloat16()
-    want = f.want(q, [100])
+@pytest.mark.parametrize("new, dim", [(100, 64), (300, 64), (300, 128)])
+def test_a_row_of_nan_in_a_chunk(new, dim):
+    f = Filled([700], 16, 8, dim, 64, spare=new)
+    plan = f.add([new])
+    q = torch.randn(new, 16, dim, device="cuda", generator=f.g).bfloat16()
+    want = f.want(q, [new])
     bad = q.clone()
     bad[31, 7, 5], bad[90, 2, 0] = float("nan"), float("inf")
     out = f.cache.attention(0, bad, plan)
@@ -512,6 +528,64 @@ def test_captured_steps_cross_blocks():
         assert cache.seq_lens.tolist() == [45] * 3
 
 
+def test_captured_chunks():
+    """Two caches' graphs of whole prompt chunks, replayed side by side for chunks of other lengths, are the same as eager calls."""
+    def step(cache, bufs):
+        k, v, q, new, at = bufs
+        plan = cache.plan(slots, new, at=at, n_rows=320, max_new=300)
+        cache.append(0, k, v, plan)
+        return plan, cache.attention(0, q, plan, out=torch.full_like(q, 5.0))
+
+    slots = torch.tensor([2, 0, 1], dtype=torch.int32, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(9)
+    runs = []
+    for _ in range(2):
+        cache, eager = make(120, 16, 3, 40), make(120, 16, 3, 40)
+        bufs = [torch.randn(320, h, 64, generator=g, device="cuda").bfloat16() for h in (8, 8, 16)]
+        bufs += [torch.zeros(3, dtype=torch.int32, device="cuda") for _ in range(2)]
+        step(cache, bufs)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            plan, out = step(cache, bufs)
+        runs.append((cache, eager, bufs, graph, plan, out, torch.cuda.Stream()))
+    for new, at in (([300, 1, 19], [0, 0, 0]), ([0, 200, 120], [300, 1, 19]), ([20, 0, 300], [300, 0, 139]), ([0, 0, 0], [320, 0, 0]),
+                    ([290, 30, 0], [320, 0, 0]), ([1, 1, 1], [610, 30, 0])):
+        for cache, eager, bufs, graph, plan, out, stream in runs:
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                for b in bufs[:3]:
+                    b.normal_(generator=g)
+                for b, x in zip(bufs[3:], (new, at)):
+                    b.copy_(torch.tensor(x, dtype=torch.int32))
+                graph.replay()
+        torch.cuda.synchronize()
+        for cache, eager, bufs, graph, plan, out, stream in runs:
+            want_plan, want = step(eager, bufs)
+            assert torch.equal(plan.slot_map, want_plan.slot_map) and torch.equal(out, want) and (out[sum(new):] == 5).all()
+            cache.check_device()
+            eager.check_device()
+
+
+def test_one_plan_on_two_streams():
+    """Two layers of one plan at the same time: each stream has partial sums of its own."""
+    for new, heads, kv in (([1, 1], 16, 8), ([20, 40], 16, 8), ([300, 9], 16, 8)):
+        f = Filled([3000, 800], heads, kv, 64, 64, spare=max(new))
+        plan = f.add(new)
+        qs = [torch.randn(sum(new), heads, 64, device="cuda", generator=f.g).bfloat16() for _ in range(2)]
+        want = [f.cache.attention(0, q, plan) for q in qs]
+        streams = [torch.cuda.Stream() for _ in qs]
+        got = [[], []]
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+        for _ in range(8):
+            for i, s in enumerate(streams):
+                with torch.cuda.stream(s):
+                    got[i].append(f.cache.attention(0, qs[i], plan))
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, w) for g, w in zip(got, want) for x in g)
+
+
 def test_on_another_stream():
     side = torch.cuda.Stream()
     with torch.cuda.stream(side):
@@ -554,7 +628,8 @@ def test_a_conversation_is_put_away_and_taken_up_again(nano_model):
         ref = torch.einsum("hn,nhd->hd", p, vv).flatten()
         mag = torch.einsum("hn,nhd->hd", p, vv.abs()).flatten()
         move = torch.einsum("hd,nhd->hn", qh.abs(), kk.abs()).amax(-1).repeat_interleave(64) / 8 * 2.0 ** -8
-        assert ((a[0] - ref).abs() <= 2.0 ** -8 * ref.abs() + 2.0 ** -10 * mag).all()
+        more = fixed(qh[None], kk, vv, p[:, None], mag.view(1, 16, 64), 0.125).flatten()
+        assert ((a[0] - ref).abs() <= 2.0 ** -8 * ref.abs() + 2.0 ** -10 * mag + more).all()
         assert ((b[0] - ref).abs() <= 2.0 ** -8 * ref.abs() + (2.0 ** -8 + 2.2 * move + 2.0 ** -10) * mag).all()
     cache.check_device()
     eng.check_device()

@@ -70,9 +70,6 @@ long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 // A few columns: splits of 256 positions in sequences of up to 1024, 512 beyond, whatever the batch.
 // Up to 16 columns the form for a few (2, 4, 8 or 16 columns a tile), else the one for many.
 enum Form { FEW_HALVES, FEW_4, FEW_8, FEW_16, MANY, CHUNK };
-#ifndef KV4_CHUNK
-#define KV4_CHUNK 64
-#endif
 struct Shape { Form form; int cols; Kv4Split split; };
 Shape shape_of(const VuibKv4* c, const VuibKv4Plan* p) {
     const int group = c->cfg.n_heads / c->cfg.n_kv_heads;
@@ -82,7 +79,7 @@ Shape shape_of(const VuibKv4* c, const VuibKv4Plan* p) {
         return {f, f == FEW_HALVES ? 2 : f == FEW_4 ? 4 : f == FEW_8 ? 8 : 16, {512, 256, 512, 1 << 30, true}};
     }
     Shape s = {MANY, c->ng > 2 ? 16 : 32, {}};
-    if (most >= KV4_CHUNK) return {CHUNK, KC_COLS, {1 << 30, 1 << 30, 1 << 30, 1, false}};
+    if (most >= 128 && (long long)p->n_rows * c->cfg.n_heads >= 4096) return {CHUNK, KC_COLS, {1 << 30, 1 << 30, 1 << 30, 1, false}};
     const long long tiles = ceil_div((long long)p->n_rows * group, s.cols) + p->n_seqs;
     // enough tiles for the SMs: no splits; else at most 8 of a sequence, so that their sums stay a few megabytes
     const long long len = (long long)c->cfg.max_blocks << c->block_shift;
@@ -268,7 +265,8 @@ extern "C" int32_t vuib_kv4_plan(VuibKv4* c, const VuibKv4Plan* p, const int32_t
     a.row_slot = p->row_slot; a.row_pos = p->row_pos; a.slot_map = reinterpret_cast<long long*>(p->slot_map);
     const size_t smem = (8 * (size_t)p->n_seqs + 3 + c->cfg.max_seqs) * 4;
     if (smem > 48 * 1024) CK(cudaFuncSetAttribute(k_kv4_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    const int cluster = p->n_rows > 4096 ? 8 : 1;
+    // One CTA where little is written: a cluster's barriers cost 2 us.  Rows are known here; cut-backs can give back any number of blocks.
+    const int cluster = p->n_rows > 4096 || (at_dev && p->n_seqs > 64 && c->cfg.n_blocks > 4096) ? 8 : 1;
     const int threads = p->n_seqs <= 256 && p->n_rows <= 1024 ? 256 : 1024;
     CK(launch(c, k_kv4_plan, dim3(cluster), threads, smem, cluster, stream, a));
     return VUIB_OK;

@@ -276,33 +276,68 @@ __global__ void __launch_bounds__(1024) k_kv4_plan(const Kv4PlanArgs a) {
     }
     // Blocks given back go on the stack so that the first entry's first one is on top; those taken come off the top in entry order:
     // what was given back and is taken again in the same order gets its places again.
-    for (int r = me; r < dropped; r += step) {
-        const int i = find_in(s_drop, n, r);
-        int32_t* at = a.c.table + (size_t)s_slot[i] * a.c.max_blocks + s_need[i] + (r - s_drop[i]);
-        if (top - 1 - r < a.c.n_blocks) a.c.free_blocks[top - 1 - r] = *at;
-        *at = -1;
+    // Four at a time, so that their reads of the L2 are under way together.
+    for (int r0 = me; r0 < dropped; r0 += 4 * step) {
+        int32_t* at[4];
+        int id[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int r = r0 + k * step;
+            at[k] = nullptr;
+            if (r >= dropped) continue;
+            const int i = find_in(s_drop, n, r);
+            at[k] = a.c.table + (size_t)s_slot[i] * a.c.max_blocks + s_need[i] + (r - s_drop[i]);
+            id[k] = __ldcg(at[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (!at[k]) continue;
+            const int to = top - 1 - (r0 + k * step);
+            if (to < a.c.n_blocks) a.c.free_blocks[to] = id[k];
+            *at[k] = -1;
+        }
     }
     if (dropped) plan_sync(size);
-    for (int r = me; r < grown; r += step) {
-        const int i = find_in(s_grow, n, r);
-        a.c.table[(size_t)s_slot[i] * a.c.max_blocks + s_have[i] + (r - s_grow[i])] = __ldcg(a.c.free_blocks + (top - 1 - r));
+    for (int r0 = me; r0 < grown; r0 += 4 * step) {
+        int32_t* at[4];
+        int id[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int r = r0 + k * step;
+            at[k] = nullptr;
+            if (r >= grown) continue;
+            id[k] = __ldcg(a.c.free_blocks + (top - 1 - r));
+            const int i = find_in(s_grow, n, r);
+            at[k] = a.c.table + (size_t)s_slot[i] * a.c.max_blocks + s_have[i] + (r - s_grow[i]);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (at[k]) *at[k] = id[k];
     }
     if (grown || dropped) plan_sync(size);
-    for (int r = me; r < a.n_rows; r += step) {
-        int slot = -1, pos = -1, i = -1;
-        long long where = -1;
-        if (r < rows) {
-            i = find_in(s_cu, n, r);
-            slot = s_slot[i];
-            pos = s_start[i] + (r - s_cu[i]);
-            const int b = __ldcg(a.c.table + (size_t)slot * a.c.max_blocks + (pos >> a.c.block_shift));
-            if (b >= 0 && b < a.c.n_blocks) where = ((long long)b << a.c.block_shift) + (pos & (bs - 1));
-            else atomicOr(a.c.flag, KV4_BAD_BLOCK);
+    for (int r0 = me; r0 < a.n_rows; r0 += 4 * step) {
+        int entry[4], pos[4], block[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int r = r0 + k * step;
+            entry[k] = pos[k] = block[k] = -1;
+            if (r >= rows) continue;
+            const int i = find_in(s_cu, n, r);
+            entry[k] = i;
+            pos[k] = s_start[i] + (r - s_cu[i]);
+            block[k] = __ldcg(a.c.table + (size_t)s_slot[i] * a.c.max_blocks + (pos[k] >> a.c.block_shift));
         }
-        a.row_entry[r] = i;
-        a.row_slot[r] = slot;
-        a.row_pos[r] = pos;
-        a.slot_map[r] = where;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int r = r0 + k * step;
+            if (r >= a.n_rows) continue;
+            const bool fine = (unsigned)block[k] < (unsigned)a.c.n_blocks;
+            if (!fine && entry[k] >= 0) atomicOr(a.c.flag, KV4_BAD_BLOCK);
+            a.row_entry[r] = entry[k];
+            a.row_slot[r] = entry[k] >= 0 ? s_slot[entry[k]] : -1;
+            a.row_pos[r] = pos[k];
+            a.slot_map[r] = fine ? ((long long)block[k] << a.c.block_shift) + (pos[k] & (bs - 1)) : -1;
+        }
     }
 }
 
@@ -341,23 +376,22 @@ __device__ __forceinline__ uint32_t most_bits(const uint4& r) {
     const uint32_t m = __vmaxu2(__vmaxu2(r.x & 0x7fff7fffu, r.y & 0x7fff7fffu), __vmaxu2(r.z & 0x7fff7fffu, r.w & 0x7fff7fffu));
     return max(m & 0xffffu, m >> 16);
 }
-constexpr uint32_t KV4_LIMIT_BITS = 0x476a;   // 59904, the largest bf16 below KV4_LIMIT
 
-__device__ __noinline__ float tame(float x) { return x == x ? fminf(fmaxf(x, -KV4_LIMIT), KV4_LIMIT) : 0.f; }
-__device__ __noinline__ void codes_by_division(const float (&x)[8], float z, float s, uint32_t (&code)[8]) {
-    for (int j = 0; j < 8; ++j) code[j] = (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[j], z), s)), 0.f), 15.f);
-}
+__device__ __forceinline__ float tame(float x) { return x == x ? fminf(fmaxf(x, -KV4_LIMIT), KV4_LIMIT) : 0.f; }
+// Element j of 16 bf16.
+__device__ __forceinline__ float element(const uint32_t (&w)[8], int j) { return __uint_as_float(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16); }
 
-// A warp stores one tile of 16 positions of one kv head, or those of its positions that are new: NG * 4 lanes a row, 8 elements a lane,
-// the four lanes of a group share its extremes; the codes are gathered in shared memory as they lie in the pool and leave it 16 bytes a
-// lane where the whole tile is new, else in the words and bytes of the new positions.
-// The nearest code: (x - zero) times the reciprocal of the scale is 2^-19 off at most (three roundings of a quotient below 16), so unless
-// that lies within 2^-17 of the middle between two codes it rounds as the quotient does; the few that do are divided.
+// A warp stores one tile of 16 positions of one kv head, or those of its positions that are new: 16 elements a lane, two lanes a group, which
+// share its extremes; the codes are gathered in shared memory as they lie in the pool and leave it 16 bytes a lane where the whole tile is
+// new, else in the words and bytes of the new positions.
+// The nearest code: (x - zero) times the reciprocal of 15 scales, kept within [0, 1] and times 15, is 2^-17.4 off at most (a division of two ulp and two roundings, of a
+// quotient below 16), so unless that lies within 2^-17 of the middle between two codes it rounds as the quotient does; the few lanes that
+// have such an element divide.
 template <int NG>
 __global__ void __launch_bounds__(128) k_kv4_append(const Kv4RowsArgs a) {
-    constexpr int LANES = NG * 4, ROWS = 32 / LANES;     // lanes of a row, rows side by side: 4, 2 (8 lanes idle), 2
-    constexpr int IMG = NG * KV4_GT;
-    __shared__ __align__(16) unsigned char image[4][IMG];
+    constexpr int LANES = NG * 2, ROWS = 32 / LANES, TURNS = (16 + ROWS - 1) / ROWS;     // lanes of a row; rows side by side: 8, 5 (2 lanes idle), 4
+    constexpr int PITCH = KV4_GT + 16;                       // a group's image: 4 banks further than the one before
+    __shared__ __align__(16) unsigned char image[4][NG * PITCH];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     unsigned char* const img = image[warp];
     const long long id = (long long)blockIdx.x * 4 + warp;
@@ -378,96 +412,118 @@ __global__ void __launch_bounds__(128) k_kv4_append(const Kv4RowsArgs a) {
     const int4 e = __ldcg(a.entries + lo);
     const int pos0 = ((e.y >> 4) + want - before) << 4;                       // the tile's first position
     const int from = max(e.y, pos0) - pos0, to = min(e.y + e.z, pos0 + 16) - pos0;
-    int b = __ldcg(a.c.table + (size_t)e.x * a.c.max_blocks + (pos0 >> a.c.block_shift));
+    const int b = __ldcg(a.c.table + (size_t)e.x * a.c.max_blocks + (pos0 >> a.c.block_shift));
     if ((unsigned)b >= (unsigned)a.c.n_blocks) {
         if (lane == 0) atomicOr(a.c.flag, KV4_BAD_BLOCK);
         return;
     }
     unsigned char* const tile = a.c.pool + tile_at<NG>(a.c, ((long long)b << a.c.block_shift) + (pos0 & ((1 << a.c.block_shift) - 1)), h);
-    const int sub = lane / LANES, ch = lane % LANES, grp = ch >> 2, t = ch & 3;
-    unsigned char* const gimg = img + grp * KV4_GT;
+    const int sub = lane / LANES, ch = lane % LANES;
+    unsigned char* const gimg = img + (ch >> 1) * PITCH;
+    // keys, then values, a few rows at a time, the next ones on their way meanwhile.  (One loop body: unrolled it is 50 KB of code, and 72 us
+    // for 16000 rows of 8 heads of 128 where this takes 40.)
+    auto rows_of = [&](int it, uint4 (&raw)[2]) {
+        const bool value = it >= TURNS;
+        const int key = (value ? it - TURNS : it) * ROWS + sub;
+        raw[0] = raw[1] = make_uint4(0, 0, 0, 0);
+        if (it < 2 * TURNS && sub < ROWS && key >= from && key < to) {
+            const __nv_bfloat16* src = (value ? a.v : a.k) + (long long)(e.w + pos0 - e.y + key) * (value ? a.v_stride : a.k_stride) + h * (NG * KV4_GROUP) + ch * 16;
+            raw[0] = __ldcg(reinterpret_cast<const uint4*>(src));
+            raw[1] = __ldcg(reinterpret_cast<const uint4*>(src) + 1);
+        }
+    };
+    // turns that hold a new position: [first, end) of keys, and the same of values
+    const int first = from / ROWS, end = (to + ROWS - 1) / ROWS;
+    uint4 next[2];
+    rows_of(first, next);
+    {
+#pragma unroll 1
+        for (int it = first; it < TURNS + end; it = it + 1 == end ? TURNS + first : it + 1) {
+            const uint4 raw[2] = {next[0], next[1]};
+            rows_of(it + 1 == end ? TURNS + first : it + 1, next);
+            const bool half = it >= TURNS;
+            const int key = (half ? it - TURNS : it) * ROWS + sub;
+            uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+            __nv_bfloat162 least = *reinterpret_cast<const __nv_bfloat162*>(&w[0]), most = least;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {       // keys, values
-        const __nv_bfloat16* src = (half ? a.v : a.k) + (long long)(e.w + pos0 - e.y) * (half ? a.v_stride : a.k_stride) + h * (NG * KV4_GROUP) + ch * 8;
-        const long long stride = half ? a.v_stride : a.k_stride;
-#pragma unroll
-        for (int part = 0; part < 16 / ROWS; part += 4) {       // four rows a lane in flight
-            uint4 raw[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int key = (part + j) * ROWS + sub;
-                raw[j] = make_uint4(0, 0, 0, 0);
-                if (sub < ROWS && key >= from && key < to) raw[j] = __ldcg(reinterpret_cast<const uint4*>(src + key * stride));
+            for (int j = 1; j < 8; ++j) {
+                const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(&w[j]);
+                least = __hmin2(least, v);
+                most = __hmax2_nan(most, v);
             }
+            float low = fminf(__low2float(least), __high2float(least)), high = __low2float(most);
+            high = high <= __high2float(most) ? __high2float(most) : high;       // NaN stays if it is in the first
+            const bool odd = !(high <= KV4_LIMIT) || !(low >= -KV4_LIMIT) || __hisnan(__high2bfloat16(most));
+            if (odd) {                                                           // so that what is stored is finite
+                atomicOr(a.c.flag, KV4_BAD_VALUE);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int key = (part + r) * ROWS + sub;
-                if ((part + r) * ROWS >= to) break;              // the whole warp
-                if ((part + r + 1) * ROWS <= from) continue;
-                const uint32_t w[4] = {raw[r].x, raw[r].y, raw[r].z, raw[r].w};
-                float x[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16);
-                if (most_bits(raw[r]) > KV4_LIMIT_BITS) {      // so that what is stored is finite
-                    atomicOr(a.c.flag, KV4_BAD_VALUE);
-                    for (int j = 0; j < 8; ++j) x[j] = tame(x[j]);
+                for (int j = 0; j < 16; ++j) {
+                    const float x = tame(element(w, j));
+                    low = j ? fminf(low, x) : x;
+                    high = j ? fmaxf(high, x) : x;
                 }
-                float low = x[0], high = x[0];
+            }
+            low = fminf(low, __shfl_xor_sync(0xffffffffu, low, 1));
+            high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 1));
+            const __half zero = __float2half_rn(low);
+            const float z = __half2float(zero);
+            const __half scale = __float2half_rn(__fmul_rn(__fsub_rn(high, z), 1.f / 15.f));
+            const float s = __half2float(scale), inv = s > 0.f ? __fdividef(1.f, 15.f * s) : 0.f;
+            uint32_t code[16];      // in the low bits of 2^23 + code
+            float near = 0.f;
 #pragma unroll
-                for (int j = 1; j < 8; ++j) { low = fminf(low, x[j]); high = fmaxf(high, x[j]); }
+            for (int j = 0; j < 16; ++j) {
+                const float x = odd ? tame(element(w, j)) : element(w, j);
+                const float q = __saturatef((x - z) * inv), c = fmaf(q, 15.f, 8388608.f);
+                near = fmaxf(near, fabsf(fmaf(q, 15.f, 8388608.f - c)));
+                code[j] = __float_as_uint(c);
+            }
+            if (near > 0.5f - 7.62939453125e-6f && s > 0.f) {
 #pragma unroll
-                for (int o = 1; o < 4; o <<= 1) {
-                    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
-                    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+                for (int j = 0; j < 16; ++j) {
+                    const float x = odd ? tame(element(w, j)) : element(w, j);
+                    code[j] = __float_as_uint(8388608.f + fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x, z), s)), 0.f), 15.f));
                 }
-                const __half zero = __float2half_rn(low);
-                const float z = __half2float(zero);
-                const __half scale = __float2half_rn(__fmul_rn(__fsub_rn(high, z), 1.f / 15.f));
-                const float s = __half2float(scale), inv = s > 0.f ? __frcp_rn(s) : 0.f;
-                uint32_t code[8];
-                float near = 0.f;
+            }
+            if (sub >= ROWS || key < from || key >= to) continue;
+            const int key8 = key & 7, upper = key >> 3;
+            constexpr uint32_t BASE = 0x4B000000u;      // the bits of 2^23
+            if (!half) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float q = fminf(fmaxf(__fsub_rn(x[j], z), 0.f) * inv, 15.f);
-                    const float c = q + 8388608.f;             // 2^23: the nearest whole number is in the low bits
-                    near = fmaxf(near, fabsf(q - (c - 8388608.f)));
-                    code[j] = __float_as_uint(c) & 15u;
+                for (int q = 0; q < 2; ++q) {
+                    uint32_t word = 0u - BASE * 0x11111111u;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) word += code[8 * q + j] << (4 * (j >> 1) + 16 * (j & 1));
+                    *reinterpret_cast<uint32_t*>(gimg + (key8 * 4 + (ch & 1) * 2 + q) * 8 + upper * 4) = word;
                 }
-                if (near > 0.5f - 7.62939453125e-6f && s > 0.f) codes_by_division(x, z, s, code);
-                if (sub >= ROWS || key < from || key >= to) continue;
-                const int key8 = key & 7, upper = key >> 3;
-                if (!half) {
-                    uint32_t word = 0;
+                if (!(ch & 1)) *reinterpret_cast<__half2*>(gimg + KV4_KPAR + key8 * 8 + upper * 4) = __halves2half2(scale, zero);
+            } else {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) word |= code[j] << (4 * (j >> 1) + 16 * (j & 1));
-                    *reinterpret_cast<uint32_t*>(gimg + (key8 * 4 + t) * 8 + upper * 4) = word;
-                    if (t == 0) *reinterpret_cast<__half2*>(gimg + KV4_KPAR + key8 * 8 + upper * 4) = __halves2half2(scale, zero);
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        gimg[KV4_VCODE + ((2 * t + (q >> 1)) * 4 + (key8 >> 1)) * 8 + (q & 1) * 4 + (key8 & 1) * 2 + upper] =
-                            (unsigned char)(code[2 * q] | code[2 * q + 1] << 4);
-                    if (t == 0) *reinterpret_cast<__half2*>(gimg + KV4_VPAR + key8 * 8 + upper * 4) = __halves2half2(scale, zero);
-                }
+                for (int q = 0; q < 8; ++q)
+                    gimg[KV4_VCODE + (((ch & 1) * 4 + (q >> 1)) * 4 + (key8 >> 1)) * 8 + (q & 1) * 4 + (key8 & 1) * 2 + upper] =
+                        (unsigned char)(code[2 * q] + (code[2 * q + 1] << 4));
+                if (!(ch & 1)) *reinterpret_cast<__half2*>(gimg + KV4_VPAR + key8 * 8 + upper * 4) = __halves2half2(scale, zero);
             }
         }
     }
     __syncwarp();
     if (to - from == 16) {
-        for (int i = lane; i < IMG / 16; i += 32) reinterpret_cast<uint4*>(tile)[i] = reinterpret_cast<const uint4*>(img)[i];
+        for (int i = lane; i < NG * (KV4_GT / 16); i += 32)
+            reinterpret_cast<uint4*>(tile)[i] = *reinterpret_cast<const uint4*>(img + i / (KV4_GT / 16) * PITCH + i % (KV4_GT / 16) * 16);
         return;
     }
-    for (int i = lane; i < IMG / 4; i += 32) {      // word i of the image: whose is it?
+    for (int i = lane; i < NG * (KV4_GT / 4); i += 32) {      // word i of the tile: whose is it?
         const int in = i * 4 % KV4_GT;
+        const unsigned char* const from_img = img + i / (KV4_GT / 4) * PITCH + in;
         if (in < KV4_VCODE || in >= KV4_VPAR) {     // one key's
             const int key = (in < KV4_KPAR ? in >> 5 : in < KV4_VCODE ? (in - KV4_KPAR) >> 3 : (in - KV4_VPAR) >> 3) + (in >> 2 & 1) * 8;
-            if (key >= from && key < to) reinterpret_cast<uint32_t*>(tile)[i] = reinterpret_cast<const uint32_t*>(img)[i];
+            if (key >= from && key < to) reinterpret_cast<uint32_t*>(tile)[i] = *reinterpret_cast<const uint32_t*>(from_img);
         } else {                                    // four keys', a byte each
             const int key = (in >> 3 & 3) * 2;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int k = key + (q >> 1) + (q & 1) * 8;
-                if (k >= from && k < to) tile[4 * i + q] = img[4 * i + q];
+                if (k >= from && k < to) tile[4 * i + q] = from_img[q];
             }
         }
     }
@@ -490,35 +546,38 @@ __global__ void __launch_bounds__(256) k_kv4_read(const Kv4RowsArgs a) {
         if (b >= 0 && b < a.c.n_blocks) where = ((long long)b << a.c.block_shift) + (pos & ((1 << a.c.block_shift) - 1));
     }
     if (where < 0 && slot != -1) atomicOr(a.c.flag, KV4_BAD_SLOT);
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    uint32_t w[4] = {0, 0, 0, 0};
     if (where >= 0) {
         const int key = (int)(where & 15), key8 = key & 7, upper = key >> 3, grp = ch >> 2, t = ch & 3;
         const unsigned char* tile = a.c.pool + tile_at<NG>(a.c, where, h) + grp * KV4_GT;
-        float s, z;
-        uint32_t code[8];
         const uint32_t par = __ldg(reinterpret_cast<const uint32_t*>(tile + (value ? KV4_VPAR : KV4_KPAR) + key8 * 8 + upper * 4));
-        s = __half2float(__ushort_as_half((unsigned short)(par & 0xffff)));
-        z = __half2float(__ushort_as_half((unsigned short)(par >> 16)));
+        const __half2 sz = *reinterpret_cast<const __half2*>(&par), s = __low2half2(sz), z = __high2half2(sz);
+        // pairs of codes as 1024 + c and 1024 + 16 c (a nibble, and one four bits higher, under the exponent of 1024), exact in f16
+        uint32_t pair[4];
         if (!value) {
             const uint32_t word = __ldg(reinterpret_cast<const uint32_t*>(tile + (key8 * 4 + t) * 8 + upper * 4));
 #pragma unroll
-            for (int j = 0; j < 8; ++j) code[j] = word >> (4 * (j >> 1) + 16 * (j & 1)) & 15;
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t two = word >> (4 * j);
+                pair[j] = (two & 0xfu) | (two & 0xf0000u) << 4 | 0x64006400u;      // the odd element four bits higher
+            }
         } else {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const uint32_t two = __ldg(tile + KV4_VCODE + ((2 * t + (q >> 1)) * 4 + (key8 >> 1)) * 8 + (q & 1) * 4 + (key8 & 1) * 2 + upper);
-                code[2 * q] = two & 15;
-                code[2 * q + 1] = two >> 4;
+            for (int q = 0; q < 2; ++q) {
+                const uint2 four = __ldg(reinterpret_cast<const uint2*>(tile + KV4_VCODE + ((2 * t + q) * 4 + (key8 >> 1)) * 8));
+                const unsigned at = (key8 & 1) * 2 + upper;
+                pair[2 * q] = (__byte_perm(four.x, 0, at | at << 8 | 0x4040) & 0x00f0000fu) | 0x64006400u;
+                pair[2 * q + 1] = (__byte_perm(four.y, 0, at | at << 8 | 0x4040) & 0x00f0000fu) | 0x64006400u;
             }
         }
+        const __half2 unit = __halves2half2(__ushort_as_half(0x3C00), __ushort_as_half(0x2C00));      // 1, 1 / 16
+        const __half2 less = __halves2half2(__ushort_as_half(0xE400), __ushort_as_half(0xD400));      // -1024, -64
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = __half2float(__float2half_rn(__fmaf_rn(s, (float)code[j], z)));   // the product is exact
-    }
-    uint32_t w[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const __nv_bfloat162 p = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
-        w[j] = *reinterpret_cast<const uint32_t*>(&p);
+        for (int j = 0; j < 4; ++j) {
+            const __half2 code = __hfma2(*reinterpret_cast<const __half2*>(&pair[j]), unit, less), v = __hfma2(s, code, z);
+            const __nv_bfloat162 p = __floats2bfloat162_rn(__low2float(v), __high2float(v));
+            w[j] = *reinterpret_cast<const uint32_t*>(&p);
+        }
     }
     __nv_bfloat16* dst = (value ? a.v_out + row * a.v_stride : a.k_out + row * a.k_stride) + (size_t)h * (NG * KV4_GROUP) + ch * 8;
     *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
