@@ -29,6 +29,10 @@ struct KcShared {
     static constexpr int SLOTS = 4;
     static constexpr int BARS = 2 * Q + SLOTS * SLOT;
     static constexpr int TOTAL = BARS + 256 + 1024;        // and room to start at a multiple of 1024
+    // Columns of tensor memory: the tiles' scores, 128 each; their sums, HD each; weights (two f16 a column) behind them where there is
+    // room, else over the scores that they came from.
+    static constexpr bool APART = HD == 64;
+    __host__ __device__ static constexpr uint32_t weights(int x) { return APART ? 256 + 2 * HD + x * (KC_STEP / 2) : x * KC_TILE; }
 };
 
 // The CTAs share out all steps of all column tiles and kv heads evenly, in the order sequence, column tile, kv head, step.  A run is what a
@@ -126,6 +130,7 @@ struct KcBars {
     __device__ __forceinline__ uint32_t kv_full(int s) const { return at + 48 + 8 * s; }
     __device__ __forceinline__ uint32_t kv_empty(int s) const { return at + 80 + 8 * s; }
     __device__ __forceinline__ uint32_t tmem() const { return at + 112; }
+    __device__ __forceinline__ uint32_t summed(int x) const { return at + 128 + 8 * x; }
     __device__ __forceinline__ uint32_t again(int x) const { return at + 116 + 4 * x; }     // the round of P whose step is to be taken again
 };
 
@@ -323,6 +328,7 @@ __device__ __forceinline__ void kc_issue(const Kv4AttnArgs& a, uint32_t smem, co
     const uint32_t ring = smem + 2 * S::Q;
     KcRun u;
     unsigned n = 0, runs[2] = {0, 0}, rounds[2] = {0, 0};     // tiles of keys and values, runs with steps, rounds of P
+    unsigned waits[2] = {0, 0};
     auto scores = [&](int x, unsigned slot) {       // S of tile x
         const uint32_t q = tile_desc(smem + x * S::Q), k = tile_desc(ring + slot * S::SLOT), d = tmem + x * KC_TILE;
         mma_ss<4, true>(d, q, k, kc_idesc(KC_STEP));
@@ -330,7 +336,7 @@ __device__ __forceinline__ void kc_issue(const Kv4AttnArgs& a, uint32_t smem, co
         tc_commit(bars.s_full(x));
     };
     auto sums = [&](int x, unsigned slot, bool add) {
-        const uint32_t v = tile_desc(ring + slot * S::SLOT), p = tmem + x * KC_TILE, d = tmem + 256 + x * S::HD;
+        const uint32_t v = tile_desc(ring + slot * S::SLOT), p = tmem + S::weights(x), d = tmem + 256 + x * S::HD;
         if (add) mma_ts<false>(d, p, v, kc_idesc(S::HD));
         else mma_ts<true>(d, p, v, kc_idesc(S::HD));
         mma_ts<false>(d, p + 32, v + (S::HD * 128 >> 4), kc_idesc(S::HD));
@@ -363,10 +369,13 @@ __device__ __forceinline__ void kc_issue(const Kv4AttnArgs& a, uint32_t smem, co
                 if (elect_one()) {
                     sums(x, vslot, j > 0);
                     if (j + 1 == steps[x]) tc_commit(bars.s_full(x));
+                    else if (!S::APART) tc_commit(bars.summed(x));
                 }
                 __syncwarp();
                 if (j + 1 == steps[x]) continue;
                 if (!bar_wait(bars.kv_full(next), ((n + 2) / S::SLOTS) & 1)) return give_up(a.c.flag);
+                // products of different sums are not in order by themselves: the new scores lie where the weights are read
+                if (!S::APART && !bar_wait(bars.summed(x), waits[x]++ & 1)) return give_up(a.c.flag);
                 tc_after();
                 if (elect_one()) scores(x, next);
                 __syncwarp();
@@ -385,7 +394,7 @@ template <int NG>
 __device__ __forceinline__ void kc_softmax(const Kv4AttnArgs& a, uint32_t smem, const KcBars bars, uint32_t tmem, int x, int r, int lane) {
     using S = KcShared<NG>;
     constexpr int HD = S::HD;
-    const uint32_t lanes = tmem + ((uint32_t)(r & ~31) << 16), scores = lanes + x * KC_TILE, sums = lanes + 256 + x * HD;
+    const uint32_t lanes = tmem + ((uint32_t)(r & ~31) << 16), scores = lanes + x * KC_TILE, weights = lanes + S::weights(x), sums = lanes + 256 + x * HD;
     KcRun u;
     unsigned ns = 0, np = 0;       // rounds of S and of P
     for (bool more = kc_begin(a, u, lane); more; more = kc_next(a, u)) {
@@ -490,13 +499,13 @@ __device__ __forceinline__ void kc_softmax(const Kv4AttnArgs& a, uint32_t smem, 
                     tm_wait(s0);
                     tm_load16(scores + i + 16, s1);
                     weigh(s0, i, p0);
-                    if (i > 0) tm_store8(scores + (i >> 1) - 8, p1);
+                    if (i > 0) tm_store8(weights + (i >> 1) - 8, p1);
                     tm_wait(s1);
                     if (i + 32 < KC_STEP) tm_load16(scores + i + 32, s0);
                     weigh(s1, i + 16, p1);
-                    tm_store8(scores + (i >> 1), p0);
+                    tm_store8(weights + (i >> 1), p0);
                 }
-                tm_store8(scores + KC_STEP / 2 - 8, p1);
+                tm_store8(weights + KC_STEP / 2 - 8, p1);
                 step = (part[0] + part[1]) + (part[2] + part[3]);
                 top *= factor;
                 if (__any_sync(0xffffffffu, top > m + 14.f) && lane == 0) sts32(bars.again(x), np);
@@ -554,6 +563,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv4_attn_chunk(const Kv4AttnA
         for (int x = 0; x < 2; ++x) {
             bar_init(bars.q_full(x), 4);
             bar_init(bars.s_full(x), 1);
+            bar_init(bars.summed(x), 1);
             bar_init(bars.p_full(x), 4);
             sts32(bars.again(x), 0xffffffffu);
         }
