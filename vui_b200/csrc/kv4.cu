@@ -290,7 +290,7 @@ extern "C" int32_t vuib_kv4_append(VuibKv4* c, int32_t layer, const VuibKv4Plan*
     a.n_rows = p->n_rows;
     // a sequence's m rows touch (m + 30) / 16 tiles at most, and no more than m
     const long long tiles = min((long long)p->n_rows, p->n_rows / 16 + 2ll * p->n_seqs);
-    const dim3 grid((unsigned)ceil_div(tiles * c->cfg.n_kv_heads, 4));
+    const dim3 grid((unsigned)ceil_div(tiles * c->cfg.n_kv_heads, 4), 2);
     CK(c->ng == 2 ? launch(c, k_kv4_append<2>, grid, 128, 0, 1, stream, a)
                   : c->ng == 3 ? launch(c, k_kv4_append<3>, grid, 128, 0, 1, stream, a) : launch(c, k_kv4_append<4>, grid, 128, 0, 1, stream, a));
     return VUIB_OK;
@@ -314,7 +314,7 @@ extern "C" int32_t vuib_kv4_read(VuibKv4* c, int32_t layer, int32_t n_rows, cons
     a.v_out = static_cast<__nv_bfloat16*>(v_out_dev); a.v_stride = v_stride;
     a.row_slot = row_slot_dev; a.row_pos = row_pos_dev;
     a.n_rows = n_rows;
-    const dim3 grid((unsigned)ceil_div(n_rows, 256 / (c->ng * 4)), c->cfg.n_kv_heads, 2);
+    const dim3 grid((unsigned)ceil_div(n_rows, 256 / (c->ng * 4)), (unsigned)ceil_div(c->cfg.n_kv_heads, KV4_READ_HEADS), 2);
     CK(c->ng == 2 ? launch(c, k_kv4_read<2>, grid, 256, 0, 0, stream, a)
                   : c->ng == 3 ? launch(c, k_kv4_read<3>, grid, 256, 0, 0, stream, a) : launch(c, k_kv4_read<4>, grid, 256, 0, 0, stream, a));
     return VUIB_OK;

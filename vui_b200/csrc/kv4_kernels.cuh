@@ -26,6 +26,7 @@ constexpr int KV4_GROUP = 32;
 constexpr int KV4_TILE = 16;              // positions of a tile
 constexpr int KV4_GT = 640;               // bytes of a tile's group
 constexpr int KV4_KPAR = 256, KV4_VCODE = 320, KV4_VPAR = 576;
+static_assert(KV4_VCODE == KV4_GT / 2 && KV4_VPAR - KV4_VCODE == KV4_KPAR, "a group's values lie as its keys do");
 constexpr float KV4_LIMIT = 60000.f;      // larger magnitudes are stored as this (f16 ends at 65504)
 constexpr int KV4_MAX_SEQS = 4096;
 
@@ -381,21 +382,32 @@ __device__ __forceinline__ float tame(float x) { return x == x ? fminf(fmaxf(x, 
 // Element j of 16 bf16.
 __device__ __forceinline__ float element(const uint32_t (&w)[8], int j) { return __uint_as_float(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16); }
 
-// A warp stores one tile of 16 positions of one kv head, or those of its positions that are new: 16 elements a lane, two lanes a group, which
-// share its extremes; the codes are gathered in shared memory as they lie in the pool and leave it 16 bytes a lane where the whole tile is
-// new, else in the words and bytes of the new positions.
+// Which of the codes k and k + 1 (k = 0 .. 14) the quotient f / s, rounded to fp32, rounds to; it is within 2^-16 of their middle t.  The distance
+// f - t s is exact (t s has 15 bits, f is next to it); the quotient rounds to t itself, and then to the even code, if it is half a unit in
+// the last place of t off or less (below 0.5, a power of two, units are half as large).
+__device__ __forceinline__ float code_between(float f, float s, float k) {
+    const float t = k + 0.5f, r = fmaf(-t, s, f), half_ulp = __int_as_float((__float_as_int(t) & 0x7f800000) - (24 << 23)) * s;
+    const bool up = r > half_ulp, down = r < (k == 0.f ? -0.5f * half_ulp : -half_ulp);
+    return k + (up || (!down && ((int)k & 1)) ? 1.f : 0.f);
+}
+
+// A warp stores the keys or the values (blockIdx.y) of one tile of 16 positions of one kv head, or of those of its positions that are new: 16
+// elements a lane, two lanes a group, which share its extremes; the codes are gathered in shared memory as they lie in the pool and leave
+// it 16 bytes a lane where the whole tile is new, else in the words and bytes of the new positions.
 // The nearest code: (x - zero) times the reciprocal of 15 scales, kept within [0, 1] and times 15, is 2^-17.4 off at most (a division of two ulp and two roundings, of a
-// quotient below 16), so unless that lies within 2^-17 of the middle between two codes it rounds as the quotient does; the few lanes that
-// have such an element divide.
+// quotient below 16), so unless that lies within 2^-17 of the middle between two codes it rounds as the quotient does; lanes that have such an
+// element (exact middles are not rare among bf16 numbers: one group of normal ones in fifty) look closer.
 template <int NG>
 __global__ void __launch_bounds__(128) k_kv4_append(const Kv4RowsArgs a) {
-    constexpr int LANES = NG * 2, ROWS = 32 / LANES, TURNS = (16 + ROWS - 1) / ROWS;     // lanes of a row; rows side by side: 8, 5 (2 lanes idle), 4
-    constexpr int PITCH = KV4_GT + 16;                       // a group's image: 4 banks further than the one before
+    constexpr int LANES = NG * 2, ROWS = 32 / LANES;     // lanes of a row; rows side by side: 8, 5 (2 lanes idle), 4
+    constexpr float NEAR = 0.5f - 7.62939453125e-6f;         // 2^-17 from the middle between two codes
+    constexpr int PITCH = KV4_GT / 2 + 16;                       // a group's image: 4 banks further than the one before
     __shared__ __align__(16) unsigned char image[4][NG * PITCH];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     unsigned char* const img = image[warp];
     const long long id = (long long)blockIdx.x * 4 + warp;
     const int h = (int)(id % a.c.n_kv), want = (int)(id / a.c.n_kv);
+    const bool half = blockIdx.y != 0;         // values
     pdl_wait();
     pdl_launch();
     int lo = 0, hi = a.n;      // the entry that tile number `want` belongs to
@@ -420,29 +432,25 @@ __global__ void __launch_bounds__(128) k_kv4_append(const Kv4RowsArgs a) {
     unsigned char* const tile = a.c.pool + tile_at<NG>(a.c, ((long long)b << a.c.block_shift) + (pos0 & ((1 << a.c.block_shift) - 1)), h);
     const int sub = lane / LANES, ch = lane % LANES;
     unsigned char* const gimg = img + (ch >> 1) * PITCH;
-    // keys, then values, a few rows at a time, the next ones on their way meanwhile.  (One loop body: unrolled it is 50 KB of code, and 72 us
-    // for 16000 rows of 8 heads of 128 where this takes 40.)
+    // a few rows at a time, the next ones on their way meanwhile
+    const long long stride = half ? a.v_stride : a.k_stride;
+    const __nv_bfloat16* const rows = (half ? a.v : a.k) + (long long)(e.w + pos0 - e.y) * stride + h * (NG * KV4_GROUP) + ch * 16;
     auto rows_of = [&](int it, uint4 (&raw)[2]) {
-        const bool value = it >= TURNS;
-        const int key = (value ? it - TURNS : it) * ROWS + sub;
+        const int key = it * ROWS + sub;
         raw[0] = raw[1] = make_uint4(0, 0, 0, 0);
-        if (it < 2 * TURNS && sub < ROWS && key >= from && key < to) {
-            const __nv_bfloat16* src = (value ? a.v : a.k) + (long long)(e.w + pos0 - e.y + key) * (value ? a.v_stride : a.k_stride) + h * (NG * KV4_GROUP) + ch * 16;
-            raw[0] = __ldcg(reinterpret_cast<const uint4*>(src));
-            raw[1] = __ldcg(reinterpret_cast<const uint4*>(src) + 1);
+        if (sub < ROWS && key >= from && key < to) {
+            raw[0] = __ldcg(reinterpret_cast<const uint4*>(rows + key * stride));
+            raw[1] = __ldcg(reinterpret_cast<const uint4*>(rows + key * stride) + 1);
         }
     };
-    // turns that hold a new position: [first, end) of keys, and the same of values
-    const int first = from / ROWS, end = (to + ROWS - 1) / ROWS;
     uint4 next[2];
-    rows_of(first, next);
+    rows_of(from / ROWS, next);
     {
 #pragma unroll 1
-        for (int it = first; it < TURNS + end; it = it + 1 == end ? TURNS + first : it + 1) {
+        for (int it = from / ROWS; it * ROWS < to; ++it) {
             const uint4 raw[2] = {next[0], next[1]};
-            rows_of(it + 1 == end ? TURNS + first : it + 1, next);
-            const bool half = it >= TURNS;
-            const int key = (half ? it - TURNS : it) * ROWS + sub;
+            rows_of(it + 1, next);
+            const int key = it * ROWS + sub;
             uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
             __nv_bfloat162 least = *reinterpret_cast<const __nv_bfloat162*>(&w[0]), most = least;
 #pragma unroll
@@ -473,16 +481,17 @@ __global__ void __launch_bounds__(128) k_kv4_append(const Kv4RowsArgs a) {
             float near = 0.f;
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-                const float x = odd ? tame(element(w, j)) : element(w, j);
-                const float q = __saturatef((x - z) * inv), c = fmaf(q, 15.f, 8388608.f);
+                const float q = __saturatef((element(w, j) - z) * inv), c = fmaf(q, 15.f, 8388608.f);
                 near = fmaxf(near, fabsf(fmaf(q, 15.f, 8388608.f - c)));
                 code[j] = __float_as_uint(c);
             }
-            if (near > 0.5f - 7.62939453125e-6f && s > 0.f) {
+            if (near > NEAR || odd) {
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                    const float x = odd ? tame(element(w, j)) : element(w, j);
-                    code[j] = __float_as_uint(8388608.f + fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x, z), s)), 0.f), 15.f));
+                    const float f = (odd ? tame(element(w, j)) : element(w, j)) - z, q = __saturatef(f * inv);
+                    float c = fmaf(q, 15.f, 8388608.f);
+                    if (fabsf(fmaf(q, 15.f, 8388608.f - c)) > NEAR) c = 8388608.f + code_between(f, s, floorf(q * 15.f));
+                    code[j] = __float_as_uint(c);
                 }
             }
             if (sub >= ROWS || key < from || key >= to) continue;
@@ -500,43 +509,48 @@ __global__ void __launch_bounds__(128) k_kv4_append(const Kv4RowsArgs a) {
             } else {
 #pragma unroll
                 for (int q = 0; q < 8; ++q)
-                    gimg[KV4_VCODE + (((ch & 1) * 4 + (q >> 1)) * 4 + (key8 >> 1)) * 8 + (q & 1) * 4 + (key8 & 1) * 2 + upper] =
+                    gimg[(((ch & 1) * 4 + (q >> 1)) * 4 + (key8 >> 1)) * 8 + (q & 1) * 4 + (key8 & 1) * 2 + upper] =
                         (unsigned char)(code[2 * q] + (code[2 * q + 1] << 4));
-                if (!(ch & 1)) *reinterpret_cast<__half2*>(gimg + KV4_VPAR + key8 * 8 + upper * 4) = __halves2half2(scale, zero);
+                if (!(ch & 1)) *reinterpret_cast<__half2*>(gimg + KV4_KPAR + key8 * 8 + upper * 4) = __halves2half2(scale, zero);
             }
         }
     }
     __syncwarp();
+    constexpr int SIDE = KV4_GT / 2;           // bytes of a group's keys, and of its values
+    unsigned char* const out = tile + (half ? SIDE : 0);
     if (to - from == 16) {
-        for (int i = lane; i < NG * (KV4_GT / 16); i += 32)
-            reinterpret_cast<uint4*>(tile)[i] = *reinterpret_cast<const uint4*>(img + i / (KV4_GT / 16) * PITCH + i % (KV4_GT / 16) * 16);
+        for (int i = lane; i < NG * (SIDE / 16); i += 32)
+            *reinterpret_cast<uint4*>(out + i / (SIDE / 16) * KV4_GT + i % (SIDE / 16) * 16) =
+                *reinterpret_cast<const uint4*>(img + i / (SIDE / 16) * PITCH + i % (SIDE / 16) * 16);
         return;
     }
-    for (int i = lane; i < NG * (KV4_GT / 4); i += 32) {      // word i of the tile: whose is it?
-        const int in = i * 4 % KV4_GT;
-        const unsigned char* const from_img = img + i / (KV4_GT / 4) * PITCH + in;
-        if (in < KV4_VCODE || in >= KV4_VPAR) {     // one key's
-            const int key = (in < KV4_KPAR ? in >> 5 : in < KV4_VCODE ? (in - KV4_KPAR) >> 3 : (in - KV4_VPAR) >> 3) + (in >> 2 & 1) * 8;
-            if (key >= from && key < to) reinterpret_cast<uint32_t*>(tile)[i] = *reinterpret_cast<const uint32_t*>(from_img);
+    for (int i = lane; i < NG * (SIDE / 4); i += 32) {      // word i: whose is it?
+        const int in = i * 4 % SIDE;
+        const unsigned char* const from_img = img + i / (SIDE / 4) * PITCH + in;
+        unsigned char* const to_pool = out + i / (SIDE / 4) * KV4_GT + in;
+        if (!half || in >= KV4_KPAR) {              // one key's
+            const int key = (in < KV4_KPAR ? in >> 5 : (in - KV4_KPAR) >> 3) + (in >> 2 & 1) * 8;
+            if (key >= from && key < to) *reinterpret_cast<uint32_t*>(to_pool) = *reinterpret_cast<const uint32_t*>(from_img);
         } else {                                    // four keys', a byte each
             const int key = (in >> 3 & 3) * 2;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int k = key + (q >> 1) + (q & 1) * 8;
-                if (k >= from && k < to) tile[4 * i + q] = from_img[q];
+                if (k >= from && k < to) to_pool[q] = from_img[q];
             }
         }
     }
 }
 
-// The reverse: 8 elements a thread, bf16 out.  Rows whose slot or position is out of range, or whose block the table lacks, come out as
-// zeros.  A CTA takes the rows next to one another of one kv head, keys or values (blockIdx.z), because those of a tile share its lines in
+// The reverse: 8 elements of four kv heads a thread, bf16 out.  Rows whose slot or position is out of range, or whose block the table lacks, come out as
+// zeros.  A CTA takes the rows next to one another, keys or values (blockIdx.z), because those of a tile share its lines in
 // the L1; that is why this kernel starts only when the kernel before it has ended (no early launch: an SM's L1 could hold older lines).
+constexpr int KV4_READ_HEADS = 4;
 template <int NG>
 __global__ void __launch_bounds__(256) k_kv4_read(const Kv4RowsArgs a) {
     constexpr int CH = NG * 4, ROWS = 256 / CH;
     const bool value = blockIdx.z != 0;
-    const int ch = threadIdx.x % CH, h = blockIdx.y;
+    const int ch = threadIdx.x % CH, h0 = blockIdx.y * KV4_READ_HEADS;
     const long long row = (long long)blockIdx.x * ROWS + threadIdx.x / CH;
     if (threadIdx.x >= ROWS * CH || row >= a.n_rows) return;
     const int slot = __ldg(a.row_slot + row), pos = __ldg(a.row_pos + row);
@@ -546,41 +560,55 @@ __global__ void __launch_bounds__(256) k_kv4_read(const Kv4RowsArgs a) {
         if (b >= 0 && b < a.c.n_blocks) where = ((long long)b << a.c.block_shift) + (pos & ((1 << a.c.block_shift) - 1));
     }
     if (where < 0 && slot != -1) atomicOr(a.c.flag, KV4_BAD_SLOT);
-    uint32_t w[4] = {0, 0, 0, 0};
-    if (where >= 0) {
-        const int key = (int)(where & 15), key8 = key & 7, upper = key >> 3, grp = ch >> 2, t = ch & 3;
-        const unsigned char* tile = a.c.pool + tile_at<NG>(a.c, where, h) + grp * KV4_GT;
-        const uint32_t par = __ldg(reinterpret_cast<const uint32_t*>(tile + (value ? KV4_VPAR : KV4_KPAR) + key8 * 8 + upper * 4));
-        const __half2 sz = *reinterpret_cast<const __half2*>(&par), s = __low2half2(sz), z = __high2half2(sz);
-        // pairs of codes as 1024 + c and 1024 + 16 c (a nibble, and one four bits higher, under the exponent of 1024), exact in f16
-        uint32_t pair[4];
+    const int key = (int)(where & 15), key8 = key & 7, upper = key >> 3, grp = ch >> 2, t = ch & 3, heads = min(a.c.n_kv - h0, KV4_READ_HEADS);
+    const int skip = NG * KV4_GT << (a.c.block_shift - 4);      // from a head to the next in a block
+    const unsigned char* const tile = a.c.pool + (where >= 0 ? tile_at<NG>(a.c, where, h0) + grp * KV4_GT : 0);
+    uint32_t par[KV4_READ_HEADS];
+    uint2 code[KV4_READ_HEADS];
+#pragma unroll
+    for (int i = 0; i < KV4_READ_HEADS; ++i) {
+        par[i] = 0;
+        code[i] = make_uint2(0, 0);
+        if (where < 0 || i >= heads) continue;
+        const unsigned char* const at = tile + i * skip;
+        par[i] = __ldg(reinterpret_cast<const uint32_t*>(at + (value ? KV4_VPAR : KV4_KPAR) + key8 * 8 + upper * 4));
         if (!value) {
-            const uint32_t word = __ldg(reinterpret_cast<const uint32_t*>(tile + (key8 * 4 + t) * 8 + upper * 4));
+            code[i].x = __ldg(reinterpret_cast<const uint32_t*>(at + (key8 * 4 + t) * 8 + upper * 4));
+        } else {      // the key's bytes of two words each
+            const uint2 lo = __ldg(reinterpret_cast<const uint2*>(at + KV4_VCODE + (2 * t * 4 + (key8 >> 1)) * 8));
+            const uint2 hi = __ldg(reinterpret_cast<const uint2*>(at + KV4_VCODE + ((2 * t + 1) * 4 + (key8 >> 1)) * 8));
+            const unsigned in = (key8 & 1) * 2 + upper, two = in | in + 4 << 4;
+            code[i] = make_uint2(__byte_perm(lo.x, lo.y, two), __byte_perm(hi.x, hi.y, two));
+        }
+    }
+    const __half2 unit = __halves2half2(__ushort_as_half(0x3C00), __ushort_as_half(0x2C00));      // 1, 1 / 16
+    const __half2 less = __halves2half2(__ushort_as_half(0xE400), __ushort_as_half(0xD400));      // -1024, -64
+    __nv_bfloat16* dst = (value ? a.v_out + row * a.v_stride : a.k_out + row * a.k_stride) + (size_t)h0 * (NG * KV4_GROUP) + ch * 8;
+#pragma unroll
+    for (int i = 0; i < KV4_READ_HEADS; ++i) {
+        if (i >= heads) break;
+        // pairs of codes as 1024 + c and 1024 + 16 c (a nibble, and one four bits higher, under the exponent of 1024), exact in f16
+        uint32_t pair[4], w[4];
+        if (!value) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const uint32_t two = word >> (4 * j);
+                const uint32_t two = code[i].x >> (4 * j);
                 pair[j] = (two & 0xfu) | (two & 0xf0000u) << 4 | 0x64006400u;      // the odd element four bits higher
             }
         } else {
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const uint2 four = __ldg(reinterpret_cast<const uint2*>(tile + KV4_VCODE + ((2 * t + q) * 4 + (key8 >> 1)) * 8));
-                const unsigned at = (key8 & 1) * 2 + upper;
-                pair[2 * q] = (__byte_perm(four.x, 0, at | at << 8 | 0x4040) & 0x00f0000fu) | 0x64006400u;
-                pair[2 * q + 1] = (__byte_perm(four.y, 0, at | at << 8 | 0x4040) & 0x00f0000fu) | 0x64006400u;
-            }
+            for (int j = 0; j < 4; ++j)      // a byte holds both codes of a pair
+                pair[j] = (__byte_perm(j < 2 ? code[i].x : code[i].y, 0, j & 1 ? 0x4141 : 0x4040) & 0x00f0000fu) | 0x64006400u;
         }
-        const __half2 unit = __halves2half2(__ushort_as_half(0x3C00), __ushort_as_half(0x2C00));      // 1, 1 / 16
-        const __half2 less = __halves2half2(__ushort_as_half(0xE400), __ushort_as_half(0xD400));      // -1024, -64
+        const __half2 sz = *reinterpret_cast<const __half2*>(&par[i]), s = __low2half2(sz), z = __high2half2(sz);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const __half2 code = __hfma2(*reinterpret_cast<const __half2*>(&pair[j]), unit, less), v = __hfma2(s, code, z);
+            const __half2 c = __hfma2(*reinterpret_cast<const __half2*>(&pair[j]), unit, less), v = __hfma2(s, c, z);
             const __nv_bfloat162 p = __floats2bfloat162_rn(__low2float(v), __high2float(v));
             w[j] = *reinterpret_cast<const uint32_t*>(&p);
         }
+        *reinterpret_cast<uint4*>(dst + i * (NG * KV4_GROUP)) = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    __nv_bfloat16* dst = (value ? a.v_out + row * a.v_stride : a.k_out + row * a.k_stride) + (size_t)h * (NG * KV4_GROUP) + ch * 8;
-    *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 }  // namespace vuik
