@@ -389,6 +389,28 @@ __device__ __forceinline__ void kc_issue(const Kv4AttnArgs& a, uint32_t smem, co
     }
 }
 
+// Two numbers at a time: half the instructions.
+__device__ __forceinline__ unsigned long long two(uint32_t lo, uint32_t hi) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 halves(unsigned long long x) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+    return r;
+}
+__device__ __forceinline__ unsigned long long fma_two(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ unsigned long long add_two(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 // ---- the softmax warps of tile x: thread r of 128 has column r, which is its lane of tensor memory
 template <int NG>
 __device__ __forceinline__ void kc_softmax(const Kv4AttnArgs& a, uint32_t smem, const KcBars bars, uint32_t tmem, int x, int r, int lane) {
@@ -480,14 +502,15 @@ __device__ __forceinline__ void kc_softmax(const Kv4AttnArgs& a, uint32_t smem, 
                     top = -INFINITY;
                 }
                 const float less = m == -INFINITY ? 0.f : -m;        // still nothing seen: weights of exp(-inf) = 0
-                float part[4] = {0.f, 0.f, 0.f, 0.f};
+                const unsigned long long factors = two(__float_as_uint(factor), __float_as_uint(factor)), lesses = two(__float_as_uint(less), __float_as_uint(less));
+                unsigned long long part[2] = {0, 0};
                 auto weigh = [&](uint32_t (&s)[16], int first, uint32_t (&p)[8]) {
                     look(s, first);
 #pragma unroll
                     for (int i = 0; i < 16; i += 2) {
-                        const float w0 = ex2(fmaf(__uint_as_float(s[i]), factor, less)), w1 = ex2(fmaf(__uint_as_float(s[i + 1]), factor, less));
-                        part[i & 2] += w0;
-                        part[(i & 2) + 1] += w1;
+                        const float2 e = halves(fma_two(two(s[i], s[i + 1]), factors, lesses));
+                        const float w0 = ex2(e.x), w1 = ex2(e.y);
+                        part[i >> 1 & 1] = add_two(part[i >> 1 & 1], two(__float_as_uint(w0), __float_as_uint(w1)));
                         p[i >> 1] = pack_h2(w0, w1);
                     }
                 };
@@ -506,7 +529,8 @@ __device__ __forceinline__ void kc_softmax(const Kv4AttnArgs& a, uint32_t smem, 
                     tm_store8(weights + (i >> 1), p0);
                 }
                 tm_store8(weights + KC_STEP / 2 - 8, p1);
-                step = (part[0] + part[1]) + (part[2] + part[3]);
+                const float2 sum = halves(add_two(part[0], part[1]));
+                step = sum.x + sum.y;
                 top *= factor;
                 if (__any_sync(0xffffffffu, top > m + 14.f) && lane == 0) sts32(bars.again(x), np);
                 ++np;
