@@ -525,7 +525,8 @@ typedef struct VuibKv4Config {
 } VuibKv4Config;
 
 /* One step's rows: n_seqs entries (a sequence and the rows it brings) and at most n_rows rows in all, max_new of one
- * entry.  The arrays are the caller's, written by vuib_kv4_plan and read by the calls that take the plan. */
+ * entry.  The arrays are the caller's, written by vuib_kv4_plan and read by the calls of the same VuibKv4 that take the
+ * plan (with n_seqs, n_rows and max_new as they were). */
 typedef struct VuibKv4Plan {
     int32_t n_seqs, n_rows, max_new;
     int32_t* work;       /* (7 * n_seqs + 3 + n_rows), 16-byte aligned: how the calls share out the rows */

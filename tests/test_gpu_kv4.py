@@ -258,11 +258,11 @@ def fixed(x, k, v, p, mag, scale):
 class Filled:
     """A cache with sequences of the given lengths, stored in rounds so that their blocks lie in turn, and its contents in fp64."""
 
-    def __init__(self, lens, heads, kv, dim, block, seed=0, spare=3, key_scale=1.0, max_blocks=None, turn=300):
+    def __init__(self, lens, heads, kv, dim, block, seed=0, spare=3, key_scale=1.0, max_blocks=None, turn=300, n_blocks=None):
         n = len(lens)
         self.lens, self.heads, self.kv, self.dim = list(lens), heads, kv, dim
         most = -(-(max(lens) + spare) // block)
-        self.cache = make(sum(-(-(x + spare) // block) for x in lens) + 2, block, n + 2, max_blocks or most, heads, kv, dim)
+        self.cache = make(n_blocks or sum(-(-(x + spare) // block) for x in lens) + 2, block, n + 2, max_blocks or most, heads, kv, dim)
         self.slots = [(3 * i + 1) % n if n % 3 else i for i in range(n)]
         self.g = torch.Generator(device="cuda").manual_seed(seed)
         self.k = [torch.zeros(0, kv, dim, device="cuda", dtype=torch.float64) for _ in lens]
@@ -373,6 +373,21 @@ def test_long_contexts():
         q = torch.randn(sum(new), heads, dim, device="cuda", generator=f.g).bfloat16()
         close(f.cache.attention(0, q, plan), f.want(q, new))
         f.cache.check_device()
+
+
+@pytest.mark.parametrize("heads, new", [(8, [1, 1]), (64, [1, 1]), (8, [20, 3]), (64, [70, 64])])
+def test_offsets_beyond_32_bits(heads, new):
+    """A pool of 4.6 GB, whose blocks are taken from the far end: every form of attention, rows in and out."""
+    f = Filled([700, 90], heads, 8, 128, 256, max_blocks=8, n_blocks=14000)
+    plan = f.add(new)
+    assert int(plan.slot_map.min()) * 8 * 128 // 32 * 40 > 2 ** 32
+    q = torch.randn(sum(new), heads, 128, device="cuda", generator=f.g).bfloat16()
+    close(f.cache.attention(0, q, plan), f.want(q, new))
+    for i, slot in enumerate(f.slots):
+        n = f.k[i].shape[0]
+        k, v = f.cache.read(0, [slot] * n, list(range(n)))
+        assert torch.equal(k, f.k[i].bfloat16()) and torch.equal(v, f.v[i].bfloat16())
+    f.cache.check_device()
 
 
 @pytest.mark.parametrize("size", [1e-30, 2.0 ** -12, 1.0, 300.0, 1e30])
@@ -640,6 +655,7 @@ def test_refusals():
 
     cache = make(10, 16, 3, heads=16, kv=8)
     plan = cache.plan([0, 1], [2, 3])
+    other = make(10, 16, 300, heads=16, kv=8).plan([280, 1], [2, 3])      # of another cache
     k, q = (torch.zeros(5, h, 64, device="cuda", dtype=torch.bfloat16) for h in (8, 16))
     for bad in (lambda: cache.append(0, k[:4], k[:4], plan), lambda: cache.append(0, q, q, plan), lambda: cache.attention(0, k, plan),
                 lambda: cache.attention(0, q, plan, scale=0.0), lambda: cache.attention(0, q, plan, scale=-1.0),
@@ -647,7 +663,8 @@ def test_refusals():
                 lambda: cache.attention(0, q, plan, out=q[:, :8]), lambda: cache.plan([]), lambda: cache.plan([0.5]), lambda: cache.plan([[0]]),
                 lambda: cache.plan([0, 1], [1]), lambda: cache.plan([0], [1], at=[0, 0]), lambda: cache.read(0, [0, 1], [0]),
                 lambda: cache.plan([0], torch.ones(1, dtype=torch.int32, device="cuda")), lambda: cache.plan([0], [1], n_rows=-1),
-                lambda: cache.read(0, [0], [0], k_out=k[:1, :, :32])):
+                lambda: cache.read(0, [0], [0], k_out=k[:1, :, :32]), lambda: cache.plan([2 ** 32]), lambda: cache.plan([0], [2 ** 40], n_rows=1),
+                lambda: cache.attention(0, q, other), lambda: cache.append(0, k, k, other), lambda: cache.attention(0, q, None)):
         with pytest.raises(ValueError):
             bad()
     for bad in (lambda: cache.append(1, k, k, plan), lambda: cache.attention(-1, q, plan), lambda: cache.read(7, [0], [0])):

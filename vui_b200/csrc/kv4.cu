@@ -263,7 +263,7 @@ extern "C" int32_t vuib_kv4_plan(VuibKv4* c, const VuibKv4Plan* p, const int32_t
     a.entries = plan_entries(p); a.cu_units = plan_units(p); a.cu_work = plan_work(p); a.cu_tiles = plan_tiles(p); a.row_entry = plan_row_entry(p);
     a.cu_rows = p->cu_rows;
     a.row_slot = p->row_slot; a.row_pos = p->row_pos; a.slot_map = reinterpret_cast<long long*>(p->slot_map);
-    const size_t smem = (8 * (size_t)p->n_seqs + 3 + c->cfg.max_seqs) * 4;
+    const size_t smem = (9 * (size_t)p->n_seqs + 3 + c->cfg.max_seqs) * 4;
     if (smem > 48 * 1024) CK(cudaFuncSetAttribute(k_kv4_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     // One CTA where little is written: a cluster's barriers cost 2 us.  Rows are known here; cut-backs can give back any number of blocks.
     const int cluster = p->n_rows > 4096 || (at_dev && p->n_seqs > 64 && c->cfg.n_blocks > 4096) ? 8 : 1;

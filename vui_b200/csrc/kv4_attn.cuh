@@ -201,9 +201,6 @@ __device__ __noinline__ void give_up(int32_t* flag) {
     for (int i = 0; i < 100; ++i) __nanosleep(100000);
 }
 
-#ifndef KV4_STAGES
-#define KV4_STAGES 2
-#endif
 // Shared memory of the mma.sync forms, in bytes.
 template <int NG, int COLS>
 struct KaShared {
@@ -212,7 +209,7 @@ struct KaShared {
     static constexpr int TILE = NG * KV4_GT, QCOL = NG * KV4_GROUP * 2;
     static constexpr int KV = KA_WARPS * KT * TILE, Q = COLS * QCOL;
     static constexpr int STAGE = KV + Q + (int)sizeof(Kv4Item);
-    static constexpr int STAGES = KV4_STAGES;
+    static constexpr int STAGES = 2;
     static constexpr int ACC = KA_WARPS * COLS * (NG * KV4_GROUP + 4) * 4, ML = KA_WARPS * COLS * 8;
     static constexpr int TOTAL = STAGES * STAGE + ACC + ML + 8 * (2 * STAGES + 2);
 };

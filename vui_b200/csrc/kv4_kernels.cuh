@@ -37,8 +37,7 @@ constexpr unsigned KV4_POLLS = 1u << 22;  // bound of every wait
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// A plan's entry, as int4: slot (-1: takes no part), first new position, rows, first row.
-
+// What all kernels know of a cache.  (A plan's entry is an int4: slot, -1 if it takes no part; first new position; rows; first row.)
 struct Kv4Cache {
     unsigned char* pool;        // of the layer
     int32_t* table;             // (max_seqs, max_blocks)
@@ -155,7 +154,8 @@ __global__ void __launch_bounds__(1024) k_kv4_plan(const Kv4PlanArgs a) {
     int* s_cu = s_need + n;         // n + 1 each
     int* s_grow = s_cu + n + 1;
     int* s_drop = s_grow + n + 1;
-    int* owner = s_drop + n + 1;    // max_seqs
+    int* s_work = s_drop + n + 1;   // n: steps of the form for chunks
+    int* owner = s_work + n;        // max_seqs
     const unsigned size = cluster_size(), rank = cluster_rank();
     const int tid = threadIdx.x, first = tid * per, last = min(n, first + per);
     const int bs = 1 << a.c.block_shift;
@@ -196,6 +196,24 @@ __global__ void __launch_bounds__(1024) k_kv4_plan(const Kv4PlanArgs a) {
         s_need[i] = ok ? (int)((start + want + bs - 1) >> a.c.block_shift) : 0;
     }
     __syncthreads();
+    if (a.steps) {     // a thread an entry of a few tiles, its warp one of many (16000 rows of 7 query heads a kv head are 438)
+        const int lane = tid & 31;
+        for (int base = tid - lane; base < n; base += blockDim.x) {
+            const int mine = base + lane, cols = mine < n ? s_new[mine] * a.group : 0;
+            long long sum = 0;
+            if (cols <= 4 * KC_COLS)
+                for (int t = 0; t * KC_COLS < cols; ++t) sum += kc_cost(s_start[mine], s_new[mine], a.group, t);
+            for (unsigned left = __ballot_sync(0xffffffffu, cols > 4 * KC_COLS); left; left &= left - 1) {
+                const int k = __ffs(left) - 1, i = base + k;
+                long long part = 0;
+                for (int t = lane; t * KC_COLS < s_new[i] * a.group; t += 32) part += kc_cost(s_start[i], s_new[i], a.group, t);
+#pragma unroll
+                for (int o = 16; o; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+                if (lane == k) sum = part;
+            }
+            if (mine < n) s_work[mine] = (int)min(sum, (long long)KV4_MANY);
+        }
+    }
     // Who is served: the rows of the entries so far have to fit, and so have the blocks that they ask for (an entry that asks for none
     // is served all the same).
     auto leave_out = [&](int i) { s_slot[i] = -1; s_new[i] = 0; s_need[i] = s_have[i]; };
@@ -218,11 +236,7 @@ __global__ void __launch_bounds__(1024) k_kv4_plan(const Kv4PlanArgs a) {
     auto times_tiles = [&](int i, int of_one) { return (int)min(((long long)s_new[i] * a.group + a.cols - 1) / a.cols * of_one, (long long)KV4_MANY); };
     auto units_of = [&](int i) { return s_new[i] ? times_tiles(i, a.split.parts(s_start[i] + (long long)s_new[i])) : 0; };
     auto work_of = [&](int i) {
-        if (a.steps) {
-            int sum = 0;
-            for (int t = 0; t * KC_COLS < s_new[i] * a.group; ++t) sum = min(sum + kc_cost(s_start[i], s_new[i], a.group, t), KV4_MANY);
-            return sum;
-        }
+        if (a.steps) return s_new[i] ? s_work[i] : 0;
         return s_new[i] ? times_tiles(i, a.split.work(s_start[i] + (long long)s_new[i])) : 0;
     };
     auto tiles_of = [&](int i) { return s_new[i] ? ((s_start[i] + s_new[i] - 1) >> 4) - (s_start[i] >> 4) + 1 : 0; };

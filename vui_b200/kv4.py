@@ -34,9 +34,11 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i:
 class Kv4Plan:
     """The rows of one step, all on the device: ``row_slot`` and ``row_pos`` (int32) say which position of which sequence
     a row is, ``slot_map`` (int64) where it lies (block * block_size + offset), ``cu_rows`` (int32, one more than
-    sequences) where each sequence's rows begin.  Rows behind the last are -1."""
+    sequences) where each sequence's rows begin.  Rows behind the last are -1.  The calls that take a plan read these
+    arrays, those in a captured graph at every replay: the plan has to live as long."""
 
-    def __init__(self, device, n_seqs: int, n_rows: int, max_new: int):
+    def __init__(self, cache: "Kv4Cache", n_seqs: int, n_rows: int, max_new: int):
+        device, self._cache = cache.device, cache
         self.n_seqs, self.n_rows, self.max_new = n_seqs, n_rows, max_new
         work = (7 * n_seqs + 3 + n_rows + 3) & ~3          # the parts behind it: 16-byte aligned
         row = (n_rows + 3) & ~3
@@ -130,6 +132,8 @@ class Kv4Cache:
         if t.dim() != 1 or t.is_floating_point() or t.is_complex() or (n is not None and t.numel() != n):
             raise ValueError(f"{name}: a one-dimensional list of {'whole numbers' if n is None else f'{n} whole numbers'} is wanted, "
                              f"got {t.dtype} {tuple(t.shape)}")
+        if not t.is_cuda and t.numel() and not (-2 ** 31 <= int(t.min()) and int(t.max()) < 2 ** 31):
+            raise ValueError(f"{name}: numbers beyond 32 bits")
         return t.to(self.device, torch.int32).contiguous()
 
     # ------------------------------------------------------------------ tables
@@ -161,7 +165,7 @@ class Kv4Cache:
             at = None if at is None else self._ints(at, "at", n)
             if n_rows < 0 or max_new < 0:
                 raise ValueError("n_rows and max_new must not be negative")
-            plan = Kv4Plan(self.device, n, int(n_rows), min(int(max_new), int(n_rows)))
+            plan = Kv4Plan(self, n, int(n_rows), min(int(max_new), int(n_rows)))
             self._ck(self._lib.vuib_kv4_plan(self._h, plan._ref, slots.data_ptr(), None if new is None else new.data_ptr(),
                                              None if at is None else at.data_ptr(), self._stream))
         return plan
@@ -173,6 +177,10 @@ class Kv4Cache:
         self.plan(slots, none, at=none, n_rows=0, max_new=0)
 
     # -------------------------------------------------------------------- rows
+    def _own(self, plan: Kv4Plan) -> None:
+        if not isinstance(plan, Kv4Plan) or plan._cache is not self:
+            raise ValueError("plan: one that this cache made is wanted")
+
     def _rows(self, t: Tensor, name: str, n: int, heads: int, *, out: bool = False) -> Tensor:
         """(n, heads, head_dim) or (n, heads * head_dim) as the library takes it: bf16 on this device, heads behind one
         another, rows a multiple of 16 bytes apart.  An input that lies otherwise is copied, an output refused."""
@@ -199,6 +207,7 @@ class Kv4Cache:
     def append(self, layer: int, k: Tensor, v: Tensor, plan: Kv4Plan) -> None:
         """Stores the plan's rows: k, v (n_rows, n_kv_heads, head_dim), keys with RoPE applied.  NaN is stored as 0 and
         magnitudes beyond 60000 as 60000, which ``check_device`` reports."""
+        self._own(plan)
         with self._here():
             n, heads = plan.n_rows, self.n_kv_heads
             k, v = self._rows(k, "k", n, heads), self._rows(v, "v", n, heads)
@@ -228,6 +237,7 @@ class Kv4Cache:
         Rows behind the plan's last are not written."""
         if scale is not None and not 0 < scale <= 1e30:
             raise ValueError("scale must be positive")
+        self._own(plan)
         if torch.cuda.current_device() != self._index:
             with torch.cuda.device(self._index):
                 return self.attention(layer, q, plan, scale=scale, out=out)
