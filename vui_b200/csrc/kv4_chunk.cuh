@@ -315,14 +315,13 @@ __device__ __forceinline__ void kc_fill(const Kv4AttnArgs& a, uint32_t ring, con
     }
 }
 
-// ---- the issuing warp
+// ---- the issuing thread.  What it does between one product and the next the tensor cores wait for, and each instruction takes its turn among
+// those of four busy warps: so one thread runs the whole loop, and both tiles' code is written out.
 template <int NG>
-__device__ __forceinline__ void kc_issue(const Kv4AttnArgs& a, uint32_t smem, const KcBars bars, uint32_t tmem, int lane) {
+__device__ __forceinline__ void kc_issue_all(const Kv4AttnArgs& a, uint32_t smem, const KcBars bars, uint32_t tmem, KcRun& u) {
     using S = KcShared<NG>;
     const uint32_t ring = smem + 2 * S::Q;
-    KcRun u;
-    unsigned n = 0, runs[2] = {0, 0}, rounds[2] = {0, 0};     // tiles of keys and values, runs with steps, rounds of P
-    unsigned waits[2] = {0, 0};
+    unsigned n = 0, runs[2] = {0, 0}, rounds[2] = {0, 0}, waits[2] = {0, 0};     // tiles of keys and values, runs with steps, rounds of P, waits for sums
     auto scores = [&](int x, unsigned slot) {       // S of tile x
         const uint32_t q = tile_desc(smem + x * S::Q), k = tile_desc(ring + slot * S::SLOT), d = tmem + x * KC_TILE;
         mma_ss<4, true>(d, q, k, kc_idesc(KC_STEP));
@@ -335,52 +334,53 @@ __device__ __forceinline__ void kc_issue(const Kv4AttnArgs& a, uint32_t smem, co
         else mma_ts<true>(d, p, v, kc_idesc(S::HD));
         mma_ts<false>(d, p + 32, v + (S::HD * 128 >> 4), kc_idesc(S::HD));
     };
-    for (bool more = kc_begin(a, u, lane); more; more = kc_next(a, u)) {
-        const int(&steps)[2] = u.steps;
-        const int last = max(steps[0], steps[1]);
+    for (bool more = true; more; more = kc_next(a, u)) {
+        const int last = max(u.steps[0], u.steps[1]);
         if (last == 0) continue;
-        if (!bar_wait(bars.kv_full(n % S::SLOTS), (n / S::SLOTS) & 1)) return give_up(a.c.flag);
+        if (!bar_wait_one(bars.kv_full(n % S::SLOTS), (n / S::SLOTS) & 1)) return give_up(a.c.flag);
+#pragma unroll
         for (int x = 0; x < 2; ++x) {
-            if (!steps[x]) continue;
-            if (!bar_wait(bars.q_full(x), runs[x] & 1)) return give_up(a.c.flag);
+            if (!u.steps[x]) continue;
+            if (!bar_wait_one(bars.q_full(x), runs[x] & 1)) return give_up(a.c.flag);
             ++runs[x];
             tc_after();
-            if (elect_one()) scores(x, n % S::SLOTS);
-            __syncwarp();
+            scores(x, n % S::SLOTS);
         }
         for (int j = 0; j < last; ++j, n += 2) {
             const unsigned kslot = n % S::SLOTS, vslot = (n + 1) % S::SLOTS, next = (n + 2) % S::SLOTS;
-            if (!bar_wait(bars.kv_full(vslot), ((n + 1) / S::SLOTS) & 1)) return give_up(a.c.flag);
+            if (!bar_wait_one(bars.kv_full(vslot), ((n + 1) / S::SLOTS) & 1)) return give_up(a.c.flag);
+#pragma unroll
             for (int x = 0; x < 2; ++x) {
-                if (j >= steps[x]) continue;
+                if (j >= u.steps[x]) continue;
                 for (;;) {
-                    if (!bar_wait(bars.p_full(x), rounds[x] & 1)) return give_up(a.c.flag);
+                    if (!bar_wait_one(bars.p_full(x), rounds[x] & 1)) return give_up(a.c.flag);
                     tc_after();
                     if (lds32(bars.again(x)) != rounds[x]++) break;
-                    if (elect_one()) scores(x, kslot);
-                    __syncwarp();
+                    scores(x, kslot);
                 }
-                if (elect_one()) {
-                    sums(x, vslot, j > 0);
-                    if (j + 1 == steps[x]) tc_commit(bars.s_full(x));
-                    else if (!S::APART) tc_commit(bars.summed(x));
+                sums(x, vslot, j > 0);
+                if (j + 1 == u.steps[x]) {
+                    tc_commit(bars.s_full(x));
+                    continue;
                 }
-                __syncwarp();
-                if (j + 1 == steps[x]) continue;
-                if (!bar_wait(bars.kv_full(next), ((n + 2) / S::SLOTS) & 1)) return give_up(a.c.flag);
+                if (!S::APART) tc_commit(bars.summed(x));
+                if (!bar_wait_one(bars.kv_full(next), ((n + 2) / S::SLOTS) & 1)) return give_up(a.c.flag);
                 // products of different sums are not in order by themselves: the new scores lie where the weights are read
-                if (!S::APART && !bar_wait(bars.summed(x), waits[x]++ & 1)) return give_up(a.c.flag);
+                if (!S::APART && !bar_wait_one(bars.summed(x), waits[x]++ & 1)) return give_up(a.c.flag);
                 tc_after();
-                if (elect_one()) scores(x, next);
-                __syncwarp();
+                scores(x, next);
             }
-            if (elect_one()) {
-                tc_commit(bars.kv_empty(kslot));
-                tc_commit(bars.kv_empty(vslot));
-            }
-            __syncwarp();
+            tc_commit(bars.kv_empty(kslot));
+            tc_commit(bars.kv_empty(vslot));
         }
     }
+}
+
+template <int NG>
+__device__ __forceinline__ void kc_issue(const Kv4AttnArgs& a, uint32_t smem, const KcBars bars, uint32_t tmem, int lane) {
+    KcRun u;
+    if (kc_begin(a, u, lane) && elect_one()) kc_issue_all<NG>(a, smem, bars, tmem, u);
+    __syncwarp();
 }
 
 // Two numbers at a time: half the instructions.
