@@ -20,7 +20,7 @@ struct VuibKv4 {
     size_t layer_bytes;
     bool bound;
     int block_shift, ng, sms, device;
-    int resident[6];          // CTAs of each attention form that fit an SM of the device, 0: not asked for yet
+    int resident[6];          // (FORMS) CTAs of each attention form that fit an SM of the device, 0: not asked for yet
     int64_t launches;
     char err[256];
 };
@@ -66,20 +66,18 @@ cudaError_t launch(VuibKv4* c, void (*kern)(KArgs...), dim3 grid, dim3 block, si
 
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
-// What a plan's shape decides for attention: columns of a tile (rows x query heads of a kv head) and positions of a split.
-// A few columns: splits of 256 positions in sequences of up to 1024, 512 beyond, whatever the batch.
-// Up to 16 columns the form for a few (2, 4, 8 or 16 columns a tile), else the one for many.
-enum Form { FEW_HALVES, FEW_4, FEW_8, FEW_16, MANY, CHUNK };
+// What a plan's shape decides for attention: the form, the columns of a tile (rows x query heads of a kv head) and the positions of a split.
+enum Form { FEW_HALVES, FEW_4, FEW_8, MANY_16, MANY_32, CHUNK, FORMS };
 struct Shape { Form form; int cols; Kv4Split split; };
 Shape shape_of(const VuibKv4* c, const VuibKv4Plan* p) {
     const int group = c->cfg.n_heads / c->cfg.n_kv_heads;
     const long long most = (long long)p->max_new * group;       // columns of one sequence
-    if (most <= 16) {
-        const Form f = most <= 2 && c->ng != 3 ? FEW_HALVES : most <= 4 ? FEW_4 : most <= 8 ? FEW_8 : FEW_16;
-        return {f, f == FEW_HALVES ? 2 : f == FEW_4 ? 4 : f == FEW_8 ? 8 : 16, {512, 256, 512, 1 << 30, true}};
+    if (most <= 8) {
+        const Form f = most <= 2 && c->ng != 3 ? FEW_HALVES : most <= 4 ? FEW_4 : FEW_8;
+        return {f, f == FEW_HALVES ? 2 : f == FEW_4 ? 4 : 8, {512, 256, 512, 1 << 30, true}};
     }
-    Shape s = {MANY, c->ng > 2 ? 16 : 32, {}};
     if (most >= 128 && (long long)p->n_rows * c->cfg.n_heads >= 4096) return {CHUNK, KC_COLS, {1 << 30, 1 << 30, 1 << 30, 1, false}};
+    Shape s = {most <= 16 || c->ng > 2 ? MANY_16 : MANY_32, most <= 16 || c->ng > 2 ? 16 : 32, {}};
     const long long tiles = ceil_div((long long)p->n_rows * group, s.cols) + p->n_seqs;
     // enough tiles for the SMs: no splits; else at most 8 of a sequence, so that their sums stay a few megabytes
     const long long len = (long long)c->cfg.max_blocks << c->block_shift;
@@ -165,14 +163,15 @@ cudaError_t launch_attn(VuibKv4* c, const Shape& s, void (*kern)(Kv4AttnArgs), i
 
 template <int NG>
 cudaError_t launch_form(VuibKv4* c, const Shape& s, const Kv4AttnArgs& a, long long items, bool merge, void* stream) {
-    constexpr int T = KA_THREADS + 32, MANY_NT = NG == 2 ? 4 : 2;
+    constexpr int T = KA_THREADS + 32;
     switch (s.form) {
         case FEW_HALVES:
             if constexpr (NG != 3) return launch_attn<NG>(c, s, k_kv4_attn_few<NG, 1, true>, T, KaShared<NG, 2>::TOTAL, a, items, merge, stream);
         case FEW_4: return launch_attn<NG>(c, s, k_kv4_attn_few<NG, 1, false>, T, KaShared<NG, 4>::TOTAL, a, items, merge, stream);
         case FEW_8: return launch_attn<NG>(c, s, k_kv4_attn_few<NG, 2, false>, T, KaShared<NG, 8>::TOTAL, a, items, merge, stream);
-        case FEW_16: return launch_attn<NG>(c, s, k_kv4_attn_few<NG, 4, false>, T, KaShared<NG, 16>::TOTAL, a, items, merge, stream);
-        case MANY: return launch_attn<NG>(c, s, k_kv4_attn<NG, MANY_NT>, T, KaShared<NG, 8 * MANY_NT>::TOTAL, a, items, merge, stream);
+        case MANY_32:
+            if constexpr (NG == 2) return launch_attn<NG>(c, s, k_kv4_attn<NG, 4>, T, KaShared<NG, 32>::TOTAL, a, items, merge, stream);
+        case MANY_16: return launch_attn<NG>(c, s, k_kv4_attn<NG, 2>, T, KaShared<NG, 16>::TOTAL, a, items, merge, stream);
         default: return launch_attn<NG>(c, s, k_kv4_attn_chunk<NG>, KC_THREADS, KcShared<NG>::TOTAL, a, items, merge, stream);
     }
 }
