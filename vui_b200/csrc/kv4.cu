@@ -20,7 +20,7 @@ struct VuibKv4 {
     size_t layer_bytes;
     bool bound;
     int block_shift, ng, sms, device;
-    int resident[6];          // (FORMS) CTAs of each attention form that fit an SM of the device, 0: not asked for yet
+    int resident[5];          // CTAs of each attention form that fit an SM of the device, 0: not asked for yet
     int64_t launches;
     char err[256];
 };
@@ -67,24 +67,21 @@ cudaError_t launch(VuibKv4* c, void (*kern)(KArgs...), dim3 grid, dim3 block, si
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
 // What a plan's shape decides for attention: the form, the columns of a tile (rows x query heads of a kv head) and the positions of a split.
-enum Form { FEW_HALVES, FEW_4, FEW_8, MANY_16, MANY_32, CHUNK, FORMS };
+enum Form { FEW_2, FEW_4, MANY_8, MANY_16, CHUNK };
 struct Shape { Form form; int cols; Kv4Split split; };
 Shape shape_of(const VuibKv4* c, const VuibKv4Plan* p) {
     const int group = c->cfg.n_heads / c->cfg.n_kv_heads;
     const long long most = (long long)p->max_new * group;       // columns of one sequence
-    if (most <= 8) {
-        const Form f = most <= 2 && c->ng != 3 ? FEW_HALVES : most <= 4 ? FEW_4 : FEW_8;
-        return {f, f == FEW_HALVES ? 2 : f == FEW_4 ? 4 : 8, {512, 256, 512, 1 << 30, true}};
-    }
+    const Form form = most <= 2 && c->ng != 3 ? FEW_2 : most <= 4 ? FEW_4 : most <= 8 ? MANY_8 : MANY_16;
+    const int cols = form == FEW_2 ? 2 : form == FEW_4 ? 4 : form == MANY_8 ? 8 : 16;
+    if (most <= 16) return {form, cols, {512, 256, 512, 1 << 30, true}};
     if (most >= 128 && (long long)p->n_rows * c->cfg.n_heads >= 4096) return {CHUNK, KC_COLS, {1 << 30, 1 << 30, 1 << 30, 1, false}};
-    Shape s = {most <= 16 || c->ng > 2 ? MANY_16 : MANY_32, most <= 16 || c->ng > 2 ? 16 : 32, {}};
-    const long long tiles = ceil_div((long long)p->n_rows * group, s.cols) + p->n_seqs;
+    const long long tiles = ceil_div((long long)p->n_rows * group, cols) + p->n_seqs;
     // enough tiles for the SMs: no splits; else at most 8 of a sequence, so that their sums stay a few megabytes
     const long long len = (long long)c->cfg.max_blocks << c->block_shift;
     const bool enough = tiles * c->cfg.n_kv_heads >= 2 * c->sms;
     const int split = enough ? 1 << 30 : 512;
-    s.split = {split, split, split, 8, tiles * (len / 64 + 16) < KV4_MANY};
-    return s;
+    return {form, cols, {split, split, split, 8, tiles * (len / 64 + 16) < KV4_MANY}};
 }
 
 // Most splits of one sequence.
@@ -165,12 +162,10 @@ template <int NG>
 cudaError_t launch_form(VuibKv4* c, const Shape& s, const Kv4AttnArgs& a, long long items, bool merge, void* stream) {
     constexpr int T = KA_THREADS + 32;
     switch (s.form) {
-        case FEW_HALVES:
+        case FEW_2:
             if constexpr (NG != 3) return launch_attn<NG>(c, s, k_kv4_attn_few<NG, 1, true>, T, KaShared<NG, 2>::TOTAL, a, items, merge, stream);
         case FEW_4: return launch_attn<NG>(c, s, k_kv4_attn_few<NG, 1, false>, T, KaShared<NG, 4>::TOTAL, a, items, merge, stream);
-        case FEW_8: return launch_attn<NG>(c, s, k_kv4_attn_few<NG, 2, false>, T, KaShared<NG, 8>::TOTAL, a, items, merge, stream);
-        case MANY_32:
-            if constexpr (NG == 2) return launch_attn<NG>(c, s, k_kv4_attn<NG, 4>, T, KaShared<NG, 32>::TOTAL, a, items, merge, stream);
+        case MANY_8: return launch_attn<NG>(c, s, k_kv4_attn<NG, 1>, T, KaShared<NG, 8>::TOTAL, a, items, merge, stream);
         case MANY_16: return launch_attn<NG>(c, s, k_kv4_attn<NG, 2>, T, KaShared<NG, 16>::TOTAL, a, items, merge, stream);
         default: return launch_attn<NG>(c, s, k_kv4_attn_chunk<NG>, KC_THREADS, KcShared<NG>::TOTAL, a, items, merge, stream);
     }
