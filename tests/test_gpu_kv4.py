@@ -366,6 +366,23 @@ def test_chunks_of_prompts(heads, kv, dim, block, before, new):
     f.cache.check_device()
 
 
+@pytest.mark.parametrize("heads, kv, dim, seqs, new", [(32, 8, 96, 64, 68), (12, 4, 96, 8, 200), (12, 4, 64, 40, 90), (16, 4, 128, 30, 71)])
+def test_many_tiles_that_end_inside_a_warp(heads, kv, dim, seqs, new):
+    """Columns that end within 32 of one another, over and over, call after call: all bits the same, none of them anywhere else."""
+    f = Filled([200 + 5 * i % 190 for i in range(seqs)], heads, kv, dim, 64, spare=new)
+    plan = f.add([new] * seqs)
+    q = torch.randn(seqs * new, heads, dim, device="cuda", generator=f.g).bfloat16()
+    big = torch.full((seqs * new + 2, heads + 2, dim), 5.0, device="cuda", dtype=torch.bfloat16)
+    out = big[1:-1, 1:-1]
+    f.cache.attention(0, q, plan, out=out)
+    close(out, f.want(q, [new] * seqs))
+    first = big.clone()
+    for _ in range(20):
+        f.cache.attention(0, q, plan, out=out)
+    assert torch.equal(big, first) and (big[0] == 5).all() and (big[-1] == 5).all() and (big[:, 0] == 5).all() and (big[:, -1] == 5).all()
+    f.cache.check_device()
+
+
 def test_long_contexts():
     for lens, heads, kv, dim, new in (([40000, 9000], 8, 2, 64, [1, 1]), ([20000, 3], 4, 1, 128, [1, 1]), ([30000], 2, 1, 64, [40])):
         f = Filled([n - m for n, m in zip(lens, new)], heads, kv, dim, 256, turn=8000, spare=max(new))

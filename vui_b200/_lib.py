@@ -22,7 +22,7 @@ UNITS = {
     "vuib200.cu": ["decode_kernels.cuh", "tc_gemm.cuh", "fused_blocks.cuh", "fused_rows.cuh", "depth_tc.cuh", "prefill_attn.cuh"],
     "codec.cu": ["codec_kernels.cuh", "codec_batch.cuh", "split_ops.cuh", "split_gemm.cuh"],
     "codec_enc.cu": ["codec_enc_kernels.cuh", "split_ops.cuh", "split_gemm.cuh"],
-    "kv4.cu": ["kv4_kernels.cuh", "kv4_attn.cuh", "kv4_chunk.cuh"],
+    "kv4.cu": ["kv4_kernels.cuh", "kv4_attn.cuh"],
 }
 SOURCES = [os.path.join(_CSRC, u) for u in UNITS]
 HEADERS = sorted({os.path.join(_CSRC, h) for hs in UNITS.values() for h in hs}) + [_API_H]

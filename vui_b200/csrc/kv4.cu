@@ -9,7 +9,6 @@
 
 #include "../../include/vuib200.h"
 #include "kv4_attn.cuh"
-#include "kv4_chunk.cuh"
 #include "kv4_kernels.cuh"
 
 using namespace vuik;
@@ -20,7 +19,7 @@ struct VuibKv4 {
     size_t layer_bytes;
     bool bound;
     int block_shift, ng, sms, device;
-    int resident[5];          // CTAs of each attention form that fit an SM of the device, 0: not asked for yet
+    int resident[4];          // CTAs of each attention form that fit an SM of the device, 0: not asked for yet
     int64_t launches;
     char err[256];
 };
@@ -67,7 +66,7 @@ cudaError_t launch(VuibKv4* c, void (*kern)(KArgs...), dim3 grid, dim3 block, si
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
 // What a plan's shape decides for attention: the form, the columns of a tile (rows x query heads of a kv head) and the positions of a split.
-enum Form { FEW_2, FEW_4, MANY_8, MANY_16, CHUNK };
+enum Form { FEW_2, FEW_4, MANY_8, MANY_16 };
 struct Shape { Form form; int cols; Kv4Split split; };
 Shape shape_of(const VuibKv4* c, const VuibKv4Plan* p) {
     const int group = c->cfg.n_heads / c->cfg.n_kv_heads;
@@ -75,7 +74,6 @@ Shape shape_of(const VuibKv4* c, const VuibKv4Plan* p) {
     const Form form = most <= 2 && c->ng != 3 ? FEW_2 : most <= 4 ? FEW_4 : most <= 8 ? MANY_8 : MANY_16;
     const int cols = form == FEW_2 ? 2 : form == FEW_4 ? 4 : form == MANY_8 ? 8 : 16;
     if (most <= 16) return {form, cols, {512, 256, 512, 1 << 30, true}};
-    if (most >= 128 && (long long)p->n_rows * c->cfg.n_heads >= 4096) return {CHUNK, KC_COLS, {1 << 30, 1 << 30, 1 << 30, 1, false}};
     const long long tiles = ceil_div((long long)p->n_rows * group, cols) + p->n_seqs;
     // enough tiles for the SMs: no splits; else at most 8 of a sequence, so that their sums stay a few megabytes
     const long long len = (long long)c->cfg.max_blocks << c->block_shift;
@@ -100,10 +98,8 @@ long long most_units(const VuibKv4* c, const VuibKv4Plan* p, const Shape& s) {
     return min(tiles * most_parts(c, s), a_seq * (p->n_seqs + pool / min(s.split.up_to_512, s.split.up_to_1024)));
 }
 
-// Units whose sums may have to be kept: of the form for chunks, two a CTA.
-long long most_items(const VuibKv4* c, const VuibKv4Plan* p, const Shape& s) {
-    return s.form == CHUNK ? 2ll * c->sms : most_units(c, p, s) * c->cfg.n_kv_heads;
-}
+// Units whose sums may have to be kept.
+long long most_items(const VuibKv4* c, const VuibKv4Plan* p, const Shape& s) { return most_units(c, p, s) * c->cfg.n_kv_heads; }
 
 size_t acc_bytes(const VuibKv4* c, long long items, int cols) { return ((size_t)items * cols * c->cfg.head_dim * 4 + 255) & ~size_t(255); }
 
@@ -143,16 +139,15 @@ cudaError_t launch_attn(VuibKv4* c, const Shape& s, void (*kern)(Kv4AttnArgs), i
         if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
         if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kern, threads, smem);
         if (e != cudaSuccess) return e;
-        if (resident < 1 || s.form == CHUNK) resident = 1;      // CHUNK: a CTA takes all of an SM's tensor memory
+        if (resident < 1) resident = 1;
     }
     const long long room = (long long)c->sms * resident;
     // A kernel that starts beside the merge finds its SMs partly taken, and one that fills them all then has late CTAs: 256 sequences of
     // 512 to 2048 positions call after call 61.0 us with an early start and 53.0 without, one sequence of 300 6.3 and 6.7.
     a.early = 2 * items < room;
-    const long long grid = s.form == CHUNK ? c->sms : min(items, room), rows = (long long)a.n_rows * c->cfg.n_heads;
+    const long long grid = min(items, room), rows = (long long)a.n_rows * c->cfg.n_heads;
     e = launch(c, kern, dim3((unsigned)grid), threads, smem, 1, stream, a);
     if (e != cudaSuccess || !merge) return e;
-    if (s.form == CHUNK) return launch(c, k_kv4_chunk_merge<NG>, dim3((unsigned)grid, KC_COLS / KC_MERGE), 256, 0, 1, stream, a);
     if (most_parts(c, s) <= 32)
         return launch(c, k_kv4_merge<NG, 1>, dim3((unsigned)ceil_div(rows, 4)), 128, 0, 1, stream, a, s.cols);
     return launch(c, k_kv4_merge<NG, 8>, dim3((unsigned)rows), 256, 0, 1, stream, a, s.cols);
@@ -166,8 +161,7 @@ cudaError_t launch_form(VuibKv4* c, const Shape& s, const Kv4AttnArgs& a, long l
             if constexpr (NG != 3) return launch_attn<NG>(c, s, k_kv4_attn_few<NG, 1, true>, T, KaShared<NG, 2>::TOTAL, a, items, merge, stream);
         case FEW_4: return launch_attn<NG>(c, s, k_kv4_attn_few<NG, 1, false>, T, KaShared<NG, 4>::TOTAL, a, items, merge, stream);
         case MANY_8: return launch_attn<NG>(c, s, k_kv4_attn<NG, 1>, T, KaShared<NG, 8>::TOTAL, a, items, merge, stream);
-        case MANY_16: return launch_attn<NG>(c, s, k_kv4_attn<NG, 2>, T, KaShared<NG, 16>::TOTAL, a, items, merge, stream);
-        default: return launch_attn<NG>(c, s, k_kv4_attn_chunk<NG>, KC_THREADS, KcShared<NG>::TOTAL, a, items, merge, stream);
+        default: return launch_attn<NG>(c, s, k_kv4_attn<NG, 2>, T, KaShared<NG, 16>::TOTAL, a, items, merge, stream);
     }
 }
 
@@ -246,18 +240,16 @@ extern "C" int32_t vuib_kv4_plan(VuibKv4* c, const VuibKv4Plan* p, const int32_t
     if (!slots_dev) return fail(c, VUIB_ERR_NULL, "slots is NULL");
     if (!new_dev && p->max_new < 1) return fail(c, VUIB_ERR_RANGE, "one new row each, but max_new is %d", p->max_new);
     const Shape s = shape_of(c, p);
-    const long long len = (long long)c->cfg.max_blocks << c->block_shift;
-    const long long tiles = ceil_div((long long)p->n_rows * (c->cfg.n_heads / c->cfg.n_kv_heads), s.cols) + p->n_seqs;
-    if (s.form == CHUNK ? tiles * (len / KC_STEP + 1) >= KV4_MANY : most_units(c, p, s) >= KV4_MANY) return fail(c, VUIB_ERR_RANGE, "too many units of work for one plan");
+    if (most_units(c, p, s) >= KV4_MANY) return fail(c, VUIB_ERR_RANGE, "too many units of work for one plan");
     Kv4PlanArgs a = {};
     a.c = c->cache;
     a.slots = slots_dev; a.new_lens = new_dev; a.at = at_dev;
     a.n = p->n_seqs; a.n_rows = p->n_rows; a.max_new = p->max_new;
-    a.group = c->cfg.n_heads / c->cfg.n_kv_heads; a.cols = s.cols; a.split = s.split; a.steps = s.form == CHUNK;
+    a.group = c->cfg.n_heads / c->cfg.n_kv_heads; a.cols = s.cols; a.split = s.split;
     a.entries = plan_entries(p); a.cu_units = plan_units(p); a.cu_work = plan_work(p); a.cu_tiles = plan_tiles(p); a.row_entry = plan_row_entry(p);
     a.cu_rows = p->cu_rows;
     a.row_slot = p->row_slot; a.row_pos = p->row_pos; a.slot_map = reinterpret_cast<long long*>(p->slot_map);
-    const size_t smem = (9 * (size_t)p->n_seqs + 3 + c->cfg.max_seqs) * 4;
+    const size_t smem = (8 * (size_t)p->n_seqs + 3 + c->cfg.max_seqs) * 4;
     if (smem > 48 * 1024) CK(cudaFuncSetAttribute(k_kv4_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     // One CTA where little is written: a cluster's barriers cost 2 us.  Rows are known here; cut-backs can give back any number of blocks.
     const int cluster = p->n_rows > 4096 || (at_dev && p->n_seqs > 64 && c->cfg.n_blocks > 4096) ? 8 : 1;
@@ -320,7 +312,7 @@ extern "C" int32_t vuib_kv4_attention_workspace(VuibKv4* c, const VuibKv4Plan* p
     *bytes = 0;
     if (!p->n_rows || !p->max_new) return VUIB_OK;
     const Shape s = shape_of(c, p);
-    if (s.form != CHUNK && most_parts(c, s) <= 1) return VUIB_OK;
+    if (most_parts(c, s) <= 1) return VUIB_OK;
     const long long items = most_items(c, p, s);
     *bytes = acc_bytes(c, items, s.cols) + (size_t)items * s.cols * 8;
     return VUIB_OK;

@@ -62,14 +62,6 @@ struct Kv4Split {
     __host__ __device__ int work_of(int positions) const { return 1 + (weigh ? (positions + 63) / 64 : 0); }            // of one
 };
 
-// Work of attention in the form for chunks: steps of 128 positions that a tile of 256 columns (rows x query heads of a kv head) takes, from
-// the sequence's first position to the last that any of its rows sees.
-constexpr int KC_COLS = 256, KC_STEP = 128;
-__device__ __forceinline__ int kc_cost(int start, int rows, int group, int ctile) {
-    const int last = (min((ctile + 1) * KC_COLS, rows * group) - 1) / group;
-    return (start + last + KC_STEP) / KC_STEP;
-}
-
 // ------------------------------------------------------------------------------------------------ tables and maps
 struct Kv4PlanArgs {
     Kv4Cache c;
@@ -77,7 +69,6 @@ struct Kv4PlanArgs {
     int n, n_rows, max_new;
     int group, cols;            // query heads a kv head, columns of a tile: attention's units are counted here
     Kv4Split split;
-    bool steps;                 // work is counted in steps of tiles (kc_cost)
     int4* entries; int32_t* cu_units; int32_t* cu_work; int32_t* cu_tiles; int32_t* row_entry;    // the plan's work array
     int32_t* cu_rows; int32_t* row_slot; int32_t* row_pos; long long* slot_map;
 };
@@ -154,8 +145,7 @@ __global__ void __launch_bounds__(1024) k_kv4_plan(const Kv4PlanArgs a) {
     int* s_cu = s_need + n;         // n + 1 each
     int* s_grow = s_cu + n + 1;
     int* s_drop = s_grow + n + 1;
-    int* s_work = s_drop + n + 1;   // n: steps of the form for chunks
-    int* owner = s_work + n;        // max_seqs
+    int* owner = s_drop + n + 1;    // max_seqs
     const unsigned size = cluster_size(), rank = cluster_rank();
     const int tid = threadIdx.x, first = tid * per, last = min(n, first + per);
     const int bs = 1 << a.c.block_shift;
@@ -196,24 +186,6 @@ __global__ void __launch_bounds__(1024) k_kv4_plan(const Kv4PlanArgs a) {
         s_need[i] = ok ? (int)((start + want + bs - 1) >> a.c.block_shift) : 0;
     }
     __syncthreads();
-    if (a.steps) {     // a thread an entry of a few tiles, its warp one of many (16000 rows of 7 query heads a kv head are 438)
-        const int lane = tid & 31;
-        for (int base = tid - lane; base < n; base += blockDim.x) {
-            const int mine = base + lane, cols = mine < n ? s_new[mine] * a.group : 0;
-            long long sum = 0;
-            if (cols <= 4 * KC_COLS)
-                for (int t = 0; t * KC_COLS < cols; ++t) sum += kc_cost(s_start[mine], s_new[mine], a.group, t);
-            for (unsigned left = __ballot_sync(0xffffffffu, cols > 4 * KC_COLS); left; left &= left - 1) {
-                const int k = __ffs(left) - 1, i = base + k;
-                long long part = 0;
-                for (int t = lane; t * KC_COLS < s_new[i] * a.group; t += 32) part += kc_cost(s_start[i], s_new[i], a.group, t);
-#pragma unroll
-                for (int o = 16; o; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-                if (lane == k) sum = part;
-            }
-            if (mine < n) s_work[mine] = (int)min(sum, (long long)KV4_MANY);
-        }
-    }
     // Who is served: the rows of the entries so far have to fit, and so have the blocks that they ask for (an entry that asks for none
     // is served all the same).
     auto leave_out = [&](int i) { s_slot[i] = -1; s_new[i] = 0; s_need[i] = s_have[i]; };
@@ -235,10 +207,7 @@ __global__ void __launch_bounds__(1024) k_kv4_plan(const Kv4PlanArgs a) {
     int part[5] = {0, 0, 0, 0, 0}, whole[5];   // blocks got, rows, units of attention (of a kv head) and their work, tiles of 16 positions written
     auto times_tiles = [&](int i, int of_one) { return (int)min(((long long)s_new[i] * a.group + a.cols - 1) / a.cols * of_one, (long long)KV4_MANY); };
     auto units_of = [&](int i) { return s_new[i] ? times_tiles(i, a.split.parts(s_start[i] + (long long)s_new[i])) : 0; };
-    auto work_of = [&](int i) {
-        if (a.steps) return s_new[i] ? s_work[i] : 0;
-        return s_new[i] ? times_tiles(i, a.split.work(s_start[i] + (long long)s_new[i])) : 0;
-    };
+    auto work_of = [&](int i) { return s_new[i] ? times_tiles(i, a.split.work(s_start[i] + (long long)s_new[i])) : 0; };
     auto tiles_of = [&](int i) { return s_new[i] ? ((s_start[i] + s_new[i] - 1) >> 4) - (s_start[i] >> 4) + 1 : 0; };
     for (int i = first; i < last; ++i) {
         s_drop[i] = blocks[0];
@@ -267,6 +236,7 @@ __global__ void __launch_bounds__(1024) k_kv4_plan(const Kv4PlanArgs a) {
     }
     if (tid == 0) { s_cu[n] = rows; s_grow[n] = grown; s_drop[n] = dropped; }
     if (bad && rank == 0) atomicOr(a.c.flag, bad);
+    __syncwarp();
     plan_sync(size);                   // every CTA has read the lengths and the number of free blocks
     const int step = blockDim.x * size, me = rank * blockDim.x + tid;
     if (rank == 0) {
