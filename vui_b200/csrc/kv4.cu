@@ -19,7 +19,7 @@ struct VuibKv4 {
     size_t layer_bytes;
     bool bound;
     int block_shift, ng, sms, device;
-    int resident[4];          // CTAs of each attention form that fit an SM of the device, 0: not asked for yet
+    int resident[5];          // CTAs of each attention form that fit an SM of the device, 0: not asked for yet
     int64_t launches;
     char err[256];
 };
@@ -66,19 +66,30 @@ cudaError_t launch(VuibKv4* c, void (*kern)(KArgs...), dim3 grid, dim3 block, si
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
 // What a plan's shape decides for attention: the form, the columns of a tile (rows x query heads of a kv head) and the positions of a split.
-enum Form { FEW_2, FEW_4, MANY_8, MANY_16 };
+//   FEW_2, FEW_4   bytes: up to 2 columns (heads of 64 and 128) and up to 4.  256 sequences of 512 to 2048 positions, two query heads a kv head of 64:
+//                  53 us with FEW_2, 62 with FEW_4, 203 with the f16 form for 16; 4 query heads of 128, 4 x 64k positions: 75 with FEW_4, 92 with MANY_8.
+//   MANY_8, _16    f16, a warp's own keys: up to 8 and 16 columns a tile.  64 sequences of up to 4000, 8 query heads of 128: 85 us with MANY_8, 109
+//                  with the byte form for 8; 16 rows' columns of 4 heads of 128: 23 us with MANY_16, 37 with the byte form for 16; tiles of 32
+//                  columns are slower wherever they fill (64 x 24 rows of 2 query heads of 64: 30 us with 16, 45 with 32).
+//   ROWS           f16, shared keys, 128 columns: from 128 columns of heads of 128 on, 256 of 64, 512 of 96.  Against MANY_16, us: heads of 128, 128
+//                  columns 28 and 30, 256 32 and 47, 2 x 1000 rows 952 and 1408; heads of 64, 128 columns 38 and 32, 256 43 and 54, 2000 38 and
+//                  40; heads of 96, 300 columns 39 and 31, 600 54 and 54.
+// Splits.  Up to 16 columns by the sequence's length alone, so that a row's bits do not depend on what else is there: one of up to 512 positions is one
+// piece (64 sequences of 64 to 512: 10.3 us, in pieces of 256 12.4), up to 1024 pieces of 256 (16 sequences of up to 1000, 8 query heads of 128:
+// 19.7, in pieces of 512 23.1), beyond of 512 (4 x 64k: 74.7, 256 79.4, 1024 76.4).  More columns: none where the tiles fill the SMs, else pieces of 512,
+// at most 8 of a sequence, so that their sums stay a few megabytes.
+enum Form { FEW_2, FEW_4, MANY_8, MANY_16, ROWS };
 struct Shape { Form form; int cols; Kv4Split split; };
 Shape shape_of(const VuibKv4* c, const VuibKv4Plan* p) {
     const int group = c->cfg.n_heads / c->cfg.n_kv_heads;
     const long long most = (long long)p->max_new * group;       // columns of one sequence
-    const Form form = most <= 2 && c->ng != 3 ? FEW_2 : most <= 4 ? FEW_4 : most <= 8 ? MANY_8 : MANY_16;
-    const int cols = form == FEW_2 ? 2 : form == FEW_4 ? 4 : form == MANY_8 ? 8 : 16;
+    const int rows_from = c->ng == 4 ? 128 : c->ng == 3 ? 512 : 256;
+    const Form form = most <= 2 && c->ng != 3 ? FEW_2 : most <= 4 ? FEW_4 : most <= 8 ? MANY_8 : most < rows_from ? MANY_16 : ROWS;
+    const int cols = form == FEW_2 ? 2 : form == FEW_4 ? 4 : form == MANY_8 ? 8 : form == MANY_16 ? 16 : KR_COLS;
     if (most <= 16) return {form, cols, {512, 256, 512, 1 << 30, true}};
     const long long tiles = ceil_div((long long)p->n_rows * group, cols) + p->n_seqs;
-    // enough tiles for the SMs: no splits; else at most 8 of a sequence, so that their sums stay a few megabytes
     const long long len = (long long)c->cfg.max_blocks << c->block_shift;
-    const bool enough = tiles * c->cfg.n_kv_heads >= 2 * c->sms;
-    const int split = enough ? 1 << 30 : 512;
+    const int split = tiles * c->cfg.n_kv_heads >= 2 * c->sms ? 1 << 30 : 512;
     return {form, cols, {split, split, split, 8, tiles * (len / 64 + 16) < KV4_MANY}};
 }
 
@@ -158,9 +169,10 @@ cudaError_t launch_form(VuibKv4* c, const Shape& s, const Kv4AttnArgs& a, long l
     constexpr int T = KA_THREADS + 32;
     switch (s.form) {
         case FEW_2:
-            if constexpr (NG != 3) return launch_attn<NG>(c, s, k_kv4_attn_few<NG, 1, true>, T, KaShared<NG, 2>::TOTAL, a, items, merge, stream);
-        case FEW_4: return launch_attn<NG>(c, s, k_kv4_attn_few<NG, 1, false>, T, KaShared<NG, 4>::TOTAL, a, items, merge, stream);
+            if constexpr (NG != 3) return launch_attn<NG>(c, s, k_kv4_attn_few<NG, true>, T, KaShared<NG, 2>::TOTAL, a, items, merge, stream);
+        case FEW_4: return launch_attn<NG>(c, s, k_kv4_attn_few<NG, false>, T, KaShared<NG, 4>::TOTAL, a, items, merge, stream);
         case MANY_8: return launch_attn<NG>(c, s, k_kv4_attn<NG, 1>, T, KaShared<NG, 8>::TOTAL, a, items, merge, stream);
+        case ROWS: return launch_attn<NG>(c, s, k_kv4_attn_rows<NG>, KR_THREADS, KrShared<NG>::TOTAL, a, items, merge, stream);
         default: return launch_attn<NG>(c, s, k_kv4_attn<NG, 2>, T, KaShared<NG, 16>::TOTAL, a, items, merge, stream);
     }
 }

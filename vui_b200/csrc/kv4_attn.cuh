@@ -343,8 +343,9 @@ __device__ __forceinline__ void ka_finish(const Kv4AttnArgs& a, const KaRing<NG,
     }
 }
 
-// Form for tiles of more columns than a few: keys as the A operand, queries as the B operand (8 columns), values as f16; the scores'
-// transpose for the second product is one movmatrix a fragment.  Softmax statistics and sums are fp32; the weights enter the second
+// Form for tiles of 8 or 16 columns: keys as the A operand, queries as the B operand (8 columns), values as f16; the scores'
+// transpose for the second product is one movmatrix a fragment.  Each warp has its own positions and makes f16 of them in registers, 13
+// instructions for eight codes: with 16 columns about what their products cost.  Softmax statistics and sums are fp32; the weights enter the second
 // product as f16 (2^-11 of each, where bf16's 2^-8 would be as much as the output's own rounding).
 template <int NG, int NT>
 __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn(const Kv4AttnArgs a) {
@@ -587,10 +588,10 @@ __device__ __forceinline__ float two_bytes(int high, int low) {
     return fmaf(__int_as_float(high) - 12582912.f, 256.f, __int_as_float(low) - 12582912.f);
 }
 
-template <int NG, int NT, bool HALVES>
+template <int NG, bool HALVES>
 __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn_few(const Kv4AttnArgs a) {
-    static_assert(!HALVES || (NT == 1 && NG % 2 == 0), "two halves of an even number of groups");
-    constexpr int HD = NG * KV4_GROUP, COLS = HALVES ? 2 : NT * 4;
+    static_assert(!HALVES || NG % 2 == 0, "two halves of an even number of groups");
+    constexpr int HD = NG * KV4_GROUP, COLS = HALVES ? 2 : 4;
     constexpr int OWN = HALVES ? NG / 2 : NG, SIDES = HALVES ? 2 : 1;      // groups that a lane scales; group i * SIDES + side
     using S = KaShared<NG, COLS>;
     constexpr int KT = S::KT, D = S::STAGES, NEXT = KA_WARPS * S::TILE;
@@ -604,10 +605,10 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn_few(const Kv4AttnA
 
     const int side = HALVES ? t & 1 : 0, query = HALVES ? t >> 1 : t;
     const uint32_t pick = g & 1 ? 0x6240 : 0x7351;      // low or high bytes of four 16-bit weights, in the order of a word's keys
-    uint32_t qf[NT][NG][2];         // bytes of column g: high byte (even g) or low byte of its query
-    float qsum[NT][OWN], factor[NT];  // of the lane's query, as all below
-    int limit[NT];                  // last position that it sees
-    float acc[NT][2 * OWN][2], zsum[NT][OWN], m[NT], l[NT];
+    uint32_t qf[NG][2];         // bytes of column g: high byte (even g) or low byte of its query
+    float qsum[OWN], factor;    // of the lane's query, as all below
+    int limit;                  // last position that it sees
+    float acc[2 * OWN][2], zsum[OWN], m, l;
     unsigned merged = 0;
     for (unsigned k = 0;; ++k) {
         const int s = k % D;
@@ -620,144 +621,124 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn_few(const Kv4AttnA
         const bool whole = d.base + S::KEYS - 1 <= d.all;                   // every column sees all of the stage
         if (flags & KI_QUERIES) {
             const int cols = d.rows * a.group - d.ctile * COLS;
+            const int col = HALVES ? g >> 2 : g >> 1;
+            uint4 raw[NG];
+            uint32_t big = 0;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const int col = HALVES ? g >> 2 : nt * 4 + (g >> 1);
-                uint4 raw[NG];
-                uint32_t big = 0;
-#pragma unroll
-                for (int i = 0; i < NG; ++i) {
-                    raw[i] = make_uint4(0, 0, 0, 0);
-                    if (col < cols) raw[i] = *reinterpret_cast<const uint4*>(stage + S::KV + col * S::QCOL + i * 64 + t * 16);
-                    big = max(big, most_bits(raw[i]));
-                }
-                big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
-                big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
-                // times a power of two, so that the largest element lies in [2^13, 2^14)
-                const int e = min(max((int)(big >> 7), 1), 253);
-                const float down = __int_as_float((254 - e) << 23), up = __int_as_float(e << 23);
-                float total[NG];
-#pragma unroll
-                for (int i = 0; i < NG; ++i) {
-                    const uint32_t x[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-                    int v[8], part = 0;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        v[j] = __float2int_rn(__uint_as_float(j & 1 ? x[j >> 1] & 0xffff0000u : x[j >> 1] << 16) * down * 8192.f);
-                        part += v[j];
-                        const int low = (int)(signed char)(v[j] & 255);
-                        v[j] = g & 1 ? low & 255 : (v[j] - low) >> 8 & 255;
-                    }
-                    qf[nt][i][0] = v[0] | v[4] << 8 | v[1] << 16 | v[5] << 24;      // the order of a key word's low nibbles
-                    qf[nt][i][1] = v[2] | v[6] << 8 | v[3] << 16 | v[7] << 24;      // and of its high ones
-                    if (HALVES && (g >> 1 & 1) != (i & 1)) qf[nt][i][0] = qf[nt][i][1] = 0;
-                    part += __shfl_xor_sync(0xffffffffu, part, 1);
-                    part += __shfl_xor_sync(0xffffffffu, part, 2);
-                    total[i] = (float)part;
-                }
-                // a masked score times the factor has to stay -inf, and a query that is not finite makes all its weights NaN
-                const float f = big >= 0x7f80u ? __int_as_float(0x7fffffff) : fmaxf(a.scale_log2 * up * (1.f / 8192.f), 1e-37f);
-                const int from = HALVES ? query * 16 : t * 8;        // a lane of the query's columns
-                factor[nt] = __shfl_sync(0xffffffffu, f, from);
-#pragma unroll
-                for (int i = 0; i < OWN; ++i) {
-                    qsum[nt][i] = __shfl_sync(0xffffffffu, total[i * SIDES], from);
-                    if constexpr (HALVES) {
-                        const float other = __shfl_sync(0xffffffffu, total[i * SIDES + 1], from);
-                        if (side) qsum[nt][i] = other;
-                    }
-                }
-                const int mine = nt * 4 + query;
-                limit[nt] = mine < cols ? d.start + by_group(a, d.ctile * COLS + mine) : -1;
+            for (int i = 0; i < NG; ++i) {
+                raw[i] = make_uint4(0, 0, 0, 0);
+                if (col < cols) raw[i] = *reinterpret_cast<const uint4*>(stage + S::KV + col * S::QCOL + i * 64 + t * 16);
+                big = max(big, most_bits(raw[i]));
             }
+            big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+            big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+            // times a power of two, so that the largest element lies in [2^13, 2^14)
+            const int e = min(max((int)(big >> 7), 1), 253);
+            const float down = __int_as_float((254 - e) << 23), up = __int_as_float(e << 23);
+            float total[NG];
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                const uint32_t x[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                int v[8], part = 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    v[j] = __float2int_rn(__uint_as_float(j & 1 ? x[j >> 1] & 0xffff0000u : x[j >> 1] << 16) * down * 8192.f);
+                    part += v[j];
+                    const int low = (int)(signed char)(v[j] & 255);
+                    v[j] = g & 1 ? low & 255 : (v[j] - low) >> 8 & 255;
+                }
+                qf[i][0] = v[0] | v[4] << 8 | v[1] << 16 | v[5] << 24;      // the order of a key word's low nibbles
+                qf[i][1] = v[2] | v[6] << 8 | v[3] << 16 | v[7] << 24;      // and of its high ones
+                if (HALVES && (g >> 1 & 1) != (i & 1)) qf[i][0] = qf[i][1] = 0;
+                part += __shfl_xor_sync(0xffffffffu, part, 1);
+                part += __shfl_xor_sync(0xffffffffu, part, 2);
+                total[i] = (float)part;
+            }
+            // a masked score times the factor has to stay -inf, and a query that is not finite makes all its weights NaN
+            const float f = big >= 0x7f80u ? __int_as_float(0x7fffffff) : fmaxf(a.scale_log2 * up * (1.f / 8192.f), 1e-37f);
+            const int from = HALVES ? query * 16 : t * 8;        // a lane of the query's columns
+            factor = __shfl_sync(0xffffffffu, f, from);
+#pragma unroll
+            for (int i = 0; i < OWN; ++i) {
+                qsum[i] = __shfl_sync(0xffffffffu, total[i * SIDES], from);
+                if constexpr (HALVES) {
+                    const float other = __shfl_sync(0xffffffffu, total[i * SIDES + 1], from);
+                    if (side) qsum[i] = other;
+                }
+            }
+            limit = query < cols ? d.start + by_group(a, d.ctile * COLS + query) : -1;
         }
         if (flags & KI_FIRST) {
+            m = -INFINITY;
+            l = factor * 0.f;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                m[nt] = -INFINITY;
-                l[nt] = factor[nt] * 0.f;
+            for (int i = 0; i < OWN; ++i) zsum[i] = 0.f;
 #pragma unroll
-                for (int i = 0; i < OWN; ++i) zsum[nt][i] = 0.f;
-#pragma unroll
-                for (int i = 0; i < 2 * OWN; ++i) acc[nt][i][0] = acc[nt][i][1] = 0.f;
-            }
+            for (int i = 0; i < 2 * OWN; ++i) acc[i][0] = acc[i][1] = 0.f;
         }
         if (left > 0) {
             const unsigned char* const mine = stage + warp * S::TILE;
             auto there = [&](int k2) { return k2 * (KA_WARPS * KV4_TILE) < left; };     // whether the warp has a tile number k2
-            float sc[KT][NT][2];      // scores of keys g and g + 8 of every tile, then weights
+            float sc[KT][2];      // scores of keys g and g + 8 of every tile, then weights
 #pragma unroll
             for (int k2 = 0; k2 < KT; ++k2) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) sc[k2][nt][0] = sc[k2][nt][1] = 0.f;
+                sc[k2][0] = sc[k2][1] = 0.f;
                 if (there(k2)) {
 #pragma unroll
                     for (int i = 0; i < OWN; ++i) {
                         const unsigned char* const p = mine + k2 * NEXT + i * SIDES * KV4_GT;
                         const uint2 par = *reinterpret_cast<const uint2*>(p + side * KV4_GT + KV4_KPAR + g * 8);
                         const float2 p0 = __half22float2(as_h2(par.x)), p1 = __half22float2(as_h2(par.y));     // scale, zero
-                        int x[NT][4];
+                        int x[4];
 #pragma unroll
                         for (int j = 0; j < SIDES; ++j) {
                             const uint2 code = *reinterpret_cast<const uint2*>(p + j * KV4_GT + lane * 8);
                             const uint32_t a0 = code.x & 0x0f0f0f0fu, a1 = code.y & 0x0f0f0f0fu;
                             const uint32_t a2 = code.x >> 4 & 0x0f0f0f0fu, a3 = code.y >> 4 & 0x0f0f0f0fu;
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) {
-                                const uint32_t* const q = qf[nt][i * SIDES + j];
-                                if (j == 0) mma16832<true>(x[nt], a0, a1, a2, a3, q[0], q[1], KA_ORIGIN, KA_ORIGIN, KA_ORIGIN, KA_ORIGIN);
-                                else mma16832<true>(x[nt], a0, a1, a2, a3, q[0], q[1], x[nt][0], x[nt][1], x[nt][2], x[nt][3]);
-                            }
+                            const uint32_t* const q = qf[i * SIDES + j];
+                            if (j == 0) mma16832<true>(x, a0, a1, a2, a3, q[0], q[1], KA_ORIGIN, KA_ORIGIN, KA_ORIGIN, KA_ORIGIN);
+                            else mma16832<true>(x, a0, a1, a2, a3, q[0], q[1], x[0], x[1], x[2], x[3]);
                         }
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            sc[k2][nt][0] = fmaf(p0.x, two_bytes(x[nt][0], x[nt][1]), fmaf(p0.y, qsum[nt][i], sc[k2][nt][0]));
-                            sc[k2][nt][1] = fmaf(p1.x, two_bytes(x[nt][2], x[nt][3]), fmaf(p1.y, qsum[nt][i], sc[k2][nt][1]));
-                        }
+                        sc[k2][0] = fmaf(p0.x, two_bytes(x[0], x[1]), fmaf(p0.y, qsum[i], sc[k2][0]));
+                        sc[k2][1] = fmaf(p1.x, two_bytes(x[2], x[3]), fmaf(p1.y, qsum[i], sc[k2][1]));
                     }
                     if constexpr (HALVES) {
-                        sc[k2][0][0] += __shfl_xor_sync(0xffffffffu, sc[k2][0][0], 1);
-                        sc[k2][0][1] += __shfl_xor_sync(0xffffffffu, sc[k2][0][1], 1);
+                        sc[k2][0] += __shfl_xor_sync(0xffffffffu, sc[k2][0], 1);
+                        sc[k2][1] += __shfl_xor_sync(0xffffffffu, sc[k2][1], 1);
                     }
                 }
             }
             if (!whole) {
 #pragma unroll
                 for (int k2 = 0; k2 < KT; ++k2) {
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        if (base + k2 * (KA_WARPS * KV4_TILE) + g > limit[nt]) sc[k2][nt][0] = -INFINITY;
-                        if (base + k2 * (KA_WARPS * KV4_TILE) + g + 8 > limit[nt]) sc[k2][nt][1] = -INFINITY;
-                    }
+                    if (base + k2 * (KA_WARPS * KV4_TILE) + g > limit) sc[k2][0] = -INFINITY;
+                    if (base + k2 * (KA_WARPS * KV4_TILE) + g + 8 > limit) sc[k2][1] = -INFINITY;
                 }
             }
+            float top = sc[0][0];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                float top = sc[0][nt][0];
+            for (int k2 = 0; k2 < KT; ++k2) top = fmaxf(fmaxf(top, sc[k2][0]), sc[k2][1]);
 #pragma unroll
-                for (int k2 = 0; k2 < KT; ++k2) top = fmaxf(fmaxf(top, sc[k2][nt][0]), sc[k2][nt][1]);
+            for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            top *= factor;
+            if (flags & KI_FIRST) {
+                m = top;
+            } else if (__any_sync(0xffffffffu, top > m)) {
+                const float best = fmaxf(m, top), old = best == -INFINITY ? 1.f : ex2(m - best);
+                m = best;
+                l *= old;
 #pragma unroll
-                for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                top *= factor[nt];
-                if (flags & KI_FIRST) {
-                    m[nt] = top;
-                } else if (__any_sync(0xffffffffu, top > m[nt])) {
-                    const float best = fmaxf(m[nt], top), old = best == -INFINITY ? 1.f : ex2(m[nt] - best);
-                    m[nt] = best;
-                    l[nt] *= old;
+                for (int i = 0; i < OWN; ++i) zsum[i] *= old;
 #pragma unroll
-                    for (int i = 0; i < OWN; ++i) zsum[nt][i] *= old;
+                for (int i = 0; i < 2 * OWN; ++i) { acc[i][0] *= old; acc[i][1] *= old; }
+            }
+            const float less = m == -INFINITY ? 0.f : -m;       // nothing seen yet: weights of exp(-inf) = 0
 #pragma unroll
-                    for (int i = 0; i < 2 * OWN; ++i) { acc[nt][i][0] *= old; acc[nt][i][1] *= old; }
-                }
-                const float less = m[nt] == -INFINITY ? 0.f : -m[nt];       // nothing seen yet: weights of exp(-inf) = 0
+            for (int k2 = 0; k2 < KT; ++k2) {
 #pragma unroll
-                for (int k2 = 0; k2 < KT; ++k2) {
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        sc[k2][nt][j] = ex2(fminf(fmaf(sc[k2][nt][j], factor[nt], less), 0.f));
-                        l[nt] += sc[k2][nt][j];
-                    }
+                for (int j = 0; j < 2; ++j) {
+                    sc[k2][j] = ex2(fminf(fmaf(sc[k2][j], factor, less), 0.f));
+                    l += sc[k2][j];
                 }
             }
             // value scales, and the largest of each group
@@ -775,8 +756,7 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn_few(const Kv4AttnA
                         vs[k2][i][0] = p0.x;
                         vs[k2][i][1] = p1.x;
                         unit[i] = fmaxf(fmaxf(unit[i], p0.x), p1.x);
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) zsum[nt][i] = fmaf(sc[k2][nt][0], p0.y, fmaf(sc[k2][nt][1], p1.y, zsum[nt][i]));
+                        zsum[i] = fmaf(sc[k2][0], p0.y, fmaf(sc[k2][1], p1.y, zsum[i]));
                     }
                 }
             }
@@ -798,50 +778,41 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn_few(const Kv4AttnA
             }
 #pragma unroll
             for (int i = 0; i < OWN; ++i) {
-                int x[NT][SIDES][2][4];
+                int x[SIDES][2][4];
 #pragma unroll
                 for (int k2 = 0; k2 < KT; k2 += 2) {
                     if (k2 == 0 || there(k2)) {       // of a second tile that is not there the weights are 0
-                        uint32_t b[NT][2];
+                        uint32_t b[2];
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                // the nearest whole number in the low 16 bits, twice over, for the columns of both bytes
-                                const uint32_t w0 = __float_as_uint(fmaf(sc[k2 + j][nt][0], vs[k2 + j][i][0], 8388608.f));
-                                const uint32_t w8 = __float_as_uint(fmaf(sc[k2 + j][nt][1], vs[k2 + j][i][1], 8388608.f));
-                                b[nt][j] = __byte_perm(movmatrix(__byte_perm(w0, 0, 0x1010)), movmatrix(__byte_perm(w8, 0, 0x1010)), pick);
-                            }
+                        for (int j = 0; j < 2; ++j) {
+                            // the nearest whole number in the low 16 bits, twice over, for the columns of both bytes
+                            const uint32_t w0 = __float_as_uint(fmaf(sc[k2 + j][0], vs[k2 + j][i][0], 8388608.f));
+                            const uint32_t w8 = __float_as_uint(fmaf(sc[k2 + j][1], vs[k2 + j][i][1], 8388608.f));
+                            b[j] = __byte_perm(movmatrix(__byte_perm(w0, 0, 0x1010)), movmatrix(__byte_perm(w8, 0, 0x1010)), pick);
                         }
 #pragma unroll
                         for (int j = 0; j < SIDES; ++j) {
                             const unsigned char* const p = mine + k2 * NEXT + (i * SIDES + j) * KV4_GT + KV4_VCODE + lane * 8;
                             const uint2 c0 = *reinterpret_cast<const uint2*>(p), c1 = *reinterpret_cast<const uint2*>(p + NEXT);
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) {
-                                // elements in the high nibbles come out 16 times as large
-                                int(&y)[4] = x[nt][j][0], (&z)[4] = x[nt][j][1];
-                                if (k2 == 0) {
-                                    mma16832<false>(y, c0.x & 0x0f0f0f0fu, c0.x & 0xf0f0f0f0u, c1.x & 0x0f0f0f0fu, c1.x & 0xf0f0f0f0u, b[nt][0], b[nt][1], KA_ORIGIN, KA_ORIGIN, KA_ORIGIN, KA_ORIGIN);
-                                    mma16832<false>(z, c0.y & 0x0f0f0f0fu, c0.y & 0xf0f0f0f0u, c1.y & 0x0f0f0f0fu, c1.y & 0xf0f0f0f0u, b[nt][0], b[nt][1], KA_ORIGIN, KA_ORIGIN, KA_ORIGIN, KA_ORIGIN);
-                                } else {
-                                    mma16832<false>(y, c0.x & 0x0f0f0f0fu, c0.x & 0xf0f0f0f0u, c1.x & 0x0f0f0f0fu, c1.x & 0xf0f0f0f0u, b[nt][0], b[nt][1], y[0], y[1], y[2], y[3]);
-                                    mma16832<false>(z, c0.y & 0x0f0f0f0fu, c0.y & 0xf0f0f0f0u, c1.y & 0x0f0f0f0fu, c1.y & 0xf0f0f0f0u, b[nt][0], b[nt][1], z[0], z[1], z[2], z[3]);
-                                }
+                            // elements in the high nibbles come out 16 times as large
+                            int(&y)[4] = x[j][0], (&z)[4] = x[j][1];
+                            if (k2 == 0) {
+                                mma16832<false>(y, c0.x & 0x0f0f0f0fu, c0.x & 0xf0f0f0f0u, c1.x & 0x0f0f0f0fu, c1.x & 0xf0f0f0f0u, b[0], b[1], KA_ORIGIN, KA_ORIGIN, KA_ORIGIN, KA_ORIGIN);
+                                mma16832<false>(z, c0.y & 0x0f0f0f0fu, c0.y & 0xf0f0f0f0u, c1.y & 0x0f0f0f0fu, c1.y & 0xf0f0f0f0u, b[0], b[1], KA_ORIGIN, KA_ORIGIN, KA_ORIGIN, KA_ORIGIN);
+                            } else {
+                                mma16832<false>(y, c0.x & 0x0f0f0f0fu, c0.x & 0xf0f0f0f0u, c1.x & 0x0f0f0f0fu, c1.x & 0xf0f0f0f0u, b[0], b[1], y[0], y[1], y[2], y[3]);
+                                mma16832<false>(z, c0.y & 0x0f0f0f0fu, c0.y & 0xf0f0f0f0u, c1.y & 0x0f0f0f0fu, c1.y & 0xf0f0f0f0u, b[0], b[1], z[0], z[1], z[2], z[3]);
                             }
                         }
                     }
                 }
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
+                for (int j = 0; j < 2; ++j) {
+                    int y[4];
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        int y[4];
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) y[r] = HALVES && side ? x[nt][SIDES - 1][j][r] : x[nt][0][j][r];
-                        acc[nt][2 * i + j][0] = fmaf(unit[i], two_bytes(y[0], y[1]), acc[nt][2 * i + j][0]);
-                        acc[nt][2 * i + j][1] = fmaf(unit[i] * 0.0625f, two_bytes(y[2], y[3]), acc[nt][2 * i + j][1]);
-                    }
+                    for (int r = 0; r < 4; ++r) y[r] = HALVES && side ? x[SIDES - 1][j][r] : x[0][j][r];
+                    acc[2 * i + j][0] = fmaf(unit[i], two_bytes(y[0], y[1]), acc[2 * i + j][0]);
+                    acc[2 * i + j][1] = fmaf(unit[i] * 0.0625f, two_bytes(y[2], y[3]), acc[2 * i + j][1]);
                 }
             }
         }
@@ -855,22 +826,19 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn_few(const Kv4AttnA
         if (lane == 0) bar_arrive(ring.empty(s));
         const int cols = last.rows * a.group - last.ctile * COLS;           // valid ones of this tile, if fewer than COLS
         if (merged && !bar_wait(ring.acc_empty(), (merged - 1) & 1)) { give_up(a.c.flag); return; }
+        const int col = query;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int col = nt * 4 + query;
+        for (int o = 4; o < 32; o <<= 1) {
+            l += __shfl_xor_sync(0xffffffffu, l, o);
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) {
-                l[nt] += __shfl_xor_sync(0xffffffffu, l[nt], o);
+            for (int i = 0; i < OWN; ++i) zsum[i] += __shfl_xor_sync(0xffffffffu, zsum[i], o);
+        }
+        if (col < cols) {
+            if (g == 0 && side == 0) ring.ml[warp * COLS + col] = make_float2(m, l);
 #pragma unroll
-                for (int i = 0; i < OWN; ++i) zsum[nt][i] += __shfl_xor_sync(0xffffffffu, zsum[nt][i], o);
-            }
-            if (col < cols) {
-                if (g == 0 && side == 0) ring.ml[warp * COLS + col] = make_float2(m[nt], l[nt]);
-#pragma unroll
-                for (int i = 0; i < OWN; ++i)
-                    *reinterpret_cast<float4*>(ring.acc + (warp * COLS + col) * (HD + 4) + (i * SIDES + side) * KV4_GROUP + 4 * g) =
-                        make_float4(acc[nt][2 * i][0] + zsum[nt][i], acc[nt][2 * i][1] + zsum[nt][i], acc[nt][2 * i + 1][0] + zsum[nt][i], acc[nt][2 * i + 1][1] + zsum[nt][i]);
-            }
+            for (int i = 0; i < OWN; ++i)
+                *reinterpret_cast<float4*>(ring.acc + (warp * COLS + col) * (HD + 4) + (i * SIDES + side) * KV4_GROUP + 4 * g) =
+                    make_float4(acc[2 * i][0] + zsum[i], acc[2 * i][1] + zsum[i], acc[2 * i + 1][0] + zsum[i], acc[2 * i + 1][1] + zsum[i]);
         }
         __syncwarp();
         if (lane == 0) bar_arrive(ring.acc_full());
@@ -879,6 +847,260 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn_few(const Kv4AttnA
         __syncwarp();
         if (lane == 0) bar_arrive(ring.acc_empty());
         ++merged;
+    }
+}
+
+// Form for chunks of prompts: a CTA takes 128 columns, 16 a warp, and 64 positions at a time.  Codes become f16 once a CTA, one tile of 16 keys or
+// values a warp, and lie in shared memory in the order in which lanes need them as the B operands of m16n8k16: 16 bytes a lane, no conflicts.
+// The queries are the A operand of the first product and stay in registers; the weights, as the first product leaves them, are the A operand of
+// the second.  A lane ends with eight neighbouring elements of its rows.  (Weights below 2^-25 of a column's largest are lost in f16.)
+// Each step's codes are read while the step before is computed; two buffers, so that one barrier a step is enough.
+// Bound: at heads of 128 a step's products take the tensor cores 2130 cycles at mma.sync's rate (8.3 a product and scheduler) and its operands
+// 2050 of shared memory's; measured, about 4500 with the exponentials and the conversion in between, as two warps a scheduler overlap them
+// only in part.  2 x 1000 rows of 32 query and 8 kv heads of 128 against 6000 to 9000 positions: 952 us, 243 TFLOP/s of some 540 that mma.sync
+// can do.  12 warps with 96 positions at a time (168 registers, spills) take 994 us, 16 warps 1339.
+constexpr int KR_COLS = 128, KR_WARPS = 8, KR_THREADS = KR_WARPS * 32, KR_STEP = 64;
+template <int NG>
+struct KrShared {
+    static constexpr int HALF = 4 * NG * 2 * 32;            // 16-byte pieces of a step's keys, and of its values
+    static constexpr int TOTAL = 2 * 2 * HALF * 16;
+};
+
+template <int NG>
+__global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const Kv4AttnArgs a) {
+    constexpr int HD = NG * KV4_GROUP, HALF = KrShared<NG>::HALF;
+    extern __shared__ __align__(128) unsigned char smem[];
+    uint4* const ring = reinterpret_cast<uint4*>(smem);     // [buffer][keys, values][tile][group][half][lane]
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int tile = warp & 3, tiles = 1 << (a.c.block_shift - 4);      // the tile of a step that this warp fills, keys or values
+    const bool value = warp >= 4;
+    pdl_wait();
+    pdl_launch();
+    Kv4Walk u = {};
+    long long share = 0;
+    int buffer = 0;
+    for (bool more = walk_begin<KR_COLS>(a, u, share, lane); more; walk_next<KR_COLS>(a, u), more = u.at < share && u.entry < a.n) {
+        const int first = u.ctile * KR_COLS, cols = min(u.e.z * a.group - first, KR_COLS), mine = warp * 16 + g;
+        const int steps = max((u.hi - u.base + KR_STEP - 1) / KR_STEP, 0);
+        const int32_t* const table = a.c.table + (size_t)u.e.x * a.c.max_blocks;
+        auto block_of = [&](int j) {
+            const int pos = u.base + j * KR_STEP + tile * KV4_TILE;
+            return pos < u.hi ? __ldcg(table + (pos >> a.c.block_shift)) : 0;
+        };
+        uint2 code[NG];
+        uint4 par[NG];
+        auto read = [&](int j, int id) {        // what is not there is zeros
+            const int pos = u.base + j * KR_STEP + tile * KV4_TILE;
+            const bool there = pos < u.hi;
+            if ((unsigned)id >= (unsigned)a.c.n_blocks) {
+                if (lane == 0) atomicOr(a.c.flag, KV4_BAD_BLOCK);
+                id = 0;
+            }
+            const unsigned char* const at = a.c.pool + ((size_t)((long long)id * a.c.n_kv + u.head) * tiles + ((pos & ((1 << a.c.block_shift) - 1)) >> 4)) * (NG * KV4_GT);
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                code[i] = make_uint2(0, 0);
+                par[i] = make_uint4(0, 0, 0, 0);
+                if (!there) continue;
+                code[i] = __ldcg(reinterpret_cast<const uint2*>(at + i * KV4_GT + (value ? KV4_VCODE : 0) + lane * 8));
+                if (value) {
+                    par[i] = __ldcg(reinterpret_cast<const uint4*>(at + i * KV4_GT + KV4_VPAR + t * 16));      // of keys 2t, 2t+8, 2t+1, 2t+9
+                } else {
+                    const uint2 p = __ldcg(reinterpret_cast<const uint2*>(at + i * KV4_GT + KV4_KPAR + g * 8));
+                    par[i].x = p.x;
+                    par[i].y = p.y;
+                }
+            }
+        };
+        auto fill = [&](uint4* to) {
+            to += (value ? HALF : 0) + tile * (NG * 64) + lane;
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                uint32_t x[4], y[4];
+                if (value) {
+                    const __half2 s0 = as_h2(__byte_perm(par[i].x, par[i].z, 0x5410)), z0 = as_h2(__byte_perm(par[i].x, par[i].z, 0x7632));
+                    const __half2 s8 = as_h2(__byte_perm(par[i].y, par[i].w, 0x5410)), z8 = as_h2(__byte_perm(par[i].y, par[i].w, 0x7632));
+                    kv4_values(code[i].x, s0, z0, s8, z8, x);
+                    kv4_values(code[i].y, s0, z0, s8, z8, y);
+                    to[i * 64] = make_uint4(x[0], x[2], x[1], x[3]);           // elements 4 g, then 4 g + 1 of keys 2t, 2t+1 and 2t+8, 2t+9
+                    to[i * 64 + 32] = make_uint4(y[0], y[2], y[1], y[3]);      // elements 4 g + 2, then 4 g + 3
+                } else {
+                    const __half2 s0 = __low2half2(as_h2(par[i].x)), z0 = __high2half2(as_h2(par[i].x));
+                    const __half2 s8 = __low2half2(as_h2(par[i].y)), z8 = __high2half2(as_h2(par[i].y));
+                    kv4_values(code[i].x, s0, z0, s0, z0, x);
+                    kv4_values(code[i].y, s8, z8, s8, z8, y);
+                    to[i * 64] = make_uint4(x[0], x[1], x[2], x[3]);           // elements 8 t .. 8 t + 7 of key g
+                    to[i * 64 + 32] = make_uint4(y[0], y[1], y[2], y[3]);      // of key g + 8
+                }
+            }
+        };
+        int id = block_of(0);
+        read(0, id);
+        id = block_of(1);
+
+        // the lane's two columns: queries (times a power of two, so that the largest element lies in [1, 2): exact in f16 but for elements 2^14
+        // times smaller), the last position seen
+        uint32_t q[NG][8];
+        float factor[2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, acc[NG][4][4];
+        int limit[2], row[2], head[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int c = first + mine + 8 * r;
+            const bool there = mine + 8 * r < cols;
+            row[r] = there ? by_group(a, c) : 0;
+            head[r] = u.head * a.group + (there ? c - row[r] * a.group : 0);
+            limit[r] = there ? min(u.e.y + row[r], u.hi - 1) : -1;
+            const uint4* const src = reinterpret_cast<const uint4*>(a.q + (long long)(u.e.w + row[r]) * a.q_stride + head[r] * HD) + t;
+            uint4 raw[NG];
+            uint32_t big = 0;
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                raw[i] = make_uint4(0, 0, 0, 0);
+                if (there) raw[i] = __ldcg(src + i * 4);
+                big = max(big, most_bits(raw[i]));
+            }
+            big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+            big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+            const int e = min(max((int)(big >> 7), 1), 253);
+            const float down = __int_as_float((254 - e) << 23), up = __int_as_float(e << 23);
+            factor[r] = fmaxf(a.scale_log2 * up, 1e-37f);       // not 0, which would make NaN of masked scores
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                const uint32_t v[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j)      // elements 8 t + 2 j: first or second half of the first (j < 2) or second product's k
+                    q[i][(j >> 1) * 4 + (j & 1) * 2 + r] = pack_h2(__uint_as_float(v[j] << 16) * down, __uint_as_float(v[j] & 0xffff0000u) * down);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.f;
+        }
+        // the last position that some, and that every, column of the warp sees (a split need not end with a step)
+        const int some = warp * 16 < cols ? min(u.e.y + by_group(a, first + min(warp * 16 + 15, cols - 1)), u.hi - 1) : -1;
+        const int every = min(u.e.y + by_group(a, first + warp * 16), u.hi - 1);
+
+        for (int j = 0; j < steps; ++j) {
+            uint4* const at = ring + buffer * (2 * HALF);
+            buffer ^= 1;
+            fill(at);
+            __syncthreads();
+            if (j + 1 < steps) {
+                read(j + 1, id);
+                id = block_of(j + 2);
+            }
+            const int base = u.base + j * KR_STEP;
+            if (base > some) continue;
+            const uint4* const keys = at + lane;
+            float s[4][2][4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    s[k][h][0] = s[k][h][1] = s[k][h][2] = s[k][h][3] = 0.f;
+#pragma unroll
+                    for (int i = 0; i < NG; ++i) {
+                        const uint4 b = keys[(k * NG + i) * 64 + h * 32];
+                        mma16816(s[k][h], q[i][0], q[i][1], q[i][2], q[i][3], b.x, b.y);
+                        mma16816(s[k][h], q[i][4], q[i][5], q[i][6], q[i][7], b.z, b.w);
+                    }
+                }
+            }
+            if (base + KR_STEP - 1 > every) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                        for (int x = 0; x < 4; ++x)
+                            if (base + k * KV4_TILE + h * 8 + 2 * t + (x & 1) > limit[x >> 1]) s[k][h][x] = -INFINITY;
+                    }
+                }
+            }
+            float top[2] = {s[0][0][0], s[0][0][2]};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    top[0] = fmaxf(fmaxf(top[0], s[k][h][0]), s[k][h][1]);
+                    top[1] = fmaxf(fmaxf(top[1], s[k][h][2]), s[k][h][3]);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2)) * factor[r];
+            }
+            if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float best = fmaxf(m[r], top[r]), old = best == -INFINITY ? 1.f : ex2(m[r] - best);
+                    m[r] = best;
+                    l[r] *= old;
+#pragma unroll
+                    for (int i = 0; i < NG; ++i) {
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            acc[i][x][2 * r] *= old;
+                            acc[i][x][2 * r + 1] *= old;
+                        }
+                    }
+                }
+            }
+            const float less[2] = {m[0] == -INFINITY ? 0.f : -m[0], m[1] == -INFINITY ? 0.f : -m[1]};     // nothing seen yet: weights of exp(-inf) = 0
+            const uint4* const values = at + HALF + lane;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                uint32_t p[4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        s[k][h][x] = ex2(fmaf(s[k][h][x], factor[x >> 1], less[x >> 1]));
+                        l[x >> 1] += s[k][h][x];
+                    }
+                    p[2 * h] = pack_h2(s[k][h][0], s[k][h][1]);
+                    p[2 * h + 1] = pack_h2(s[k][h][2], s[k][h][3]);
+                }
+#pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    const uint4 b = values[(k * NG + i) * 64], d = values[(k * NG + i) * 64 + 32];
+                    mma16816(acc[i][0], p[0], p[1], p[2], p[3], b.x, b.y);
+                    mma16816(acc[i][1], p[0], p[1], p[2], p[3], b.z, b.w);
+                    mma16816(acc[i][2], p[0], p[1], p[2], p[3], d.x, d.y);
+                    mma16816(acc[i][3], p[0], p[1], p[2], p[3], d.z, d.w);
+                }
+            }
+        }
+        // the lane's elements 8 t .. 8 t + 7 of every group: column 2 t of product x is element 8 t + x, column 2 t + 1 element 8 t + 4 + x
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+            if (mine + 8 * r >= cols) continue;
+            const size_t place = (size_t)u.w * KR_COLS + mine + 8 * r;
+            const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
+            if (u.splits > 1 && t == 0) a.ml[place] = make_float2(m[r], l[r]);
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                if (u.splits > 1) {
+                    float4* const dst = reinterpret_cast<float4*>(a.acc + place * HD + i * KV4_GROUP + t * 8);
+                    dst[0] = make_float4(acc[i][0][2 * r], acc[i][1][2 * r], acc[i][2][2 * r], acc[i][3][2 * r]);
+                    dst[1] = make_float4(acc[i][0][2 * r + 1], acc[i][1][2 * r + 1], acc[i][2][2 * r + 1], acc[i][3][2 * r + 1]);
+                } else {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const int half = 2 * r + (x >> 1), of = x % 2 * 2;
+                        const __nv_bfloat162 h = __floats2bfloat162_rn(acc[i][of][half] * inv, acc[i][of + 1][half] * inv);
+                        w[x] = *reinterpret_cast<const uint32_t*>(&h);
+                    }
+                    *reinterpret_cast<uint4*>(a.out + (long long)(u.e.w + row[r]) * a.out_stride + head[r] * HD + i * KV4_GROUP + t * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+        }
+        __syncwarp();
     }
 }
 
