@@ -997,14 +997,17 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const Kv4AttnAr
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    s[k][h][0] = s[k][h][1] = s[k][h][2] = s[k][h][3] = 0.f;
+                for (int h = 0; h < 2; ++h) s[k][h][0] = s[k][h][1] = s[k][h][2] = s[k][h][3] = 0.f;
+            }
 #pragma unroll
-                    for (int i = 0; i < NG; ++i) {
-                        const uint4 b = keys[(k * NG + i) * 64 + h * 32];
-                        mma16816(s[k][h], q[i][0], q[i][1], q[i][2], q[i][3], b.x, b.y);
-                        mma16816(s[k][h], q[i][4], q[i][5], q[i][6], q[i][7], b.z, b.w);
-                    }
+            for (int i = 0; i < NG; ++i) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint4 b = keys[(k * NG + i) * 64], d = keys[(k * NG + i) * 64 + 32];
+                    mma16816(s[k][0], q[i][0], q[i][1], q[i][2], q[i][3], b.x, b.y);
+                    mma16816(s[k][1], q[i][0], q[i][1], q[i][2], q[i][3], d.x, d.y);
+                    mma16816(s[k][0], q[i][4], q[i][5], q[i][6], q[i][7], b.z, b.w);
+                    mma16816(s[k][1], q[i][4], q[i][5], q[i][6], q[i][7], d.z, d.w);
                 }
             }
             if (base + KR_STEP - 1 > every) {
