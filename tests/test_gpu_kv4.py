@@ -366,6 +366,19 @@ def test_chunks_of_prompts(heads, kv, dim, block, before, new):
     f.cache.check_device()
 
 
+@pytest.mark.parametrize("seqs", [31, 32, 33, 39, 63, 65, 66, 85, 97, 129, 1025])
+def test_any_number_of_sequences(seqs):
+    """Work is shared out by searching the sequences 32 at a time: numbers that leave a group of one, of two, and of none."""
+    for heads, kv, dim, new in ((2, 1, 64, 1), (8, 2, 64, 1), (12, 2, 96, 1), (9, 1, 128, 1), (8, 2, 64, 7), (4, 1, 128, 40))[:6 if seqs < 130 else 2]:
+        f = Filled([1 + 37 * i % 90 for i in range(seqs)], heads, kv, dim, 16, spare=new)
+        plan = f.add([new] * seqs)
+        q = torch.randn(seqs * new, heads, dim, device="cuda", generator=f.g).bfloat16()
+        out = torch.full_like(q, float("nan"))
+        f.cache.attention(0, q, plan, out=out)
+        close(out, f.want(q, [new] * seqs))
+        f.cache.check_device()
+
+
 @pytest.mark.parametrize("heads, kv, dim, seqs, new", [(32, 8, 96, 64, 68), (12, 4, 96, 8, 200), (12, 4, 64, 40, 90), (16, 4, 128, 30, 71)])
 def test_many_tiles_that_end_inside_a_warp(heads, kv, dim, seqs, new):
     """Columns that end within 32 of one another, over and over, call after call: all bits the same, none of them anywhere else."""
