@@ -132,7 +132,8 @@ __device__ __forceinline__ int find_in(const int* first, int n, int x) {
 }
 
 // One CTA, or one cluster whose CTAs all compute the same few prefix sums and share out what is written: a step's entries are few, its
-// rows and blocks many.  Latency bound: three dependent reads (entry, length, table) and five barriers.
+// rows and blocks many.  Latency bound: three dependent reads (entry, length, table) and five barriers.  64 sequences of one row: 5.6 us a call in a
+// graph; 512 sequences emptied, then filled again with 4 to 300 positions each (81000 rows): 15 us each of the two calls.
 __global__ void __launch_bounds__(1024) k_kv4_plan(const Kv4PlanArgs a) {
     extern __shared__ int sm[];
     __shared__ int scan_a[1][32], scan_b[2][32], scan_c[5][32];
@@ -381,6 +382,8 @@ __device__ __forceinline__ float code_between(float f, float s, float k) {
 // The nearest code: (x - zero) times the reciprocal of 15 scales, kept within [0, 1] and times 15, is 2^-17.4 off at most (a division of two ulp and two roundings, of a
 // quotient below 16), so unless that lies within 2^-17 of the middle between two codes it rounds as the quotient does; lanes that have such an
 // element (exact middles are not rare among bf16 numbers: one group of normal ones in fifty) look closer.
+// Bound by instructions: 16000 rows of 8 heads of 128 are 33 million elements, 22 an element and lane; 37 us (65 MB in and 20 out: 13 us).  Keys and
+// values in one warp, unrolled, took 72 us (50 KB of code), 8 elements a lane with a division each 55.
 template <int NG>
 __global__ void __launch_bounds__(128) k_kv4_append(const Kv4RowsArgs a) {
     constexpr int LANES = NG * 2, ROWS = 32 / LANES;     // lanes of a row; rows side by side: 8, 5 (2 lanes idle), 4
@@ -529,6 +532,7 @@ __global__ void __launch_bounds__(128) k_kv4_append(const Kv4RowsArgs a) {
 // The reverse: 8 elements of four kv heads a thread, bf16 out.  Rows whose slot or position is out of range, or whose block the table lacks, come out as
 // zeros.  A CTA takes the rows next to one another, keys or values (blockIdx.z), because those of a tile share its lines in
 // the L1; that is why this kernel starts only when the kernel before it has ended (no early launch: an SM's L1 could hold older lines).
+// 16000 rows of 8 heads of 128: 25 us (20 MB in and 65 out: 13 us); with one head a thread, which looks its row up for 8 elements, 29.
 constexpr int KV4_READ_HEADS = 4;
 template <int NG>
 __global__ void __launch_bounds__(256) k_kv4_read(const Kv4RowsArgs a) {
