@@ -349,6 +349,11 @@ def test_single_tokens(heads, kv, dim, block):
     (15, 5, 128, 16, [127, 1, 0], [129, 128, 127]),
     (64, 4, 128, 256, [0, 0, 2000], [1, 8, 64]),
     (16, 16, 64, 64, [100, 5], [1100, 7]),
+    # contexts beyond eight pieces of 512, whose pieces are longer
+    (16, 8, 64, 256, [4400, 6700], [20, 9]),
+    (8, 8, 96, 64, [4200], [30]),
+    (6, 2, 128, 64, [5000, 4097], [7, 40]),
+    (4, 1, 64, 64, [4500], [90]),
     (32, 8, 128, 32, [0, 0, 0, 900], [380, 257, 128, 5]),
 ])
 def test_chunks_of_prompts(heads, kv, dim, block, before, new):

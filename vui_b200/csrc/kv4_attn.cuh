@@ -209,6 +209,7 @@ template <int NG, int COLS>
 struct KaShared {
     static constexpr int KT = NG == 2 ? 4 : 2;                                  // tiles of 16 positions a warp takes at once
     static constexpr int KEYS = KA_WARPS * KT * KV4_TILE;                         // positions of a stage
+    static_assert(256 % KEYS == 0, "splits are whole stages, but for a sequence's last");
     static constexpr int TILE = NG * KV4_GT, QCOL = NG * KV4_GROUP * 2;
     static constexpr int KV = KA_WARPS * KT * TILE, Q = COLS * QCOL;
     static constexpr int STAGE = KV + Q + (int)sizeof(Kv4Item);

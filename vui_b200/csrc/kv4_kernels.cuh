@@ -51,11 +51,11 @@ struct Kv4Cache {
 // Positions of a split of attention's work: by the length of the sequence alone, so that a row's bits do not depend on what else is there.
 struct Kv4Split {
     int up_to_512, up_to_1024, beyond;
-    int most;        // splits of one sequence: longer ones get larger splits, multiples of 128 positions
+    int most;        // splits of one sequence: longer ones get larger splits, multiples of 256 positions, so that a stage ends with its split
     bool weigh;      // units count for what they cost: their positions by 64, and one more
     __host__ __device__ int of(long long len) const {
         const int s = len <= 512 ? up_to_512 : len <= 1024 ? up_to_1024 : beyond;
-        return (long long)s * most >= len ? s : (int)(((len + most - 1) / most + 127) & ~127ll);
+        return (long long)s * most >= len ? s : (int)(((len + most - 1) / most + 255) & ~255ll);
     }
     __host__ __device__ int parts(long long len) const { const int s = of(len); return (int)((len + s - 1) / s); }
     __host__ __device__ int work(long long len) const { return parts(len) + (weigh ? (int)((len + 63) / 64) : 0); }     // of all parts
