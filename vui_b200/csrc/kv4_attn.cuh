@@ -182,17 +182,15 @@ __device__ __forceinline__ void bar_arrive(uint32_t bar) {
 __device__ __forceinline__ void bar_expect(uint32_t bar, unsigned bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-// Waits for a phase, a bounded number of polls; false when they run out.
-__device__ __forceinline__ bool bar_wait_one(uint32_t bar, unsigned parity) {
+// Waits for a phase, a bounded number of polls; false for the whole warp when they run out.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, unsigned parity) {
     uint32_t ok = 0;
     for (unsigned i = 0; i < KV4_POLLS && !ok; ++i)
         asm volatile(
             "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
             : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    return ok;
+    return __all_sync(0xffffffffu, ok);
 }
-// The same for a whole warp.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, unsigned parity) { return __all_sync(0xffffffffu, bar_wait_one(bar, parity)); }
 __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, unsigned bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
