@@ -1,0 +1,88 @@
+"""The paged 4-bit cache where it can go wrong: what blocks held before, outliers, sizes and values at the borders of what a call takes."""
+import pytest
+import torch
+from test_gpu_kv4 import Filled, close, fixed, make, stored
+
+pytestmark = pytest.mark.gpu
+
+
+# columns of a tile (rows x query heads of a kv head): 1 to 4, at every width
+FEW = [(8, 8, 64), (16, 8, 64), (9, 3, 64), (16, 4, 64), (4, 4, 96), (12, 4, 96), (2, 2, 128), (4, 2, 128), (32, 8, 128)]
+
+
+@pytest.mark.parametrize("heads, kv, dim", FEW + [(16, 2, 64), (32, 2, 128)])
+def test_what_a_block_held_before_does_not_count(heads, kv, dim):
+    """Sequences that end inside a tile whose other positions still hold what was there before: another sequence's values, or the
+    sequence's own from before a cut-back.  The same bits as in a cache where nothing was."""
+    lens = [*range(1, 18), 33, 70, 650]
+    g = torch.Generator(device="cuda").manual_seed(3)
+    n = sum(lens)
+    k, v, q = ((torch.randn(n, h, dim, generator=g, device="cuda") * s).bfloat16() for h, s in ((kv, 1), (kv, 0.5), (heads, 1)))
+    q = q[:len(lens)].contiguous()
+    last = torch.tensor(lens, device="cuda").cumsum(0) - 1
+    before = torch.ones(n, dtype=torch.bool, device="cuda")
+    before[last] = False
+    outs = []
+    for kind in ("fresh", "another's", "its own"):
+        cache = make(sum(-(-x // 16) + 2 for x in lens), 16, len(lens), heads=heads, kv=kv, dim=dim)
+        slots = list(range(len(lens)))
+        if kind != "fresh":
+            more = [x + 17 for x in lens]
+            big = [((torch.rand(sum(more), kv, dim, generator=g, device="cuda") - 0.5) * 60000).bfloat16() for _ in range(2)]
+            cache.append(0, *big, cache.plan(slots, more))
+        plan = cache.plan(slots, [x - 1 for x in lens], at=[0] * len(lens) if kind == "its own" else None) if kind != "another's" else None
+        if kind == "another's":
+            cache.release(slots)
+            plan = cache.plan(slots, [x - 1 for x in lens])
+        cache.append(0, k[before], v[before], plan)
+        plan = cache.plan(slots)
+        cache.append(0, k[last], v[last], plan)
+        outs.append(cache.attention(0, q, plan))
+        cache.check_device()
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+@pytest.mark.parametrize("heads, kv, dim, new", [(8, 8, 64, 2), (8, 8, 64, 4), (16, 8, 64, 2), (4, 4, 96, 3), (4, 2, 96, 2), (2, 2, 128, 2), (8, 4, 128, 2)])
+def test_later_rows_do_not_count(heads, kv, dim, new):
+    """A chunk's first row has the same bits whatever the rows behind it store."""
+    outs = []
+    for size in (1.0, 20000.0):
+        f = Filled([1, 21, 60, 700], heads, kv, dim, 64, spare=new)
+        g = torch.Generator(device="cuda").manual_seed(4)
+        k, v, q = (torch.randn(4 * new, h, dim, generator=g, device="cuda").bfloat16() for h in (kv, kv, heads))
+        v.view(4, new, kv, dim)[:, 1:] *= size
+        plan = f.cache.plan(f.slots, [new] * 4)
+        f.cache.append(0, k, v, plan)
+        outs.append(f.cache.attention(0, q, plan).view(4, new, heads, dim))
+    assert torch.equal(outs[0][:, 0], outs[1][:, 0]) and not torch.equal(outs[0], outs[1])
+
+
+def weighed(x, k, v, p, mag, scale):
+    """As fixed(), with the weights' part taken from what is summed: weights times value scales enter in units of 2^-16 of the largest such
+    product of a query and group of 32 elements, up to 1.01 of it, half a unit off each, against codes up to 15; independent errors, six
+    standard deviations."""
+    span = (v.unflatten(-1, (-1, 32)).amax(-1) - v.unflatten(-1, (-1, 32)).amin(-1)) / 15 * 1.001      # (n, heads, groups)
+    unit = 1.01 * torch.einsum("hrn,nhg->rhgn", p, span).amax(-1) * 2.0 ** -16
+    sums = k.shape[0] ** 0.5 * 15 * 6 / 12 ** 0.5 * unit.repeat_interleave(32, -1)
+    return fixed(x, k, torch.zeros_like(v), p, mag, scale) + sums
+
+
+@pytest.mark.parametrize("heads, kv, dim", FEW)
+@pytest.mark.parametrize("size", [1000.0, 30000.0])
+def test_outliers_of_no_weight(heads, kv, dim, size):
+    """Positions with values far larger than the others' and next to no weight: the others lose nothing by them."""
+    f = Filled([1], heads, kv, dim, 64, spare=1200, max_blocks=20)
+    for n in (40, 300, 900):
+        plan = f.cache.plan(f.slots, [n], at=[0])
+        k, v = (torch.randn(n, kv, dim, generator=f.g, device="cuda") for _ in range(2))
+        k[3::50], v[3::50] = -30.0, v[3::50] * size
+        k, v = k.bfloat16(), v.clamp(-60000, 60000).bfloat16()
+        f.cache.append(0, k, v, plan)
+        f.k[0], f.v[0] = stored(k), stored(v)
+        plan = f.cache.plan(f.slots, [1], at=[n - 1])
+        f.cache.append(0, k[-1:], v[-1:], plan)
+        q = torch.randn(1, heads, dim, device="cuda", generator=f.g).abs().bfloat16()
+        ref, mag, _ = f.want(q, [1])
+        kk, vv = (x[0].repeat_interleave(heads // kv, 1) for x in (f.k, f.v))
+        p = (torch.einsum("rhd,nhd->hrn", q.double(), kk) * dim ** -0.5).softmax(-1)
+        close(f.cache.attention(0, q, plan), (ref, mag, weighed(q.double(), kk, vv, p, mag, dim ** -0.5)))

@@ -577,10 +577,10 @@ __device__ __forceinline__ void mma16832(int (&d)[4], uint32_t a0, uint32_t a1, 
 //   scores:  q . K = sum over groups of scale * (q . code) + zero * (sum of the group's q)
 //   outputs: sum_i w_i V_i = sum_i (w_i scale_i) code_i + sum_i w_i zero_i
 // A query column, times a power of two, is a 15-bit whole number: exact for elements down to 2^-6 of the largest, the others to 2^-14 of
-// it.  The weights times the value scales are 16-bit whole numbers in units of 2^-16 of the largest value scale among the warp's positions
-// (half a unit off, each on its own, a quarter of what bf16 weights would be off at one position and less the more there are).  Both are
-// cut into two bytes that take two of the 8 columns of a product.  The tensor cores' sums are exact; what is added to them, statistics and
-// outputs, is fp32.
+// it.  The weights times the value scales are 16-bit whole numbers in units of 2^-16 of the largest such product of the query and group
+// among the warp's positions (half a unit off, each on its own): positions that a query does not see, or whose weight is nothing, take no part
+// in the unit, whatever they hold.  Both are cut into two bytes that take two of the 8 columns of a product.  The tensor cores' sums are exact;
+// what is added to them, statistics and outputs, is fp32.
 // A product's columns hold four queries; or (HALVES, for up to two queries a tile, heads of 64 and 128) two queries twice, once for the
 // even groups of 32 elements and once for the odd ones, zeros elsewhere: a lane then has one group of two to scale and to weigh.
 // 256 sequences of 512 to 2048 positions, two query heads a kv head of 64: 53 us (219 MB: 34 us), the copies alone 52; with f16 values and a
@@ -743,7 +743,7 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn_few(const Kv4AttnA
                     l += sc[k2][j];
                 }
             }
-            // value scales, and the largest of each group
+            // weights times value scales, and the largest of each group
             float vs[KT][OWN][2], unit[OWN], units[OWN];
 #pragma unroll
             for (int i = 0; i < OWN; ++i) unit[i] = 0.f;
@@ -755,28 +755,28 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn_few(const Kv4AttnA
                     if (there(k2)) {
                         const uint2 par = *reinterpret_cast<const uint2*>(mine + k2 * NEXT + (i * SIDES + side) * KV4_GT + KV4_VPAR + g * 8);
                         const float2 p0 = __half22float2(as_h2(par.x)), p1 = __half22float2(as_h2(par.y));
-                        vs[k2][i][0] = p0.x;
-                        vs[k2][i][1] = p1.x;
-                        unit[i] = fmaxf(fmaxf(unit[i], p0.x), p1.x);
+                        vs[k2][i][0] = sc[k2][0] * p0.x;
+                        vs[k2][i][1] = sc[k2][1] * p1.x;
+                        unit[i] = fmaxf(fmaxf(unit[i], vs[k2][i][0]), vs[k2][i][1]);
                         zsum[i] = fmaf(sc[k2][0], p0.y, fmaf(sc[k2][1], p1.y, zsum[i]));
                     }
                 }
             }
+            // Of the lane's query over all keys: two groups at a time as bf16, rounded up.  Products below 1e-30 are nothing beside the weight of 1
+            // that the maximum has.
 #pragma unroll
-            for (int i = 0; i < OWN; ++i) {
-                if constexpr (HALVES) {
+            for (int i = 0; i < OWN; i += 2) {
+                const bool two = i + 1 < OWN;
+                uint32_t top2 = __byte_perm(__float_as_uint(unit[i]), __float_as_uint(unit[two ? i + 1 : i]), 0x7632) + 0x00010001u;
 #pragma unroll
-                    for (int o = 4; o < 32; o <<= 1) unit[i] = fmaxf(unit[i], __shfl_xor_sync(0xffffffffu, unit[i], o));
-                } else {
-                    unit[i] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(unit[i])));
-                }
-                units[i] = unit[i] > 0.f ? __fdividef(65280.f, unit[i]) : 0.f;
-                unit[i] *= 1.f / 65280.f;
+                for (int o = 4; o < 32; o <<= 1) top2 = __vmaxu2(top2, __shfl_xor_sync(0xffffffffu, top2, o));
+                unit[i] = __uint_as_float(top2 << 16);
+                if (two) unit[i + 1] = __uint_as_float(top2 & 0xffff0000u);
             }
 #pragma unroll
-            for (int k2 = 0; k2 < KT; ++k2) {
-#pragma unroll
-                for (int i = 0; i < OWN; ++i) { vs[k2][i][0] *= units[i]; vs[k2][i][1] *= units[i]; }
+            for (int i = 0; i < OWN; ++i) {
+                units[i] = unit[i] > 1e-30f ? __fdividef(65280.f, unit[i]) : 0.f;
+                unit[i] *= 1.f / 65280.f;
             }
 #pragma unroll
             for (int i = 0; i < OWN; ++i) {
@@ -788,8 +788,8 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn_few(const Kv4AttnA
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
                             // the nearest whole number in the low 16 bits, twice over, for the columns of both bytes
-                            const uint32_t w0 = __float_as_uint(fmaf(sc[k2 + j][0], vs[k2 + j][i][0], 8388608.f));
-                            const uint32_t w8 = __float_as_uint(fmaf(sc[k2 + j][1], vs[k2 + j][i][1], 8388608.f));
+                            const uint32_t w0 = __float_as_uint(fmaf(vs[k2 + j][i][0], units[i], 8388608.f));
+                            const uint32_t w8 = __float_as_uint(fmaf(vs[k2 + j][i][1], units[i], 8388608.f));
                             b[j] = __byte_perm(movmatrix(__byte_perm(w0, 0, 0x1010)), movmatrix(__byte_perm(w8, 0, 0x1010)), pick);
                         }
 #pragma unroll
