@@ -1,4 +1,7 @@
 """The paged 4-bit cache where it can go wrong: what blocks held before, outliers, sizes and values at the borders of what a call takes."""
+import subprocess
+import sys
+
 import pytest
 import torch
 from test_gpu_kv4 import Filled, close, fixed, make, stored
@@ -86,3 +89,18 @@ def test_outliers_of_no_weight(heads, kv, dim, size):
         kk, vv = (x[0].repeat_interleave(heads // kv, 1) for x in (f.k, f.v))
         p = (torch.einsum("rhd,nhd->hrn", q.double(), kk) * dim ** -0.5).softmax(-1)
         close(f.cache.attention(0, q, plan), (ref, mag, weighed(q.double(), kk, vv, p, mag, dim ** -0.5)))
+
+
+def test_plans_at_the_border_of_a_blocks_shared_memory():
+    """Numbers of sequences whose tables take about as much shared memory as a launch gets unasked, as a process's first plans."""
+    program = """
+from vui_b200 import Kv4Cache
+for seqs, slots in ((1000, 4096), (1023, 4096), (1340, 1500), (1365, 1365), (1022, 4096), (4096, 4096)):
+    cache = Kv4Cache(n_layers=1, n_heads=2, n_kv_heads=1, head_dim=64, n_blocks=seqs + 1, block_size=16, max_seqs=slots, max_blocks=2)
+    plan = cache.plan(list(range(seqs)))
+    cache.check_device()
+    assert plan.cu_rows.tolist() == list(range(seqs + 1)) and cache.seq_lens.tolist() == [1] * seqs + [0] * (slots - seqs)
+print("fine")
+"""
+    done = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "fine" in done.stdout, done.stderr[-2000:]

@@ -114,6 +114,9 @@ long long most_items(const VuibKv4* c, const VuibKv4Plan* p, const Shape& s) { r
 
 size_t acc_bytes(const VuibKv4* c, long long items, int cols) { return ((size_t)items * cols * c->cfg.head_dim * 4 + 255) & ~size_t(255); }
 
+// Shared memory of the plan's kernel.
+size_t plan_smem(int n_seqs, int max_seqs) { return (8 * (size_t)n_seqs + 3 + max_seqs) * 4; }
+
 // The parts of a plan's work array.
 int4* plan_entries(const VuibKv4Plan* p) { return reinterpret_cast<int4*>(p->work); }
 int32_t* plan_units(const VuibKv4Plan* p) { return p->work + 4 * (size_t)p->n_seqs; }
@@ -231,6 +234,9 @@ extern "C" int32_t vuib_kv4_bind(VuibKv4* c, void* pool, size_t bytes, int32_t* 
     memset(c->resident, 0, sizeof(c->resident));
     CK(cudaGetDevice(&c->device));
     CK(cudaDeviceGetAttribute(&c->sms, cudaDevAttrMultiProcessorCount, c->device));
+    // For the largest plan there can be: the attribute is the kernel's, not a call's, and what a launch gets without it holds the kernel's
+    // static arrays too.
+    CK(cudaFuncSetAttribute(k_kv4_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)plan_smem(KV4_MAX_SEQS, KV4_MAX_SEQS)));
     c->cache = {static_cast<unsigned char*>(pool), block_table, seq_lens, free_blocks, n_free, flag, c->cfg.n_kv_heads, c->block_shift,
                 c->cfg.n_blocks, c->cfg.max_seqs, c->cfg.max_blocks};
     c->bound = true;
@@ -261,8 +267,7 @@ extern "C" int32_t vuib_kv4_plan(VuibKv4* c, const VuibKv4Plan* p, const int32_t
     a.entries = plan_entries(p); a.cu_units = plan_units(p); a.cu_work = plan_work(p); a.cu_tiles = plan_tiles(p); a.row_entry = plan_row_entry(p);
     a.cu_rows = p->cu_rows;
     a.row_slot = p->row_slot; a.row_pos = p->row_pos; a.slot_map = reinterpret_cast<long long*>(p->slot_map);
-    const size_t smem = (8 * (size_t)p->n_seqs + 3 + c->cfg.max_seqs) * 4;
-    if (smem > 48 * 1024) CK(cudaFuncSetAttribute(k_kv4_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    const size_t smem = plan_smem(p->n_seqs, c->cfg.max_seqs);
     // One CTA where little is written: a cluster's barriers cost 2 us.  Rows are known here; cut-backs can give back any number of blocks.
     const int cluster = p->n_rows > 4096 || (at_dev && p->n_seqs > 64 && c->cfg.n_blocks > 4096) ? 8 : 1;
     const int threads = p->n_seqs <= 256 && p->n_rows <= 1024 ? 256 : 1024;
