@@ -564,7 +564,8 @@ int32_t vuib_kv4_plan(VuibKv4* c, const VuibKv4Plan* plan, const int32_t* slots_
  * of 8, 16-byte aligned).  NaN is stored as 0, magnitudes beyond 60000 as 60000 (recorded in the flag). */
 int32_t vuib_kv4_append(VuibKv4* c, int32_t layer, const VuibKv4Plan* plan, const void* k_dev, int64_t k_stride,
                         const void* v_dev, int64_t v_stride, void* stream);
-/* What is stored for rows (row_slot, row_pos), as bf16 (n_rows, n_kv_heads * head_dim); slot -1 gives zeros. */
+/* What is stored for rows (row_slot, row_pos), as bf16 (n_rows, n_kv_heads * head_dim); slot -1 gives zeros, and so does a row
+ * whose slot is out of range or whose position is not below its sequence's length (recorded in the flag). */
 int32_t vuib_kv4_read(VuibKv4* c, int32_t layer, int32_t n_rows, const int32_t* row_slot_dev, const int32_t* row_pos_dev,
                       void* k_out_dev, int64_t k_stride, void* v_out_dev, int64_t v_stride, void* stream);
 

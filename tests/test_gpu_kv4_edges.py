@@ -104,3 +104,29 @@ print("fine")
 """
     done = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0 and "fine" in done.stdout, done.stderr[-2000:]
+
+
+def test_positions_behind_a_sequences_end_are_not_read():
+    """In a block that holds what another sequence left there."""
+    from vui_b200._lib import VuibError
+
+    cache = make(2, 32, 2, heads=2, kv=2)
+    x = torch.full((64, 2, 64), 77.0, device="cuda", dtype=torch.bfloat16)
+    cache.append(0, x, x, cache.plan([1], [64]))
+    cache.release([1])
+    plan = cache.plan([0], [20])
+    cache.append(0, x[:20] * 0 + 5, x[:20] * 0 + 5, plan)
+    for t in cache.read(0, [0] * 20, list(range(20))):
+        assert (t == 5).all()
+    cache.check_device()
+    for p in (20, 21, 31, 32):
+        for t in cache.read(0, [0, 0], [p, 19]):
+            assert (t[0] == 0).all() and (t[1] == 5).all()
+        with pytest.raises(VuibError, match="position"):
+            cache.check_device()
+    cache.plan([0], [0], at=[3])
+    assert all((t == 0).all() for t in cache.read(0, [0], [3]))
+    with pytest.raises(VuibError, match="position"):
+        cache.check_device()
+    assert all((t == 5).all() for t in cache.read(0, [0], [2]))
+    cache.check_device()

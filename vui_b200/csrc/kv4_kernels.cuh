@@ -529,7 +529,7 @@ __global__ void __launch_bounds__(128) k_kv4_append(const Kv4RowsArgs a) {
     }
 }
 
-// The reverse: 8 elements of four kv heads a thread, bf16 out.  Rows whose slot or position is out of range, or whose block the table lacks, come out as
+// The reverse: 8 elements of four kv heads a thread, bf16 out.  Rows whose slot is out of range or whose position lies behind the sequence's end come out as
 // zeros.  A CTA takes the rows next to one another, keys or values (blockIdx.z), because those of a tile share its lines in
 // the L1; that is why this kernel starts only when the kernel before it has ended (no early launch: an SM's L1 could hold older lines).
 // 16000 rows of 8 heads of 128: 25 us (20 MB in and 65 out: 13 us); with one head a thread, which looks its row up for 8 elements, 29.
@@ -544,8 +544,9 @@ __global__ void __launch_bounds__(256) k_kv4_read(const Kv4RowsArgs a) {
     const int slot = __ldg(a.row_slot + row), pos = __ldg(a.row_pos + row);
     long long where = -1;
     if (slot >= 0 && slot < a.c.max_seqs && pos >= 0 && (pos >> a.c.block_shift) < a.c.max_blocks) {
-        const int b = __ldg(a.c.table + (size_t)slot * a.c.max_blocks + (pos >> a.c.block_shift));
-        if (b >= 0 && b < a.c.n_blocks) where = ((long long)b << a.c.block_shift) + (pos & ((1 << a.c.block_shift) - 1));
+        const int b = __ldg(a.c.table + (size_t)slot * a.c.max_blocks + (pos >> a.c.block_shift)), len = __ldg(a.c.lens + slot);
+        // behind the end lies what the block's last owner stored
+        if (b >= 0 && b < a.c.n_blocks && pos < len) where = ((long long)b << a.c.block_shift) + (pos & ((1 << a.c.block_shift) - 1));
     }
     if (where < 0 && slot != -1) atomicOr(a.c.flag, KV4_BAD_SLOT);
     const int key = (int)(where & 15), key8 = key & 7, upper = key >> 3, grp = ch >> 2, t = ch & 3, heads = min(a.c.n_kv - h0, KV4_READ_HEADS);

@@ -218,7 +218,8 @@ class Kv4Cache:
 
     def read(self, layer: int, row_slot, row_pos, *, k_out: Tensor | None = None, v_out: Tensor | None = None) -> tuple[Tensor, Tensor]:
         """The keys and values stored for position ``row_pos[i]`` of sequence ``row_slot[i]``: (n, n_kv_heads, head_dim) bf16,
-        new tensors or ``k_out`` and ``v_out`` (a stretch of an engine's bf16 cache, say).  Slot -1 gives zeros."""
+        new tensors or ``k_out`` and ``v_out`` (a stretch of an engine's bf16 cache, say).  Slot -1 gives zeros; so do positions that
+        the sequence does not have, which are recorded (``check_device``)."""
         with self._here():
             row_slot = self._ints(row_slot, "row_slot")
             n = row_slot.numel()
