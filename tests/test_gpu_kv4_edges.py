@@ -130,3 +130,41 @@ def test_positions_behind_a_sequences_end_are_not_read():
         cache.check_device()
     assert all((t == 5).all() for t in cache.read(0, [0], [2]))
     cache.check_device()
+
+
+def test_numbers_beyond_32_bits_on_the_device():
+    """They are as out of range as any other, not what is left of them in 32 bits."""
+    from vui_b200._lib import VuibError
+
+    far = lambda *v: torch.tensor(v, dtype=torch.int64, device="cuda")  # noqa: E731
+    cache = make(10, 16, 3)
+    cache.plan([0, 1], [5, 5])
+    for call in (lambda: cache.plan(far(2 ** 32)), lambda: cache.plan(far(-2 ** 32)), lambda: cache.plan(far(2 ** 32 - 1)),
+                 lambda: cache.plan(far(0), far(2 ** 32 + 1), n_rows=4, max_new=4),
+                 lambda: cache.plan(far(0), far(1), at=far(2 ** 33 + 2), n_rows=4, max_new=4), lambda: cache.release(far(2 ** 32 + 1)),
+                 lambda: cache.read(0, far(2 ** 32), far(0)), lambda: cache.read(0, far(0), far(2 ** 32 + 1))):
+        call()
+        with pytest.raises(VuibError):
+            cache.check_device()
+        assert cache.seq_lens.tolist() == [5, 5, 0]
+    plan = cache.plan(far(1, -1), far(2, 0), at=far(4, 0), n_rows=4, max_new=4)
+    assert plan.row_pos.tolist() == [4, 5, -1, -1] and cache.seq_lens.tolist() == [5, 6, 0]
+    cache.check_device()
+
+
+def test_unsigned_numbers():
+    from vui_b200._lib import VuibError
+
+    cache = make(10, 16, 3)
+    for where in ("cpu", "cuda"):
+        for t in (torch.uint8, torch.uint16, torch.uint32):
+            assert cache.plan(torch.tensor([1]).to(t).to(where)).row_slot.tolist() == [1]
+        with pytest.raises(ValueError):
+            cache.plan(torch.tensor([1]).to(torch.uint64).to(where))
+    far = torch.tensor([2 ** 32 - 1], dtype=torch.uint32)
+    with pytest.raises(ValueError, match="32 bits"):
+        cache.plan(far)
+    cache.check_device()
+    assert cache.plan(far.cuda()).row_slot.tolist() == [-1]
+    with pytest.raises(VuibError):
+        cache.check_device()

@@ -132,8 +132,14 @@ class Kv4Cache:
         if t.dim() != 1 or t.is_floating_point() or t.is_complex() or (n is not None and t.numel() != n):
             raise ValueError(f"{name}: a one-dimensional list of {'whole numbers' if n is None else f'{n} whole numbers'} is wanted, "
                              f"got {t.dtype} {tuple(t.shape)}")
+        if t.dtype is torch.uint64:
+            raise ValueError(f"{name}: int32 or int64 is wanted, got {t.dtype}")
+        if t.dtype in (torch.uint16, torch.uint32):
+            t = t.to(torch.int64)
         if not t.is_cuda and t.numel() and not (-2 ** 31 <= int(t.min()) and int(t.max()) < 2 ** 31):
             raise ValueError(f"{name}: numbers beyond 32 bits")
+        if t.dtype is torch.int64:      # on the device: the ends of 32 bits, which are out of range too
+            t = t.clamp(-2 ** 31, 2 ** 31 - 1)
         return t.to(self.device, torch.int32).contiguous()
 
     # ------------------------------------------------------------------ tables
