@@ -168,3 +168,21 @@ def test_unsigned_numbers():
     assert cache.plan(far.cuda()).row_slot.tolist() == [-1]
     with pytest.raises(VuibError):
         cache.check_device()
+
+
+def test_sizes_beyond_32_bits():
+    from vui_b200._lib import VuibError
+
+    cache = make(10, 16, 3)
+    plan = cache.plan([0], [1])
+    k, q = (torch.zeros(1, h, 64, device="cuda", dtype=torch.bfloat16) for h in (8, 16))
+    for bad in (lambda: cache.append(2 ** 32, k, k, plan), lambda: cache.attention(2 ** 32, q, plan), lambda: cache.read(-2 ** 32, [0], [0])):
+        with pytest.raises(VuibError, match="layer"):
+            bad()
+    for n in (2 ** 24 + 1, 2 ** 31, 2 ** 32 + 1):
+        with pytest.raises(ValueError, match="n_rows"):
+            cache.plan([0], [1], n_rows=n, max_new=1)
+    with pytest.raises(ValueError, match="n_rows"):
+        cache.plan([0, 1], [2 ** 31 - 1, 2 ** 31 - 1])
+    cache.check_device()
+    assert cache.seq_lens.tolist() == [1, 0, 0]

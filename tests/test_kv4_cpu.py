@@ -69,3 +69,12 @@ def test_null_and_unbound():
     assert lib.vuib_kv4_plan(h, None, p, p, None, None) == -1
     assert lib.vuib_kv4_launch_count(h) == 0
     assert lib.vuib_kv4_destroy(h) == 0
+
+
+@pytest.mark.parametrize("name", [n for n, _ in _lib.VuibKv4Config._fields_])
+def test_sizes_beyond_32_bits_are_refused(name):
+    """Not taken for what 32 bits leave of them."""
+    kw = {n: getattr(_cfg(), n) for n, _ in _lib.VuibKv4Config._fields_}
+    for more in (2 ** 32, -2 ** 32, 2 ** 40):
+        with pytest.raises(ValueError):
+            Kv4Cache(**{**kw, name: kw[name] + more})

@@ -31,6 +31,14 @@ _NOTHING = contextlib.nullcontext()
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
+_MOST_ROWS = 1 << 24      # of a plan
+
+
+def _int32(x: int) -> int:
+    """x, or the end of 32 bits that is next to it: out of range all the same, where ctypes would drop the higher bits."""
+    return min(max(x, -2 ** 31), 2 ** 31 - 1)
+
+
 class Kv4Plan:
     """The rows of one step, all on the device: ``row_slot`` and ``row_pos`` (int32) say which position of which sequence
     a row is, ``slot_map`` (int64) where it lies (block * block_size + offset), ``cu_rows`` (int32, one more than
@@ -77,7 +85,8 @@ class Kv4Cache:
                  max_seqs: int, max_blocks: int | None = None, device="cuda"):
         self._h = C.c_void_p()
         max_blocks = n_blocks if max_blocks is None else max_blocks
-        cfg = _lib.VuibKv4Config(n_layers, n_heads, n_kv_heads, head_dim, n_blocks, block_size, max_seqs, max_blocks)
+        sizes = (n_layers, n_heads, n_kv_heads, head_dim, n_blocks, block_size, max_seqs, max_blocks)
+        cfg = _lib.VuibKv4Config(*(_int32(x) for x in sizes))
         self._lib = _lib.load()
         rc = self._lib.vuib_kv4_create(C.byref(cfg), C.byref(self._h))
         if rc:
@@ -171,6 +180,8 @@ class Kv4Cache:
             at = None if at is None else self._ints(at, "at", n)
             if n_rows < 0 or max_new < 0:
                 raise ValueError("n_rows and max_new must not be negative")
+            if n_rows > _MOST_ROWS:
+                raise ValueError(f"n_rows {n_rows}: a plan holds up to {_MOST_ROWS}")
             plan = Kv4Plan(self, n, int(n_rows), min(int(max_new), int(n_rows)))
             self._ck(self._lib.vuib_kv4_plan(self._h, plan._ref, slots.data_ptr(), None if new is None else new.data_ptr(),
                                              None if at is None else at.data_ptr(), self._stream))
@@ -217,7 +228,7 @@ class Kv4Cache:
         with self._here():
             n, heads = plan.n_rows, self.n_kv_heads
             k, v = self._rows(k, "k", n, heads), self._rows(v, "v", n, heads)
-            rc = self._lib.vuib_kv4_append(self._h, layer, plan._ref, k.data_ptr(), self._step(k, heads), v.data_ptr(), self._step(v, heads),
+            rc = self._lib.vuib_kv4_append(self._h, _int32(layer), plan._ref, k.data_ptr(), self._step(k, heads), v.data_ptr(), self._step(v, heads),
                                            _raw_stream(self._index))
             if rc:
                 self._ck(rc)
@@ -234,7 +245,7 @@ class Kv4Cache:
             k = new() if k_out is None else self._rows(k_out, "k_out", n, self.n_kv_heads, out=True)
             v = new() if v_out is None else self._rows(v_out, "v_out", n, self.n_kv_heads, out=True)
             if n:
-                self._ck(self._lib.vuib_kv4_read(self._h, layer, n, row_slot.data_ptr(), row_pos.data_ptr(), k.data_ptr(),
+                self._ck(self._lib.vuib_kv4_read(self._h, _int32(layer), n, row_slot.data_ptr(), row_pos.data_ptr(), k.data_ptr(),
                                                  self._step(k, self.n_kv_heads), v.data_ptr(), self._step(v, self.n_kv_heads), self._stream))
         return k, v
 
@@ -269,7 +280,7 @@ class Kv4Cache:
                 ws = torch.empty(plan._ws_bytes, dtype=torch.uint8, device=self.device)
                 if not torch.cuda.is_current_stream_capturing():
                     plan._ws[stream] = ws
-        rc = self._lib.vuib_kv4_attention(self._h, layer, plan._ref, q.data_ptr(), self._step(q, heads), out.data_ptr(), step, scale or 0.0,
+        rc = self._lib.vuib_kv4_attention(self._h, _int32(layer), plan._ref, q.data_ptr(), self._step(q, heads), out.data_ptr(), step, scale or 0.0,
                                           None if ws is None else ws.data_ptr(), plan._ws_bytes, stream)
         if rc:
             self._ck(rc)
