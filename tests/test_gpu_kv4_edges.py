@@ -186,3 +186,14 @@ def test_sizes_beyond_32_bits():
         cache.plan([0, 1], [2 ** 31 - 1, 2 ** 31 - 1])
     cache.check_device()
     assert cache.seq_lens.tolist() == [1, 0, 0]
+
+
+def test_scales_that_are_0_in_32_bits():
+    f = Filled([70], 16, 8, 64, 64)
+    plan = f.add([1])
+    q = torch.randn(1, 16, 64, device="cuda", generator=f.g).bfloat16()
+    for scale in (1e-50, 1e-46, 5e-324, 1e31, float("inf")):
+        with pytest.raises(ValueError, match="scale"):
+            f.cache.attention(0, q, plan, scale=scale)
+    for scale in (1e-40, 2.0 ** -126):
+        close(f.cache.attention(0, q, plan, scale=scale), f.want(q, [1], scale))

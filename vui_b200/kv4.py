@@ -253,8 +253,8 @@ class Kv4Cache:
         """Causal attention of the plan's rows, each over its sequence up to and with its own position (append first):
         q (n_rows, n_heads, head_dim) with RoPE applied -> the same shape, bf16.  ``scale`` defaults to 1 / sqrt(head_dim).
         Rows behind the plan's last are not written."""
-        if scale is not None and not 0 < scale <= 1e30:
-            raise ValueError("scale must be positive")
+        if scale is not None and not (scale <= 1e30 and C.c_float(scale).value > 0):       # 0 is the library's word for the default
+            raise ValueError("scale must be positive, also in 32 bits, and at most 1e30")
         self._own(plan)
         if torch.cuda.current_device() != self._index:
             with torch.cuda.device(self._index):
