@@ -197,3 +197,26 @@ def test_scales_that_are_0_in_32_bits():
             f.cache.attention(0, q, plan, scale=scale)
     for scale in (1e-40, 2.0 ** -126):
         close(f.cache.attention(0, q, plan, scale=scale), f.want(q, [1], scale))
+
+
+@pytest.mark.parametrize("seqs, first", [(600, 100), (4096, 100), (600, 0)])
+def test_lengths_whose_sum_is_beyond_32_bits(seqs, first):
+    """Each in range by itself; all but the first are left as they are."""
+    from vui_b200._lib import VuibError
+
+    most = 1 << 22
+    cache = make(64, 256, seqs, most // 256, heads=2, kv=1)
+    new = torch.full((seqs,), most, dtype=torch.int32, device="cuda")
+    new[0] = first
+    for at in (None, torch.zeros_like(new)):
+        plan = cache.plan(list(range(seqs)), new, at=at, n_rows=most, max_new=most)
+        with pytest.raises(VuibError, match="more rows" if first else "more rows.*out of blocks"):
+            cache.check_device()
+        assert cache.seq_lens.tolist() == [first] + [0] * (seqs - 1) and int(cache.n_free.item()) == 64 - (first > 0)
+        assert plan.cu_rows.tolist() == [0] + [first] * seqs and (plan.row_slot[first:] == -1).all() and (plan.slot_map[first:] == -1).all()
+        assert plan.row_pos[:first].tolist() == list(range(first)) and int((cache.block_table >= 0).sum()) == (first > 0)
+        cache.release([0])
+        cache.check_device()
+    plan = cache.plan([0, 5], [20, 1])
+    assert plan.cu_rows.tolist() == [0, 20, 21]
+    cache.check_device()

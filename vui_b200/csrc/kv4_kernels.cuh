@@ -83,8 +83,8 @@ __device__ __forceinline__ void plan_sync(unsigned size) {
 }
 
 // Exclusive prefix sums over the block of N non-negative numbers a thread, side by side; v becomes the sum before the thread, total the
-// whole.  Sums stop at KV4_MANY, which no size that can be served reaches.
-constexpr int KV4_MANY = 1 << 30;
+// whole.  Sums stop at KV4_MANY, which no size that can be served reaches; two of them still fit an int.
+constexpr int KV4_MANY = (1 << 30) - 1;
 template <int N>
 __device__ __forceinline__ void block_scan(int (&v)[N], int (*warp_sums)[32], int (&total)[N]) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
