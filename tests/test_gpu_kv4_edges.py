@@ -220,3 +220,25 @@ def test_lengths_whose_sum_is_beyond_32_bits(seqs, first):
     plan = cache.plan([0, 5], [20, 1])
     assert plan.cu_rows.tolist() == [0, 20, 21]
     cache.check_device()
+
+
+FORMS = [(16, 8, 64, 1), (16, 4, 64, 1), (12, 4, 96, 1), (4, 2, 128, 1), (32, 8, 128, 1), (16, 2, 64, 1), (26, 2, 128, 1), (12, 2, 96, 3), (4, 4, 64, 20),
+         (16, 8, 64, 150), (12, 4, 96, 180), (32, 8, 128, 40)]
+
+
+@pytest.mark.parametrize("heads, kv, dim, new", FORMS)
+@pytest.mark.parametrize("size", [1e6, 1e7, 1e9, 1e20, 1e33])
+def test_scores_of_any_size(heads, kv, dim, new, size):
+    """One position's score is far above the others', wherever they lie: it alone is what comes out."""
+    for n, best in ((30, 7), (700, 300), (1500, 1)):
+        f = Filled([1], heads, kv, dim, 64, spare=1800, max_blocks=30)
+        plan = f.cache.plan(f.slots, [n + new], at=[0])
+        k, v = (torch.randn(n + new, kv, dim, generator=f.g, device="cuda").bfloat16() for _ in range(2))
+        k[best] = 8.0
+        f.cache.append(0, k, v, plan)
+        plan = f.cache.plan(f.slots, [new], at=[n])
+        f.cache.append(0, k[n:], v[n:], plan)
+        q = ((1 + torch.rand(new, heads, dim, device="cuda", generator=f.g)) * size).bfloat16()
+        want = stored(v[best]).repeat_interleave(heads // kv, 0)
+        # one rounding to bf16, the stored value's own rounding to f16 (where it is left out), 16-bit weights
+        assert ((f.cache.attention(0, q, plan).double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -9).all()

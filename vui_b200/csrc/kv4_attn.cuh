@@ -40,6 +40,18 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// What a product of a query and a key is multiplied by to be a log2 score.  The maximum is kept of the products themselves and taken off before they
+// are multiplied, so that the largest weight is 1 whatever the scores' size (as a fused multiply, scores of 2^28 would leave it at
+// 2^16 or 2^-16: the maximum's rounding).  Limited to where products up to 2^38, the largest that stored keys allow, stay finite and masked
+// ones -inf: products next to one another are 1e-15 apart or more, so beyond 1e26 all but the largest weigh nothing as it is.
+__device__ __forceinline__ float score_factor(float f) { return fminf(fmaxf(f, 1e-37f), 1e26f); }
+
+// Two products by two factors in one instruction.
+__device__ __forceinline__ void mul2(float& a, float& b, float factor_a, float factor_b) {
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tmul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "+f"(a), "+f"(b) : "f"(factor_a), "f"(factor_b));
+}
+
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -398,7 +410,7 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn(const Kv4AttnArgs 
                     for (int j = 0; j < 4; ++j)
                         qf[nt][i][j] = pack_h2(__uint_as_float(x[j] << 16) * down, __uint_as_float(x[j] & 0xffff0000u) * down);
                 }
-                const float f = fmaxf(a.scale_log2 * up, 1e-37f);      // not 0, which would make NaN of masked scores
+                const float f = score_factor(a.scale_log2 * up);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const int c2 = nt * 8 + 2 * t + j;
@@ -469,8 +481,6 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn(const Kv4AttnArgs 
                     top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], o));
                     top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], o));
                 }
-                top[0] *= factor[nt][0];
-                top[1] *= factor[nt][1];
                 if (d.flags & KI_FIRST) {
                     m[nt][0] = top[0];
                     m[nt][1] = top[1];
@@ -479,7 +489,7 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn(const Kv4AttnArgs 
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         const float best = fmaxf(m[nt][j], top[j]);
-                        old[j] = best == -INFINITY ? 1.f : ex2(m[nt][j] - best);
+                        old[j] = best == -INFINITY ? 1.f : ex2((m[nt][j] - best) * factor[nt][j]);
                         m[nt][j] = best;
                         l[nt][j] *= old[j];
                     }
@@ -489,15 +499,20 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn(const Kv4AttnArgs 
                         acc[nt][i][2] *= old[0]; acc[nt][i][3] *= old[1];
                     }
                 }
-                // minus the maximum, as the addend of a fused multiply; nothing seen yet: weights of exp(-inf) = 0
+                // minus the maximum; nothing seen yet: weights of exp(-inf) = 0
                 const float less[2] = {m[nt][0] == -INFINITY ? 0.f : -m[nt][0], m[nt][1] == -INFINITY ? 0.f : -m[nt][1]};
 #pragma unroll
                 for (int k2 = 0; k2 < KT; ++k2) {
                     float e[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        e[j] = ex2(fmaf(sc[k2][nt][j], factor[nt][j & 1], less[j & 1]));
-                        l[nt][j & 1] += e[j];
+                    for (int j = 0; j < 4; j += 2) {
+                        e[j] = sc[k2][nt][j] + less[0];
+                        e[j + 1] = sc[k2][nt][j + 1] + less[1];
+                        mul2(e[j], e[j + 1], factor[nt][0], factor[nt][1]);
+                        e[j] = ex2(e[j]);
+                        e[j + 1] = ex2(e[j + 1]);
+                        l[nt][0] += e[j];
+                        l[nt][1] += e[j + 1];
                     }
                     p[k2][nt][0] = movmatrix(pack_h2(e[0], e[1]));
                     p[k2][nt][1] = movmatrix(pack_h2(e[2], e[3]));
@@ -541,7 +556,7 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn(const Kv4AttnArgs 
             for (int j = 0; j < 2; ++j) {
                 const int col = nt * 8 + 2 * t + j;
                 if (col < cols) {
-                    if (g == 0) ring.ml[warp * COLS + col] = make_float2(m[nt][j], l[nt][j]);
+                    if (g == 0) ring.ml[warp * COLS + col] = make_float2(m[nt][j] * factor[nt][j], l[nt][j]);
 #pragma unroll
                     for (int i = 0; i < NG; ++i)
                         *reinterpret_cast<float4*>(ring.acc + (warp * COLS + col) * (HD + 4) + i * KV4_GROUP + 4 * g) =
@@ -656,8 +671,8 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn_few(const Kv4AttnA
                 part += __shfl_xor_sync(0xffffffffu, part, 2);
                 total[i] = (float)part;
             }
-            // a masked score times the factor has to stay -inf, and a query that is not finite makes all its weights NaN
-            const float f = big >= 0x7f80u ? __int_as_float(0x7fffffff) : fmaxf(a.scale_log2 * up * (1.f / 8192.f), 1e-37f);
+            // a query that is not finite makes all its weights NaN
+            const float f = big >= 0x7f80u ? __int_as_float(0x7fffffff) : score_factor(a.scale_log2 * up * (1.f / 8192.f));
             const int from = HALVES ? query * 16 : t * 8;        // a lane of the query's columns
             factor = __shfl_sync(0xffffffffu, f, from);
 #pragma unroll
@@ -722,11 +737,10 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn_few(const Kv4AttnA
             for (int k2 = 0; k2 < KT; ++k2) top = fmaxf(fmaxf(top, sc[k2][0]), sc[k2][1]);
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            top *= factor;
             if (flags & KI_FIRST) {
                 m = top;
             } else if (__any_sync(0xffffffffu, top > m)) {
-                const float best = fmaxf(m, top), old = best == -INFINITY ? 1.f : ex2(m - best);
+                const float best = fmaxf(m, top), old = best == -INFINITY ? 1.f : ex2((m - best) * factor);
                 m = best;
                 l *= old;
 #pragma unroll
@@ -739,7 +753,7 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn_few(const Kv4AttnA
             for (int k2 = 0; k2 < KT; ++k2) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    sc[k2][j] = ex2(fminf(fmaf(sc[k2][j], factor, less), 0.f));
+                    sc[k2][j] = ex2((sc[k2][j] + less) * factor);
                     l += sc[k2][j];
                 }
             }
@@ -836,7 +850,7 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn_few(const Kv4AttnA
             for (int i = 0; i < OWN; ++i) zsum[i] += __shfl_xor_sync(0xffffffffu, zsum[i], o);
         }
         if (col < cols) {
-            if (g == 0 && side == 0) ring.ml[warp * COLS + col] = make_float2(m, l);
+            if (g == 0 && side == 0) ring.ml[warp * COLS + col] = make_float2(m * factor, l);
 #pragma unroll
             for (int i = 0; i < OWN; ++i)
                 *reinterpret_cast<float4*>(ring.acc + (warp * COLS + col) * (HD + 4) + (i * SIDES + side) * KV4_GROUP + 4 * g) =
@@ -965,7 +979,7 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const Kv4AttnAr
             big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
             const int e = min(max((int)(big >> 7), 1), 253);
             const float down = __int_as_float((254 - e) << 23), up = __int_as_float(e << 23);
-            factor[r] = fmaxf(a.scale_log2 * up, 1e-37f);       // not 0, which would make NaN of masked scores
+            factor[r] = score_factor(a.scale_log2 * up);
 #pragma unroll
             for (int i = 0; i < NG; ++i) {
                 const uint32_t v[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
@@ -1035,12 +1049,12 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const Kv4AttnAr
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2)) * factor[r];
+                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
             }
             if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const float best = fmaxf(m[r], top[r]), old = best == -INFINITY ? 1.f : ex2(m[r] - best);
+                    const float best = fmaxf(m[r], top[r]), old = best == -INFINITY ? 1.f : ex2((m[r] - best) * factor[r]);
                     m[r] = best;
                     l[r] *= old;
 #pragma unroll
@@ -1061,9 +1075,15 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const Kv4AttnAr
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        s[k][h][x] = ex2(fmaf(s[k][h][x], factor[x >> 1], less[x >> 1]));
-                        l[x >> 1] += s[k][h][x];
+                    for (int r = 0; r < 2; ++r) {
+                        float &u0 = s[k][h][2 * r], &u1 = s[k][h][2 * r + 1];
+                        u0 += less[r];
+                        u1 += less[r];
+                        mul2(u0, u1, factor[r], factor[r]);
+                        u0 = ex2(u0);
+                        u1 = ex2(u1);
+                        l[r] += u0;
+                        l[r] += u1;
                     }
                     p[2 * h] = pack_h2(s[k][h][0], s[k][h][1]);
                     p[2 * h + 1] = pack_h2(s[k][h][2], s[k][h][3]);
@@ -1086,7 +1106,7 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const Kv4AttnAr
             if (mine + 8 * r >= cols) continue;
             const size_t place = (size_t)u.w * KR_COLS + mine + 8 * r;
             const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
-            if (u.splits > 1 && t == 0) a.ml[place] = make_float2(m[r], l[r]);
+            if (u.splits > 1 && t == 0) a.ml[place] = make_float2(m[r] * factor[r], l[r]);
 #pragma unroll
             for (int i = 0; i < NG; ++i) {
                 if (u.splits > 1) {
