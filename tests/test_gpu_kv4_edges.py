@@ -242,3 +242,27 @@ def test_scores_of_any_size(heads, kv, dim, new, size):
         want = stored(v[best]).repeat_interleave(heads // kv, 0)
         # one rounding to bf16, the stored value's own rounding to f16 (where it is left out), 16-bit weights
         assert ((f.cache.attention(0, q, plan).double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -9).all()
+
+
+@pytest.mark.parametrize("heads, kv, dim, new", FORMS)
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+def test_queries_that_are_not_finite(heads, kv, dim, new, value):
+    """Infinity times keys of one sign leaves scores of one sign: infinite all the same, whose softmax is not defined."""
+    f = Filled([1], heads, kv, dim, 64, spare=1800, max_blocks=30)
+    for n in (30, 700):
+        plan = f.cache.plan(f.slots, [n + new], at=[0])
+        k, v = (torch.randn(n + new, kv, dim, generator=f.g, device="cuda").bfloat16() for _ in range(2))
+        k[:, :, 5] = 1.0
+        f.cache.append(0, k, v, plan)
+        f.k[0], f.v[0] = stored(k), stored(v)
+        plan = f.cache.plan(f.slots, [new], at=[n])
+        f.cache.append(0, k[n:], v[n:], plan)
+        q = torch.randn(new, heads, dim, device="cuda", generator=f.g).bfloat16()
+        want = f.want(q, [new])
+        row, head = new // 2, heads - 1
+        bad = q.clone()
+        bad[row, head, 5] = value
+        out = f.cache.attention(0, bad, plan)
+        assert out[row, head].isnan().all()
+        out[row, head] = want[0][row, head].bfloat16()
+        close(out, want)

@@ -44,7 +44,10 @@ __device__ __forceinline__ float ex2(float x) {
 // are multiplied, so that the largest weight is 1 whatever the scores' size (as a fused multiply, scores of 2^28 would leave it at
 // 2^16 or 2^-16: the maximum's rounding).  Limited to where products up to 2^38, the largest that stored keys allow, stay finite and masked
 // ones -inf: products next to one another are 1e-15 apart or more, so beyond 1e26 all but the largest weigh nothing as it is.
-__device__ __forceinline__ float score_factor(float f) { return fminf(fmaxf(f, 1e-37f), 1e26f); }
+// For a query that is not finite (`big`: the bits of its largest element) it is NaN, and so are all its weights: infinite scores have no softmax.
+__device__ __forceinline__ float score_factor(float f, uint32_t big) {
+    return fminf(fmaxf(f, 1e-37f), 1e26f) + (big >= 0x7f80u ? __int_as_float(0x7fffffff) : 0.f);
+}
 
 // Two products by two factors in one instruction.
 __device__ __forceinline__ void mul2(float& a, float& b, float factor_a, float factor_b) {
@@ -410,7 +413,7 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn(const Kv4AttnArgs 
                     for (int j = 0; j < 4; ++j)
                         qf[nt][i][j] = pack_h2(__uint_as_float(x[j] << 16) * down, __uint_as_float(x[j] & 0xffff0000u) * down);
                 }
-                const float f = score_factor(a.scale_log2 * up);
+                const float f = score_factor(a.scale_log2 * up, big);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const int c2 = nt * 8 + 2 * t + j;
@@ -671,8 +674,7 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn_few(const Kv4AttnA
                 part += __shfl_xor_sync(0xffffffffu, part, 2);
                 total[i] = (float)part;
             }
-            // a query that is not finite makes all its weights NaN
-            const float f = big >= 0x7f80u ? __int_as_float(0x7fffffff) : score_factor(a.scale_log2 * up * (1.f / 8192.f));
+            const float f = score_factor(a.scale_log2 * up * (1.f / 8192.f), big);
             const int from = HALVES ? query * 16 : t * 8;        // a lane of the query's columns
             factor = __shfl_sync(0xffffffffu, f, from);
 #pragma unroll
@@ -979,7 +981,7 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const Kv4AttnAr
             big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
             const int e = min(max((int)(big >> 7), 1), 253);
             const float down = __int_as_float((254 - e) << 23), up = __int_as_float(e << 23);
-            factor[r] = score_factor(a.scale_log2 * up);
+            factor[r] = score_factor(a.scale_log2 * up, big);
 #pragma unroll
             for (int i = 0; i < NG; ++i) {
                 const uint32_t v[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
