@@ -78,3 +78,11 @@ def test_sizes_beyond_32_bits_are_refused(name):
     for more in (2 ** 32, -2 ** 32, 2 ** 40):
         with pytest.raises(ValueError):
             Kv4Cache(**{**kw, name: kw[name] + more})
+
+
+@pytest.mark.parametrize("device", ["cpu", "cpu:0", "meta"])
+def test_other_devices_are_refused(device):
+    """With an index they went to the kernels as addresses on the GPU."""
+    kw = {n: getattr(_cfg(), n) for n, _ in _lib.VuibKv4Config._fields_}
+    with pytest.raises(ValueError, match="CUDA"):
+        Kv4Cache(**kw, device=device)

@@ -84,6 +84,9 @@ class Kv4Cache:
     def __init__(self, *, n_layers: int, n_heads: int, n_kv_heads: int, head_dim: int, n_blocks: int, block_size: int = 64,
                  max_seqs: int, max_blocks: int | None = None, device="cuda"):
         self._h = C.c_void_p()
+        dev = torch.device(device)
+        if dev.type != "cuda":
+            raise ValueError(f"device {dev}: a CUDA device is wanted; there is no CPU path")
         max_blocks = n_blocks if max_blocks is None else max_blocks
         sizes = (n_layers, n_heads, n_kv_heads, head_dim, n_blocks, block_size, max_seqs, max_blocks)
         cfg = _lib.VuibKv4Config(*(_int32(x) for x in sizes))
@@ -94,7 +97,6 @@ class Kv4Cache:
                              f"{n_blocks} blocks of {block_size}, {max_seqs} sequences of up to {max_blocks} blocks")
         if not torch.cuda.is_available():
             raise RuntimeError("vui_b200.Kv4Cache needs a CUDA device (sm_100a); there is no CPU path")
-        dev = torch.device(device)
         self.device = dev if dev.index is not None else torch.device("cuda", torch.cuda.current_device())
         self._index = self.device.index
         self.n_layers, self.n_heads, self.n_kv_heads, self.head_dim = n_layers, n_heads, n_kv_heads, head_dim
