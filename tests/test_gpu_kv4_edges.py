@@ -266,3 +266,39 @@ def test_queries_that_are_not_finite(heads, kv, dim, new, value):
         assert out[row, head].isnan().all()
         out[row, head] = want[0][row, head].bfloat16()
         close(out, want)
+
+
+@pytest.mark.parametrize("heads, kv, dim, chunk", [(16, 8, 64, 200), (32, 8, 128, 70), (12, 4, 96, 30)])
+def test_a_mixed_step_as_two_plans(heads, kv, dim, chunk):
+    """A prompt's chunk and single tokens of other sequences in one step, a plan for each: the single tokens' bits are those of a step of
+    their own, and both are right; as one plan too."""
+    lens = [400, 37, 900, 1, 2100]
+    outs = []
+    for kind in ("two", "alone", "one"):
+        f = Filled(lens, heads, kv, dim, 64, seed=8, spare=chunk)
+        new = [1, 1, chunk, 1, 1]
+        few = [i for i in range(5) if i != 2]
+        k, v, q = (torch.randn(sum(new), h, dim, device="cuda", generator=f.g).bfloat16() for h in (kv, kv, heads))
+        first = [0, 1, 2, 2 + chunk, 3 + chunk]
+        rows = torch.tensor([first[i] for i in few], device="cuda")
+        for i, m in enumerate(new):
+            a = first[i]
+            f.k[i], f.v[i] = torch.cat([f.k[i], stored(k[a:a + m])]), torch.cat([f.v[i], stored(v[a:a + m])])
+        if kind == "one":
+            plan = f.cache.plan(f.slots, new)
+            f.cache.append(0, k, v, plan)
+            close(f.cache.attention(0, q, plan), f.want(q, new))
+            continue
+        plans = [(f.cache.plan([f.slots[i] for i in few]), rows)]
+        if kind == "two":
+            plans.append((f.cache.plan([f.slots[2]], [chunk]), torch.arange(2, 2 + chunk, device="cuda")))
+        out = torch.zeros_like(q)
+        for plan, r in plans:
+            f.cache.append(0, k[r], v[r], plan)
+        for plan, r in plans:
+            out[r] = f.cache.attention(0, q[r], plan)
+        if kind == "two":
+            close(out, f.want(q, new))
+        outs.append(out[rows])
+        f.cache.check_device()
+    assert torch.equal(*outs)

@@ -149,7 +149,7 @@ class Kv4Cache:
             t = t.to(torch.int64)
         if not t.is_cuda and t.numel() and not (-2 ** 31 <= int(t.min()) and int(t.max()) < 2 ** 31):
             raise ValueError(f"{name}: numbers beyond 32 bits")
-        if t.dtype is torch.int64:      # on the device: the ends of 32 bits, which are out of range too
+        if t.is_cuda and t.dtype is torch.int64:      # the ends of 32 bits, which are out of range too
             t = t.clamp(-2 ** 31, 2 ** 31 - 1)
         return t.to(self.device, torch.int32).contiguous()
 
