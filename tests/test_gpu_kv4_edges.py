@@ -302,3 +302,24 @@ def test_a_mixed_step_as_two_plans(heads, kv, dim, chunk):
         outs.append(out[rows])
         f.cache.check_device()
     assert torch.equal(*outs)
+
+
+@pytest.mark.parametrize("heads, kv, dim, new", [(32, 4, 64, 1), (16, 2, 96, 1), (26, 2, 128, 1), (12, 2, 96, 3), (4, 4, 64, 20), (16, 8, 64, 150), (12, 4, 96, 180),
+                                                 (32, 8, 128, 40)])
+def test_large_values_of_little_weight(heads, kv, dim, new):
+    """Weights of 2^-15 to 2^-30 on values a million times the others': they are a part of the sum that is right to their own 11 bits."""
+    f = Filled([1], heads, kv, dim, 64, spare=1300, max_blocks=30)
+    for n in (60, 900):
+        plan = f.cache.plan(f.slots, [n + new], at=[0])
+        k, v = (torch.randn(n + new, kv, dim, generator=f.g, device="cuda") for _ in range(2))
+        v *= 0.01
+        k[5:n:9], v[5:n:9] = -2.0, v[5:n:9] * 2e6
+        k, v = k.bfloat16(), v.clamp(-60000, 60000).bfloat16()
+        f.cache.append(0, k, v, plan)
+        f.k[0], f.v[0] = stored(k), stored(v)
+        plan = f.cache.plan(f.slots, [new], at=[n])
+        f.cache.append(0, k[n:], v[n:], plan)
+        q = torch.randn(new, heads, dim, device="cuda", generator=f.g).abs().bfloat16()
+        ref, mag, _ = f.want(q, [new])
+        # weights below 2^-29 of the largest: half a unit of 2^-39 each
+        close(f.cache.attention(0, q, plan), (ref, mag, 2.0 ** -40 * f.v[0].abs().sum(0).amax()))

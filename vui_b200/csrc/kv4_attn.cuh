@@ -49,10 +49,12 @@ __device__ __forceinline__ float score_factor(float f, uint32_t big) {
     return fminf(fmaxf(f, 1e-37f), 1e26f) + (big >= 0x7f80u ? __int_as_float(0x7fffffff) : 0.f);
 }
 
-// Two products by two factors in one instruction.
-__device__ __forceinline__ void mul2(float& a, float& b, float factor_a, float factor_b) {
-    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tmul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
-        : "+f"(a), "+f"(b) : "f"(factor_a), "f"(factor_b));
+// Two scores, 15 higher, in one instruction: weights that become f16 are 2^15 times as large as the maximum's distance says, as are their sums, so
+// that they keep their 11 bits down to 2^-29 of the largest and are lost below 2^-40, not 2^-14 and 2^-25: positions of little weight
+// may hold large values.
+__device__ __forceinline__ void lifted2(float& a, float& b, float factor_a, float factor_b) {
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tmov.b64 z, {%4, %4};\n\tfma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "+f"(a), "+f"(b) : "f"(factor_a), "f"(factor_b), "f"(15.f));
 }
 
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
@@ -361,7 +363,7 @@ __device__ __forceinline__ void ka_finish(const Kv4AttnArgs& a, const KaRing<NG,
 // Form for tiles of 8 or 16 columns: keys as the A operand, queries as the B operand (8 columns), values as f16; the scores'
 // transpose for the second product is one movmatrix a fragment.  Each warp has its own positions and makes f16 of them in registers, 13
 // instructions for eight codes: with 16 columns about what their products cost.  Softmax statistics and sums are fp32; the weights enter the second
-// product as f16 (2^-11 of each, where bf16's 2^-8 would be as much as the output's own rounding).
+// product as f16, 2^15 times as large (2^-11 of each, where bf16's 2^-8 would be as much as the output's own rounding).
 template <int NG, int NT>
 __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn(const Kv4AttnArgs a) {
     constexpr int HD = NG * KV4_GROUP, COLS = NT * 8;
@@ -511,7 +513,7 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn(const Kv4AttnArgs 
                     for (int j = 0; j < 4; j += 2) {
                         e[j] = sc[k2][nt][j] + less[0];
                         e[j + 1] = sc[k2][nt][j + 1] + less[1];
-                        mul2(e[j], e[j + 1], factor[nt][0], factor[nt][1]);
+                        lifted2(e[j], e[j + 1], factor[nt][0], factor[nt][1]);
                         e[j] = ex2(e[j]);
                         e[j + 1] = ex2(e[j + 1]);
                         l[nt][0] += e[j];
@@ -871,7 +873,7 @@ __global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn_few(const Kv4AttnA
 // Form for chunks of prompts: a CTA takes 128 columns, 16 a warp, and 64 positions at a time.  Codes become f16 once a CTA, one tile of 16 keys or
 // values a warp, and lie in shared memory in the order in which lanes need them as the B operands of m16n8k16: 16 bytes a lane, no conflicts.
 // The queries are the A operand of the first product and stay in registers; the weights, as the first product leaves them, are the A operand of
-// the second.  A lane ends with eight neighbouring elements of its rows.  (Weights below 2^-25 of a column's largest are lost in f16.)
+// the second.  A lane ends with eight neighbouring elements of its rows.  (Weights are 2^15 times as large here too.)
 // Each step's codes are read while the step before is computed; two buffers, so that one barrier a step is enough.
 // Bound: at heads of 128 a step's products take the tensor cores 2130 cycles at mma.sync's rate (8.3 a product and scheduler) and its operands
 // 2050 of shared memory's; measured, about 4500 with the exponentials and the conversion in between, as two warps a scheduler overlap them
@@ -1081,7 +1083,7 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kv4_attn_rows(const Kv4AttnAr
                         float &u0 = s[k][h][2 * r], &u1 = s[k][h][2 * r + 1];
                         u0 += less[r];
                         u1 += less[r];
-                        mul2(u0, u1, factor[r], factor[r]);
+                        lifted2(u0, u1, factor[r], factor[r]);
                         u0 = ex2(u0);
                         u1 = ex2(u1);
                         l[r] += u0;
