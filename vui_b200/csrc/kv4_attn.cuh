@@ -610,8 +610,10 @@ __device__ __forceinline__ float two_bytes(int high, int low) {
     return fmaf(__int_as_float(high) - 12582912.f, 256.f, __int_as_float(low) - 12582912.f);
 }
 
+// At least 4 CTAs an SM, which shared memory allows at every width: with no number the compiler kept to 72 registers and spilled at three
+// of five widths (4 x 64k 78.1 us, heads of 96 17.5 for 17.2), with 5 at two (85.0).
 template <int NG, bool HALVES>
-__global__ void __launch_bounds__(KA_THREADS + 32) k_kv4_attn_few(const Kv4AttnArgs a) {
+__global__ void __launch_bounds__(KA_THREADS + 32, 4) k_kv4_attn_few(const Kv4AttnArgs a) {
     static_assert(!HALVES || NG % 2 == 0, "two halves of an even number of groups");
     constexpr int HD = NG * KV4_GROUP, COLS = HALVES ? 2 : 4;
     constexpr int OWN = HALVES ? NG / 2 : NG, SIDES = HALVES ? 2 : 1;      // groups that a lane scales; group i * SIDES + side
