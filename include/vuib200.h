@@ -509,6 +509,8 @@ int64_t vuib_codec_enc_launch_count(VuibCodecEnc* c);
  * a new block.  A vector (position, kv head) is stored in groups of 32 elements as 4-bit codes with an f16 scale and
  * zero: 80 bytes a position and kv head at head_dim 64 (keys and values), where bf16 takes 256.
  *   zero = f16(min x), scale = f16((max x - zero) / 15), code = nearest of 0..15; it stands for f16(scale*code + zero).
+ * vuib_kv4_read and attention of more than 4 columns (rows of a sequence x query heads of a kv head) take that value;
+ * attention of up to 4 takes scale*code + zero without the last rounding, 2^-11 of the value.
  * Sequences are slots 0 .. max_seqs-1; their lengths are the device's.  A step is
  *   vuib_kv4_plan once, then for every layer vuib_kv4_append and vuib_kv4_attention with that plan.
  * All calls are asynchronous on `stream`, can be captured, allocate nothing and launch on the current device, which is
@@ -571,8 +573,10 @@ int32_t vuib_kv4_read(VuibKv4* c, int32_t layer, int32_t n_rows, const int32_t* 
 
 /* Causal attention of the plan's rows over their sequences: row r of a sequence attends positions [0, its own], its own
  * row included (store it first).  q, out: bf16 (n_rows, n_heads * head_dim), strides as in vuib_kv4_append; query head j
- * reads kv head j / (n_heads / n_kv_heads).  scale 0: 1/sqrt(head_dim).  Rows behind the plan's last row are not
- * written.  The workspace (256-byte aligned, contents of no account) holds the parts of long sequences. */
+ * reads kv head j / (n_heads / n_kv_heads).  scale 0: 1/sqrt(head_dim).  A query that is not finite gives NaN.  Rows
+ * behind the plan's last row are not written.  All of a plan's rows go by one form, which max_new decides: single
+ * tokens beside a prompt's chunk are served better, and with the bits of a step of their own, by a plan of their own.
+ * The workspace (256-byte aligned, contents of no account) holds the parts of long sequences. */
 int32_t vuib_kv4_attention_workspace(VuibKv4* c, const VuibKv4Plan* plan, size_t* bytes);
 int32_t vuib_kv4_attention(VuibKv4* c, int32_t layer, const VuibKv4Plan* plan, const void* q_dev, int64_t q_stride,
                            void* out_dev, int64_t out_stride, float scale, void* ws_dev, size_t ws_bytes, void* stream);

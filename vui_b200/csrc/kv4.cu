@@ -67,16 +67,16 @@ long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
 // What a plan's shape decides for attention: the form, the columns of a tile (rows x query heads of a kv head) and the positions of a split.
 //   FEW_2, FEW_4   bytes: up to 2 columns (heads of 64 and 128) and up to 4.  256 sequences of 512 to 2048 positions, two query heads a kv head of 64:
-//                  53 us with FEW_2, 62 with FEW_4, 203 with the f16 form for 16; 4 query heads of 128, 4 x 64k positions: 75 with FEW_4, 92 with MANY_8.
-//   MANY_8, _16    f16, a warp's own keys: up to 8 and 16 columns a tile.  64 sequences of up to 4000, 8 query heads of 128: 85 us with MANY_8, 109
-//                  with the byte form for 8; 16 rows' columns of 4 heads of 128: 23 us with MANY_16, 37 with the byte form for 16; tiles of 32
-//                  columns are slower wherever they fill (64 x 24 rows of 2 query heads of 64: 30 us with 16, 45 with 32).
+//                  53 us with FEW_2, 64 with FEW_4, 105 with MANY_16; 4 query heads of 128, 4 x 64k positions: 77 with FEW_4, 92 with MANY_8.
+//   MANY_8, _16    f16, a warp's own keys: up to 8 and 16 columns a tile.  64 sequences of 800 to 4000, 8 query heads a kv head of 128 (8 kv heads): 71 us
+//                  with MANY_8, 91 with MANY_16; 16 query heads (4 kv heads): 69 and 57; tiles of 32 columns, when they were built, were
+//                  slower wherever they fill (64 x 24 rows of 2 query heads of 64: 30 us with 16, 45 with 32).
 //   ROWS           f16, shared keys, 128 columns: from 128 columns of heads of 128 on, 256 of 64, 512 of 96.  Against MANY_16, us: heads of 128, 128
-//                  columns 28 and 30, 256 32 and 47, 2 x 1000 rows 952 and 1408; heads of 64, 128 columns 38 and 32, 256 43 and 54, 2000 38 and
-//                  40; heads of 96, 300 columns 39 and 31, 600 54 and 54.
+//                  columns 28 and 29, 256 32 and 47, 2 x 1000 rows 1060 and 1556; heads of 64, 128 columns 38 and 32, 256 43 and 55, 2000 38 and
+//                  40; heads of 96, 300 columns 39 and 32, 600 54 and 54.
 // Splits.  Up to 16 columns by the sequence's length alone, so that a row's bits do not depend on what else is there: one of up to 512 positions is one
-// piece (64 sequences of 64 to 512: 10.3 us, in pieces of 256 12.4), up to 1024 pieces of 256 (16 sequences of up to 1000, 8 query heads of 128:
-// 19.7, in pieces of 512 23.1), beyond of 512 (4 x 64k: 74.7, 256 79.4, 1024 76.4).  More columns: none where the tiles fill the SMs, else pieces of 512,
+// piece (64 sequences of 64 to 512: 10.4 us, in pieces of 256 12.9), up to 1024 pieces of 256 (16 sequences of 600 to 1000, 8 query heads a kv head of
+// 128: 12.5, in pieces of 512 15.7), beyond of 512 (4 x 64k: 77, 256 82, 1024 80).  More columns: none where the tiles fill the SMs, else pieces of 512,
 // at most 8 of a sequence, so that their sums stay a few megabytes.
 enum Form { FEW_2, FEW_4, MANY_8, MANY_16, ROWS };
 struct Shape { Form form; int cols; Kv4Split split; };
@@ -157,7 +157,7 @@ cudaError_t launch_attn(VuibKv4* c, const Shape& s, void (*kern)(Kv4AttnArgs), i
     }
     const long long room = (long long)c->sms * resident;
     // A kernel that starts beside the merge finds its SMs partly taken, and one that fills them all then has late CTAs: 256 sequences of
-    // 512 to 2048 positions call after call 61.0 us with an early start and 53.0 without, one sequence of 300 6.3 and 6.7.
+    // 512 to 2048 positions call after call 61.7 us with an early start and 53.4 without, one sequence of 1300 7.8 and 7.9.
     a.early = 2 * items < room;
     const long long grid = min(items, room), rows = (long long)a.n_rows * c->cfg.n_heads;
     e = launch(c, kern, dim3((unsigned)grid), threads, smem, 1, stream, a);

@@ -596,6 +596,7 @@ __device__ __forceinline__ void mma16832(int (&d)[4], uint32_t a0, uint32_t a1, 
 // them at half rate.
 //   scores:  q . K = sum over groups of scale * (q . code) + zero * (sum of the group's q)
 //   outputs: sum_i w_i V_i = sum_i (w_i scale_i) code_i + sum_i w_i zero_i
+// So K and V are scale * code + zero here, without the rounding to f16 (2^-11 of the value) that the other forms and k_kv4_read make.
 // A query column, times a power of two, is a 15-bit whole number: exact for elements down to 2^-6 of the largest, the others to 2^-14 of
 // it.  The weights times the value scales are 16-bit whole numbers in units of 2^-16 of the largest such product of the query and group
 // among the warp's positions (half a unit off, each on its own): positions that a query does not see, or whose weight is nothing, take no part
@@ -603,8 +604,8 @@ __device__ __forceinline__ void mma16832(int (&d)[4], uint32_t a0, uint32_t a1, 
 // what is added to them, statistics and outputs, is fp32.
 // A product's columns hold four queries; or (HALVES, for up to two queries a tile, heads of 64 and 128) two queries twice, once for the
 // even groups of 32 elements and once for the odd ones, zeros elsewhere: a lane then has one group of two to scale and to weigh.
-// 256 sequences of 512 to 2048 positions, two query heads a kv head of 64: 53 us (219 MB: 34 us), the copies alone 52; with f16 values and a
-// product's 8 columns a query each, 93.  4 sequences of 64k, four query heads of 128: 75 us (313 MB: 48).
+// 256 sequences of 512 to 2048 positions, two query heads a kv head of 64: 53.5 us (219 MB: 34 us), the copies alone 52; with f16 values and a
+// product's 8 columns a query each, 93.  4 sequences of 64k, four query heads of 128: 77 us (313 MB: 48).
 constexpr int KA_ORIGIN = 0x4B400000;   // sums that start as the bits of 1.5 * 2^23 are that float plus the sum (below 2^22 in magnitude)
 __device__ __forceinline__ float two_bytes(int high, int low) {
     return fmaf(__int_as_float(high) - 12582912.f, 256.f, __int_as_float(low) - 12582912.f);
@@ -879,8 +880,8 @@ __global__ void __launch_bounds__(KA_THREADS + 32, 4) k_kv4_attn_few(const Kv4At
 // Each step's codes are read while the step before is computed; two buffers, so that one barrier a step is enough.
 // Bound: at heads of 128 a step's products take the tensor cores 2130 cycles at mma.sync's rate (8.3 a product and scheduler) and its operands
 // 2050 of shared memory's; measured, about 4500 with the exponentials and the conversion in between, as two warps a scheduler overlap them
-// only in part.  2 x 1000 rows of 32 query and 8 kv heads of 128 against 6000 to 9000 positions: 952 us, 243 TFLOP/s of some 540 that mma.sync
-// can do.  12 warps with 96 positions at a time (168 registers, spills) take 994 us, 16 warps 1339.
+// only in part.  2 x 1000 rows of 32 query and 8 kv heads of 128 against 6000 to 9000 positions: 1061 us, 216 TFLOP/s of some 540 that mma.sync
+// can do.  12 warps with 96 positions at a time (168 registers, spills) and 16 warps were slower.
 constexpr int KR_COLS = 128, KR_WARPS = 8, KR_THREADS = KR_WARPS * 32, KR_STEP = 64;
 template <int NG>
 struct KrShared {

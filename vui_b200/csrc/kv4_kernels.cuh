@@ -2,7 +2,7 @@
 //
 // A stored vector (one position, one kv head, keys or values) is cut into groups of 32 elements:
 //   zero = f16(min x), scale = f16((max x - zero) * fl(1/15)), code = rint((x - zero) / scale) in 0 .. 15,
-// and a code stands for f16(scale * code + zero).
+// and a code stands for f16(scale * code + zero).  (Attention of up to 4 columns takes scale * code + zero as it is.)
 //
 // Layout of a layer's pool: [block][kv head][16 positions][32 elements] -> 640 bytes, laid out as the fragments that the attention
 // feeds to the tensor cores (lane = 4 g + t of a warp; keys 0 .. 15 are the positions of a tile):

@@ -202,7 +202,8 @@ class Kv4Cache:
 
     def _rows(self, t: Tensor, name: str, n: int, heads: int, *, out: bool = False) -> Tensor:
         """(n, heads, head_dim) or (n, heads * head_dim) as the library takes it: bf16 on this device, heads behind one
-        another, rows a multiple of 16 bytes apart.  An input that lies otherwise is copied, an output refused."""
+        another, rows a multiple of 16 bytes apart.  An input that lies otherwise, or is of another type or device, is copied (and
+        rounded to bf16), an output refused."""
         if torch.is_tensor(t) and t.dtype is torch.bfloat16 and t.device == self.device and t.shape == (n, heads, self.head_dim) and \
                 t.is_contiguous() and t.data_ptr() % 16 == 0:
             return t
@@ -225,7 +226,8 @@ class Kv4Cache:
 
     def append(self, layer: int, k: Tensor, v: Tensor, plan: Kv4Plan) -> None:
         """Stores the plan's rows: k, v (n_rows, n_kv_heads, head_dim), keys with RoPE applied.  NaN is stored as 0 and
-        magnitudes beyond 60000 as 60000, which ``check_device`` reports."""
+        magnitudes beyond 60000 as 60000, which ``check_device`` reports.  Other types than bf16, other devices and rows that are not
+        16-byte aligned are copied first."""
         self._own(plan)
         with self._here():
             n, heads = plan.n_rows, self.n_kv_heads
@@ -254,7 +256,10 @@ class Kv4Cache:
     def attention(self, layer: int, q: Tensor, plan: Kv4Plan, *, scale: float | None = None, out: Tensor | None = None) -> Tensor:
         """Causal attention of the plan's rows, each over its sequence up to and with its own position (append first):
         q (n_rows, n_heads, head_dim) with RoPE applied -> the same shape, bf16.  ``scale`` defaults to 1 / sqrt(head_dim).
-        Rows behind the plan's last are not written."""
+        Rows behind the plan's last are not written.  ``q`` is copied first where ``append`` would copy.
+
+        All of a plan's rows are served in one way, by its ``max_new``: a prompt's chunk of a hundred rows and more and single tokens of
+        other sequences in one step are faster as two plans, and the single tokens then have the bits of a step of their own."""
         if scale is not None and not (scale <= 1e30 and C.c_float(scale).value > 0):       # 0 is the library's word for the default
             raise ValueError("scale must be positive, also in 32 bits, and at most 1e30")
         self._own(plan)
